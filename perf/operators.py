@@ -381,12 +381,17 @@ def work(case):
 
 
 # ----------------------------------------------------------------------------- in 64 bits
+def _two64(e):
+    """2^e as float64, exactly, for whole e of any type."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _decode64(codes, exps):
     """e4m3 codes and biased exponents as float64, from the format's definition."""
     c = codes.long()
     sign, e, m = 1.0 - 2.0 * (c >> 7), (c >> 3) & 15, (c & 7).double()
-    x = torch.where(e > 0, (1 + m / 8) * 2.0 ** (e - 7).double(), m / 8 * 2.0 ** -6)
-    return sign * x * 2.0 ** (exps.double() - 127).unsqueeze(-1)
+    x = torch.where(e > 0, (1 + m / 8) * _two64(e - 7), m / 8 * 2.0 ** -6)
+    return sign * x * _two64(exps.long() - 127).unsqueeze(-1)
 
 
 def exact(case, seed):
@@ -411,10 +416,10 @@ def exact(case, seed):
                 if case["cache"] == "e4m3":
                     top = x.abs().amax(-1)
                     e = torch.ceil(torch.log2(top / E4M3_MAX))
-                    e = e + (top > E4M3_MAX * 2.0 ** e).double() - (top <= E4M3_MAX * 2.0 ** (e - 1)).double()
+                    e = e + (top > E4M3_MAX * _two64(e)).double() - (top <= E4M3_MAX * _two64(e - 1)).double()
                     out[2 + i][page, :, slot] = e.long() + 127
-                    y = x * 2.0 ** -e.unsqueeze(-1)
-                    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)  # e4m3's spacing at y
+                    y = x * _two64(-e).unsqueeze(-1)
+                    step = _two64(torch.frexp(y.abs().clamp(min=2.0 ** -6))[1] - 4)  # e4m3's spacing at y
                     x = torch.round(y / step) * step  # to nearest, ties to even
                 out[i][page, :, slot] = x
         return tuple(out)
