@@ -46,6 +46,13 @@ class GemmDesc(C.Structure):
                 ("B", vp), ("ldb", i64), ("C", vp), ("ldc", i64)]
 
 
+class KVPages(C.Structure):
+    """aic_kv_pages: a layer's paged key/value cache."""
+    _fields_ = [("k_pages", vp), ("v_pages", vp), ("k_exps", vp), ("v_exps", vp), ("page_table", vp),
+                ("ld_table", i64), ("n_pages", i64), ("page_size", i64), ("kv_heads", i64), ("head_dim", i64),
+                ("type", i32)]
+
+
 class LMConfig(C.Structure):
     _fields_ = [("vocab", i64), ("d_model", i64), ("n_layers", i64), ("n_heads", i64), ("d_ffn", i64),
                 ("max_seq_len", i64), ("norm_eps", f32), ("rope_base", f32), ("tied", i32), ("compute", i32),
@@ -100,6 +107,14 @@ SIGNATURES = {
                                   vp]),
     "aic_hip_attn_bwd_rope": (i32, [vp, vp, vp, i64, vp, vp, i64, vp, vp, vp, vp, i64, i64, i64, i64, i64, i32, f32,
                                     vp, vp, i32, vp]),
+    "aic_hip_kv_write": (i32, [C.POINTER(KVPages), vp, vp, i64, vp, vp, i64, i64, i32, vp]),
+    "aic_hip_kv_read": (i32, [C.POINTER(KVPages), vp, vp, i64, vp, vp, i64, i64, i32, vp]),
+    "aic_hip_attn_paged_workspace": (i64, [C.POINTER(KVPages), i64, i64, i64, i64, i64]),
+    "aic_hip_attn_paged": (i32, [C.POINTER(KVPages), vp, i64, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, f32,
+                                 vp, i64, i32, vp]),
+    "aic_hip_verify_drafts_workspace": (i64, [i64, i64, i64]),
+    "aic_hip_verify_drafts": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, vp, i64, i64, i64, i64, f32, vp, vp, vp, vp, i64,
+                                    i32, vp]),
     "aic_hip_swiglu_fwd": (i32, [vp, vp, i64, vp, i64, i64, i64, i32, vp]),
     "aic_hip_swiglu_bwd": (i32, [vp, vp, i64, vp, i64, vp, vp, i64, i64, i64, i32, vp]),
     "aic_hip_ce_fwd": (i32, [vp, i64, vp, i64, i64, i64, vp, vp, vp, vp, i32, vp]),

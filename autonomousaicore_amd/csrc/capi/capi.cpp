@@ -100,6 +100,20 @@ int guard(F&& f) {
 aic::DType dt(aic_dtype d) { return static_cast<aic::DType>(static_cast<int>(d)); }
 hipStream_t st(aic_stream s) { return static_cast<hipStream_t>(s); }
 
+aic::hip::KVPages pages(const aic_kv_pages* c) {
+    AIC_CHECK(c, InvalidArgument, "null cache descriptor");
+    return {c->k_pages, c->v_pages,   c->k_exps,   c->v_exps,   c->page_table, c->ld_table,
+            c->n_pages, c->page_size, c->kv_heads, c->head_dim, dt(c->type)};
+}
+
+// A size, or minus the error code.
+template <typename F>
+int64_t guard_size(F&& f) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = f(); });
+    return rc == 0 ? n : -static_cast<int64_t>(rc);
+}
+
 }  // namespace
 
 extern "C" {
@@ -239,6 +253,46 @@ int aic_hip_attn_bwd(const void* q, const void* k, const void* v, int64_t ld_qkv
     return guard([&] {
         aic::hip::attn_bwd(q, k, v, ld_qkv, o, dout, ld_o, lse, dq, dk, dv, ld_d, B, H, S, hd, causal != 0, scale,
                            dt(d), st(stream));
+    });
+}
+
+int aic_hip_kv_write(const aic_kv_pages* cache, const void* k, const void* v, int64_t ld, const int64_t* offsets,
+                     const int64_t* lens, int64_t B, int64_t T, aic_dtype d, aic_stream stream) {
+    return guard([&] { aic::hip::kv_write(pages(cache), k, v, ld, offsets, lens, B, T, dt(d), st(stream)); });
+}
+
+int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, const int64_t* offsets,
+                    const int64_t* lens, int64_t B, int64_t T, aic_dtype d, aic_stream stream) {
+    return guard([&] { aic::hip::kv_read(pages(cache), k, v, ld, offsets, lens, B, T, dt(d), st(stream)); });
+}
+
+int64_t aic_hip_attn_paged_workspace(const aic_kv_pages* cache, int64_t B, int64_t T, int64_t max_q, int64_t max_len,
+                                     int64_t H) {
+    return guard_size([&] { return aic::hip::attn_paged_workspace(pages(cache), B, T, max_q, max_len, H); });
+}
+
+int aic_hip_attn_paged(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse,
+                       const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, int64_t max_q,
+                       int64_t max_len, int64_t H, int64_t window, float scale, void* workspace,
+                       int64_t workspace_bytes, aic_dtype d, aic_stream stream) {
+    return guard([&] {
+        aic::hip::attn_paged(pages(cache), q, ld_q, o, ld_o, lse, offsets, lens, B, T, max_q, max_len, H, window, scale,
+                             workspace, workspace_bytes, dt(d), st(stream));
+    });
+}
+
+int64_t aic_hip_verify_drafts_workspace(int64_t B, int64_t T, int64_t V) {
+    return guard_size([&] { return aic::hip::verify_drafts_workspace(B, T, V); });
+}
+
+int aic_hip_verify_drafts(const void* logits, int64_t ld, const void* draft_logits, int64_t ld_draft,
+                          const int64_t* ids, const float* u, const float* u_next, const int64_t* offsets,
+                          const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t V, float temperature,
+                          int64_t* tokens, int64_t* counts, int64_t* new_lens, void* workspace,
+                          int64_t workspace_bytes, aic_dtype d, aic_stream stream) {
+    return guard([&] {
+        aic::hip::verify_drafts(logits, ld, draft_logits, ld_draft, ids, u, u_next, offsets, lens, B, T, max_q, V,
+                                temperature, tokens, counts, new_lens, workspace, workspace_bytes, dt(d), st(stream));
     });
 }
 

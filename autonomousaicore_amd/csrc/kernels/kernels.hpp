@@ -161,6 +161,33 @@ void attn_cached(const void* q, int64_t ldq, const void* kc, const void* vc, int
 void kv_append(const void* qkv, void* kc, void* vc, int64_t B, int64_t S, int64_t d, int64_t cache_rows,
                int64_t start_pos, DType dt, hipStream_t s);
 
+// The paged key/value cache (paged_kv.hip): pools [n_pages][kv_heads][page_size][head_dim] of type
+// (UInt8: e4m3 codes with an exponent byte per [n_pages][kv_heads][page_size]) and the sequences' page
+// ids.  Sequence b's rows offsets[b] .. offsets[b + 1] are the last of its lens[b] cached tokens.
+struct KVPages {
+    void *k_pages = nullptr, *v_pages = nullptr;
+    uint8_t *k_exps = nullptr, *v_exps = nullptr;
+    const int32_t* page_table = nullptr;
+    int64_t ld_table = 0, n_pages = 0, page_size = 0, kv_heads = 0, head_dim = 0;
+    DType type = DType::BFloat16;
+};
+void kv_write(const KVPages& c, const void* k, const void* v, int64_t ld, const int64_t* offsets, const int64_t* lens,
+              int64_t B, int64_t T, DType dt, hipStream_t s);
+void kv_read(const KVPages& c, void* k, void* v, int64_t ld, const int64_t* offsets, const int64_t* lens, int64_t B,
+             int64_t T, DType dt, hipStream_t s);
+// Attention over it (attention_paged.hip).  workspace null: the stream's scratch, or no split of the
+// keys where the call is captured.
+int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H);
+void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int64_t* offsets,
+                const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t window,
+                float scale, void* workspace, int64_t workspace_bytes, DType dt, hipStream_t s);
+// Verification of drafted tokens (drafts.hip); draft null: one-hot drafts.
+int64_t verify_drafts_workspace(int64_t B, int64_t T, int64_t V);
+void verify_drafts(const void* logits, int64_t ld, const void* draft, int64_t ld_draft, const int64_t* ids, const float* u,
+                   const float* u_next, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, int64_t max_q,
+                   int64_t V, float temperature, int64_t* tokens, int64_t* counts, int64_t* new_lens, void* workspace,
+                   int64_t workspace_bytes, DType dt, hipStream_t s);
+
 // Optimizer tail (optim.hip)
 struct OptimCtl;  // = aic_optim_ctl (include/aic_hip.h)
 void grad_sqnorm_multi(const float* const* grads, const int64_t* sizes, int count, double* sqnorm, int* nonfinite,

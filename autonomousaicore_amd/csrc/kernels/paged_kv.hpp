@@ -1,0 +1,72 @@
+// The paged key/value cache as its kernels see it (paged_kv.hip, attention_paged.hip).
+#pragma once
+
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace aic::hip {
+
+// Pools [n_pages][Hkv][ps][hd]: a page holds each head's rows one after another, so that the rows
+// of a head that one block reads are whole runs of ps * hd elements.  e4m3 pools carry one byte per
+// (page, head, slot): the row is code * 2^(byte - 127).  Powers of two cost no precision that the
+// codes have (e4m3 is a floating format: moving a row by up to one binade leaves its relative steps),
+// make the values exact in bf16, and go through the hardware's scaled conversion for free.
+struct PageView {
+    char *kp, *vp;
+    uint8_t *ke, *ve;
+    const int32_t* table;
+    int64_t ld_table;
+    int32_t n_pages, ps, Hkv;
+    uint32_t mul;  // position / ps = position * mul >> shift, exact below 2^31
+    int shift;
+
+    __device__ __forceinline__ int page_index(int pos) const {
+        return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(pos)) * mul) >> shift);
+    }
+    // Row index (in rows of hd elements) of position pos of the sequence whose table row is `tr`, head
+    // h; -1 where the table has no valid page there.
+    __device__ __forceinline__ int64_t row(const int32_t* tr, int pos, int h) const {
+        const int pi = page_index(pos);
+        const int page = pi < ld_table ? tr[pi] : -1;
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(n_pages)) return -1;
+        return (static_cast<int64_t>(page) * Hkv + h) * ps + (pos - pi * ps);
+    }
+};
+
+// Arguments checked, and the view made of them.  `what` names the entry in the messages.
+PageView page_view(const KVPages& c, const char* what);
+
+constexpr int kBlock = 256;
+
+// Block-wide: how many of offsets[0 .. B-1] are <= t, minus one: the sequence of packed row t, or one
+// before it in a run of empty sequences.  One parallel load instead of a chain of dependent ones.
+__device__ __forceinline__ int block_sequence(const int64_t* offsets, int B, int64_t t) {
+    int n = 0;
+    for (int i0 = 0; i0 < B; i0 += kBlock) {
+        const int i = i0 + static_cast<int>(threadIdx.x);
+        n += __syncthreads_count(i < B && offsets[i] <= t);
+    }
+    return n - 1;
+}
+
+// The eight e4m3 codes of w times the power of two s, as floats: element j in byte j.
+__device__ __forceinline__ void e4m3_floats(uint2 w, float s, float (&v)[8]) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w.x, s, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w.x, s, true);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w.y, s, false);
+    const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w.y, s, true);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
+}
+// The same as bf16, where code * s is exact.
+__device__ __forceinline__ uint4 e4m3_bf16(uint2 w, float s) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, true)));
+}
+// 2^(b - 127) of a stored exponent byte (1 .. 254; 0 and 255 cannot be written and read as 2^-126, 2^127).
+__device__ __forceinline__ float exp_scale(uint32_t b) {
+    return __uint_as_float(min(max(b, 1u), 254u) << 23);
+}
+
+}  // namespace aic::hip

@@ -250,6 +250,88 @@ int aic_hip_attn_bwd_qk(const void* q, int64_t ld_q, const void* k, const void* 
                         int64_t ld_dkv, int64_t B, int64_t H, int64_t Sq, int64_t Sk, int64_t hd, int causal,
                         float scale, aic_dtype dt, aic_stream stream);
 
+/* ---------------------------------------------------------------- paged KV cache ----- */
+/* A key/value cache of one layer in pages: k_pages and v_pages are pools
+ * [n_pages][kv_heads][page_size][head_dim] (16-byte aligned; head_dim 32, 64 or 128; any page_size
+ * from 1 to 65536), and position j of sequence b is slot j % page_size of page
+ * page_table[b * ld_table + j / page_size] (device memory; several sequences may read one page).
+ * type: AIC_F32, AIC_BF16, or AIC_U8 for e4m3 codes (4 exponent, 3 mantissa bits, largest 448):
+ * a row's head is code * 2^(byte - 127), byte in k_exps / v_exps [n_pages][kv_heads][page_size].
+ *
+ * The calls below share a ragged batch's description, in device memory: offsets [B + 1] and lens [B]
+ * (int64).  Sequence b's packed rows offsets[b] .. offsets[b + 1] - 1 are the last ones of its
+ * lens[b] cached tokens, the new ones included: row i of n stands at position lens[b] - n + i.
+ * offsets do not decrease; T bounds offsets[B] (the row buffers' size).  A sequence may have no rows
+ * or an empty cache.  Rows that belong to no sequence are left as they are.  Lengths reach
+ * 2^31 - 4096.  A position before 0, past the page table's row, or whose page id is outside
+ * [0, n_pages) has no place in the cache: see each call.
+ * No reference counterpart: the reference keeps one contiguous cache per layer
+ * (CausalSelfAttention::forward_with_cache, include/nn/attention.hpp:49-120). */
+typedef struct {
+    void* k_pages;
+    void* v_pages;
+    uint8_t* k_exps; /* AIC_U8 only */
+    uint8_t* v_exps;
+    const int32_t* page_table;
+    int64_t ld_table, n_pages, page_size, kv_heads, head_dim;
+    aic_dtype type;
+} aic_kv_pages;
+/* The new rows k, v [T, kv_heads * head_dim] (leading dimension ld, dtype dt F32 or BF16) into their
+ * places.  A cache of dt takes them as they are.  An e4m3 cache takes each row's head with the least
+ * power of two 2^e >= max|x| / 448 (e >= -126), codes rounded to nearest, ties to even; an
+ * infinity or NaN is held as NaN.  Rows without a place are not written.  Two rows of one call must
+ * not share a place. */
+int aic_hip_kv_write(const aic_kv_pages* cache, const void* k, const void* v, int64_t ld, const int64_t* offsets,
+                     const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
+/* The other way: the cached rows at the batch's positions to k, v [T, kv_heads * head_dim] (e4m3 to
+ * bf16 is exact); rows without a place are zero. */
+int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, const int64_t* offsets,
+                    const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
+/* Attention of the batch's rows over the cache, for chunks of a prompt, drafted tokens and single tokens
+ * alike.  q and o are [T, H * head_dim] (leading dimensions ld_q, ld_o; dtype dt: the cache's, or
+ * either with an e4m3 cache); query head h reads key/value head h / (H / kv_heads).  The row at
+ * position pos sees the cached positions j <= pos, with window > 0 only those above pos - window:
+ *   o = sum_j softmax_j(scale q . k_j) v_j,   lse[t * H + h] = log sum_j exp(scale q . k_j)
+ * (lse fp32, nullable).  A row that sees nothing (position before 0) has o = 0 and lse = -infinity.  A
+ * row that sees a position without a place in the cache is NaN.  What a row does not see does not
+ * reach it, infinities and NaN included.  scale > 0.
+ * max_q and max_len: the most rows of a sequence and the longest lens[b], for the choice of
+ * kernels; larger values in offsets and lens give right results, slower.
+ * workspace: device memory of at least aic_hip_attn_paged_workspace(...) bytes for the same sizes,
+ * 16-byte aligned, of this call alone until it is done; NULL: the stream's scratch memory.  A captured
+ * call with NULL does not split the keys among blocks (slow for few rows): give it one that
+ * lives as long as the graph.  Deterministic for given sizes and workspace use. */
+int64_t aic_hip_attn_paged_workspace(const aic_kv_pages* cache, int64_t B, int64_t T, int64_t max_q, int64_t max_len,
+                                     int64_t H); /* negative: -(error code) */
+int aic_hip_attn_paged(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse,
+                       const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, int64_t max_q,
+                       int64_t max_len, int64_t H, int64_t window, float scale, void* workspace,
+                       int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
+/* Speculative sampling's verification.  Sequence b's rows are its newest token and the drafted ones
+ * behind it, ids [T] (int64); logits [T, V] (dtype dt F32 or BF16, leading dimension ld) are the target's
+ * after each of them, draft_logits (nullable, the same layout, ld_draft; a sequence's last row is not
+ * used) those that the next id was drawn from.  With p = softmax(logits[t] / temperature) and d =
+ * softmax(draft_logits[t] / temperature) (NULL: all on ids[t + 1]), ids[t + 1] is kept where
+ * u[t] d < p (u [T] fp32 in [0, 1)).  The first that is not kept is replaced by a draw from
+ * max(0, p - d); if all are, one token more is drawn from the last row's p.  The draw is the first
+ * token whose running sum passes u_next[b] (fp32 in [0, 1)) times the whole; sums in 64 bits.
+ * temperature <= 0.001: greedy, as aic_lm_generate (a draft is kept if it is the largest logit, the
+ * lowest index of equal ones; draft_logits, u and u_next are not used).  A NaN logit counts as
+ * -infinity; where no logit is above -infinity the token is -1.
+ * tokens [B, max_q]: the kept drafts and the new token, then -1; counts [B]: how many (0 for a sequence
+ * without rows); new_lens [B] (nullable, may be lens): lens[b] less the rows past the new token's
+ * place, so that the cache goes on behind the kept drafts.  Rows of a sequence past max_q are not
+ * looked at.  workspace: as aic_hip_attn_paged, aic_hip_verify_drafts_workspace(B, T, V) bytes; a
+ * captured call must bring one (InvalidState).
+ * No reference counterpart: TransformerLM::generate draws token by token on the host
+ * (src/models/transformer_lm.cpp:113-213). */
+int64_t aic_hip_verify_drafts_workspace(int64_t B, int64_t T, int64_t V); /* negative: -(error code) */
+int aic_hip_verify_drafts(const void* logits, int64_t ld, const void* draft_logits, int64_t ld_draft,
+                          const int64_t* ids, const float* u, const float* u_next, const int64_t* offsets,
+                          const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t V, float temperature,
+                          int64_t* tokens, int64_t* counts, int64_t* new_lens, void* workspace,
+                          int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
+
 /* ---------------------------------------------------------------- SwiGLU ----------- */
 /* h = silu(g) * u, silu(x) = x / (1 + exp(-x)); g, u, h [T, f] with leading dims ld_gu, ld_h.
  * Replaces: silu + mul of SwiGLU::forward (include/nn/swiglu.hpp:21-33). */
