@@ -10,31 +10,50 @@
 //
 // The running sum's steps are as close as 1e-5 of the whole at a vocabulary of 32000, and p - d
 // cancels: sums, p and d are kept in 64 bits (a sum in 32 bits would move one draw in a few hundred
-// to a neighbouring token).  exp in 64 bits is reduced to 2^f, |f| <= 1/2, and the Taylor polynomial
-// of degree 10 (remainder (ln 2 / 2)^11 / 11! = 2e-13 of the value).
+// to a neighbouring token).
 //
-// Three launches: the rows' statistics by parts of kPart logits (one pass over all logits: the only
-// work that grows with the batch's bytes), then per sequence the decision and the parts' residual
-// sums, then the draw inside the one part it falls into.  Nothing is returned to the host.
+// Three launches: the rows' statistics by parts of kPart logits, a wave each, in one pass over all
+// logits (the only work that grows with the batch's bytes; the parts need no barrier); then per
+// sequence the decision and the residual's sums by runs of kRun; then the draw inside the one run it falls into.
+// Nothing is returned to the host.
 #include <algorithm>
 #include <cmath>
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "wave_dpp.hpp"
 #include "../runtime/memory_pool.hpp"
 
 namespace aic::hip {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kPer = 16;                    // logits per thread
-constexpr int kPart = kThreads * kPer;      // logits per block
+constexpr int kPer = 16;             // logits per lane
+constexpr int kPart = kWave * kPer;  // logits of a part: one wave's
+constexpr int kStatWaves = 4;        // waves of a block: statistics
+constexpr int kWaves = 8;            // decision: rows looked at side by side
+// Logits per lane and per wave of the residual: few, for the weights are straight-line code that each launch
+// fetches anew (16 per lane measured 12.4 us for one sequence, 4 per lane the time in DESIGN).
+constexpr int kFew = 4;
+constexpr int kRun = kWave * kFew;
 
 struct Stat {
-    double sum;   // of 2^((z - max) c) over the part
+    double sum;    // of the weights against max over the part
     float max;
-    int32_t best;  // lowest index of the maximum, -1 if every logit is -infinity or NaN
+    int32_t best;  // lowest index of the maximum (target rows)
+};
+// A row's maximum and the sum of its weights.
+struct Whole {
+    double sum;
+    float max;
+    int32_t best;
+};
+struct Decision {
+    int64_t row;   // the packed row whose distribution the new token comes from
+    int64_t off;   // the token taken out of it (a refused one-hot draft), -1: none
+    int n, kept;
+    int minus;     // the draft's distribution is taken off
+    Whole p, d;
 };
 
 struct DraftArgs {
@@ -43,294 +62,320 @@ struct DraftArgs {
     const int64_t* ids;
     const float *u, *u_next;
     const int64_t *offsets, *lens;
-    int B, V, parts;
+    int B, V, parts, runs;
     int64_t T, max_q;
     double c;  // log2(e) / temperature; 0: greedy
+    // logits below the maximum less reach weigh under 2^-1000, and fp32 tells them from a maximum under plain_top
+    float reach, plain_top;
     int64_t *tokens, *counts, *new_lens;
-    Stat *sz, *sy;     // [T][parts]
-    double* left;      // [B][parts]: residual sums
+    Stat *sz, *sy;       // [T][parts]
+    double* left;        // [B][runs]: residual sums
+    Decision* decided;   // [B]
     bool vec_z, vec_y;
 };
 
-// 2^x for x <= 0, to 3e-13 of the value.
-__device__ __forceinline__ double exp2_neg(double x) {
-    x = fmax(x, -1100.0);  // below the smallest number: zero
-    const double n = rint(x), f = x - n;
-    double p = 7.054911620801123e-9;  // (ln 2)^k / k!, k = 10 .. 0
-    p = fma(p, f, 1.0178086009239699e-7);
-    p = fma(p, f, 1.3215486790144309e-6);
-    p = fma(p, f, 1.5252733804059841e-5);
-    p = fma(p, f, 1.5403530393381609e-4);
-    p = fma(p, f, 1.3333558146428443e-3);
-    p = fma(p, f, 9.6181291076284770e-3);
-    p = fma(p, f, 5.5504108664821580e-2);
-    p = fma(p, f, 2.4022650695910072e-1);
-    p = fma(p, f, 6.9314718055994531e-1);
-    p = fma(p, f, 1.0);
-    return ldexp(p, static_cast<int>(n));
+// 2^x for x <= 0, to 1e-12 of the value: x = n + f with |f| <= 1/2 by adding and taking off 1.5 2^52 (whose
+// low word then is n), a polynomial of 2^f (Chebyshev interpolation of degree 8 on [-1/2, 1/2], off by at most
+// 1.07e-12), and n into the exponent.  x >= -1001.
+__device__ __forceinline__ double exp2_poly(double x) {
+    const double big = x + 6755399441055744.0, f = x - (big - 6755399441055744.0);
+    double p = 1.3255394667825251e-06;
+    p = fma(p, f, 1.531008371327383e-05);
+    p = fma(p, f, 0.00015403455050654204);
+    p = fma(p, f, 0.0013333450549365335);
+    p = fma(p, f, 0.009618129160545788);
+    p = fma(p, f, 0.055504109412293744);
+    p = fma(p, f, 0.24022650695808107);
+    p = fma(p, f, 0.6931471805459256);
+    p = fma(p, f, 1.0000000000000004);
+    return ldexp(p, static_cast<int>(static_cast<uint32_t>(__double_as_longlong(big))));
 }
-// Weight of a logit against its row's maximum; an infinite maximum shares the mass among the infinities.
+__device__ __forceinline__ double exp2_neg(double x) { return x < -1000.0 ? 0.0 : exp2_poly(fmax(x, -1000.0)); }
+// Weight of a logit against its row's maximum.  An infinite maximum shares the mass among the infinities.
 __device__ __forceinline__ double weight(float z, float top, double c) {
-    if (z == top) return 1.0;
-    return exp2_neg((static_cast<double>(z) - static_cast<double>(top)) * c);
+    if (top == INFINITY) return z == top ? 1.0 : 0.0;
+    return z > -INFINITY ? exp2_neg((static_cast<double>(z) - static_cast<double>(top)) * c) : 0.0;
 }
 
-// kPer logits of a row from i0 on; -infinity past the row's end and in the place of a NaN.
-template <typename T>
-__device__ __forceinline__ void load_logits(const T* row, int i0, int V, bool vec, float (&z)[kPer]) {
-    constexpr int W = 16 / sizeof(T);
+// This lane's PER logits of a run that starts at i0: groups of kWave vectors of up to 16 bytes.
+// -infinity past the row's end.
+template <typename T, int PER> constexpr int vec_width = PER < 16 / static_cast<int>(sizeof(T)) ? PER : 16 / static_cast<int>(sizeof(T));
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const T* row, int i0, int V, bool vec, float (&z)[PER]) {
+    constexpr int W = vec_width<T, PER>;
     typedef T vec_t __attribute__((ext_vector_type(W)));
+    const int i = i0 + static_cast<int>(threadIdx.x & 63) * W;
+    if (vec && i0 + PER * kWave <= V) {  // wave-uniform: the loads go out together
+        vec_t x[PER / W];
 #pragma unroll
-    for (int j0 = 0; j0 < kPer; j0 += W) {
-        // lane-contiguous vectors: element j of group j0 sits at i0 + j0 * kThreads + lane * W
-        const int i = i0 + j0 * kThreads + static_cast<int>(threadIdx.x) * W;
-        if (vec && i + W <= V) {
-            const vec_t x = *reinterpret_cast<const vec_t*>(row + i);
+        for (int g = 0; g < PER / W; ++g) x[g] = *reinterpret_cast<const vec_t*>(row + i + g * W * kWave);
 #pragma unroll
-            for (int j = 0; j < W; ++j) z[j0 + j] = static_cast<float>(x[j]);
-        } else {
+        for (int j = 0; j < PER; ++j) z[j] = static_cast<float>(x[j / W][j % W]);
+    } else {
 #pragma unroll
-            for (int j = 0; j < W; ++j) z[j0 + j] = i + j < V ? static_cast<float>(row[i + j]) : -INFINITY;
+        for (int j = 0; j < PER; ++j) {
+            const int at = i + j / W * W * kWave + j % W;
+            const float x = static_cast<float>(row[min(at, V - 1)]);
+            z[j] = at < V ? x : -INFINITY;
         }
     }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) z[j] = z[j] == z[j] ? z[j] : -INFINITY;
 }
-template <typename T>
+template <typename T, int PER>
 __device__ __forceinline__ int logit_index(int i0, int j) {
-    constexpr int W = 16 / sizeof(T);
-    return i0 + (j / W) * W * kThreads + static_cast<int>(threadIdx.x) * W + j % W;
+    constexpr int W = vec_width<T, PER>;
+    return i0 + (j / W) * W * kWave + static_cast<int>(threadIdx.x & 63) * W + j % W;
 }
-
-__device__ __forceinline__ double block_sum_d(double v, double* red) {
-    v = wave_sum_d(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
-}
+struct Max {
+    template <typename X> __device__ __forceinline__ X operator()(X a, X b) const { return a > b ? a : b; }
+};
+struct Min {
+    template <typename X> __device__ __forceinline__ X operator()(X a, X b) const { return a < b ? a : b; }
+};
+struct Sum {
+    template <typename X> __device__ __forceinline__ X operator()(X a, X b) const { return a + b; }
+};
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void draft_stats_k(DraftArgs a) {
-    __shared__ double red[4];
-    __shared__ float redf[16];
-    __shared__ int redi[4];
-    const int part = static_cast<int>(blockIdx.x) % a.parts;
-    int64_t row = static_cast<int64_t>(blockIdx.x) / a.parts;
+__global__ __launch_bounds__(kStatWaves * kWave) void draft_stats_k(DraftArgs a) {
+    const int lane = threadIdx.x & 63, blocks = (a.parts + kStatWaves - 1) / kStatWaves;
+    const int part = static_cast<int>(blockIdx.x) % blocks * kStatWaves + static_cast<int>(threadIdx.x >> 6);
+    int64_t row = static_cast<int64_t>(blockIdx.x) / blocks;
+    if (part >= a.parts) return;
     const bool draft = row >= a.T;
-    if (draft) row -= a.T;
+    if (draft) {
+        row -= a.T;
+        if (a.B <= 256) {  // a sequence's last row judges no draft (more sequences: the search costs more than the row)
+            bool end = false;
+            for (int b = lane; b < a.B; b += kWave) end |= a.offsets[b + 1] == row + 1;
+            if (__any(end)) return;
+        }
+    }
     const T* src = draft ? static_cast<const T*>(a.y) + row * a.ldy : static_cast<const T*>(a.z) + row * a.ldz;
     float z[kPer];
-    load_logits(src, part * kPart, a.V, draft ? a.vec_y : a.vec_z, z);
-    float mx = z[0];
+    load_logits<T, kPer>(src, part * kPart, a.V, draft ? a.vec_y : a.vec_z, z);
+    float mx = -INFINITY;  // a NaN does not count
 #pragma unroll
-    for (int j = 1; j < kPer; ++j) mx = fmaxf(mx, z[j]);
-    mx = block_max(mx, redf);
+    for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, z[j]);
+    mx = wave_all(mx, Max{});
     Stat st{0.0, mx, -1};
     if (mx > -INFINITY) {
-        if (!draft) {
+        if (a.c == 0.0) {
             int best = INT32_MAX;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (z[j] == mx) best = min(best, logit_index<T>(part * kPart, j));
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, kWave));
-            if ((threadIdx.x & 63) == 0) redi[threadIdx.x >> 6] = best;
-            __syncthreads();
-            st.best = min(min(redi[0], redi[1]), min(redi[2], redi[3]));
-        }
-        if (a.c > 0.0) {
+            for (int j = 0; j < kPer; ++j) best = z[j] == mx ? min(best, logit_index<T, kPer>(part * kPart, j)) : best;
+            st.best = wave_all(best, Min{});
+        } else {
             double sum = 0.0;
+            if (fabsf(mx) < a.plain_top) {  // 2^-1000 of the maximum is a step that fp32 resolves: clamped there, also NaN
+                const float low = mx - a.reach;
+                const double top = -static_cast<double>(mx) * a.c;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) sum += weight(z[j], mx, a.c);
-            st.sum = block_sum_d(sum, red);
+                for (int j = 0; j < kPer; ++j) sum += exp2_poly(fma(static_cast<double>(fmaxf(z[j], low)), a.c, top));
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < kPer; ++j) sum += weight(z[j], mx, a.c);
+            }
+            st.sum = wave_all(sum, Sum{});
         }
     }
-    if (threadIdx.x == 0) (draft ? a.sy : a.sz)[row * a.parts + part] = st;
+    if (lane == 0) (draft ? a.sy : a.sz)[row * a.parts + part] = st;
 }
 
-// A row's maximum and sum from its parts.
-struct Whole {
-    float max;
-    double sum;
-};
-__device__ __forceinline__ Whole whole(const Stat* s, int parts, double c) {
-    float m = -INFINITY;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, s[i].max);
-    double sum = 0.0;
-    for (int i = 0; i < parts; ++i)
-        if (s[i].max > -INFINITY) sum += s[i].sum * weight(s[i].max, m, c);
-    return {m, sum};
+// A row's whole from its parts, by a wave; x: this lane's part, loaded by the caller, if there is one.
+__device__ __forceinline__ Whole whole(const Stat* s, Stat x, int parts, double c) {
+    const int lane = threadIdx.x & 63;
+    float m = x.max;
+    for (int i = lane + kWave; i < parts; i += kWave) m = fmaxf(m, s[i].max);
+    Whole w{0.0, wave_all(m, Max{}), INT32_MAX};
+    if (c == 0.0) {
+        int best = x.max == w.max ? x.best : INT32_MAX;
+        for (int i = lane + kWave; i < parts; i += kWave)
+            if (s[i].max == w.max) best = min(best, s[i].best);
+        w.best = wave_all(best, Min{});
+    } else if (w.max > -INFINITY) {
+        double sum = x.max > -INFINITY ? x.sum * weight(x.max, w.max, c) : 0.0;
+        for (int i = lane + kWave; i < parts; i += kWave)
+            if (s[i].max > -INFINITY) sum += s[i].sum * weight(s[i].max, w.max, c);
+        w.sum = wave_all(sum, Sum{});
+    }
+    return w;
 }
-template <typename T>
-__device__ __forceinline__ double prob(const T* row, int64_t x, int V, const Whole& w, double c) {
-    if (x < 0 || x >= V || w.max == -INFINITY) return 0.0;
-    const float z = static_cast<float>(row[x]);
-    return z == z ? weight(z, w.max, c) / w.sum : 0.0;
+// p of a logit; exp2 of the library: down to the smallest number.
+__device__ __forceinline__ double prob(float z, const Whole& w, double c) {
+    if (!(z > -INFINITY)) return 0.0;
+    const double v = w.max == INFINITY ? (z == w.max ? 1.0 : 0.0) : exp2((static_cast<double>(z) - static_cast<double>(w.max)) * c);
+    return v / w.sum;
 }
 
-struct Decision {
-    int64_t row;    // the packed row whose distribution the new token comes from
-    int64_t off;    // the draft token taken out of it (one-hot drafts), -1: none
-    int n, kept;
-    bool short_;    // a draft was refused
-};
-// How many drafts of sequence b are kept.  Every thread of the block asks; drafts go by lanes of a wave.
+// How many drafts of sequence b are kept, and where its new token comes from.  The block's waves take its rows
+// in turn, kWaves at a time, up to the first draft that is refused.  What a row needs is loaded before its
+// statistics are joined: the chain of dependent loads is offsets, ids, logits.
 template <typename T>
-__device__ __forceinline__ Decision decide(const DraftArgs& a, int b, int* first_bad) {
+__device__ __forceinline__ Decision decide(const DraftArgs& a, int b) {
+    __shared__ Whole ps[kWaves], ds[kWaves];
+    __shared__ int bad[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t lo = min(max(a.offsets[b], int64_t{0}), a.T);
     const int64_t hi = min(max(a.offsets[b + 1], lo), a.T);
-    Decision d{lo, -1, static_cast<int>(min(hi - lo, a.max_q)), 0, false};
-    if (threadIdx.x == 0) *first_bad = INT32_MAX;
-    __syncthreads();
-    for (int i0 = 0; i0 + 1 < d.n; i0 += kThreads) {
-        const int i = i0 + static_cast<int>(threadIdx.x);
-        if (i + 1 < d.n) {
-            const int64_t t = lo + i, x = a.ids[t + 1];
-            bool keep;
-            if (a.c == 0.0) {
-                float m = -INFINITY;
-                int64_t best = -1;
-                for (int s = 0; s < a.parts; ++s)
-                    if (a.sz[t * a.parts + s].max > m) {
-                        m = a.sz[t * a.parts + s].max;
-                        best = a.sz[t * a.parts + s].best;
-                    }
-                keep = x == best && best >= 0;
-            } else {
-                const Whole p = whole(a.sz + t * a.parts, a.parts, a.c);
-                const double px = prob(static_cast<const T*>(a.z) + t * a.ldz, x, a.V, p, a.c);
-                double dx = 1.0;
-                if (a.y) dx = prob(static_cast<const T*>(a.y) + t * a.ldy, x, a.V, whole(a.sy + t * a.parts, a.parts, a.c), a.c);
-                keep = static_cast<double>(a.u[t]) * dx < px;
+    Decision d{lo, -1, static_cast<int>(min(hi - lo, a.max_q)), 0, 0, {}, {}};
+    for (int i0 = 0; i0 < d.n; i0 += kWaves) {
+        const int i = i0 + wave;
+        const int64_t t = lo + i;
+        if (i < d.n) {
+            const bool judges = i + 1 < d.n, two = judges && a.y;  // the last row gives one token more
+            const Stat none{0.0, -INFINITY, INT32_MAX};
+            const Stat *sz = a.sz + t * a.parts, *sy = a.sy + t * a.parts;
+            const Stat xz = lane < a.parts ? sz[lane] : none, xy = two && lane < a.parts ? sy[lane] : none;
+            int64_t x = -1;
+            float zx = -INFINITY, yx = -INFINITY, u = 0.0f;
+            if (judges) {
+                x = a.ids[t + 1];
+                if (a.c > 0.0) u = a.u[t];
+                if (a.c > 0.0 && x >= 0 && x < a.V) {
+                    zx = static_cast<float>(static_cast<const T*>(a.z)[t * a.ldz + x]);
+                    if (two) yx = static_cast<float>(static_cast<const T*>(a.y)[t * a.ldy + x]);
+                }
             }
-            if (!keep) atomicMin(first_bad, i);
+            const Whole p = whole(sz, xz, a.parts, a.c);
+            Whole q{0.0, -INFINITY, -1};
+            if (two) q = whole(sy, xy, a.parts, a.c);
+            if (lane == 0) {
+                int refuse = 1;
+                if (judges && a.c == 0.0) refuse = !(p.max > -INFINITY && x == p.best);
+                else if (judges) refuse = !(static_cast<double>(u) * (two ? prob(yx, q, a.c) : 1.0) < prob(zx, p, a.c));
+                ps[wave] = p;
+                ds[wave] = q;
+                bad[wave] = refuse;
+            }
+        } else if (lane == 0) {
+            bad[wave] = 0;
         }
+        __syncthreads();
+        int first = 0;
+        while (first < kWaves && !bad[first]) ++first;
+        if (first < kWaves) {
+            d.kept = i0 + first;
+            d.row = lo + d.kept;
+            d.p = ps[first];
+            d.d = ds[first];
+            if (d.kept + 1 < d.n) {
+                d.minus = a.y != nullptr;
+                if (!a.y) d.off = a.ids[d.row + 1];
+            }
+            break;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    d.kept = min(*first_bad, max(d.n - 1, 0));
-    d.short_ = d.kept < d.n - 1;
-    d.row = lo + d.kept;
-    if (d.short_ && !a.y) d.off = a.ids[d.row + 1];
     return d;
 }
 
-// The residual weights max(0, p - d) of this thread's logits of one part.
-template <typename T>
-__device__ __forceinline__ void residual(const DraftArgs& a, const Decision& d, int part, double (&r)[kPer]) {
-    const Stat* sz = a.sz + d.row * a.parts;
-    const Whole p = whole(sz, a.parts, a.c);
-    float z[kPer];
-    load_logits(static_cast<const T*>(a.z) + d.row * a.ldz, part * kPart, a.V, a.vec_z, z);
-    const bool some = p.max > -INFINITY;
-    const double ip = some ? 1.0 / p.sum : 0.0;
+// This lane's target and draft logits of a run that starts at i0.
+template <int PER>
+struct Pair {
+    float z[PER], y[PER];
+};
+template <typename T, int PER>
+__device__ __forceinline__ Pair<PER> load_pair(const DraftArgs& a, const Decision& d, int i0) {
+    Pair<PER> x;
+    load_logits<T, PER>(static_cast<const T*>(a.z) + d.row * a.ldz, i0, a.V, a.vec_z, x.z);
+    if (d.minus) load_logits<T, PER>(static_cast<const T*>(a.y) + d.row * a.ldy, i0, a.V, a.vec_y, x.y);
+    return x;
+}
+// Their residual weights max(0, p - d).
+template <typename T, int PER>
+__device__ __forceinline__ void residual(const DraftArgs& a, const Decision& d, int i0, const Pair<PER>& x, double (&r)[PER]) {
+    const double ip = d.p.max > -INFINITY ? 1.0 / d.p.sum : 0.0, iq = d.minus && d.d.max > -INFINITY ? 1.0 / d.d.sum : 0.0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) r[j] = some && z[j] > -INFINITY ? weight(z[j], p.max, a.c) * ip : 0.0;
-    if (!d.short_) return;
-    if (!a.y) {
+    for (int j = 0; j < PER; ++j) r[j] = weight(x.z[j], d.p.max, a.c) * ip;
+    if (iq > 0.0) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-            if (logit_index<T>(part * kPart, j) == d.off) r[j] = 0.0;
-        return;
+        for (int j = 0; j < PER; ++j) r[j] = fmax(0.0, r[j] - weight(x.y[j], d.d.max, a.c) * iq);
     }
-    const Whole q = whole(a.sy + d.row * a.parts, a.parts, a.c);
-    if (!(q.max > -INFINITY)) return;
-    load_logits(static_cast<const T*>(a.y) + d.row * a.ldy, part * kPart, a.V, a.vec_y, z);
-    const double iq = 1.0 / q.sum;
+    if (d.off >= 0) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        if (z[j] > -INFINITY) r[j] = fmax(0.0, r[j] - weight(z[j], q.max, a.c) * iq);
+        for (int j = 0; j < PER; ++j) r[j] = logit_index<T, PER>(i0, j) == d.off ? 0.0 : r[j];
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void draft_residual_k(DraftArgs a) {
-    __shared__ double red[4];
-    __shared__ int first_bad;
-    const int part = static_cast<int>(blockIdx.x) % a.parts, b = static_cast<int>(blockIdx.x) / a.parts;
-    const Decision d = decide<T>(a, b, &first_bad);
-    if (d.n == 0) return;
-    double r[kPer], sum = 0.0;
-    residual<T>(a, d, part, r);
+__global__ __launch_bounds__(kWaves * kWave) void draft_residual_k(DraftArgs a, int blocks) {
+    const int group = static_cast<int>(blockIdx.x) % blocks, b = static_cast<int>(blockIdx.x) / blocks;
+    const Decision d = decide<T>(a, b);
+    if (group == 0 && threadIdx.x == 0) a.decided[b] = d;
+    if (d.n == 0 || a.c == 0.0) return;
+    int run = group * kWaves + static_cast<int>(threadIdx.x >> 6);
+    if (run >= a.runs) return;
+    Pair<kFew> x = load_pair<T, kFew>(a, d, run * kRun);
+    while (true) {
+        const int next = run + blocks * kWaves;
+        Pair<kFew> y = x;
+        if (next < a.runs) y = load_pair<T, kFew>(a, d, next * kRun);
+        double r[kFew], sum = 0.0;
+        residual<T, kFew>(a, d, run * kRun, x, r);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += r[j];
-    sum = block_sum_d(sum, red);
-    if (threadIdx.x == 0) a.left[static_cast<int64_t>(b) * a.parts + part] = sum;
+        for (int j = 0; j < kFew; ++j) sum += r[j];
+        sum = wave_all(sum, Sum{});
+        if ((threadIdx.x & 63) == 0) a.left[static_cast<int64_t>(b) * a.runs + run] = sum;
+        if (next >= a.runs) return;
+        x = y;
+        run = next;
+    }
 }
 
+// One wave per sequence: the run, then the token, whose running sum first passes the target.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void draft_pick_k(DraftArgs a) {
-    constexpr int W = 16 / sizeof(T);
-    __shared__ int first_bad, pick, last;
-    __shared__ double wsum[4];
-    const int b = static_cast<int>(blockIdx.x);
-    const Decision d = decide<T>(a, b, &first_bad);
+__global__ __launch_bounds__(kWave) void draft_pick_k(DraftArgs a) {
+    constexpr int W = vec_width<T, kFew>;
+    static_assert(W == kFew, "a lane's logits of a run are neighbours");
+    const int b = static_cast<int>(blockIdx.x), lane = threadIdx.x;
+    const double* left = a.left + static_cast<int64_t>(b) * a.runs;
+    const Decision d = a.decided[b];
     int64_t token = -1;
-    if (d.n > 0) {
+    if (d.n > 0 && d.p.max > -INFINITY) {
         if (a.c == 0.0) {
-            float m = -INFINITY;
-            for (int s = 0; s < a.parts; ++s)
-                if (a.sz[d.row * a.parts + s].max > m) {
-                    m = a.sz[d.row * a.parts + s].max;
-                    token = a.sz[d.row * a.parts + s].best;
-                }
+            token = d.p.best;
         } else {
-            // the part that the target sum falls into; parts of weight zero hold no token
-            const double* left = a.left + static_cast<int64_t>(b) * a.parts;
             double total = 0.0;
-            for (int s = 0; s < a.parts; ++s) total += left[s];
-            const double target = total * static_cast<double>(a.u_next[b]);
-            int part = -1;
-            double below = 0.0, run = 0.0;
-            for (int s = 0; s < a.parts; ++s) {
-                if (left[s] > 0.0) {
-                    part = s;
-                    below = run;
-                    if (run + left[s] > target) break;
+            for (int i = lane; i < a.runs; i += kWave) total += left[i];
+            const double target = wave_all(total, Sum{}) * static_cast<double>(a.u_next[b]);
+            int run = -1;  // runs of weight zero hold no token
+            double below = 0.0, sofar = 0.0;
+            for (int i0 = 0; i0 < a.runs; i0 += kWave) {
+                const double w = i0 + lane < a.runs ? left[i0 + lane] : 0.0;
+                const double upto = sofar + wave_running_sum(w);
+                const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && upto > target);
+                if (some) {
+                    const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+                    run = i0 + l;
+                    below = __shfl(upto - w, l, kWave);
                 }
-                run += left[s];
+                if (past) break;
+                sofar = __shfl(upto, kWave - 1, kWave);
             }
-            if (part >= 0) {
-                if (threadIdx.x == 0) pick = INT32_MAX, last = -1;
-                double r[kPer];
-                residual<T>(a, d, part, r);
-                const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-                // index order: groups of W * kThreads logits, W of each thread
+            if (run >= 0) {
+                double r[kFew], mine = 0.0;
+                residual<T, kFew>(a, d, run * kRun, load_pair<T, kFew>(a, d, run * kRun), r);
 #pragma unroll
-                for (int g = 0; g < kPer / W; ++g) {
-                    double mine = 0.0;
+                for (int j = 0; j < kFew; ++j) mine += r[j];
+                double at = below + (wave_running_sum(mine) - mine);
+                int pick = INT32_MAX, last = -1;
 #pragma unroll
-                    for (int j = 0; j < W; ++j) mine += r[g * W + j];
-                    double upto = mine;
-#pragma unroll
-                    for (int o = 1; o < 64; o <<= 1) {
-                        const double x = __shfl_up(upto, o, 64);
-                        if (lane >= o) upto += x;
-                    }
-                    __syncthreads();
-                    if (lane == 63) wsum[wave] = upto;
-                    __syncthreads();
-                    double run2 = below;
-                    for (int w = 0; w < wave; ++w) run2 += wsum[w];
-                    run2 += upto - mine;
-#pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        run2 += r[g * W + j];
-                        const int i = logit_index<T>(part * kPart, g * W + j);
-                        if (r[g * W + j] > 0.0) {
-                            atomicMax(&last, i);
-                            if (run2 > target) atomicMin(&pick, i);
-                        }
-                    }
-                    below += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+                for (int j = 0; j < kFew; ++j) {
+                    at += r[j];
+                    const int i = logit_index<T, kFew>(run * kRun, j);
+                    const bool some = r[j] > 0.0;
+                    last = some ? max(last, i) : last;
+                    pick = some && at > target ? min(pick, i) : pick;
                 }
-                __syncthreads();
+                pick = wave_all(pick, Min{});
+                last = wave_all(last, Max{});
                 token = pick != INT32_MAX ? pick : last;  // the sums' last bits: none passed the target
             }
         }
     }
-    for (int64_t i = threadIdx.x; i < a.max_q; i += kThreads)
+    for (int64_t i = lane; i < a.max_q; i += kWave)
         a.tokens[b * a.max_q + i] = d.n == 0 || i > d.kept ? -1 : i == d.kept ? token : a.ids[d.row - d.kept + i + 1];
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         a.counts[b] = d.n == 0 ? 0 : d.kept + 1;
         if (a.new_lens) {
             const int64_t all = min(max(a.offsets[b + 1], int64_t{0}), a.T) - min(max(a.offsets[b], int64_t{0}), a.T);
@@ -341,7 +386,7 @@ __global__ __launch_bounds__(kThreads) void draft_pick_k(DraftArgs a) {
 
 int64_t bytes_for(int64_t B, int64_t T, int64_t V) {
     const int64_t parts = (V + kPart - 1) / kPart;
-    return 2 * T * parts * static_cast<int64_t>(sizeof(Stat)) + B * parts * 8;
+    return 2 * T * parts * static_cast<int64_t>(sizeof(Stat)) + B * ((V + kRun - 1) / kRun) * 8 + B * static_cast<int64_t>(sizeof(Decision));
 }
 
 void check_sizes(int64_t B, int64_t T, int64_t V) {
@@ -373,7 +418,7 @@ void verify_drafts(const void* logits, int64_t ld, const void* draft, int64_t ld
     const bool greedy = temperature <= 0.001f;  // as aic_lm_generate
     AIC_CHECK(T == 0 || (logits && ids && (greedy || (u && u_next))), InvalidArgument, "verify_drafts: null pointer");
 
-    const int64_t need = bytes_for(B, T, V), parts = (V + kPart - 1) / kPart;
+    const int64_t need = bytes_for(B, T, V), parts = (V + kPart - 1) / kPart, runs = (V + kRun - 1) / kRun;
     const StreamScratchUse use(s);
     if (workspace) {
         AIC_CHECK(workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
@@ -386,23 +431,28 @@ void verify_drafts(const void* logits, int64_t ld, const void* draft, int64_t ld
     a.z = logits, a.y = greedy ? nullptr : draft;
     a.ldz = ld, a.ldy = ld_draft;
     a.ids = ids, a.u = u, a.u_next = u_next, a.offsets = offsets, a.lens = lens;
-    a.B = static_cast<int>(B), a.V = static_cast<int>(V), a.parts = static_cast<int>(parts);
+    a.B = static_cast<int>(B), a.V = static_cast<int>(V), a.parts = static_cast<int>(parts), a.runs = static_cast<int>(runs);
     a.T = T, a.max_q = max_q;
     a.c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temperature);
+    a.reach = 1000.0f * temperature * 0.6931f;  // under 1000 / c: 2^-999.9
+    a.plain_top = std::min(a.reach * 0x1p20f, 1e30f);
     a.tokens = tokens, a.counts = counts, a.new_lens = new_lens;
     a.sz = static_cast<Stat*>(workspace);
     a.sy = a.sz + T * parts;
     a.left = reinterpret_cast<double*>(a.sy + T * parts);
+    a.decided = reinterpret_cast<Decision*>(a.left + B * runs);
     const int64_t size = static_cast<int64_t>(dtype_size(dt));
     a.vec_z = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld * size % 16 == 0;
     a.vec_y = reinterpret_cast<uintptr_t>(draft) % 16 == 0 && ld_draft * size % 16 == 0;
-    const int64_t rows = T * (a.y ? 2 : 1) * parts, seqs = B * parts;
+    const int64_t rows = T * (a.y ? 2 : 1) * ((parts + kStatWaves - 1) / kStatWaves);
+    // a block decides anew, so large batches give a sequence fewer blocks with several runs per wave
+    const int64_t share = greedy ? 1 : std::min((runs + kWaves - 1) / kWaves, std::max<int64_t>(4, 256 / B)), seqs = B * share;
     AIC_CHECK(rows <= INT32_MAX && seqs <= INT32_MAX, OutOfRange, "verify_drafts: too many rows in one call");
     auto run = [&](auto t) {
         using X = decltype(t);
-        if (rows > 0) draft_stats_k<X><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
-        if (!greedy) draft_residual_k<X><<<static_cast<unsigned>(seqs), kThreads, 0, s>>>(a);
-        draft_pick_k<X><<<static_cast<unsigned>(B), kThreads, 0, s>>>(a);
+        if (rows > 0) draft_stats_k<X><<<static_cast<unsigned>(rows), kStatWaves * kWave, 0, s>>>(a);
+        draft_residual_k<X><<<static_cast<unsigned>(seqs), kWaves * kWave, 0, s>>>(a, static_cast<int>(share));
+        draft_pick_k<X><<<static_cast<unsigned>(B), kWave, 0, s>>>(a);
     };
     if (dt == DType::Float32) run(float{});
     else run(bf16{});
