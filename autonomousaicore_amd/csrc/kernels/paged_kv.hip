@@ -1,10 +1,16 @@
 // Writing rows of new keys and values into a paged cache, and reading cached rows back.
 //
 // Both are one pass over packed rows: sequence b's rows offsets[b] .. offsets[b+1] stand at the last
-// positions of its lens[b] cached tokens.  A thread carries eight elements of one (row, head), so a
-// bf16 row is read in 16-byte pieces, its head's amax is one exchange among hd / 8 lanes, and codes
-// are written 8 bytes at a time.  Bound by memory.
+// positions of its lens[b] cached tokens.  A block takes a few rows, finds their places once, and its
+// threads then carry 16-byte units of the cache, up to four each with all loads in flight together: a
+// thread that went from the offsets to the page table to its row by itself waited for four loads one
+// after the other (DESIGN has the times of both).  A head's amax is an exchange among its hd / 16
+// lanes.  Bound by memory.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged_kv.hpp"
+#include "wave_dpp.hpp"
 
 namespace aic::hip {
 
@@ -44,77 +50,92 @@ PageView page_view(const KVPages& c, const char* what) {
 
 namespace {
 
-template <typename T> struct Oct;  // eight elements of a row
-template <> struct Oct<float> {
-    static __device__ __forceinline__ void load(const float* p, bool vec, float (&v)[8]) {
-        if (vec) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
+// N neighbouring elements of a row as floats; vec: 16-byte aligned.
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const T* p, bool vec, float (&v)[N]) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec_t __attribute__((ext_vector_type(W)));
+    if (vec && N % W == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = p[j];
+        for (int i = 0; i < N / W; ++i) {
+            const vec_t x = reinterpret_cast<const vec_t*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i * W + j] = static_cast<float>(x[j]);
         }
-    }
-    static __device__ __forceinline__ void store(float* p, bool vec, const float (&v)[8]) {
-        if (vec) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = v[j];
+        for (int j = 0; j < N; ++j) v[j] = static_cast<float>(p[j]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, bool vec, const float (&v)[N]) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec_t __attribute__((ext_vector_type(W)));
+    if (vec && N % W == 0) {
+#pragma unroll
+        for (int i = 0; i < N / W; ++i) {
+            vec_t x;
+#pragma unroll
+            for (int j = 0; j < W; ++j) x[j] = static_cast<T>(v[i * W + j]);  // bf16: to nearest even
+            reinterpret_cast<vec_t*>(p)[i] = x;
         }
-    }
-};
-template <> struct Oct<bf16> {
-    static __device__ __forceinline__ void load(const bf16* p, bool vec, float (&v)[8]) {
-        if (vec) {
-            const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = bf2f(a[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = bf2f(p[j]);
-        }
+        for (int j = 0; j < N; ++j) p[j] = static_cast<T>(v[j]);
     }
-    static __device__ __forceinline__ void store(bf16* p, bool vec, const float (&v)[8]) {
-        if (vec) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                      pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = f2bf(v[j]);
-        }
-    }
+}
+
+constexpr int kMaxRows = 256;   // rows per block
+
+// A batch's rows cut into blocks of `rows` rows x ncol units (2 Hkv heads of hd * size / 16 units); wide
+// rows are shared by the blocks of the grid's second dimension.
+struct Cut {
+    const int64_t *offsets, *lens;
+    int64_t T;
+    int B, rows, ncol;
+    uint32_t mul;  // unit / ncol = unit * mul >> 32, exact for several rows' 1024 units; 0: one row
 };
 
-// One thread's eight elements: packed row t, k or v, head h, elements 8c ..
-struct Piece {
-    int64_t t = 0, row = -1;
-    int kv = 0, h = 0, c = 0;
-    bool live = false;  // row t belongs to a sequence
-};
+// The places of the block's rows: page * Hkv * ps + slot, -1: none, -2: a row of no sequence.
+__device__ __forceinline__ void block_places(const PageView& pv, const Cut& c, int64_t t0, int64_t (&at)[kMaxRows]) {
+    const int b0 = block_sequence(c.offsets, c.B, t0);
+    const int r = static_cast<int>(threadIdx.x);
+    if (r < c.rows) {
+        int64_t place = -2;
+        int b = b0;
+        const int64_t t = t0 + r;
+        int64_t end = b < c.B ? c.offsets[b + 1] : 0;
+        while (b < c.B && t >= end) {
+            ++b;
+            if (b < c.B) end = c.offsets[b + 1];
+        }
+        if (t < c.T && b >= 0 && b < c.B) {
+            const int64_t pos = c.lens[b] - (end - t);
+            place = -1;
+            if (pos >= 0 && pos <= INT32_MAX) {
+                const int64_t row = pv.row(pv.table + b * pv.ld_table, static_cast<int>(pos), 0);
+                if (row >= 0) place = row;
+            }
+        }
+        at[r] = place;
+    }
+    __syncthreads();
+}
 
-template <int HD>
-__device__ __forceinline__ Piece piece(const PageView& pv, const int64_t* offsets, const int64_t* lens, int B, int64_t T) {
-    constexpr int LPR = HD / 8;
-    const int64_t per_row = 2LL * pv.Hkv * LPR, first = static_cast<int64_t>(blockIdx.x) * kBlock;
-    const int b0 = block_sequence(offsets, B, first / per_row);
-    const int64_t i = first + threadIdx.x;
-    Piece p;
-    p.t = i / per_row;
-    const int r = static_cast<int>(i - p.t * per_row);
-    p.c = r % LPR;
-    p.h = (r / LPR) % pv.Hkv;
-    p.kv = r / LPR / pv.Hkv;
-    if (p.t >= T) return p;
-    int b = b0;
-    while (b < B && p.t >= offsets[b + 1]) ++b;
-    if (b < 0 || b >= B) return p;
-    p.live = true;
-    const int64_t pos = lens[b] - (offsets[b + 1] - p.t);
-    if (pos < 0 || pos > INT32_MAX) return p;
-    p.row = pv.row(pv.table + b * pv.ld_table, static_cast<int>(pos), p.h);
-    return p;
+// Unit u of the block: row r, k or v, head, first element.
+struct Unit {
+    int r, kv, h, d;
+};
+template <int HD, int EPU>
+__device__ __forceinline__ Unit unit(const PageView& pv, const Cut& c, int u) {
+    constexpr int LPR = HD / EPU;
+    Unit x;
+    x.r = static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(u)) * c.mul) >> 32);
+    const int col = u - x.r * c.ncol, hh = col / LPR;
+    x.kv = hh >= pv.Hkv;
+    x.h = x.kv ? hh - pv.Hkv : hh;
+    x.d = col % LPR * EPU;
+    return x;
 }
 
 // amax of a row's head -> the exponent e with the least 2^e >= amax / 448 (0 for a zero row, at
@@ -126,54 +147,102 @@ __device__ __forceinline__ int row_exponent(float amax) {
     return max(e, -126);
 }
 
-template <typename T, typename CT, int HD>
-__global__ __launch_bounds__(kBlock) void kv_write_k(PageView pv, const T* __restrict__ k, const T* __restrict__ v, int64_t ld,
-                                                     const int64_t* __restrict__ offsets, const int64_t* __restrict__ lens,
-                                                     int B, int64_t rows, bool vec) {
-    const Piece p = piece<HD>(pv, offsets, lens, B, rows);
-    float x[8] = {};
-    if (p.row >= 0) Oct<T>::load((p.kv ? v : k) + p.t * ld + p.h * HD + p.c * 8, vec, x);
-    if constexpr (sizeof(CT) == 1) {
-        float amax = 0.0f;
+template <typename T, typename CT, int HD, int U>
+__global__ __launch_bounds__(kBlock) void kv_write_k(PageView pv, Cut c, const T* __restrict__ k, const T* __restrict__ v,
+                                                     int64_t ld, bool vec) {
+    constexpr int EPU = 16 / sizeof(CT);
+    __shared__ int64_t at[kMaxRows];
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.rows;
+    const int u0 = static_cast<int>(blockIdx.y) * (kBlock * U) + static_cast<int>(threadIdx.x);
+    float x[U][EPU];
+    // the rows' data does not wait for their places
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (!(fabsf(x[j]) < INFINITY)) x[j] = NAN;  // e4m3 has no infinity: held as NaN
-            else amax = fmaxf(amax, fabsf(x[j]));
+    for (int i = 0; i < U; ++i) {
+        const int u = u0 + i * kBlock;
+        const Unit w = unit<HD, EPU>(pv, c, min(u, c.rows * c.ncol - 1));
+        const int64_t t = min(t0 + w.r, c.T - 1);
+        load_row<T, EPU>((w.kv ? v : k) + t * ld + w.h * HD + w.d, vec, x[i]);
+    }
+    block_places(pv, c, t0, at);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int u = u0 + i * kBlock;
+        const bool mine = u < c.rows * c.ncol;
+        const Unit w = unit<HD, EPU>(pv, c, mine ? u : c.rows * c.ncol - 1);
+        const int64_t place = at[w.r], row = place + static_cast<int64_t>(w.h) * pv.ps;
+        const bool go = mine && place >= 0;
+        char* pool = w.kv ? pv.vp : pv.kp;
+        if constexpr (sizeof(CT) == 1) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < EPU; ++j) {
+                const bool fine = fabsf(x[i][j]) < INFINITY;  // e4m3 has no infinity: held as NaN
+                amax = fine ? fmaxf(amax, fabsf(x[i][j])) : amax;
+                x[i][j] = fine ? x[i][j] : NAN;
+            }
+            amax = fmaxf(amax, dpp<0xb1>(amax));  // the head's lanes: 2, 4 or 8 neighbours
+            if constexpr (HD >= 64) amax = fmaxf(amax, dpp<0x4e>(amax));
+            if constexpr (HD >= 128) amax = fmaxf(amax, dpp<0x141>(amax));
+            const int e = row_exponent(amax);
+            const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            int q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // one rounding, to nearest even; |x| inv <= 448
+                q[j] = __builtin_amdgcn_cvt_pk_fp8_f32(x[i][4 * j] * inv, x[i][4 * j + 1] * inv, 0, false);
+                q[j] = __builtin_amdgcn_cvt_pk_fp8_f32(x[i][4 * j + 2] * inv, x[i][4 * j + 3] * inv, q[j], true);
+            }
+            if (go) {
+                *reinterpret_cast<int4*>(pool + row * HD + w.d) = make_int4(q[0], q[1], q[2], q[3]);
+                if (w.d == 0) (w.kv ? pv.ve : pv.ke)[row] = static_cast<uint8_t>(e + 127);
+            }
+        } else {
+            if (go) store_row<CT, EPU>(reinterpret_cast<CT*>(pool) + row * HD + w.d, true, x[i]);
         }
-#pragma unroll
-        for (int o = HD / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, kWave));  // lanes of the row's head
-        const int e = row_exponent(amax);
-        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        int w[2] = {0, 0};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {  // one rounding, to nearest even; |x| inv <= 448
-            w[u] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * u] * inv, x[4 * u + 1] * inv, w[u], false);
-            w[u] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * u + 2] * inv, x[4 * u + 3] * inv, w[u], true);
-        }
-        if (p.row < 0) return;
-        *reinterpret_cast<int2*>((p.kv ? pv.vp : pv.kp) + p.row * HD + p.c * 8) = make_int2(w[0], w[1]);
-        if (p.c == 0) (p.kv ? pv.ve : pv.ke)[p.row] = static_cast<uint8_t>(e + 127);
-    } else {
-        if (p.row < 0) return;
-        Oct<CT>::store(reinterpret_cast<CT*>(p.kv ? pv.vp : pv.kp) + p.row * HD + p.c * 8, true, x);
     }
 }
 
-template <typename T, typename CT, int HD>
-__global__ __launch_bounds__(kBlock) void kv_read_k(PageView pv, T* __restrict__ k, T* __restrict__ v, int64_t ld,
-                                                    const int64_t* __restrict__ offsets, const int64_t* __restrict__ lens, int B,
-                                                    int64_t rows, bool vec) {
-    const Piece p = piece<HD>(pv, offsets, lens, B, rows);
-    if (!p.live) return;
-    float x[8] = {};
-    if (p.row >= 0) {
-        const char* pool = p.kv ? pv.vp : pv.kp;
-        if constexpr (sizeof(CT) == 1)
-            e4m3_floats(*reinterpret_cast<const uint2*>(pool + p.row * HD + p.c * 8),
-                        exp_scale((p.kv ? pv.ve : pv.ke)[p.row]), x);
-        else Oct<CT>::load(reinterpret_cast<const CT*>(pool) + p.row * HD + p.c * 8, true, x);
+template <typename T, typename CT, int HD, int U>
+__global__ __launch_bounds__(kBlock) void kv_read_k(PageView pv, Cut c, T* __restrict__ k, T* __restrict__ v, int64_t ld, bool vec) {
+    constexpr int EPU = 16 / sizeof(CT);
+    __shared__ int64_t at[kMaxRows];
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.rows;
+    const int u0 = static_cast<int>(blockIdx.y) * (kBlock * U) + static_cast<int>(threadIdx.x);
+    block_places(pv, c, t0, at);
+    uint4 raw[U];
+    uint32_t ex[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const Unit w = unit<HD, EPU>(pv, c, min(u0 + i * kBlock, c.rows * c.ncol - 1));
+        const int64_t place = at[w.r], row = place + static_cast<int64_t>(w.h) * pv.ps;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        ex[i] = 127;
+        if (place >= 0) {
+            raw[i] = *reinterpret_cast<const uint4*>((w.kv ? pv.vp : pv.kp) + row * static_cast<int64_t>(HD * sizeof(CT)) + w.d * sizeof(CT));
+            if constexpr (sizeof(CT) == 1) ex[i] = (w.kv ? pv.ve : pv.ke)[row];
+        }
     }
-    Oct<T>::store((p.kv ? v : k) + p.t * ld + p.h * HD + p.c * 8, vec, x);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int u = u0 + i * kBlock;
+        if (u >= c.rows * c.ncol) return;
+        const Unit w = unit<HD, EPU>(pv, c, u);
+        if (at[w.r] == -2) continue;
+        float x[EPU];
+        if constexpr (sizeof(CT) == 1) {
+            const float s = exp_scale(ex[i]);
+            float a[8], b[8];
+            e4m3_floats(make_uint2(raw[i].x, raw[i].y), s, a);
+            e4m3_floats(make_uint2(raw[i].z, raw[i].w), s, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = a[j], x[8 + j] = b[j];
+        } else {
+            typedef CT vec_t __attribute__((ext_vector_type(EPU)));
+            const vec_t y = __builtin_bit_cast(vec_t, raw[i]);
+#pragma unroll
+            for (int j = 0; j < EPU; ++j) x[j] = static_cast<float>(y[j]);
+        }
+        store_row<T, EPU>((w.kv ? v : k) + (t0 + w.r) * ld + w.h * HD + w.d, vec, x);
+    }
 }
 
 template <typename F>
@@ -197,16 +266,26 @@ bool aligned16(const void* k, const void* v, int64_t ld, int64_t size) {
     return (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 && ld * size % 16 == 0;
 }
 
+// Four units per thread, or one where that leaves the card mostly empty (a decode step's few rows).
 template <typename F>
-void launch_rows(const KVPages& c, int64_t B, int64_t T, DType dt, F&& f) {
-    const int64_t blocks = (T * 2 * c.kv_heads * (c.head_dim / 8) + kBlock - 1) / kBlock;
-    AIC_CHECK(blocks <= INT32_MAX, OutOfRange, "too many rows in one call");
+void launch_rows(const KVPages& c, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, DType dt, F&& f) {
+    const int64_t ncol = 2 * c.kv_heads * (c.head_dim * static_cast<int64_t>(dtype_size(c.type)) / 16);
+    const bool few = T * ncol < kBlock * 4 * 256;
+    const int64_t per = kBlock * (few ? 1 : 4);
+    Cut cut{offsets, lens, T, static_cast<int>(B), static_cast<int>(std::clamp<int64_t>(per / ncol, 1, kMaxRows)), static_cast<int>(ncol), 0};
+    if (cut.rows > 1) cut.mul = static_cast<uint32_t>(((uint64_t{1} << 32) + ncol - 1) / ncol);
+    const int64_t blocks = (T + cut.rows - 1) / cut.rows, shares = (cut.rows * ncol + per - 1) / per;
+    AIC_CHECK(blocks <= INT32_MAX && shares <= 65535, OutOfRange, "too many rows or heads in one call");
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(shares));
+    auto types = [&](auto hd, auto u) {
+        if (dt == DType::Float32 && c.type == DType::Float32) f(float{}, float{}, hd, u, grid, cut);
+        else if (dt == DType::Float32) f(float{}, uint8_t{}, hd, u, grid, cut);
+        else if (c.type == DType::BFloat16) f(bf16{}, bf16{}, hd, u, grid, cut);
+        else f(bf16{}, uint8_t{}, hd, u, grid, cut);
+    };
     by_head_dim(c.head_dim, [&](auto hd) {
-        const auto g = static_cast<unsigned>(blocks);
-        if (dt == DType::Float32 && c.type == DType::Float32) f(float{}, float{}, hd, g);
-        else if (dt == DType::Float32) f(float{}, uint8_t{}, hd, g);
-        else if (c.type == DType::BFloat16) f(bf16{}, bf16{}, hd, g);
-        else f(bf16{}, uint8_t{}, hd, g);
+        if (few) types(hd, std::integral_constant<int, 1>{});
+        else types(hd, std::integral_constant<int, 4>{});
     });
 }
 
@@ -218,10 +297,10 @@ void kv_write(const KVPages& c, const void* k, const void* v, int64_t ld, const 
     const PageView pv = page_view(c, "kv_write");
     if (B == 0 || T == 0) return;
     const bool vec = aligned16(k, v, ld, static_cast<int64_t>(dtype_size(dt)));
-    launch_rows(c, B, T, dt, [&](auto t, auto ct, auto hd, unsigned grid) {
+    launch_rows(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
         using X = decltype(t);
-        kv_write_k<X, decltype(ct), decltype(hd)::value><<<grid, kBlock, 0, s>>>(
-            pv, static_cast<const X*>(k), static_cast<const X*>(v), ld, offsets, lens, static_cast<int>(B), T, vec);
+        kv_write_k<X, decltype(ct), decltype(hd)::value, decltype(u)::value><<<grid, kBlock, 0, s>>>(
+            pv, cut, static_cast<const X*>(k), static_cast<const X*>(v), ld, vec);
     });
     AIC_LAUNCH_CHECK("kv_write");
 }
@@ -232,10 +311,10 @@ void kv_read(const KVPages& c, void* k, void* v, int64_t ld, const int64_t* offs
     const PageView pv = page_view(c, "kv_read");
     if (B == 0 || T == 0) return;
     const bool vec = aligned16(k, v, ld, static_cast<int64_t>(dtype_size(dt)));
-    launch_rows(c, B, T, dt, [&](auto t, auto ct, auto hd, unsigned grid) {
+    launch_rows(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
         using X = decltype(t);
-        kv_read_k<X, decltype(ct), decltype(hd)::value><<<grid, kBlock, 0, s>>>(
-            pv, static_cast<X*>(k), static_cast<X*>(v), ld, offsets, lens, static_cast<int>(B), T, vec);
+        kv_read_k<X, decltype(ct), decltype(hd)::value, decltype(u)::value><<<grid, kBlock, 0, s>>>(
+            pv, cut, static_cast<X*>(k), static_cast<X*>(v), ld, vec);
     });
     AIC_LAUNCH_CHECK("kv_read");
 }
