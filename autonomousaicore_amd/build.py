@@ -45,7 +45,8 @@ def _obj(src: str) -> str:
 # MFMA of the inner loop (the AGPR form's register assignment does that for these kernels).
 FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_general.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-              "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+              "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "attention_paged_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src: str) -> tuple[str, int, str]:

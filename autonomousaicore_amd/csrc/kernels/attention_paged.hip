@@ -16,220 +16,12 @@
 #include <cmath>
 #include <type_traits>
 
-#include "attention_tiles.hpp"
-#include "paged_kv.hpp"
+#include "attention_paged.hpp"
 #include "../runtime/memory_pool.hpp"
 
 namespace aic::hip {
 
 namespace {
-
-struct PagedArgs {
-    PageView kv;
-    const void* q;
-    void* o;
-    float* lse;
-    int64_t ldq, ldo, T;
-    const int64_t *offsets, *lens;
-    int B, H, G, window;
-    float c;         // scale in log2 units
-    int chunk;       // keys of one split (0: one split over all of them)
-    int nsplit;
-    float2* part_ml;  // [nsplit][T][H]: maximum, sum (-1: only scores of -infinity)
-    float* part_o;    // [nsplit][T][H][hd]
-    bool vec_q, vec_o;
-};
-
-// All ones: a NaN in fp32, bf16 and e4m3.  Keys whose page id is out of range are read from here, so
-// that exactly the queries that would see them become NaN.
-__device__ const uint4 kNoPage = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-
-constexpr int64_t kMaxLen = INT32_MAX - 4095;  // positions and a tile past them fit in 32 bits
-
-// Weights are held times 2^-40: at most 2^8 2^-40 each, so that the sums over 2^31 keys stay below
-// the largest v, and a finite v never overflows before the division by l.  Exact, and it costs weights
-// below 2^-86 of the maximum.  bf16 takes it in exp2's argument, whose last bits (2^-19 there) are far below
-// the weight's rounding; fp32 multiplies.
-constexpr float kDown = 40.0f;
-template <typename T>
-__device__ __forceinline__ float weight(float s, float c, float off) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(fmaf(s, c, off - kDown));
-    else return __builtin_amdgcn_exp2f(fmaf(s, c, off)) * 0x1p-40f;
-}
-__device__ __forceinline__ float log_sum(float m, float l, float c) { return (m * c + log2f(l * 0x1p40f)) * kLn2; }
-
-struct Seq {
-    int64_t row0;  // first packed row
-    int n, len;    // queries, cached keys
-};
-__device__ __forceinline__ Seq sequence(const PagedArgs& a, int b) {
-    const int64_t lo = min(max(a.offsets[b], int64_t{0}), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
-    return {lo, static_cast<int>(hi - lo), static_cast<int>(min(max(a.lens[b], int64_t{0}), kMaxLen))};
-}
-
-// Tile `tile` of the batch cut into tiles of R query rows: its sequence and the tile's place in it.
-// Every wave finds it by itself: 64 sequences per step, their tile counts added up across lanes.
-template <int R>
-__device__ __forceinline__ bool find_tile(const PagedArgs& a, int tile, int& b, int& local) {
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        int tiles = 0;
-        if (b0 + lane < a.B) tiles = static_cast<int>((static_cast<int64_t>(sequence(a, b0 + lane).n) * a.G + R - 1) / R);
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
-        const uint64_t past = __ballot(tile < upto);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            b = __builtin_amdgcn_readfirstlane(b0 + l);
-            local = __builtin_amdgcn_readfirstlane(tile - (__shfl(upto, l, 64) - __shfl(tiles, l, 64)));
-            return true;
-        }
-        tile -= __shfl(upto, 63, 64);
-    }
-    return false;
-}
-
-// ------------------------------------------------------------------------------- tiles
-// [KT][HD] tiles of T in LDS, 16-byte chunks swizzled per row.
-template <typename T, int HD>
-__device__ __forceinline__ int chunk_at(int row, int ch) {
-    if constexpr (sizeof(T) == 2) return row * HD * 2 + ((ch ^ swz<HD>(row)) << 4);
-    // a ds_read_b128 phase reads one chunk of 16 consecutive rows: 16 different bank groups
-    else return row * HD * 4 + ((ch ^ (HD == 32 ? (row >> 1) & 7 : row & 15)) << 4);
-}
-
-template <typename CT> __device__ __forceinline__ bool any_non_finite(uint4 x);
-template <> __device__ __forceinline__ bool any_non_finite<bf16>(uint4 x) {
-    bool bad = false;
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u || (w[i] & 0x7f80u) == 0x7f80u;
-    return bad;
-}
-template <> __device__ __forceinline__ bool any_non_finite<float>(uint4 x) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
-    return bad;
-}
-
-// The four V values at columns d0 .. d0+3 of a tile's row.
-template <typename T, int HD>
-__device__ __forceinline__ float4 v4_at(const char* tile, int row, int d0) {
-    if constexpr (sizeof(T) == 2) {
-        const bf16x4 x = *reinterpret_cast<const bf16x4*>(tile + chunk_at<T, HD>(row, d0 >> 3) + (d0 & 7) * 2);
-        return make_float4(bf2f(x[0]), bf2f(x[1]), bf2f(x[2]), bf2f(x[3]));
-    } else {
-        return *reinterpret_cast<const float4*>(tile + chunk_at<T, HD>(row, d0 >> 2));
-    }
-}
-
-// The running state of 32 query rows: lane owns row lane % 32.
-template <int OB>
-struct Rows {
-    f32x16 o[OB];
-    float m = -INFINITY, l = 0.0f;
-    __device__ __forceinline__ void init() {
-#pragma unroll
-        for (int i = 0; i < OB; ++i) zero(o[i]);
-    }
-    // A tile's row maximum joins the reference maximum, which moves only by more than 2^8.
-    __device__ __forceinline__ void absorb(float mx, float c) {
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const bool grow = (mx - m) * c > kLazyRescale;
-        if (__any(grow)) {
-            const float m_new = grow ? mx : m;
-            const float alpha = m == -INFINITY ? 0.0f : grow ? __builtin_amdgcn_exp2f((m - m_new) * c) : 1.0f;
-            l *= alpha;
-#pragma unroll
-            for (int ob = 0; ob < OB; ++ob)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[ob][e] *= alpha;
-            m = m_new;
-        }
-    }
-    // -m in log2 units; a row that has seen only scores of -infinity counts from zero
-    __device__ __forceinline__ float offset(float c) const { return m == -INFINITY ? 0.0f : -m * c; }
-};
-
-// o += sum over the tile's keys of p v, key by key and only where the row sees the key: a hidden key has
-// weight zero in the matrix product, and zero times an infinity or NaN in its v is NaN.  For tiles
-// that hold both a hidden key and a non-finite v.  p[jb][e] is key 32 jb + 8 (e >> 2) + 4 h + (e & 3).
-template <typename T, int HD, int JB, typename Seen>
-__device__ __forceinline__ void add_seen_rows(f32x16 (&o)[HD / 32], const f32x16 (&p)[JB], const char* vt, Seen seen) {
-    const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int jb = 0; jb < JB; ++jb)
-#pragma unroll 1
-        for (int e = 0; e < 16; ++e) {
-            const float mine = p[jb][e], other = __shfl_xor(mine, 32, 64);
-#pragma unroll 1
-            for (int hh = 0; hh < 2; ++hh) {
-                const int key = 32 * jb + 8 * (e >> 2) + 4 * hh + (e & 3);
-                const float w = hh == h ? mine : other;
-                const bool s = seen(key);
-#pragma unroll
-                for (int ob = 0; ob < HD / 32; ++ob)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float4 x = v4_at<T, HD>(vt, key, 32 * ob + 8 * g + 4 * h);
-                        const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            o[ob][4 * g + u] = s ? fmaf(w, y[u], o[ob][4 * g + u]) : o[ob][4 * g + u];
-                    }
-            }
-        }
-}
-
-// Output of one query row: the lane's half of the head dimension.
-template <typename T, int HD>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const Rows<HD / 32>& r, int64_t t, int head, bool empty,
-                                          int split) {
-    constexpr int OB = HD / 32;
-    const int h = (threadIdx.x & 63) >> 5;
-    if (a.nsplit > 1) {
-        const int64_t i = (static_cast<int64_t>(split) * a.T + t) * a.H + head;
-        if (h == 0) a.part_ml[i] = make_float2(r.m, empty ? 0.0f : r.l == 0.0f ? -1.0f : r.l);
-        if (empty) return;
-        float* p = a.part_o + i * HD;
-#pragma unroll
-        for (int ob = 0; ob < OB; ++ob)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4*>(p + ob * 32 + 8 * g + 4 * h) =
-                    make_float4(r.o[ob][4 * g], r.o[ob][4 * g + 1], r.o[ob][4 * g + 2], r.o[ob][4 * g + 3]);
-        return;
-    }
-    const float inv = empty ? 0.0f : 1.0f / r.l;  // l == 0: only scores of -infinity, 0 / 0 = NaN below
-    T* op = static_cast<T*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD;
-#pragma unroll
-    for (int ob = 0; ob < OB; ++ob) {
-        if constexpr (sizeof(T) == 2) {
-            if (a.vec_o) {
-                store_t(op, r.o[ob], ob, inv);
-                continue;
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d0 = ob * 32 + 8 * g + 4 * h;
-            if (sizeof(T) == 4 && a.vec_o) {
-                *reinterpret_cast<float4*>(op + d0) = make_float4(r.o[ob][4 * g] * inv, r.o[ob][4 * g + 1] * inv,
-                                                                  r.o[ob][4 * g + 2] * inv, r.o[ob][4 * g + 3] * inv);
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) st(op, d0 + u, r.o[ob][4 * g + u] * inv);
-            }
-        }
-    }
-    if (a.lse && h == 0) a.lse[t * a.H + head] = empty ? -INFINITY : log_sum(r.m, r.l, a.c);
-}
 
 // ------------------------------------------------------------------- the general kernel
 // One block: 128 query rows (4 waves x 32) of one key/value head, over tiles of KT keys staged through
@@ -358,7 +150,7 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
         load(k_lo);
         for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
             // every row of the block sees every key of the tile?
-            const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi && r0 + 128 <= rows &&
+            const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi &&
                               (a.window <= 0 || k0 > last_pos - a.window);
             const int poison = __syncthreads_or(!open && bad_v());  // also: everyone is done with the last tile
 #pragma unroll
@@ -414,7 +206,7 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
                     sc[jb][e] = weight<T>(sc[jb][e], a.c, off);
                     sum += sc[jb][e];
                 }
-            st_.l += sum + __shfl_xor(sum, 32, 64);
+            st_.add(sum);
             if (poison) {
                 add_seen_rows<T, HD, JB>(st_.o, sc, vs, seen);
             } else if constexpr (sizeof(T) == 2) {
@@ -484,22 +276,22 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
 // --------------------------------------------------------------------------- the launch
 int64_t tile_bound(int64_t T, int64_t G, int64_t B, int64_t R) { return T * G / R + std::min(B, T); }
 
-constexpr int64_t kFill = 512;     // blocks that fill the card twice over
-constexpr int64_t kMinChunk = 256;  // keys of a split, at least
+constexpr int64_t kFewRows = 32;  // query rows per key/value head that the few-row kernel holds at a time
 
 struct Plan {
     int64_t tiles, nsplit, chunk;
+    bool few;
 };
-// Splits over the keys where the query tiles alone do not fill the card: equal chunks of a multiple of 64
-// keys that give about kFill blocks.
-Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t) {
-    Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0};
-    const int64_t blocks = p.tiles * Hkv;
-    const int64_t want = std::min(kFill / std::max<int64_t>(blocks, 1), max_len / kMinChunk);
+// Splits over the keys where the rows alone do not fill the card: equal chunks of a multiple of 128 keys.
+Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t max_q) {
+    Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0, max_q * (H / Hkv) <= kFewRows};
+    const int64_t blocks = std::max<int64_t>(1, (p.few ? B : p.tiles) * Hkv);
+    const int64_t fill = p.few ? 2048 : 512, least = p.few ? 512 : 256;  // blocks wanted, keys of a split at least
+    const int64_t want = std::min((fill + blocks - 1) / blocks, max_len / least);
     if (want > 1) {
-        p.chunk = ((max_len + want - 1) / want + 63) / 64 * 64;
+        p.chunk = ((max_len + want - 1) / want + 127) / 128 * 128;
         p.nsplit = (max_len + p.chunk - 1) / p.chunk;
-        if (p.nsplit <= 1) p = {p.tiles, 1, 0};
+        if (p.nsplit <= 1) p.nsplit = 1, p.chunk = 0;
     }
     return p;
 }
@@ -562,7 +354,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         } else if (stream_scratch_ready(s)) {
             workspace = stream_scratch(static_cast<size_t>(need), s);
         } else {
-            p = {p.tiles, 1, 0};  // captured without a workspace of its own
+            p.nsplit = 1, p.chunk = 0;  // captured without a workspace of its own
         }
     }
     a.nsplit = static_cast<int>(p.nsplit);
@@ -576,8 +368,12 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     auto run = [&](auto t, auto ct, auto hd) {
         using X = decltype(t);
         constexpr int D = decltype(hd)::value;
-        attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-        AIC_LAUNCH_CHECK("attn_paged");
+        if (p.few && sizeof(X) == 2) {
+            attn_paged_few(a, sizeof(ct) == 1, D, s);
+        } else {
+            attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+            AIC_LAUNCH_CHECK("attn_paged");
+        }
         if (a.nsplit > 1) {
             const int64_t joins = (T * H + 3) / 4;
             AIC_CHECK(joins <= INT32_MAX, OutOfRange, "attn_paged: too many rows in one call");
