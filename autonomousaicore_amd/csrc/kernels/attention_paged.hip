@@ -135,11 +135,7 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 if constexpr (E4) {
-                    const uint32_t w[4] = {rv[i].x, rv[i].y, rv[i].z, rv[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int by = 0; by < 4; ++by) bad |= ((w[j] >> (8 * by)) & 0x7fu) == 0x7fu;
+                    bad |= any_nan_code(rv[i]);
                 } else {
                     bad |= any_non_finite<CT>(rv[i]);
                 }
@@ -208,7 +204,7 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
                 }
             st_.add(sum);
             if (poison) {
-                add_seen_rows<T, HD, JB>(st_.o, sc, vs, seen);
+                add_seen_rows<HD, JB>(st_.o, sc, [&](int key, int d) { return v4_at<T, HD>(vs, key, d); }, seen);
             } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int s = 0; s < KT / 16; ++s) {
@@ -244,26 +240,37 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
     if (t < a.offsets[0] || t >= a.offsets[a.B]) return;  // rows of no sequence stay as they are
     const int lane = threadIdx.x & 63;
     const int64_t step = a.T * a.H;
-    float M = -INFINITY;
-    bool any = false;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float2 ml = a.part_ml[s * step + i];
-        if (ml.y != 0.0f) {
-            any = true;
-            M = fmaxf(M, ml.x);
-        }
-    }
+    // a lane per split: the splits of one launch are at most kMaxSplits
+    const float2 ml = lane < a.nsplit ? a.part_ml[lane * step + i] : make_float2(-INFINITY, 0.0f);
+    const bool any = __any(ml.y != 0.0f);
+    const float M = wave_all(ml.y != 0.0f ? ml.x : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
     const float base = M == -INFINITY ? 0.0f : M;
+    const bool some = ml.y != 0.0f && ml.y != -1.0f;
+    const float w = some ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) : 0.0f;
+    const float l = wave_all(some ? w * ml.y : 0.0f, [](float x, float y) { return x + y; });
     constexpr int PL = HD >= 64 ? HD / 64 : 1;
-    float o[PL] = {}, l = 0.0f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float2 ml = a.part_ml[s * step + i];
-        if (ml.y == 0.0f || ml.y == -1.0f) continue;
-        const float w = __builtin_amdgcn_exp2f((ml.x - base) * a.c);
-        l = fmaf(w, ml.y, l);
+    float o[PL] = {};
+    uint64_t left = __ballot(some);  // their partial rows, four at a time
+    while (left) {
+        int at[4];
+        float x[4][PL], ws[4];
+        bool live[4];
 #pragma unroll
-        for (int u = 0; u < PL; ++u)
-            if (lane * PL < HD) o[u] = fmaf(w, a.part_o[(s * step + i) * HD + lane * PL + u], o[u]);
+        for (int j = 0; j < 4; ++j) {
+            live[j] = left != 0;
+            at[j] = live[j] ? __builtin_ctzll(left) : at[j > 0 ? j - 1 : 0];
+            ws[j] = __shfl(w, at[j], 64);
+            left &= left - 1;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int u = 0; u < PL; ++u)
+                if (lane * PL < HD) x[j][u] = a.part_o[(at[j] * step + i) * HD + lane * PL + u];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int u = 0; u < PL; ++u) o[u] = live[j] ? fmaf(ws[j], x[j][u], o[u]) : o[u];
     }
     const float inv = any ? 1.0f / l : 0.0f;
     T* op = static_cast<T*>(a.o) + t * a.ldo + (i % a.H) * HD;
@@ -276,6 +283,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
 // --------------------------------------------------------------------------- the launch
 int64_t tile_bound(int64_t T, int64_t G, int64_t B, int64_t R) { return T * G / R + std::min(B, T); }
 
+constexpr int64_t kMaxSplits = 64;  // a wave joins them, a lane each
 constexpr int64_t kFewRows = 32;  // query rows per key/value head that the few-row kernel holds at a time
 
 struct Plan {
@@ -287,7 +295,7 @@ Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t
     Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0, max_q * (H / Hkv) <= kFewRows};
     const int64_t blocks = std::max<int64_t>(1, (p.few ? B : p.tiles) * Hkv);
     const int64_t fill = p.few ? 2048 : 512, least = p.few ? 512 : 256;  // blocks wanted, keys of a split at least
-    const int64_t want = std::min((fill + blocks - 1) / blocks, max_len / least);
+    const int64_t want = std::min({(fill + blocks - 1) / blocks, max_len / least, kMaxSplits});
     if (want > 1) {
         p.chunk = ((max_len + want - 1) / want + 127) / 128 * 128;
         p.nsplit = (max_len + p.chunk - 1) / p.chunk;

@@ -104,6 +104,16 @@ template <> __device__ __forceinline__ bool any_non_finite<float>(uint4 x) {
     return bad;
 }
 
+__device__ __forceinline__ bool any_nan_code(uint4 x) {
+    bool bad = false;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int by = 0; by < 4; ++by) bad |= ((w[i] >> (8 * by)) & 0x7fu) == 0x7fu;
+    return bad;
+}
+
 // The four V values at columns d0 .. d0+3 of a tile's row.
 template <typename T, int HD>
 __device__ __forceinline__ float4 v4_at(const char* tile, int row, int d0) {
@@ -147,9 +157,10 @@ struct Rows {
 
 // o += sum over the tile's keys of p v, key by key and only where the row sees the key: a hidden key has
 // weight zero in the matrix product, and zero times an infinity or NaN in its v is NaN.  For tiles
-// that hold both a hidden key and a non-finite v.  p[jb][e] is key 32 jb + 8 (e >> 2) + 4 h + (e & 3).
-template <typename T, int HD, int JB, typename Seen>
-__device__ __forceinline__ void add_seen_rows(f32x16 (&o)[HD / 32], const f32x16 (&p)[JB], const char* vt, Seen seen) {
+// that hold both a hidden key and a non-finite v.  p[jb][e] is key 32 jb + 8 (e >> 2) + 4 h + (e & 3);
+// v4(key, d) gives v[key][d .. d+3].
+template <int HD, int JB, typename V4, typename Seen>
+__device__ __forceinline__ void add_seen_rows(f32x16 (&o)[HD / 32], const f32x16 (&p)[JB], V4 v4, Seen seen) {
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb)
@@ -165,7 +176,7 @@ __device__ __forceinline__ void add_seen_rows(f32x16 (&o)[HD / 32], const f32x16
                 for (int ob = 0; ob < HD / 32; ++ob)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const float4 x = v4_at<T, HD>(vt, key, 32 * ob + 8 * g + 4 * h);
+                        const float4 x = v4(key, 32 * ob + 8 * g + 4 * h);
                         const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                         for (int u = 0; u < 4; ++u)

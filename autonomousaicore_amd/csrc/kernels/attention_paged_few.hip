@@ -6,10 +6,16 @@
 // tile's arrival and its use, and each wave keeps its own copies in flight; their (m, l, O) are joined
 // once at the end.  The page ids of the split are in LDS before the first tile, so a tile's
 // addresses cost no memory latency.
-//   bf16  two stages per wave, filled by direct global -> LDS copies two tiles ahead (32 KB per wave at
-//         head_dim 128: one block and up to 128 KB in flight per CU)
-//   e4m3  one stage of bf16: the next tile's codes travel to registers (8 KB per wave at head_dim 128, two
-//         blocks per CU) while this one is multiplied, and are converted as they are stored
+// Tiles arrive by direct global -> LDS copies, two stages per wave: 32 KB per wave at head_dim 128 in bf16 (one
+// block and up to 128 KB in flight per CU), 16 KB in e4m3 (two blocks).
+//
+// e4m3 tiles stay codes in LDS.  K fragments are converted as they are read, a lane holding codes of one key
+// and so one power of two; V fragments (transposed reads) hold eight keys, so they are converted with
+// the tile's largest power 2^E, and the weights take 2^(e - E).  That loses what is below 2^-86 of
+// the tile's largest: where the tile's powers differ by more than 2^40, its keys are added one by one instead,
+// so that a hidden key's large v costs a visible one nothing.
+#include <type_traits>
+
 #include "attention_paged.hpp"
 
 namespace aic::hip {
@@ -20,18 +26,64 @@ constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <int HD, bool E4>
 struct FewLds {
-    static constexpr int TILE = 32 * HD * 2;  // bytes of a tile of K or V
-    static constexpr int STAGES = E4 ? 1 : 2;
-    static constexpr int WAVE = STAGES * 2 * TILE;
+    static constexpr int TILE = 32 * HD * (E4 ? 1 : 2);          // bytes of a tile of K or V
+    static constexpr int STAGE = 2 * TILE + (E4 ? 256 : 0);      // and the exponents of 32 keys of K, then of V, a word each
+    static constexpr int WAVE = 2 * STAGE;
     static constexpr int BYTES = 4 * WAVE > 4 * 32 * HD * 4 ? 4 * WAVE : 4 * 32 * HD * 4;  // also the waves' O at the end
+    static constexpr int COPIES = 2 * (TILE / 1024) + (E4 ? 1 : 0);  // of a stage
+};
+
+// A byte per lane to LDS, zero-extended to words: lane i's at lds + 4 i.  As dma16.
+__device__ __forceinline__ void dma_byte(const void* g, const void* lds) {
+    const uint32_t l = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_ubyte %1, off"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(l)), "v"(g)
+                 : "memory", "m0");
+}
+__device__ const uint8_t kNoExponent = 1;  // of keys without a page: their codes are NaN, their power the least
+
+// [32][HD] tiles of codes, 16-byte chunks swizzled by row: 16 consecutive rows of one chunk (ds_read_b128) and the
+// rows {0-3, 8-11} + 4h of two neighbouring chunks (transposed reads) lie in different banks (the latter two-way at
+// head_dim 32).
+template <int HD>
+__device__ __forceinline__ int swz8(int row) {
+    if constexpr (HD == 128) return ((row >> 1) & 1) << 1 | ((row >> 3) & 1) << 2 | ((row >> 2) & 1);
+    else if constexpr (HD == 64) return ((row >> 3) & 1) << 1 | ((row >> 2) & 1);
+    else return (row >> 3) & 1;
+}
+typedef int v2i_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
+
+//   k(t, j):     lane = key lane % 32, its 16 codes of chunk 2 j + h: two k steps of S = K Q^T, whose Q fragments
+//                hold the columns 32 j + 16 h + 0..7 and + 8..15
+//   v(t, ob, s): lane = column 32 ob + lane % 32, 8 codes along the keys of step s in the order of Frags::tr, by
+//                one ds_read_b64_tr_b8: within 16 lanes, output lane i slot j takes byte i % 8 of the 8 at source
+//                lane 2 j + i / 8, so source lane 2 j + p addresses row j, columns 8 p .. +7
+template <int HD>
+struct Frags8 {
+    int k_off[HD / 32], v_off[HD / 32];
+    __device__ __forceinline__ void init() {
+        const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
+        const int g = lane >> 4, j = (lane & 15) >> 1, p = lane & 1, row = (j & 3) + 8 * (j >> 2) + 4 * h;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+            k_off[i] = r * HD + (((2 * i + h) ^ swz8<HD>(r)) << 4);
+            v_off[i] = row * HD + (((2 * i + (g & 1)) ^ swz8<HD>(row)) << 4) + 8 * p;
+        }
+    }
+    __device__ __forceinline__ uint4 k(const char* t, int j) const { return *reinterpret_cast<const uint4*>(t + k_off[j]); }
+    __device__ __forceinline__ uint2 v(const char* t, int ob, int s) const {
+        const v2i_t x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i_t*)(t + 16 * s * HD + v_off[ob]));
+        return make_uint2(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
+    }
 };
 
 template <int HD, bool E4>
-__global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_paged_few_k(PagedArgs a) {
+__global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_k(PagedArgs a) {
     using L = FewLds<HD, E4>;
     constexpr int KS = HD / 16, OB = HD / 32;
-    constexpr int SEG = HD / 16, RPS = 512 / HD, NC = HD / 8;  // bf16: 1 KB copies of a tile, rows of one, chunks of a row
-    constexpr int UPR = HD / 16, NU = 32 * UPR / 64;           // e4m3: units of a row, units of a tile per lane
+    constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int ids[kIds];
     __shared__ float2 mls[4][32];
@@ -44,7 +96,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_paged_few_k(Paged
     char* mine = lds + wave * L::WAVE;
     const int32_t* tr = a.kv.table + b * a.kv.ld_table;
     const int rows = sq.n * a.G;
-    Frags<HD> F;
+    std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
     F.init();
 
     for (int r0 = 0; r0 < rows; r0 += 32) {
@@ -69,30 +121,53 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_paged_few_k(Paged
             const bf16* qp = static_cast<const bf16*>(a.q) + (sq.row0 + tok) * a.ldq + static_cast<int64_t>(head) * HD;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 16 * kk + 8 * hl, real));
+                const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : 16 * kk + 8 * hl;
+                if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + col, real));
                 else
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[16 * kk + 8 * hl + j] : f2bf(0.0f);
+                    for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[col + j] : f2bf(0.0f);
             }
 
-            // one tile's products, from bf16 K and V tiles in LDS
-            auto compute = [&](const char* kt, const char* vt, int k0) {
+            // one tile's products, from the stage it arrived in
+            auto compute = [&](const char* kt, int k0) {
+                const char* vt = kt + L::TILE;
+                [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
                 f32x16 sc[1];
                 zero(sc[0]);
+                [[maybe_unused]] int e_max = 0;
+                bool one_by_one = false;
+                if constexpr (E4) {
+                    const float sk = exp_scale(ex[lane & 31]);
+                    const int ev = static_cast<int>(ex[32 + (lane & 31)]);
+                    e_max = wave_all(ev, [](int x, int y) { return max(x, y); });
+                    one_by_one = __any(e_max - ev > 40);
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk)
-                    sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
+                    for (int j = 0; j < HD / 32; ++j) {
+                        const uint4 x = F.k(kt, j);
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.x, x.y), sk)),
+                                                                        qb[2 * j], sc[0], 0, 0, 0);
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.z, x.w), sk)),
+                                                                        qb[2 * j + 1], sc[0], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < KS; ++kk)
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
+                }
                 // every row sees every key of the tile?
                 const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
                 auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
-                bool poison = false;  // a hidden key and a non-finite v
                 if (!open) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
+                    bool bad = false;  // a hidden key and a non-finite v
 #pragma unroll
-                    for (int i = 0; i < L::TILE / 1024; ++i)
-                        poison |= any_non_finite<bf16>(*reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16));
-                    poison = __any(poison);
+                    for (int i = 0; i < L::TILE / 1024; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16);
+                        if constexpr (E4) bad |= any_nan_code(x);
+                        else bad |= any_non_finite<bf16>(x);
+                    }
+                    one_by_one |= __any(bad);
                 }
                 float mx = -INFINITY;
 #pragma unroll
@@ -106,16 +181,37 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_paged_few_k(Paged
                     sum += sc[0][e];
                 }
                 st_.add(sum);
-                if (poison) {
-                    add_seen_rows<bf16, HD, 1>(st_.o, sc, vt, seen);
+                if (one_by_one) {
+                    if constexpr (E4)
+                        add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) {
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + key * HD + (((d >> 4) ^ swz8<HD>(key)) << 4) + (d & 15));
+                            const float s = exp_scale(ex[32 + key]);
+                            const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
+                            return make_float4(x[0], x[1], y[0], y[1]);
+                        }, seen);
+                    else add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<bf16, HD>(vt, key, d); }, seen);
                     return;
                 }
+                if constexpr (E4) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(ex + 32 + 8 * g + 4 * hl);
+                        const uint32_t ev[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) sc[0][4 * g + u] = __builtin_amdgcn_ldexpf(sc[0][4 * g + u], static_cast<int>(ev[u]) - e_max);
+                    }
+                }
+                [[maybe_unused]] const float sv = exp_scale(static_cast<uint32_t>(e_max));
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const bf16x8 p = pack_bf16x8(sc[0], 8 * s);
 #pragma unroll
-                    for (int ob = 0; ob < OB; ++ob)
-                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.tr(vt, ob, s), p, st_.o[ob], 0, 0, 0);
+                    for (int ob = 0; ob < OB; ++ob) {
+                        bf16x8 v;
+                        if constexpr (E4) v = __builtin_bit_cast(bf16x8, e4m3_bf16(F.v(vt, ob, s), sv));
+                        else v = F.tr(vt, ob, s);
+                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, st_.o[ob], 0, 0, 0);
+                    }
                 }
             };
 
@@ -136,64 +232,33 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void attn_paged_few_k(Paged
                     const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * ps + (key - pi * ps);
                     return page < 0 ? -1 : row;
                 };
-                if constexpr (!E4) {
-                    auto issue = [&](int t) {
-                        char* dst = mine + (t & 1) * 2 * L::TILE;
-                        const int k0 = first + 128 * t;
-                        const char* none = reinterpret_cast<const char*>(&kNoPage);
+                auto issue = [&](int t) {
+                    char* dst = mine + (t & 1) * L::STAGE;
+                    const int k0 = first + 128 * t;
+                    const char* none = reinterpret_cast<const char*>(&kNoPage);
 #pragma unroll
-                        for (int i = 0; i < SEG; ++i) {
-                            const int rr = i * RPS + lane / NC, ch = (lane % NC) ^ swz<HD>(rr);
-                            const int64_t row = row_at(k0 + rr);
-                            const int64_t at = row * (HD * 2) + ch * 16;
-                            dma16(row >= 0 ? a.kv.kp + at : none, dst + i * 1024);
-                            dma16(row >= 0 ? a.kv.vp + at : none, dst + L::TILE + i * 1024);
-                        }
-                    };
-                    if (nt > 0) issue(0);
-                    if (nt > 1) issue(1);
-                    for (int t = 0; t < nt; ++t) {
-                        if (t + 1 < nt) wait_vmcnt<2 * SEG>();  // tile t has landed; t + 1 may be in flight
-                        else wait_vmcnt<0>();
-                        const char* src = mine + (t & 1) * 2 * L::TILE;
-                        compute(src, src + L::TILE, first + 128 * t);
-                        wait_lds();  // the tile has been read
-                        if (t + 2 < nt) issue(t + 2);
+                    for (int i = 0; i < L::TILE / 1024; ++i) {
+                        const int rr = i * RPS + lane / NC;
+                        int ch = lane % NC;
+                        if constexpr (E4) ch ^= swz8<HD>(rr);
+                        else ch ^= swz<HD>(rr);
+                        const int64_t row = row_at(k0 + rr), at = row * RB + ch * 16;
+                        dma16(row >= 0 ? a.kv.kp + at : none, dst + i * 1024);
+                        dma16(row >= 0 ? a.kv.vp + at : none, dst + L::TILE + i * 1024);
                     }
-                } else {
-                    uint4 rk[NU], rv[NU];
-                    uint32_t xk[NU], xv[NU];
-                    auto load = [&](int t) {
-                        const char* none = reinterpret_cast<const char*>(&kNoPage);
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) {
-                            const int u = i * 64 + lane;
-                            const int64_t row = row_at(first + 128 * t + u / UPR), at = row * HD + (u % UPR) * 16;
-                            rk[i] = *reinterpret_cast<const uint4*>(row >= 0 ? a.kv.kp + at : none);
-                            rv[i] = *reinterpret_cast<const uint4*>(row >= 0 ? a.kv.vp + at : none);
-                            xk[i] = row >= 0 ? a.kv.ke[row] : 127;
-                            xv[i] = row >= 0 ? a.kv.ve[row] : 127;
-                        }
-                    };
-                    if (nt > 0) load(0);
-                    for (int t = 0; t < nt; ++t) {
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) {
-                            const int u = i * 64 + lane, rr = u / UPR, ch = u % UPR;
-                            const float sk = exp_scale(xk[i]), sv = exp_scale(xv[i]);
-                            char *kt = mine, *vt = mine + L::TILE;
-                            *reinterpret_cast<uint4*>(kt + chunk_at<bf16, HD>(rr, 2 * ch)) = e4m3_bf16(make_uint2(rk[i].x, rk[i].y), sk);
-                            *reinterpret_cast<uint4*>(kt + chunk_at<bf16, HD>(rr, 2 * ch + 1)) = e4m3_bf16(make_uint2(rk[i].z, rk[i].w), sk);
-                            *reinterpret_cast<uint4*>(vt + chunk_at<bf16, HD>(rr, 2 * ch)) = e4m3_bf16(make_uint2(rv[i].x, rv[i].y), sv);
-                            *reinterpret_cast<uint4*>(vt + chunk_at<bf16, HD>(rr, 2 * ch + 1)) = e4m3_bf16(make_uint2(rv[i].z, rv[i].w), sv);
-                        }
-                        if (t + 1 < nt) load(t + 1);
-                        __builtin_amdgcn_wave_barrier();
-                        wait_lds();  // the wave's own stores are there
-                        compute(mine, mine + L::TILE, first + 128 * t);
-                        wait_lds();
-                        __builtin_amdgcn_wave_barrier();
+                    if constexpr (E4) {
+                        const int64_t row = row_at(k0 + (lane & 31));
+                        dma_byte(row >= 0 ? (hl ? a.kv.ve : a.kv.ke) + row : &kNoExponent, dst + 2 * L::TILE);
                     }
+                };
+                if (nt > 0) issue(0);
+                if (nt > 1) issue(1);
+                for (int t = 0; t < nt; ++t) {
+                    if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
+                    else wait_vmcnt<0>();
+                    compute(mine + (t & 1) * L::STAGE, first + 128 * t);
+                    wait_lds();  // the tile has been read
+                    if (t + 2 < nt) issue(t + 2);
                 }
             }
         }

@@ -286,3 +286,27 @@ def test_streams_do_not_share_results():
         a.check()
     for s in streams:
         _lib.call("aic_hip_mem_release_stream", s.cuda_stream)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n,L", [(1, 300), (3, 300), (60, 300), (1, 3000)])
+def test_e4m3_rows_of_very_different_size(dt, n, L):
+    """A few cached rows 2^60 times the others, seen and hidden, and rows of 2^-100: a hidden row costs a visible one
+    nothing, and small rows keep their digits."""
+    p = Paged([n], [L], 1, 64, 16, "e4m3", seed=n + L)
+    for name in "kv":
+        codes, exps = p.pool[name]
+        for pos, by in ((3, 60), (17, -100), (L - 1, 60), (L - n // 2 - 1, 30), (40, -60)):
+            if name == "k" and by > 0:
+                by = -by  # large scores would leave one key only
+            page, slot = p.place(0, pos)
+            exps[page, 0, slot] += by
+            getattr(p, name)[page, 0, slot] *= 2.0 ** by
+    Call(p, 2, dt).run().check()
+    small = Paged([n], [L], 1, 64, 16, "e4m3", seed=n + L)
+    codes, exps = small.pool["v"]
+    exps -= 110
+    small.v *= 2.0 ** -110
+    a = Call(small, 2, dt).run()
+    a.check()
+    assert (a.o[:n, :128] != 0).any()
