@@ -96,6 +96,14 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
     char* mine = lds + wave * L::WAVE;
     const int32_t* tr = a.kv.table + b * a.kv.ld_table;
     const int rows = sq.n * a.G;
+    const bool paged = ps % (RPS > 16 ? RPS : 16) == 0;  // halves of tiles (whole ones where one copy spans both) do not leave a page
+    uint32_t voff[L::TILE / 1024];
+#pragma unroll
+    for (int i = 0; i < L::TILE / 1024; ++i) {
+        const int rr = i * RPS + lane / NC;
+        const int ch = (lane % NC) ^ (E4 ? swz8<HD>(rr) : swz<HD>(rr));
+        voff[i] = static_cast<uint32_t>((rr - (i * RPS >= 16 ? 16 : 0)) * RB + ch * 16);
+    }
     std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
     F.init();
 
@@ -235,6 +243,24 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 auto issue = [&](int t) {
                     char* dst = mine + (t & 1) * L::STAGE;
                     const int k0 = first + 128 * t;
+                    if (paged && k0 + 32 <= w1) {
+                        // each half of the tile lies in one page: uniform bases, offsets per lane made once
+                        const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
+                        const int page0 = __builtin_amdgcn_readfirstlane(ids[pi - p0]), page1 = __builtin_amdgcn_readfirstlane(ids[pj - p0]);
+                        if (page0 >= 0 && page1 >= 0) {
+                            const int64_t row[2] = {(static_cast<int64_t>(page0) * Hkv + kvh) * ps + (k0 - pi * ps),
+                                                    (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps)};
+#pragma unroll
+                            for (int i = 0; i < L::TILE / 1024; ++i) {
+                                const int64_t at = row[i * RPS >= 16 ? 1 : 0] * RB;
+                                dma16s(a.kv.kp + at, voff[i], dst + i * 1024);
+                                dma16s(a.kv.vp + at, voff[i], dst + L::TILE + i * 1024);
+                            }
+                            if constexpr (E4)
+                                dma_byte((hl ? a.kv.ve : a.kv.ke) + (lane & 16 ? row[1] : row[0]) + (lane & 15), dst + 2 * L::TILE);
+                            return;
+                        }
+                    }
                     const char* none = reinterpret_cast<const char*>(&kNoPage);
 #pragma unroll
                     for (int i = 0; i < L::TILE / 1024; ++i) {
