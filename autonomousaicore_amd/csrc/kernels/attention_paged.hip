@@ -284,18 +284,14 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
 int64_t tile_bound(int64_t T, int64_t G, int64_t B, int64_t R) { return T * G / R + std::min(B, T); }
 
 constexpr int64_t kMaxSplits = 64;  // a wave joins them, a lane each
-constexpr int64_t kFewRows = 32;  // query rows per key/value head that the few-row kernel holds at a time
-
 struct Plan {
     int64_t tiles, nsplit, chunk;
-    bool few;
 };
-// Splits over the keys where the rows alone do not fill the card: equal chunks of a multiple of 128 keys.
-Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t max_q) {
-    Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0, max_q * (H / Hkv) <= kFewRows};
-    const int64_t blocks = std::max<int64_t>(1, (p.few ? B : p.tiles) * Hkv);
-    const int64_t fill = p.few ? 2048 : 512, least = p.few ? 512 : 256;  // blocks wanted, keys of a split at least
-    const int64_t want = std::min({(fill + blocks - 1) / blocks, max_len / least, kMaxSplits});
+// Splits over the keys where the query tiles alone do not fill the card: equal chunks of a multiple of 128 keys.
+Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv) {
+    Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0};
+    const int64_t blocks = std::max<int64_t>(1, p.tiles * Hkv);
+    const int64_t want = std::min({(512 + blocks - 1) / blocks, max_len / 256, kMaxSplits});  // blocks wanted, keys of a split at least
     if (want > 1) {
         p.chunk = ((max_len + want - 1) / want + 127) / 128 * 128;
         p.nsplit = (max_len + p.chunk - 1) / p.chunk;
@@ -321,7 +317,14 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
 int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H) {
     check_sizes(c, B, T, max_q, max_len, H);
     if (B == 0 || T == 0) return 0;
-    return plan_bytes(plan(B, T, max_len, H, c.kv_heads, max_q), T, H, c.head_dim);
+    // the cache's type does not tell the queries' (e4m3 serves both): room for either
+    int64_t n = 0;
+    const int64_t G = H / c.kv_heads;
+    if (c.type != DType::Float32 && few_rows(max_q, G))
+        n = few_workspace(B, max_q, max_len, G, c.head_dim, c.type == DType::UInt8);
+    if (c.type != DType::BFloat16 || !few_rows(max_q, G))
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads), T, H, c.head_dim));
+    return n;
 }
 
 void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int64_t* offsets,
@@ -352,19 +355,21 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_q = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q * size % 16 == 0;
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
-    Plan p = plan(B, T, max_len, H, c.kv_heads, max_q);
-    const int64_t need = plan_bytes(p, T, H, c.head_dim);
+    const bool few = dt == DType::BFloat16 && few_rows(max_q, a.G);
+    Plan p = plan(B, T, max_len, H, c.kv_heads);
+    const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
-    if (need > 0) {
-        if (workspace) {
-            AIC_CHECK(workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
-                      "attn_paged: the workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
-        } else if (stream_scratch_ready(s)) {
-            workspace = stream_scratch(static_cast<size_t>(need), s);
-        } else {
-            p.nsplit = 1, p.chunk = 0;  // captured without a workspace of its own
-        }
+    if (workspace)
+        AIC_CHECK(workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
+                  "attn_paged: the workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
+    else if (need > 0 && stream_scratch_ready(s))
+        workspace = stream_scratch(static_cast<size_t>(need), s);
+    if (need == 0) workspace = nullptr;
+    if (few) {
+        attn_paged_few(a, max_q, c.type == DType::UInt8, static_cast<int>(c.head_dim), workspace, s);
+        return;
     }
+    if (!workspace) p.nsplit = 1, p.chunk = 0;  // nothing to split, or captured without a workspace of its own
     a.nsplit = static_cast<int>(p.nsplit);
     a.chunk = static_cast<int>(p.chunk);
     if (p.nsplit > 1) {
@@ -376,12 +381,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     auto run = [&](auto t, auto ct, auto hd) {
         using X = decltype(t);
         constexpr int D = decltype(hd)::value;
-        if (p.few && sizeof(X) == 2) {
-            attn_paged_few(a, sizeof(ct) == 1, D, s);
-        } else {
-            attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-            AIC_LAUNCH_CHECK("attn_paged");
-        }
+        attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+        AIC_LAUNCH_CHECK("attn_paged");
         if (a.nsplit > 1) {
             const int64_t joins = (T * H + 3) / 4;
             AIC_CHECK(joins <= INT32_MAX, OutOfRange, "attn_paged: too many rows in one call");

@@ -1,11 +1,18 @@
 // Attention over the paged cache for few query rows per key/value head (single tokens, drafted tokens): bound by
 // reading the cache once.
 //
-// One block: up to 32 query rows of one sequence and key/value head, over one split of its keys.  The
+// A group of up to 32 query rows of one sequence and key/value head is worked on by a block at a time.  The
 // four waves take tiles of 32 keys in turn, each into LDS of its own, so no barrier stands between a
 // tile's arrival and its use, and each wave keeps its own copies in flight; their (m, l, O) are joined
-// once at the end.  The page ids of the split are in LDS before the first tile, so a tile's
-// addresses cost no memory latency.
+// once at the end.  The page ids of the keys are in LDS before the first tile, so a tile's addresses
+// cost no memory latency.
+//
+// Shares: the keys of all groups, in steps of 128, form one list that is cut into as many equal parts as blocks
+// are resident at once, so that batches of uneven lengths end together; a group that a cut divides leaves
+// its parts' states in the workspace and attn_paged_few_join_k adds them.  (Equal splits per
+// sequence ran in one and a half rounds of blocks: 28.7 us at best and 40 us at worst for 32 e4m3 caches of up to
+// 8000 tokens, by the number of splits.)  Every block finds its part from offsets and lens by itself.
+//
 // Tiles arrive by direct global -> LDS copies, two stages per wave: 32 KB per wave at head_dim 128 in bf16 (one
 // block and up to 128 KB in flight per CU), 16 KB in e4m3 (two blocks).
 //
@@ -14,6 +21,8 @@
 // the tile's largest power 2^E, and the weights take 2^(e - E).  That loses what is below 2^-86 of
 // the tile's largest: where the tile's powers differ by more than 2^40, its keys are added one by one instead,
 // so that a hidden key's large v costs a visible one nothing.
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "attention_paged.hpp"
@@ -22,7 +31,82 @@ namespace aic::hip {
 
 namespace {
 
-constexpr int kIds = 512;  // page ids in LDS at a time
+constexpr int kIds = 512;    // page ids in LDS at a time
+constexpr int kStep = 128;   // keys: a tile for each wave
+constexpr int kLeast = 4;    // steps of a share at least: a part costs a block about as much as three steps
+
+struct FewArgs {
+    PagedArgs a;
+    int group;         // query rows of a group, at most 32
+    int shares;        // 0: a block per sequence and key/value head, nothing divided
+    int64_t* plan;     // [B + 1]: steps before each sequence, and a share's steps
+    float2* part_ml;   // [2 shares][group]: a share's first group's, then its last one's
+    float* part_o;     // [2 shares][group][hd]
+};
+// A sequence's place in the list of steps.
+struct Steps {
+    Seq sq;
+    int lo, steps, groups;  // first key (a multiple of kStep), steps over its keys, row groups
+};
+__device__ __forceinline__ Steps steps_of(const FewArgs& f, int b) {
+    Steps x;
+    x.sq = sequence(f.a, b);
+    const int first = max(x.sq.len - x.sq.n, 0);
+    x.lo = f.a.window > 0 ? max(0, first - f.a.window + 1) & ~(kStep - 1) : 0;
+    x.steps = max(1, (x.sq.len - x.lo + kStep - 1) / kStep);  // also of a sequence without keys: its rows are zeros
+    x.groups = (x.sq.n * f.a.G + f.group - 1) / f.group;
+    return x;
+}
+// The share of block g: sequence and steps before its begin there.  False: no steps are left for it.
+__device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, int64_t& before, int64_t& count) {
+    __shared__ double sums[4];
+    __shared__ int at_b;
+    __shared__ int64_t at_before;
+    const int per = (f.a.B + 255) / 256, tid = threadIdx.x, wave = tid >> 6;
+    const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
+    auto steps = [&](int i) {
+        const Steps x = steps_of(f, i);
+        return static_cast<double>(x.steps) * x.groups * f.a.kv.Hkv;
+    };
+    double mine = 0.0;  // whole numbers below 2^53
+    for (int i = first; i < last; ++i) mine += steps(i);
+    const double upto = wave_running_sum(mine);
+    if ((tid & 63) == 63) sums[wave] = upto;
+    __syncthreads();
+    double start = upto - mine, total = 0.0;
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) start += sums[w];
+        total += sums[w];
+    }
+    const int64_t share = max(static_cast<int64_t>(kLeast), (static_cast<int64_t>(total) + f.shares - 1) / f.shares);
+    const int64_t begin = g * share;
+    if (g == 0) {
+        double s = start;
+        for (int i = first; i < last; ++i) {
+            f.plan[i] = static_cast<int64_t>(s);
+            s += steps(i);
+        }
+        if (tid == 0) f.plan[f.a.B] = share;
+    }
+    if (begin >= static_cast<int64_t>(total)) return false;
+    if (begin >= static_cast<int64_t>(start) && begin < static_cast<int64_t>(start + mine)) {
+        double s = start;
+        for (int i = first; i < last; ++i) {
+            const double n = steps(i);
+            if (begin < static_cast<int64_t>(s + n)) {
+                at_b = i;
+                at_before = begin - static_cast<int64_t>(s);
+                break;
+            }
+            s += n;
+        }
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(at_b);
+    before = at_before;
+    count = min(share, static_cast<int64_t>(total) - begin);
+    return true;
+}
 
 template <int HD, bool E4>
 struct FewLds {
@@ -80,8 +164,9 @@ struct Frags8 {
 };
 
 template <int HD, bool E4>
-__global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_k(PagedArgs a) {
+__global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_k(FewArgs f) {
     using L = FewLds<HD, E4>;
+    const PagedArgs& a = f.a;
     constexpr int KS = HD / 16, OB = HD / 32;
     constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -89,13 +174,8 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
     __shared__ float2 mls[4][32];
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
-    const int kvh = static_cast<int>(blockIdx.x) % Hkv, rest = static_cast<int>(blockIdx.x) / Hkv;
-    const int b = rest % a.B, split = rest / a.B;
-    const Seq sq = sequence(a, b);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
     char* mine = lds + wave * L::WAVE;
-    const int32_t* tr = a.kv.table + b * a.kv.ld_table;
-    const int rows = sq.n * a.G;
     const bool paged = ps % (RPS > 16 ? RPS : 16) == 0;  // halves of tiles (whole ones where one copy spans both) do not leave a page
     uint32_t voff[L::TILE / 1024];
 #pragma unroll
@@ -107,19 +187,47 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
     std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
     F.init();
 
-    for (int r0 = 0; r0 < rows; r0 += 32) {
+    int b;
+    int64_t before, count;
+    if (f.shares > 0) {
+        if (!find_share(f, static_cast<int>(blockIdx.x), b, before, count)) return;
+    } else {
+        b = static_cast<int>(blockIdx.x) / Hkv;
+        before = 0;
+        count = INT64_MAX;
+    }
+    for (bool first_part = true; count > 0 && b < a.B;) {
+        const Steps x = steps_of(f, b);
+        const Seq sq = x.sq;
+        // groups of a sequence: all of them (shares), or those of the block's head
+        const int64_t groups = static_cast<int64_t>(x.groups) * (f.shares > 0 ? Hkv : 1);
+        if (before >= groups * x.steps) {
+            if (f.shares == 0) return;
+            before -= groups * x.steps;
+            ++b;
+            continue;
+        }
+        const int gi = static_cast<int>(before / x.steps), u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
+        const int u1 = static_cast<int>(min(static_cast<int64_t>(x.steps), u0 + min(count, int64_t{1} << 30)));
+        const int kvh = f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv, r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
+        const bool whole = u0 == 0 && u1 == x.steps;
+        const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
+        first_part = false;
+        before += u1 - u0;
+        count -= u1 - u0;
+
+        const int32_t* tr = a.kv.table + b * a.kv.ld_table;
+        const int rows = min(sq.n * a.G, r0 + f.group);
         const int r = r0 + (lane & 31);
         const bool real = r < rows;
         const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
         const int hi = real ? sq.len - sq.n + tok : -1;
         const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
-        const int first_pos = sq.len - sq.n + r0 / a.G, last_pos = sq.len - sq.n + (min(r0 + 32, rows) - 1) / a.G;
+        const int first_pos = sq.len - sq.n + r0 / a.G, last_pos = sq.len - sq.n + (rows - 1) / a.G;
+        // keys of this part that the group sees
         int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
-        if (a.chunk > 0) {
-            k_lo = max(k_lo, split * a.chunk);
-            if (split + 1 < a.nsplit) k_hi = min(k_hi, (split + 1) * a.chunk);
-        }
-        k_lo &= ~31;
+        k_lo = max(k_lo & ~31, x.lo + u0 * kStep);
+        if (u1 < x.steps) k_hi = min(k_hi, x.lo + u1 * kStep);
         const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));
 
         Rows<OB> st_;
@@ -297,7 +405,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
 #pragma unroll
         for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][q].x);
         const float base = M == -INFINITY ? 0.0f : M;
-        const float f = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
+        const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
         float* os = reinterpret_cast<float*>(lds);  // [4][32][HD], 16-byte groups swizzled by row
 #pragma unroll
         for (int ob = 0; ob < OB; ++ob)
@@ -305,7 +413,8 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
             for (int g = 0; g < 4; ++g) {
                 const int c4 = (ob * 32 + 8 * g + 4 * hl) / 4;
                 *reinterpret_cast<float4*>(os + (wave * 32 + q) * HD + ((c4 ^ (q & 7)) << 2)) =
-                    make_float4(st_.o[ob][4 * g] * f, st_.o[ob][4 * g + 1] * f, st_.o[ob][4 * g + 2] * f, st_.o[ob][4 * g + 3] * f);
+                    make_float4(st_.o[ob][4 * g] * factor, st_.o[ob][4 * g + 1] * factor, st_.o[ob][4 * g + 2] * factor,
+                                st_.o[ob][4 * g + 3] * factor);
             }
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * (HD / 4); i += 256) {
@@ -330,10 +439,10 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
             }
             const int64_t t = sq.row0 + tk;
-            if (a.nsplit > 1) {
-                const int64_t at = (static_cast<int64_t>(split) * a.T + t) * a.H + hd_;
-                if (c4 == 0) a.part_ml[at] = make_float2(mm, empty ? 0.0f : l == 0.0f ? -1.0f : l);
-                if (!empty) *reinterpret_cast<float4*>(a.part_o + at * HD + c4 * 4) = x;
+            if (!whole) {
+                const int64_t at = static_cast<int64_t>(slot) * f.group + qr;
+                if (c4 == 0) f.part_ml[at] = make_float2(mm, empty ? 0.0f : l == 0.0f ? -1.0f : l);
+                if (!empty) *reinterpret_cast<float4*>(f.part_o + at * HD + c4 * 4) = x;
                 continue;
             }
             const float inv = empty ? 0.0f : 1.0f / l;
@@ -345,28 +454,126 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
             }
             if (a.lse && c4 == 0) a.lse[t * a.H + hd_] = empty ? -INFINITY : log_sum(bs, l, a.c);
         }
-        __syncthreads();  // before the next rows' tiles
+        __syncthreads();  // before the next group's tiles
     }
 }
 
-template <int HD, bool E4>
-void launch(const PagedArgs& a, hipStream_t s) {
-    constexpr int bytes = FewLds<HD, E4>::BYTES;
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    AIC_HIP_CHECK(allowed);
-    const int64_t blocks = static_cast<int64_t>(a.kv.Hkv) * a.B * a.nsplit;
-    AIC_CHECK(blocks <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
-    attn_paged_few_k<HD, E4><<<static_cast<unsigned>(blocks), 256, bytes, s>>>(a);
-    AIC_LAUNCH_CHECK("attn_paged");
+// The groups that shares divided: one wave per row adds the parts of its group.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
+    const PagedArgs& a = f.a;
+    const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv;
+    const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
+    if (qr >= f.group) return;
+    const int64_t share = f.plan[a.B], base_step = f.plan[b];
+    const Steps x = steps_of(f, b);
+    for (int g = 0; g < x.groups; ++g) {
+        const int r = g * f.group + qr;
+        if (r >= x.sq.n * a.G) return;
+        const int64_t from = base_step + (static_cast<int64_t>(g) * Hkv + kvh) * x.steps;
+        const int s0 = static_cast<int>(from / share), s1 = static_cast<int>((from + x.steps - 1) / share);
+        if (s0 == s1) continue;  // undivided: written already
+        // part i of the group: share s0 + i, where it is the first group unless it starts behind the share's begin
+        auto at = [&](int i) {
+            return (static_cast<int64_t>(2) * (s0 + i) + (i == 0 && from != s0 * share ? 1 : 0)) * f.group + qr;
+        };
+        const int parts = s1 - s0 + 1;
+        float M = -INFINITY;
+        bool any = false;
+        for (int i = lane; i < parts; i += 64) {
+            const float2 ml = f.part_ml[at(i)];
+            any |= ml.y != 0.0f;
+            M = ml.y != 0.0f ? fmaxf(M, ml.x) : M;
+        }
+        any = __any(any);
+        M = wave_all(M, [](float p, float q) { return fmaxf(p, q); });
+        const float base = M == -INFINITY ? 0.0f : M;
+        constexpr int PL = HD >= 64 ? HD / 64 : 1;
+        float o[PL] = {}, l = 0.0f;
+        for (int i0 = 0; i0 < parts; i0 += 64) {
+            const float2 ml = i0 + lane < parts ? f.part_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+            const bool some = ml.y != 0.0f && ml.y != -1.0f;
+            const float w = some ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) : 0.0f;
+            l += wave_all(some ? w * ml.y : 0.0f, [](float p, float q) { return p + q; });
+            uint64_t left = __ballot(some);
+            while (left) {  // four parts' rows at a time
+                int j[4];
+                float v[4][PL], ws[4];
+                bool live[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    live[k] = left != 0;
+                    j[k] = live[k] ? __builtin_ctzll(left) : j[k > 0 ? k - 1 : 0];
+                    ws[k] = __shfl(w, j[k], 64);
+                    left &= left - 1;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int u = 0; u < PL; ++u)
+                        if (lane * PL < HD) v[k][u] = f.part_o[at(i0 + j[k]) * HD + lane * PL + u];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int u = 0; u < PL; ++u) o[u] = live[k] ? fmaf(ws[k], v[k][u], o[u]) : o[u];
+            }
+        }
+        const int64_t t = x.sq.row0 + r / a.G;
+        const int head = kvh * a.G + r % a.G;
+        const float inv = any ? 1.0f / l : 0.0f;
+        bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD;
+#pragma unroll
+        for (int u = 0; u < PL; ++u)
+            if (lane * PL < HD) st(op, lane * PL + u, o[u] * inv);
+        if (a.lse && lane == 0) a.lse[t * a.H + head] = any ? log_sum(base, l, a.c) : -INFINITY;
+    }
 }
+
+// Blocks that are resident at once on 256 CUs: LDS holds one of bf16 at head_dim 128, two of the others.
+int64_t resident(int64_t head_dim, bool e4m3) { return head_dim == 128 && !e4m3 ? 256 : 512; }
+
+template <int HD, bool E4>
+void launch(const FewArgs& f, hipStream_t s) {
+    constexpr int bytes = FewLds<HD, E4>::BYTES;
+    static std::atomic<bool> allowed[64];  // by device
+    int dev = 0;
+    AIC_HIP_CHECK(hipGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4>),
+                                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev >= 0 && dev < 64) allowed[dev].store(true);
+    }
+    const int64_t pairs = static_cast<int64_t>(f.a.kv.Hkv) * f.a.B;
+    AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
+    attn_paged_few_k<HD, E4><<<static_cast<unsigned>(f.shares > 0 ? f.shares : pairs), 256, bytes, s>>>(f);
+    AIC_LAUNCH_CHECK("attn_paged");
+    if (f.shares == 0) return;
+    attn_paged_few_join_k<HD><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>((f.group + 3) / 4)), 256, 0, s>>>(f);
+    AIC_LAUNCH_CHECK("attn_paged join");
+}
+
+int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * G, 1, 32); }
 
 }  // namespace
 
-void attn_paged_few(const PagedArgs& a, bool e4m3, int head_dim, hipStream_t s) {
-    if (head_dim == 32) e4m3 ? launch<32, true>(a, s) : launch<32, false>(a, s);
-    else if (head_dim == 64) e4m3 ? launch<64, true>(a, s) : launch<64, false>(a, s);
-    else e4m3 ? launch<128, true>(a, s) : launch<128, false>(a, s);
+bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
+
+int64_t few_workspace(int64_t B, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3) {
+    if (max_len <= kLeast * kStep) return 0;
+    return (2 * resident(head_dim, e4m3) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
+}
+
+void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s) {
+    FewArgs f{a, static_cast<int>(group_of(max_q, a.G)), 0, nullptr, nullptr, nullptr};
+    if (workspace) {
+        f.shares = static_cast<int>(resident(head_dim, e4m3));
+        f.part_o = static_cast<float*>(workspace);
+        f.part_ml = reinterpret_cast<float2*>(f.part_o + 2LL * f.shares * f.group * head_dim);
+        f.plan = reinterpret_cast<int64_t*>(f.part_ml + 2LL * f.shares * f.group);
+    }
+    if (head_dim == 32) e4m3 ? launch<32, true>(f, s) : launch<32, false>(f, s);
+    else if (head_dim == 64) e4m3 ? launch<64, true>(f, s) : launch<64, false>(f, s);
+    else e4m3 ? launch<128, true>(f, s) : launch<128, false>(f, s);
 }
 
 }  // namespace aic::hip
