@@ -366,7 +366,9 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         workspace = stream_scratch(static_cast<size_t>(need), s);
     if (need == 0) workspace = nullptr;
     if (few) {
-        attn_paged_few(a, max_q, c.type == DType::UInt8, static_cast<int>(c.head_dim), workspace, s);
+        const bool e4m3 = c.type == DType::UInt8;  // need may be the other kernel's alone
+        const bool shares = few_workspace(B, max_q, max_len, a.G, c.head_dim, e4m3) > 0;
+        attn_paged_few(a, max_q, e4m3, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;
     }
     if (!workspace) p.nsplit = 1, p.chunk = 0;  // nothing to split, or captured without a workspace of its own

@@ -34,6 +34,9 @@ namespace {
 constexpr int kIds = 512;    // page ids in LDS at a time
 constexpr int kStep = 128;   // keys: a tile for each wave
 constexpr int kLeast = 4;    // steps of a share at least: a part costs a block about as much as three steps
+// Longest cache whose groups are not divided: finding shares and joining them cost about 7 us, and a step of an
+// undivided group about 1 us (one 512-token sequence of 12 heads of 64: 9.6 us whole, 16.8 us in shares).
+constexpr int kWhole = 1024;
 
 struct FewArgs {
     PagedArgs a;
@@ -58,16 +61,19 @@ __device__ __forceinline__ Steps steps_of(const FewArgs& f, int b) {
     return x;
 }
 // The share of block g: sequence and steps before its begin there.  False: no steps are left for it.
-__device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, int64_t& before, int64_t& count) {
+__device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Steps& x, int64_t& before, int64_t& count) {
     __shared__ double sums[4];
     __shared__ int at_b;
+    __shared__ Steps at_x;
     __shared__ int64_t at_before;
     const int per = (f.a.B + 255) / 256, tid = threadIdx.x, wave = tid >> 6;
     const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
+    Steps own;  // the last of this thread's sequences: its only one in batches of up to 256
     auto steps = [&](int i) {
-        const Steps x = steps_of(f, i);
-        return static_cast<double>(x.steps) * x.groups * f.a.kv.Hkv;
+        if (per > 1) own = steps_of(f, i);
+        return static_cast<double>(own.steps) * own.groups * f.a.kv.Hkv;
     };
+    if (first < last) own = steps_of(f, first);
     double mine = 0.0;  // whole numbers below 2^53
     for (int i = first; i < last; ++i) mine += steps(i);
     const double upto = wave_running_sum(mine);
@@ -95,6 +101,7 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, int6
             const double n = steps(i);
             if (begin < static_cast<int64_t>(s + n)) {
                 at_b = i;
+                at_x = own;
                 at_before = begin - static_cast<int64_t>(s);
                 break;
             }
@@ -102,7 +109,10 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, int6
         }
     }
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(at_b);
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    b = same(at_b);
+    x.sq = {at_x.sq.row0, same(at_x.sq.n), same(at_x.sq.len)};
+    x.lo = same(at_x.lo), x.steps = same(at_x.steps), x.groups = same(at_x.groups);
     before = at_before;
     count = min(share, static_cast<int64_t>(total) - begin);
     return true;
@@ -188,23 +198,24 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
     F.init();
 
     int b;
+    Steps x;
     int64_t before, count;
     if (f.shares > 0) {
-        if (!find_share(f, static_cast<int>(blockIdx.x), b, before, count)) return;
+        if (!find_share(f, static_cast<int>(blockIdx.x), b, x, before, count)) return;
     } else {
         b = static_cast<int>(blockIdx.x) / Hkv;
+        x = steps_of(f, b);
         before = 0;
         count = INT64_MAX;
     }
     for (bool first_part = true; count > 0 && b < a.B;) {
-        const Steps x = steps_of(f, b);
         const Seq sq = x.sq;
         // groups of a sequence: all of them (shares), or those of the block's head
         const int64_t groups = static_cast<int64_t>(x.groups) * (f.shares > 0 ? Hkv : 1);
         if (before >= groups * x.steps) {
             if (f.shares == 0) return;
             before -= groups * x.steps;
-            ++b;
+            if (++b < a.B) x = steps_of(f, b);
             continue;
         }
         const int gi = static_cast<int>(before / x.steps), u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
@@ -432,25 +443,25 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 const float2 ml = mls[w][qr];
                 l = fmaf(__builtin_amdgcn_exp2f((ml.x - bs) * a.c), ml.y, l);
             }
-            float4 x = make_float4(0, 0, 0, 0);
+            float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const float4 y = *reinterpret_cast<const float4*>(os + (w * 32 + qr) * HD + ((c4 ^ (qr & 7)) << 2));
-                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
             const int64_t t = sq.row0 + tk;
             if (!whole) {
                 const int64_t at = static_cast<int64_t>(slot) * f.group + qr;
                 if (c4 == 0) f.part_ml[at] = make_float2(mm, empty ? 0.0f : l == 0.0f ? -1.0f : l);
-                if (!empty) *reinterpret_cast<float4*>(f.part_o + at * HD + c4 * 4) = x;
+                if (!empty) *reinterpret_cast<float4*>(f.part_o + at * HD + c4 * 4) = v;
                 continue;
             }
             const float inv = empty ? 0.0f : 1.0f / l;
             bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(hd_) * HD + c4 * 4;
             if (a.vec_o) {
-                *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+                *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
             } else {
-                op[0] = f2bf(x.x * inv), op[1] = f2bf(x.y * inv), op[2] = f2bf(x.z * inv), op[3] = f2bf(x.w * inv);
+                op[0] = f2bf(v.x * inv), op[1] = f2bf(v.y * inv), op[2] = f2bf(v.z * inv), op[3] = f2bf(v.w * inv);
             }
             if (a.lse && c4 == 0) a.lse[t * a.H + hd_] = empty ? -INFINITY : log_sum(bs, l, a.c);
         }
@@ -559,7 +570,7 @@ int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * 
 bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
 
 int64_t few_workspace(int64_t B, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3) {
-    if (max_len <= kLeast * kStep) return 0;
+    if (max_len <= kWhole) return 0;
     return (2 * resident(head_dim, e4m3) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
 }
 

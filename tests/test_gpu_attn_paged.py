@@ -310,3 +310,18 @@ def test_e4m3_rows_of_very_different_size(dt, n, L):
     a = Call(small, 2, dt).run()
     a.check()
     assert (a.o[:n, :128] != 0).any()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("n,L", [(1, 511), (1, 512), (4, 513), (1, 700), (2, 1023), (1, 1024), (1, 1025), (40, 512), (33, 700), (200, 1300)])
+def test_workspaces_are_not_overrun(dt, cache, n, L):
+    """Around the lengths where the forms change: nothing behind the bytes asked for is written."""
+    p = Paged([n, 1], [L, L // 2], 1, 64, 24, cache, seed=L)
+    a = Call(p, 8, dt)
+    size = a.bytes()
+    ws = torch.full((size + (1 << 20),), 0xa5, dtype=torch.uint8, device="cuda")
+    c = p.struct()
+    call("aic_hip_attn_paged", c, ptr(a.q), a.ld, ptr(a.o), a.ld, ptr(a.lse), ptr(p.dev_offs), ptr(p.dev_lens), *a.sizes(), a.H, 0, a.scale,
+         ptr(ws), size, CODE[dt], stream())
+    a.check()
+    assert (ws[size:] == 0xa5).all()
