@@ -46,7 +46,8 @@ def _obj(src: str) -> str:
 FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_general.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-              "attention_paged_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+              "attention_paged_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "attention_paged_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src: str) -> tuple[str, int, str]:

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
     const int split = rest % a.nsplit;
     int b, local;
     if (!find_tile<128>(a, rest / a.nsplit, b, local)) return;
-    const Seq sq = sequence(a, b);
+    const Seq sq = wave_sequence(a, b);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
     const int rows = sq.n * a.G, r0 = local * 128, r = r0 + wave * 32 + (lane & 31);
     const bool real = r < rows;
@@ -383,8 +383,12 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     auto run = [&](auto t, auto ct, auto hd) {
         using X = decltype(t);
         constexpr int D = decltype(hd)::value;
-        attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-        AIC_LAUNCH_CHECK("attn_paged");
+        if constexpr (sizeof(X) == 2) {
+            attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
+        } else {
+            attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+            AIC_LAUNCH_CHECK("attn_paged");
+        }
         if (a.nsplit > 1) {
             const int64_t joins = (T * H + 3) / 4;
             AIC_CHECK(joins <= INT32_MAX, OutOfRange, "attn_paged: too many rows in one call");

@@ -53,6 +53,16 @@ __device__ __forceinline__ Seq sequence(const PagedArgs& a, int b) {
     return {lo, static_cast<int>(hi - lo), static_cast<int>(min(max(a.lens[b], int64_t{0}), kMaxLen))};
 }
 
+// The same for a b that is one for the whole wave, in scalar registers.
+__device__ __forceinline__ Seq wave_sequence(const PagedArgs& a, int b) {
+    const Seq x = sequence(a, b);
+    const uint64_t r = static_cast<uint64_t>(x.row0);
+    const uint32_t r_lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(r)));
+    const uint32_t r_hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(r >> 32)));
+    return {static_cast<int64_t>(static_cast<uint64_t>(r_hi) << 32 | r_lo), __builtin_amdgcn_readfirstlane(x.n),
+            __builtin_amdgcn_readfirstlane(x.len)};
+}
+
 // Tile `tile` of the batch cut into tiles of R query rows: its sequence and the tile's place in it.
 // Every wave finds it by itself: 64 sequences per step, their tile counts added up across lanes.
 template <int R>
@@ -237,5 +247,8 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const Rows<HD / 32
 bool few_rows(int64_t max_q, int64_t G);
 int64_t few_workspace(int64_t B, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3);
 void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s);
+
+// Many query rows per key/value head, bf16 queries (attention_paged_tiles.hip): `blocks` as attn_paged_k's.
+void attn_paged_tiles(const PagedArgs& a, bool e4m3, int head_dim, unsigned blocks, hipStream_t s);
 
 }  // namespace aic::hip

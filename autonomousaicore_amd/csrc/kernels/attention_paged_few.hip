@@ -51,9 +51,9 @@ struct Steps {
     Seq sq;
     int lo, steps, groups;  // first key (a multiple of kStep), steps over its keys, row groups
 };
-__device__ __forceinline__ Steps steps_of(const FewArgs& f, int b) {
+__device__ __forceinline__ Steps steps_of(const FewArgs& f, const Seq& sq) {
     Steps x;
-    x.sq = sequence(f.a, b);
+    x.sq = sq;
     const int first = max(x.sq.len - x.sq.n, 0);
     x.lo = f.a.window > 0 ? max(0, first - f.a.window + 1) & ~(kStep - 1) : 0;
     x.steps = max(1, (x.sq.len - x.lo + kStep - 1) / kStep);  // also of a sequence without keys: its rows are zeros
@@ -70,10 +70,10 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
     Steps own;  // the last of this thread's sequences: its only one in batches of up to 256
     auto steps = [&](int i) {
-        if (per > 1) own = steps_of(f, i);
+        if (per > 1) own = steps_of(f, sequence(f.a, i));
         return static_cast<double>(own.steps) * own.groups * f.a.kv.Hkv;
     };
-    if (first < last) own = steps_of(f, first);
+    if (first < last) own = steps_of(f, sequence(f.a, first));
     double mine = 0.0;  // whole numbers below 2^53
     for (int i = first; i < last; ++i) mine += steps(i);
     const double upto = wave_running_sum(mine);
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
         if (!find_share(f, static_cast<int>(blockIdx.x), b, x, before, count)) return;
     } else {
         b = static_cast<int>(blockIdx.x) / Hkv;
-        x = steps_of(f, b);
+        x = steps_of(f, wave_sequence(f.a, b));
         before = 0;
         count = INT64_MAX;
     }
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
         if (before >= groups * x.steps) {
             if (f.shares == 0) return;
             before -= groups * x.steps;
-            if (++b < a.B) x = steps_of(f, b);
+            if (++b < a.B) x = steps_of(f, wave_sequence(f.a, b));
             continue;
         }
         const int gi = static_cast<int>(before / x.steps), u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
     const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
     if (qr >= f.group) return;
     const int64_t share = f.plan[a.B], base_step = f.plan[b];
-    const Steps x = steps_of(f, b);
+    const Steps x = steps_of(f, wave_sequence(f.a, b));
     for (int g = 0; g < x.groups; ++g) {
         const int r = g * f.group + qr;
         if (r >= x.sq.n * a.G) return;
