@@ -23,70 +23,61 @@ namespace aic::hip {
 
 namespace {
 
-// ------------------------------------------------------------------- the general kernel
-// One block: 128 query rows (4 waves x 32) of one key/value head, over tiles of KT keys staged through
-// registers (the next tile's loads are in flight during this one's products).
-template <typename T, typename CT, int HD>
-__global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
-    constexpr int KT = sizeof(T) == 2 ? 64 : 32, JB = KT / 32, OB = HD / 32;
-    constexpr int UPR = HD * sizeof(CT) / 16;        // 16-byte units of a cached row
-    constexpr int NU = (KT * UPR + 255) / 256;       // units of a tile per thread
+// ----------------------------------------------------------------------- the fp32 kernel
+// Blocks of 4 waves x 32 query rows over tiles of 32 keys, or (SHARE) of 32 query rows over tiles of 128 keys that the
+// waves share, 32 each, their states joined at the end: four times as many blocks with a quarter of the
+// steps, for batches that do not fill the card with the first kind.  Tiles are staged through registers: the
+// next one's loads are in flight during this one's products.  Bound by the fp32 matrix pipe (64 cycles per
+// v_mfma_f32_32x32x2_f32).
+template <typename CT, int HD, bool SHARE>
+__global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
+    constexpr int R = SHARE ? 32 : 128, KT = SHARE ? 128 : 32, OB = HD / 32;
+    constexpr int UPR = HD * sizeof(CT) / 16;   // 16-byte units of a cached row
+    constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
     constexpr bool E4 = sizeof(CT) == 1;
-    __shared__ __attribute__((aligned(16))) char ks[KT * HD * sizeof(T)];
-    __shared__ __attribute__((aligned(16))) char vs[KT * HD * sizeof(T)];
+    constexpr int TILE = KT * HD * 4;
+    __shared__ __attribute__((aligned(16))) char tiles[2 * TILE];
+    char *ks = tiles, *vs = tiles + TILE;
 
     const int Hkv = a.kv.Hkv;
     const int kvh = static_cast<int>(blockIdx.x) % Hkv;
     const int rest = static_cast<int>(blockIdx.x) / Hkv;
     const int split = rest % a.nsplit;
     int b, local;
-    if (!find_tile<128>(a, rest / a.nsplit, b, local)) return;
+    if (!find_tile<R>(a, rest / a.nsplit, b, local)) return;
     const Seq sq = wave_sequence(a, b);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5;
-    const int rows = sq.n * a.G, r0 = local * 128, r = r0 + wave * 32 + (lane & 31);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+    const int sub = SHARE ? 32 * wave : 0;  // this wave's keys of a tile
+    const int rows = sq.n * a.G, r0 = local * R, r = r0 + (SHARE ? 0 : wave * 32) + (lane & 31);
     const bool real = r < rows;
     const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
     const int64_t t = sq.row0 + tok;
-    const int hi = real ? sq.len - sq.n + tok : -1;                    // last key this row sees
+    const int hi = real ? sq.len - sq.n + tok : -1;                       // last key this row sees
     const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;  // first
 
     // keys of the block: what its first row sees first .. what its last row sees last, of this split
-    const int first_pos = sq.len - sq.n + r0 / a.G, last_pos = sq.len - sq.n + (min(r0 + 128, rows) - 1) / a.G;
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int first_pos = same(sq.len - sq.n + r0 / a.G), last_pos = same(sq.len - sq.n + (min(r0 + R, rows) - 1) / a.G);
     int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
     if (a.chunk > 0) {
         k_lo = max(k_lo, split * a.chunk);
         if (split + 1 < a.nsplit) k_hi = min(k_hi, (split + 1) * a.chunk);
     }
-    k_lo &= ~(KT - 1);
+    k_lo &= ~31;
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));  // keys from lo on that it sees here
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;                          // of this split
 
     Rows<OB> st_;
     st_.init();
     if (k_lo < k_hi) {
-        // Q fragments: bf16 8 values at 16 kk + 8 h; fp32 4 values at 8 c + 4 h
-        constexpr int KS = HD / 16, KF = HD / 8;
-        [[maybe_unused]] bf16x8 qb[KS];
-        [[maybe_unused]] float4 qf[KF];
-        const T* qp = static_cast<const T*>(a.q) + t * a.ldq + static_cast<int64_t>(head) * HD;
-        if constexpr (sizeof(T) == 2) {
+        constexpr int KF = HD / 8;
+        float4 qf[KF];  // 4 values at 8 c + 4 h
+        const float* qp = static_cast<const float*>(a.q) + t * a.ldq + static_cast<int64_t>(head) * HD;
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + 16 * kk + 8 * hl, real));
-                else
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[16 * kk + 8 * hl + j] : f2bf(0.0f);
-            }
-        } else {
-#pragma unroll
-            for (int cc = 0; cc < KF; ++cc) {
-                const T* p = qp + 8 * cc + 4 * hl;
-                qf[cc] = !real ? make_float4(0, 0, 0, 0) : a.vec_q ? *reinterpret_cast<const float4*>(p)
-                                                                   : make_float4(p[0], p[1], p[2], p[3]);
-            }
+        for (int cc = 0; cc < KF; ++cc) {
+            const float* p = qp + 8 * cc + 4 * hl;
+            qf[cc] = !real ? make_float4(0, 0, 0, 0) : a.vec_q ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
         }
-        [[maybe_unused]] Frags<sizeof(T) == 2 ? HD : 32> F;
-        if constexpr (sizeof(T) == 2) F.init();
 
         uint4 rk[NU], rv[NU];
         [[maybe_unused]] uint32_t xk[NU], xv[NU];  // exponent bytes
@@ -110,124 +101,119 @@ __global__ __launch_bounds__(256) void attn_paged_k(PagedArgs a) {
         };
         auto put = [&](char* tile, int row, int c, uint4 x, [[maybe_unused]] uint32_t xe) {
             if constexpr (!E4) {
-                *reinterpret_cast<uint4*>(tile + chunk_at<T, HD>(row, c)) = x;
+                *reinterpret_cast<uint4*>(tile + chunk_at<float, HD>(row, c)) = x;
             } else {
                 const float s = exp_scale(xe);
                 const uint2 w[2] = {make_uint2(x.x, x.y), make_uint2(x.z, x.w)};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    if constexpr (sizeof(T) == 2) {
-                        *reinterpret_cast<uint4*>(tile + chunk_at<T, HD>(row, 2 * c + j)) = e4m3_bf16(w[j], s);
-                    } else {
-                        float y[8];
-                        e4m3_floats(w[j], s, y);
-                        *reinterpret_cast<float4*>(tile + chunk_at<T, HD>(row, 4 * c + 2 * j)) =
-                            make_float4(y[0], y[1], y[2], y[3]);
-                        *reinterpret_cast<float4*>(tile + chunk_at<T, HD>(row, 4 * c + 2 * j + 1)) =
-                            make_float4(y[4], y[5], y[6], y[7]);
-                    }
+                    float y[8];
+                    e4m3_floats(w[j], s, y);
+                    *reinterpret_cast<float4*>(tile + chunk_at<float, HD>(row, 4 * c + 2 * j)) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(tile + chunk_at<float, HD>(row, 4 * c + 2 * j + 1)) = make_float4(y[4], y[5], y[6], y[7]);
                 }
             }
         };
-        // this thread's part of the V tile in registers holds an infinity or NaN
-        auto bad_v = [&] {
+        auto bad_v = [&] {  // this thread's part of the V tile in registers holds an infinity or NaN
             bool bad = false;
 #pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                if constexpr (E4) {
-                    bad |= any_nan_code(rv[i]);
-                } else {
-                    bad |= any_non_finite<CT>(rv[i]);
-                }
-            }
+            for (int i = 0; i < NU; ++i) bad |= E4 ? any_nan_code(rv[i]) : any_non_finite<float>(rv[i]);
             return bad;
         };
 
         load(k_lo);
         for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
             // every row of the block sees every key of the tile?
-            const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi &&
-                              (a.window <= 0 || k0 > last_pos - a.window);
+            const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
             const int poison = __syncthreads_or(!open && bad_v());  // also: everyone is done with the last tile
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int u = i * 256 + static_cast<int>(threadIdx.x);
-                if (u < KT * UPR) {
+                if (KT * UPR % 256 == 0 || u < KT * UPR) {
                     put(ks, u / UPR, u % UPR, rk[i], E4 ? xk[i] : 0);
                     put(vs, u / UPR, u % UPR, rv[i], E4 ? xv[i] : 0);
                 }
             }
             __syncthreads();
             if (k0 + KT < k_hi) load(k0 + KT);
+            if (SHARE && k0 + sub >= k_hi) continue;  // nothing of this tile for this wave
 
-            f32x16 sc[JB];
+            f32x16 sc[1];
+            zero(sc[0]);
 #pragma unroll
-            for (int jb = 0; jb < JB; ++jb) {
-                zero(sc[jb]);
-                if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                    for (int kk = 0; kk < KS; ++kk)
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(ks, 32 * jb, kk), qb[kk], sc[jb], 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int cc = 0; cc < KF; ++cc) {
-                        const float4 x = *reinterpret_cast<const float4*>(
-                            ks + chunk_at<T, HD>(32 * jb + (lane & 31), 2 * cc + hl));
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, qf[cc].x, sc[jb], 0, 0, 0);
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, qf[cc].y, sc[jb], 0, 0, 0);
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, qf[cc].z, sc[jb], 0, 0, 0);
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, qf[cc].w, sc[jb], 0, 0, 0);
-                    }
-                }
+            for (int cc = 0; cc < KF; ++cc) {
+                const float4 x = *reinterpret_cast<const float4*>(ks + chunk_at<float, HD>(sub + (lane & 31), 2 * cc + hl));
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, qf[cc].x, sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, qf[cc].y, sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, qf[cc].z, sc[0], 0, 0, 0);
+                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, qf[cc].w, sc[0], 0, 0, 0);
             }
-            auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
+            auto seen = [&](int j) { return static_cast<uint32_t>(k0 + sub + j - lo) < span; };
             if (!open)
 #pragma unroll
-                for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        sc[jb][e] = seen(32 * jb + 8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[jb][e] : -INFINITY;
+                for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
             float mx = -INFINITY;
 #pragma unroll
-            for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[jb][e]);
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
             st_.absorb(mx, a.c);
             const float off = st_.offset(a.c);
             float sum = 0.0f;
 #pragma unroll
-            for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[jb][e] = weight<T>(sc[jb][e], a.c, off);
-                    sum += sc[jb][e];
-                }
+            for (int e = 0; e < 16; ++e) {
+                sc[0][e] = weight<float>(sc[0][e], a.c, off);
+                sum += sc[0][e];
+            }
             st_.add(sum);
             if (poison) {
-                add_seen_rows<HD, JB>(st_.o, sc, [&](int key, int d) { return v4_at<T, HD>(vs, key, d); }, seen);
-            } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                for (int s = 0; s < KT / 16; ++s) {
-                    const bf16x8 p = pack_bf16x8(sc[s >> 1], 8 * (s & 1));
-#pragma unroll
-                    for (int ob = 0; ob < OB; ++ob)
-                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.tr(vs, ob, s), p, st_.o[ob], 0, 0, 0);
-                }
+                add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<float, HD>(vs, sub + key, d); }, seen);
             } else {
 #pragma unroll
-                for (int jb = 0; jb < JB; ++jb)
+                for (int e = 0; e < 16; ++e)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-#pragma unroll
-                        for (int ob = 0; ob < OB; ++ob) {
-                            const int d = 32 * ob + (lane & 31), row = 32 * jb + 8 * (e >> 2) + 4 * hl + (e & 3);
-                            const float x = *reinterpret_cast<const float*>(vs + chunk_at<T, HD>(row, d >> 2) + (d & 3) * 4);
-                            st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, sc[jb][e], st_.o[ob], 0, 0, 0);
-                        }
+                    for (int ob = 0; ob < OB; ++ob) {
+                        const int d = 32 * ob + (lane & 31), row = sub + 8 * (e >> 2) + 4 * hl + (e & 3);
+                        const float x = *reinterpret_cast<const float*>(vs + chunk_at<float, HD>(row, d >> 2) + (d & 3) * 4);
+                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, sc[0][e], st_.o[ob], 0, 0, 0);
+                    }
             }
         }
     }
-    if (real) store_row<T, HD>(a, st_, t, head, empty, split);
+    if constexpr (SHARE) {
+        // wave 0 takes the others' states: M = max m_w, o = sum 2^((m_w - M) c) o_w, l alike
+        float* os = reinterpret_cast<float*>(tiles);
+        __shared__ float2 mls[4][32];
+        __syncthreads();  // the tiles have been read
+        if (hl == 0) mls[wave][lane] = make_float2(st_.m, st_.l);
+        __syncthreads();
+        float M = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][lane & 31].x);
+        const float base = M == -INFINITY ? 0.0f : M;
+        const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 ml = mls[w][lane & 31];
+            l = fmaf(__builtin_amdgcn_exp2f((ml.x - base) * a.c), ml.y, l);
+        }
+#pragma unroll
+        for (int ob = 0; ob < OB; ++ob)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                st_.o[ob][e] *= factor;
+                if (wave > 0) os[((wave - 1) * OB * 16 + ob * 16 + e) * 64 + lane] = st_.o[ob][e];
+            }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int ob = 0; ob < OB; ++ob)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+#pragma unroll
+                for (int w = 0; w < 3; ++w) st_.o[ob][e] += os[(w * OB * 16 + ob * 16 + e) * 64 + lane];
+        st_.m = M;
+        st_.l = l;
+    }
+    if (real) store_row<float, HD>(a, st_, t, head, empty, split);
 }
 
 // ------------------------------------------------------------------------- joining splits
@@ -288,8 +274,9 @@ struct Plan {
     int64_t tiles, nsplit, chunk;
 };
 // Splits over the keys where the query tiles alone do not fill the card: equal chunks of a multiple of 128 keys.
-Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv) {
-    Plan p{tile_bound(T, H / Hkv, B, 128), 1, 0};
+// R: query rows of a block.
+Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t R) {
+    Plan p{tile_bound(T, H / Hkv, B, R), 1, 0};
     const int64_t blocks = std::max<int64_t>(1, p.tiles * Hkv);
     const int64_t want = std::min({(512 + blocks - 1) / blocks, max_len / 256, kMaxSplits});  // blocks wanted, keys of a split at least
     if (want > 1) {
@@ -299,6 +286,8 @@ Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv) {
     }
     return p;
 }
+// fp32: blocks of 32 rows where blocks of 128 rows are fewer than two per CU.
+int64_t f32_rows(int64_t B, int64_t T, int64_t H, int64_t Hkv) { return tile_bound(T, H / Hkv, B, 128) * Hkv < 512 ? 32 : 128; }
 int64_t plan_bytes(const Plan& p, int64_t T, int64_t H, int64_t hd) {
     return p.nsplit <= 1 ? 0 : p.nsplit * T * H * (hd + 2) * 4;
 }
@@ -322,8 +311,10 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     const int64_t G = H / c.kv_heads;
     if (c.type != DType::Float32 && few_rows(max_q, G))
         n = few_workspace(B, max_q, max_len, G, c.head_dim, c.type == DType::UInt8);
-    if (c.type != DType::BFloat16 || !few_rows(max_q, G))
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads), T, H, c.head_dim));
+    if (c.type != DType::Float32 && !few_rows(max_q, G))
+        n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
+    if (c.type != DType::BFloat16)
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, H, c.kv_heads)), T, H, c.head_dim));
     return n;
 }
 
@@ -356,7 +347,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
     const bool few = dt == DType::BFloat16 && few_rows(max_q, a.G);
-    Plan p = plan(B, T, max_len, H, c.kv_heads);
+    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, H, c.kv_heads);
+    Plan p = plan(B, T, max_len, H, c.kv_heads, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
     if (workspace)
@@ -386,7 +378,9 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         if constexpr (sizeof(X) == 2) {
             attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
         } else {
-            attn_paged_k<X, decltype(ct), D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+            const auto grid = static_cast<unsigned>(blocks);
+            if (R == 32) attn_paged_f32_k<decltype(ct), D, true><<<grid, 256, 0, s>>>(a);
+            else attn_paged_f32_k<decltype(ct), D, false><<<grid, 256, 0, s>>>(a);
             AIC_LAUNCH_CHECK("attn_paged");
         }
         if (a.nsplit > 1) {

@@ -325,3 +325,34 @@ def test_workspaces_are_not_overrun(dt, cache, n, L):
          ptr(ws), size, CODE[dt], stream())
     a.check()
     assert (ws[size:] == 0xa5).all()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("n,L,ps", [(1, 1500, 1), (40, 1500, 1), (2, 4000, 3), (70, 4000, 3), (1, 2100, 65536), (40, 700, 65536), (1, 1900, 17)])
+def test_page_ids_of_long_caches(dt, cache, n, L, ps):
+    """More pages than their ids' place in the kernels holds at a time, and one page larger than the cache."""
+    p = Paged([n], [L], 1, 32, ps, cache, seed=ps)
+    Call(p, 2, dt).run().check()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("ns,lens,window", [([300, 17], [1500, 900], 0), ([300, 17], [1500, 900], 400), ([130], [1000], 65), ([257], [257], 0)])
+@pytest.mark.parametrize("H,Hkv,hd,ps", [(4, 2, 128, 16), (3, 3, 64, 24)])
+def test_chunks_of_long_prompts(dt, cache, ns, lens, window, H, Hkv, hd, ps):
+    """Several query tiles and many tiles of keys that every row sees whole, between masked ones."""
+    p = Paged(ns, lens, Hkv, hd, ps, cache, seed=hd + window)
+    Call(p, H, dt, window).run().check()
+
+
+@pytest.mark.parametrize("dt,cache", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "e4m3")])
+def test_many_rows_and_heads_fill_the_card(dt, cache):
+    """Enough blocks that nothing is split: 700 rows of 32 heads."""
+    p = Paged([600, 100], [600, 150], 16, 32, 16, cache, seed=1)
+    a = Call(p, 32, dt, with_lse=False).run()
+    q = a.q[:, :a.w].double().cpu().numpy().reshape(a.T, 32, 32)
+    some = Paged.__new__(Paged)  # every eighth head against the definition
+    some.__dict__.update(p.__dict__)
+    for h in range(0, 32, 8):
+        some.k, some.v, some.Hkv = p.k[:, h // 2:h // 2 + 1], p.v[:, h // 2:h // 2 + 1], 1
+        got = host(a.o.contiguous()).reshape(a.T, 32, 32)[:, h:h + 1]
+        check_attention(got, None, some, q[:, h:h + 1], 1, 0, a.scale, dt)
