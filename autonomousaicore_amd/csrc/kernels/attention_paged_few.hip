@@ -11,7 +11,9 @@
 // are resident at once, so that batches of uneven lengths end together; a group that a cut divides leaves
 // its parts' states in the workspace and attn_paged_few_join_k adds them.  (Equal splits per
 // sequence ran in one and a half rounds of blocks: 28.7 us at best and 40 us at worst for 32 e4m3 caches of up to
-// 8000 tokens, by the number of splits.)  Every block finds its part from offsets and lens by itself.
+// 8000 tokens, by the number of splits.)  Where the groups are few, each is cut by itself into parts of nearly
+// a share: a block that ends one group and begins another waits twice for its first tile, which is then
+// most of its time.  Every block finds its part from offsets and lens by itself.
 //
 // Tiles arrive by direct global -> LDS copies, two stages per wave: 32 KB per wave at head_dim 128 in bf16 (one
 // block and up to 128 KB in flight per CU), 16 KB in e4m3 (two blocks).
@@ -42,7 +44,7 @@ struct FewArgs {
     PagedArgs a;
     int group;         // query rows of a group, at most 32
     int shares;        // 0: a block per sequence and key/value head, nothing divided
-    int64_t* plan;     // [B + 1]: steps before each sequence, and a share's steps
+    int64_t* plan;     // [B + 1], as find_share leaves it
     float2* part_ml;   // [2 shares][group]: a share's first group's, then its last one's
     float* part_o;     // [2 shares][group][hd]
 };
@@ -60,61 +62,90 @@ __device__ __forceinline__ Steps steps_of(const FewArgs& f, const Seq& sq) {
     x.groups = (x.sq.n * f.a.G + f.group - 1) / f.group;
     return x;
 }
-// The share of block g: sequence and steps before its begin there.  False: no steps are left for it.
+// Parts of a group of `steps` steps that is cut by itself.
+__device__ __forceinline__ int parts_of(int steps, int64_t share) {
+    return share >= steps ? 1 : (steps + static_cast<int>(share) - 1) / static_cast<int>(share);
+}
+// Whole numbers below 2^53, added over the block's threads: what comes before each, and all of them.
+__device__ __forceinline__ void block_scan(double mine, double (&sums)[4], double& before, double& total) {
+    const int wave = threadIdx.x >> 6;
+    const double upto = wave_running_sum(mine);
+    if ((threadIdx.x & 63) == 63) sums[wave] = upto;
+    __syncthreads();
+    before = upto - mine;
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        before += w < wave ? sums[w] : 0.0;
+        total += sums[w];
+    }
+}
+// The part of block g: its sequence, the steps before it there and its own.  False: nothing is left for it.
+// plan: for each sequence the steps (or, where groups are cut by themselves, the blocks) before it; behind
+// them a share's steps, negative in the second case.
 __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Steps& x, int64_t& before, int64_t& count) {
-    __shared__ double sums[4];
+    __shared__ double sums[2][4], pair_sums[4];
     __shared__ int at_b;
     __shared__ Steps at_x;
     __shared__ int64_t at_before;
-    const int per = (f.a.B + 255) / 256, tid = threadIdx.x, wave = tid >> 6;
+    const int per = (f.a.B + 255) / 256, tid = threadIdx.x;
     const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
     Steps own;  // the last of this thread's sequences: its only one in batches of up to 256
-    auto steps = [&](int i) {
-        if (per > 1) own = steps_of(f, sequence(f.a, i));
-        return static_cast<double>(own.steps) * own.groups * f.a.kv.Hkv;
-    };
     if (first < last) own = steps_of(f, sequence(f.a, first));
-    double mine = 0.0;  // whole numbers below 2^53
-    for (int i = first; i < last; ++i) mine += steps(i);
-    const double upto = wave_running_sum(mine);
-    if ((tid & 63) == 63) sums[wave] = upto;
-    __syncthreads();
-    double start = upto - mine, total = 0.0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) start += sums[w];
-        total += sums[w];
+    auto load = [&](int i) {
+        if (per > 1) own = steps_of(f, sequence(f.a, i));
+    };
+    auto groups = [&] { return static_cast<double>(own.groups) * f.a.kv.Hkv; };
+    double mine = 0.0, mine_pairs = 0.0, start, pairs_start, total, pairs;
+    for (int i = first; i < last; ++i) {
+        load(i);
+        mine += own.steps * groups();
+        mine_pairs += groups();
     }
-    const int64_t share = max(static_cast<int64_t>(kLeast), (static_cast<int64_t>(total) + f.shares - 1) / f.shares);
-    const int64_t begin = g * share;
-    if (g == 0) {
-        double s = start;
+    block_scan(mine_pairs, pair_sums, pairs_start, pairs);
+    block_scan(mine, sums[0], start, total);
+    const bool by_group = pairs * 4 <= f.shares;
+    const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
+    const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
+    auto size = [&] { return (by_group ? parts_of(own.steps, share) : own.steps) * groups(); };
+    if (by_group) {
+        mine = 0.0;
         for (int i = first; i < last; ++i) {
-            f.plan[i] = static_cast<int64_t>(s);
-            s += steps(i);
+            load(i);
+            mine += size();
         }
-        if (tid == 0) f.plan[f.a.B] = share;
+        block_scan(mine, sums[1], start, total);
     }
-    if (begin >= static_cast<int64_t>(total)) return false;
-    if (begin >= static_cast<int64_t>(start) && begin < static_cast<int64_t>(start + mine)) {
-        double s = start;
-        for (int i = first; i < last; ++i) {
-            const double n = steps(i);
-            if (begin < static_cast<int64_t>(s + n)) {
-                at_b = i;
-                at_x = own;
-                at_before = begin - static_cast<int64_t>(s);
-                break;
-            }
-            s += n;
+    const double begin = by_group ? g : static_cast<double>(g) * share;
+    double s = start;
+    for (int i = first; i < last; ++i) {
+        load(i);
+        const double n = size();
+        if (g == 0) f.plan[i] = static_cast<int64_t>(s);
+        if (begin >= s && begin < s + n) {
+            at_b = i;
+            at_x = own;
+            at_before = static_cast<int64_t>(begin - s);
         }
+        s += n;
     }
+    if (g == 0 && tid == 0) f.plan[f.a.B] = by_group ? -share : share;
+    if (begin >= total) return false;
     __syncthreads();
     auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     b = same(at_b);
     x.sq = {at_x.sq.row0, same(at_x.sq.n), same(at_x.sq.len)};
     x.lo = same(at_x.lo), x.steps = same(at_x.steps), x.groups = same(at_x.groups);
-    before = at_before;
-    count = min(share, static_cast<int64_t>(total) - begin);
+    if (by_group) {
+        const int part = same(static_cast<int>(at_before)), n = parts_of(x.steps, share);
+        const int gi = same(part / n), i = part - gi * n;
+        const int u0 = same(static_cast<int>(static_cast<int64_t>(x.steps) * i / n)), u1 = same(static_cast<int>(static_cast<int64_t>(x.steps) * (i + 1) / n));
+        before = static_cast<int64_t>(gi) * x.steps + u0;
+        count = u1 - u0;
+    } else {
+        before = at_before;
+        count = min(share, static_cast<int64_t>(total - begin));
+    }
     return true;
 }
 
@@ -218,7 +249,10 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
             if (++b < a.B) x = steps_of(f, wave_sequence(f.a, b));
             continue;
         }
-        const int gi = static_cast<int>(before / x.steps), u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
+        // (a 64-bit division takes a microsecond's worth of instructions)
+        const int gi = before >> 31 ? static_cast<int>(before / x.steps)
+                                    : __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(before) / static_cast<uint32_t>(x.steps)));
+        const int u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
         const int u1 = static_cast<int>(min(static_cast<int64_t>(x.steps), u0 + min(count, int64_t{1} << 30)));
         const int kvh = f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv, r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
         const bool whole = u0 == 0 && u1 == x.steps;
@@ -476,19 +510,27 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
     const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv;
     const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
     if (qr >= f.group) return;
-    const int64_t share = f.plan[a.B], base_step = f.plan[b];
+    const int64_t planned = f.plan[a.B], share = planned < 0 ? -planned : planned, base_step = f.plan[b];
+    const bool by_group = planned < 0;
     const Steps x = steps_of(f, wave_sequence(f.a, b));
     for (int g = 0; g < x.groups; ++g) {
         const int r = g * f.group + qr;
         if (r >= x.sq.n * a.G) return;
-        const int64_t from = base_step + (static_cast<int64_t>(g) * Hkv + kvh) * x.steps;
-        const int s0 = static_cast<int>(from / share), s1 = static_cast<int>((from + x.steps - 1) / share);
-        if (s0 == s1) continue;  // undivided: written already
-        // part i of the group: share s0 + i, where it is the first group unless it starts behind the share's begin
-        auto at = [&](int i) {
-            return (static_cast<int64_t>(2) * (s0 + i) + (i == 0 && from != s0 * share ? 1 : 0)) * f.group + qr;
-        };
-        const int parts = s1 - s0 + 1;
+        // the group's first block and its parts; a block's second slot holds a group that begins behind its own begin
+        const int64_t group = static_cast<int64_t>(g) * Hkv + kvh;
+        int64_t s0;
+        int parts, first_slot = 0;
+        if (by_group) {
+            parts = parts_of(x.steps, share);
+            s0 = base_step + group * parts;
+        } else {
+            const int64_t from = base_step + group * x.steps;
+            s0 = from / share;
+            parts = static_cast<int>((from + x.steps - 1) / share - s0) + 1;
+            first_slot = from != s0 * share;
+        }
+        if (parts == 1) continue;  // undivided: written already
+        auto at = [&](int i) { return (2 * (s0 + i) + (i == 0 ? first_slot : 0)) * f.group + qr; };
         float M = -INFINITY;
         bool any = false;
         for (int i = lane; i < parts; i += 64) {
