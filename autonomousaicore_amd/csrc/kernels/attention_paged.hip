@@ -42,9 +42,9 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     const int Hkv = a.kv.Hkv;
     const int kvh = static_cast<int>(blockIdx.x) % Hkv;
     const int rest = static_cast<int>(blockIdx.x) / Hkv;
-    const int split = rest % a.nsplit;
+    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
-    if (!find_tile<R>(a, rest / a.nsplit, b, local)) return;
+    if (!find_tile<R>(a, tile, b, local)) return;
     const Seq sq = wave_sequence(a, b);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
     const int sub = SHARE ? 32 * wave : 0;  // this wave's keys of a tile
@@ -59,11 +59,8 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     const int first_pos = same(sq.len - sq.n + r0 / a.G), last_pos = same(sq.len - sq.n + (min(r0 + R, rows) - 1) / a.G);
     int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
-    if (a.chunk > 0) {
-        k_lo = max(k_lo, split * a.chunk);
-        if (split + 1 < a.nsplit) k_hi = min(k_hi, (split + 1) * a.chunk);
-    }
-    k_lo &= ~31;
+    k_lo &= ~63;
+    part_of_keys(k_lo, k_hi, split, a.nsplit);
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));  // keys from lo on that it sees here
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;                          // of this split
 
@@ -115,10 +112,10 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
             }
         };
         auto bad_v = [&] {  // this thread's part of the V tile in registers holds an infinity or NaN
-            bool bad = false;
+            uint32_t bad = 0;
 #pragma unroll
-            for (int i = 0; i < NU; ++i) bad |= E4 ? any_nan_code(rv[i]) : any_non_finite<float>(rv[i]);
-            return bad;
+            for (int i = 0; i < NU; ++i) bad |= non_finite_bits<CT>(rv[i]);
+            return bad != 0;
         };
 
         load(k_lo);
@@ -271,19 +268,13 @@ int64_t tile_bound(int64_t T, int64_t G, int64_t B, int64_t R) { return T * G / 
 
 constexpr int64_t kMaxSplits = 64;  // a wave joins them, a lane each
 struct Plan {
-    int64_t tiles, nsplit, chunk;
+    int64_t tiles, nsplit;
 };
-// Splits over the keys where the query tiles alone do not fill the card: equal chunks of a multiple of 128 keys.
-// R: query rows of a block.
+// Parts of the keys where the query tiles alone do not fill the card.  R: query rows of a block.
 Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t R) {
-    Plan p{tile_bound(T, H / Hkv, B, R), 1, 0};
+    Plan p{tile_bound(T, H / Hkv, B, R), 1};
     const int64_t blocks = std::max<int64_t>(1, p.tiles * Hkv);
-    const int64_t want = std::min({(512 + blocks - 1) / blocks, max_len / 256, kMaxSplits});  // blocks wanted, keys of a split at least
-    if (want > 1) {
-        p.chunk = ((max_len + want - 1) / want + 127) / 128 * 128;
-        p.nsplit = (max_len + p.chunk - 1) / p.chunk;
-        if (p.nsplit <= 1) p.nsplit = 1, p.chunk = 0;
-    }
+    p.nsplit = std::max<int64_t>(1, std::min({(512 + blocks - 1) / blocks, max_len / 256, kMaxSplits}));  // blocks wanted, keys of a part
     return p;
 }
 // fp32: blocks of 32 rows where blocks of 128 rows are fewer than two per CU.
@@ -363,9 +354,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         attn_paged_few(a, max_q, e4m3, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;
     }
-    if (!workspace) p.nsplit = 1, p.chunk = 0;  // nothing to split, or captured without a workspace of its own
+    if (!workspace) p.nsplit = 1;  // nothing to split, or captured without a workspace of its own
     a.nsplit = static_cast<int>(p.nsplit);
-    a.chunk = static_cast<int>(p.chunk);
     if (p.nsplit > 1) {
         a.part_o = static_cast<float*>(workspace);
         a.part_ml = reinterpret_cast<float2*>(a.part_o + p.nsplit * T * H * c.head_dim);

@@ -17,8 +17,7 @@ struct PagedArgs {
     const int64_t *offsets, *lens;
     int B, H, G, window;
     float c;         // scale in log2 units
-    int chunk;       // keys of one split (0: one split over all of them)
-    int nsplit;
+    int nsplit;      // parts of a tile's keys, a block each
     float2* part_ml;  // [nsplit][T][H]: maximum, sum (-1: only scores of -infinity)
     float* part_o;    // [nsplit][T][H][hd]
     bool vec_q, vec_o;
@@ -89,6 +88,16 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& a, int tile, int& b, 
     return false;
 }
 
+// The keys [k_lo, k_hi) of part `split` of a query tile's, k_lo a multiple of 64: equal parts of whole tiles of 64, by
+// the tile's own range, so that the parts of one tile end together.
+__device__ __forceinline__ void part_of_keys(int& k_lo, int& k_hi, int split, int nsplit) {
+    if (nsplit == 1 || k_hi <= k_lo) return;
+    const uint32_t n = static_cast<uint32_t>(k_hi - k_lo + 63) / 64;
+    const int lo = k_lo;
+    k_lo = lo + 64 * static_cast<int>(n * static_cast<uint32_t>(split) / static_cast<uint32_t>(nsplit));
+    if (split + 1 < nsplit) k_hi = lo + 64 * static_cast<int>(n * static_cast<uint32_t>(split + 1) / static_cast<uint32_t>(nsplit));
+}
+
 // ------------------------------------------------------------------------------- tiles
 // [KT][HD] tiles of T in LDS, 16-byte chunks swizzled per row.
 template <typename T, int HD>
@@ -98,30 +107,38 @@ __device__ __forceinline__ int chunk_at(int row, int ch) {
     else return row * HD * 4 + ((ch ^ (HD == 32 ? (row >> 1) & 7 : row & 15)) << 4);
 }
 
-template <typename CT> __device__ __forceinline__ bool any_non_finite(uint4 x);
-template <> __device__ __forceinline__ bool any_non_finite<bf16>(uint4 x) {
-    bool bad = false;
+// Non-zero where one of 16 bytes' elements is an infinity or NaN; a zero field of (x ^ pattern) borrows into its
+// top bit.
+template <typename CT> __device__ __forceinline__ uint32_t non_finite_bits(uint4 x);
+template <> __device__ __forceinline__ uint32_t non_finite_bits<bf16>(uint4 x) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u || (w[i] & 0x7f80u) == 0x7f80u;
-    return bad;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = (w[i] & 0x7f807f80u) ^ 0x7f807f80u;
+        bits |= (t - 0x00010001u) & ~t & 0x80008000u;
+    }
+    return bits;
 }
-template <> __device__ __forceinline__ bool any_non_finite<float>(uint4 x) {
+template <> __device__ __forceinline__ uint32_t non_finite_bits<float>(uint4 x) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    bool bad = false;
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
-    return bad;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = (w[i] & 0x7f800000u) ^ 0x7f800000u;
+        bits |= (t - 1u) & ~t & 0x80000000u;
+    }
+    return bits;
 }
-
-__device__ __forceinline__ bool any_nan_code(uint4 x) {
-    bool bad = false;
+template <> __device__ __forceinline__ uint32_t non_finite_bits<uint8_t>(uint4 x) {  // e4m3: NaN
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int by = 0; by < 4; ++by) bad |= ((w[i] >> (8 * by)) & 0x7fu) == 0x7fu;
-    return bad;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = (w[i] & 0x7f7f7f7fu) ^ 0x7f7f7f7fu;
+        bits |= (t - 0x01010101u) & ~t & 0x80808080u;
+    }
+    return bits;
 }
 
 // The four V values at columns d0 .. d0+3 of a tile's row.

@@ -321,14 +321,11 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 if (!open) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
-                    bool bad = false;  // a hidden key and a non-finite v
+                    uint32_t bits = 0;  // a hidden key and a non-finite v
 #pragma unroll
-                    for (int i = 0; i < L::TILE / 1024; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16);
-                        if constexpr (E4) bad |= any_nan_code(x);
-                        else bad |= any_non_finite<bf16>(x);
-                    }
-                    one_by_one |= __any(bad);
+                    for (int i = 0; i < L::TILE / 1024; ++i)
+                        bits |= non_finite_bits<std::conditional_t<E4, uint8_t, bf16>>(*reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16));
+                    one_by_one |= __any(bits != 0) != 0;
                 }
                 float mx = -INFINITY;
 #pragma unroll

@@ -39,9 +39,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
     const int kvh = static_cast<int>(blockIdx.x) % Hkv, rest = static_cast<int>(blockIdx.x) / Hkv;
-    const int split = rest % a.nsplit;
+    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
-    if (!find_tile<128>(a, rest / a.nsplit, b, local)) return;
+    if (!find_tile<128>(a, tile, b, local)) return;
     const Seq sq = wave_sequence(a, b);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
     const int rows = sq.n * a.G, r0 = local * 128, r = r0 + wave * 32 + (lane & 31);
@@ -53,11 +53,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
     auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // divisions leave uniform values in vector registers
     const int first_pos = same(sq.len - sq.n + r0 / a.G), last_pos = same(sq.len - sq.n + (min(r0 + 128, rows) - 1) / a.G);
     int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
-    if (a.chunk > 0) {
-        k_lo = max(k_lo, split * a.chunk);
-        if (split + 1 < a.nsplit) k_hi = min(k_hi, (split + 1) * a.chunk);
-    }
     k_lo &= ~63;
+    part_of_keys(k_lo, k_hi, split, a.nsplit);
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;
 
@@ -182,11 +179,11 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                 const int k0 = w0 + 64 * plain_tile(i);
                 auto seen = [&](int k) { return static_cast<uint32_t>(k0 + k - lo) < span; };
                 f32x16 sc[2];
-                bool bad = false;  // a non-finite v beside a hidden key
-#pragma unroll 2
+                uint32_t bits = 0;
+#pragma unroll 4
                 for (int j = 0; j < TILE * 2 / 1024; ++j)
-                    bad |= any_non_finite<bf16>(*reinterpret_cast<const uint4*>(Vb + j * 1024 + lane * 16));
-                bad = __any(bad);
+                    bits |= non_finite_bits<bf16>(*reinterpret_cast<const uint4*>(Vb + j * 1024 + lane * 16));
+                const bool bad = __any(bits != 0);  // a non-finite v beside a hidden key
                 float mx = -INFINITY;
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb) {
@@ -242,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                 if (t + 1 < t_b) put(ck, sm[st]);
                 put(cv, sm[st] + TILE);
             };
-            f32x16 sc[2], sn[2];  // scores of tile t, then its weights; scores of tile t + 1
+            f32x16 s0[2], s1[2];  // scores of tile t, then its weights, and scores of tile t + 1: in turn
             if constexpr (E4) {
                 fetch(a.kv.kp, a.kv.ke, t_a, ck);
                 put(ck, sm[0]);
@@ -258,18 +255,18 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             __builtin_amdgcn_s_barrier();
             {
                 const char* Kb = reinterpret_cast<const char*>(sm[0]);
-                zero(sc[0]);
-                zero(sc[1]);
+                zero(s0[0]);
+                zero(s0[1]);
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
                     for (int jb = 0; jb < 2; ++jb)
-                        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(Kb, jb * 32, kk), qf[kk], sc[jb], 0, 0, 0);
+                        s0[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(Kb, jb * 32, kk), qf[kk], s0[jb], 0, 0, 0);
                 float mx = -INFINITY;
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[jb][e]);
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s0[jb][e]);
                 st_.absorb(mx, a.c);
             }
             wait_lds();
@@ -284,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             }
 
             // One iteration.  HN: tile t + 1 exists.
-            auto iter = [&](int t, auto hn) {
+            auto iter = [&](int t, auto hn, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
                 constexpr bool HN = decltype(hn)::value;
                 const int st = (t - t_a + 1) & 1;
                 const char* Kb = reinterpret_cast<const char*>(sm[st]);
@@ -329,11 +326,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     if (f + OB < NB) rd_v(f + OB);
                     if constexpr (HN) {
 #pragma unroll
-                        for (int x = f * EB; x < (f + 1) * EB; ++x) {
-                            const int jb = x >> 4, e = x & 15;
-                            sc[jb][e] = sn[jb][e];
-                            mx = fmaxf(mx, sn[jb][e]);
-                        }
+                        for (int x = f * EB; x < (f + 1) * EB; ++x) mx = fmaxf(mx, sn[x >> 4][x & 15]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -350,9 +343,19 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     }
                 }
             };
+            using T1 = std::true_type;
+            using F0 = std::false_type;
             int t = t_a;
-            for (; t + 1 < t_b; ++t) iter(t, std::true_type{});
-            iter(t, std::false_type{});
+            for (; t + 2 < t_b; t += 2) {
+                iter(t, T1{}, s0, s1);
+                iter(t + 1, T1{}, s1, s0);
+            }
+            if (t + 1 < t_b) {
+                iter(t, T1{}, s0, s1);
+                iter(t + 1, F0{}, s1, s0);
+            } else {
+                iter(t, F0{}, s0, s1);
+            }
         }
     }
     if (real) store_row<bf16, HD>(a, st_, trow, head, empty, split);
