@@ -270,11 +270,15 @@ constexpr int64_t kMaxSplits = 64;  // a wave joins them, a lane each
 struct Plan {
     int64_t tiles, nsplit;
 };
-// Parts of the keys where the query tiles alone do not fill the card.  R: query rows of a block.
+// Parts of the keys where the query tiles alone do not fill the card: as many as make one round of about 512 blocks (two
+// per CU; 2048 rows of 16 heads twice: 52.6 us in 464 blocks, 73.6 us in 928), of at least 448 keys where
+// there are more than four (256 rows on 4096 keys: 26.2 us in 8 parts, 30.5 us in 16, 33.0 us in 4).
+// R: query rows of a block.
 Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t R) {
     Plan p{tile_bound(T, H / Hkv, B, R), 1};
-    const int64_t blocks = std::max<int64_t>(1, p.tiles * Hkv);
-    p.nsplit = std::max<int64_t>(1, std::min({(512 + blocks - 1) / blocks, max_len / 256, kMaxSplits}));  // blocks wanted, keys of a part
+    const int64_t twice = (2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;  // two times the blocks there probably are
+    const int64_t most = std::max<int64_t>(std::min<int64_t>(4, max_len / 256), max_len / 448);
+    p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
 // fp32: blocks of 32 rows where blocks of 128 rows are fewer than two per CU.

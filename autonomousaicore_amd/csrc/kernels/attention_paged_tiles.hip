@@ -135,17 +135,18 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     c.e[i] = row >= 0 ? exps[row] : 127;
                 }
             };
+            auto put_unit = [&](const Codes& c, int i, bf16* dst) {
+                const int u = i * 256 + static_cast<int>(threadIdx.x);
+                if (UNITS % 256 != 0 && u >= UNITS) return;
+                const float s = exp_scale(c.e[i]);
+                char* tile = reinterpret_cast<char*>(dst);
+                const int rr = u / UPR, ch = 2 * (u % UPR);
+                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch)) = e4m3_bf16(make_uint2(c.w[i].x, c.w[i].y), s);
+                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + 1)) = e4m3_bf16(make_uint2(c.w[i].z, c.w[i].w), s);
+            };
             auto put = [&](const Codes& c, bf16* dst) {
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    const int u = i * 256 + static_cast<int>(threadIdx.x);
-                    if (UNITS % 256 != 0 && u >= UNITS) break;
-                    const float s = exp_scale(c.e[i]);
-                    char* tile = reinterpret_cast<char*>(dst);
-                    const int rr = u / UPR, ch = 2 * (u % UPR);
-                    *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch)) = e4m3_bf16(make_uint2(c.w[i].x, c.w[i].y), s);
-                    *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + 1)) = e4m3_bf16(make_uint2(c.w[i].z, c.w[i].w), s);
-                }
+                for (int i = 0; i < NU; ++i) put_unit(c, i, dst);
             };
             [[maybe_unused]] Codes ck, cv;  // the next unit's
             // tiles [t_a, t_b): every row sees every key
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             __builtin_amdgcn_s_barrier();  // the stages are free
 
             // The pipelined loop over tiles t_a .. t_b - 1; stage of unit t: (t - t_a + 1) & 1
-            // unit t on its way (bf16: into stage st; e4m3: to registers), and e4m3's codes into stage st
+            // unit t on its way (bf16: into stage st; e4m3: to registers, into the stage by iteration t - 1)
             auto begin = [&](int t, [[maybe_unused]] int st) {
                 if constexpr (E4) {
                     if (t + 1 < t_b) fetch(a.kv.kp, a.kv.ke, t + 1, ck);
@@ -235,16 +236,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     copy(a.kv.vp, t, sm[st] + TILE);
                 }
             };
-            [[maybe_unused]] auto finish = [&](int t, int st) {
-                if (t + 1 < t_b) put(ck, sm[st]);
-                put(cv, sm[st] + TILE);
-            };
             f32x16 s0[2], s1[2];  // scores of tile t, then its weights, and scores of tile t + 1: in turn
             if constexpr (E4) {
                 fetch(a.kv.kp, a.kv.ke, t_a, ck);
                 put(ck, sm[0]);
                 begin(t_a, 1);
-                finish(t_a, 1);
+                put(ck, sm[1]);
+                put(cv, sm[1] + TILE);
                 if (t_a + 1 < t_b) begin(t_a + 1, 0);
             } else {
                 copy(a.kv.kp, t_a, sm[0]);
@@ -271,14 +269,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             }
             wait_lds();
             __builtin_amdgcn_s_barrier();  // K(t_a)'s stage is free
-            if (t_a + 1 < t_b) {
-                if constexpr (E4) {
-                    finish(t_a + 1, 0);
-                    if (t_a + 2 < t_b) begin(t_a + 2, 1);
-                } else {
-                    begin(t_a + 1, 0);
-                }
-            }
+            if (!E4 && t_a + 1 < t_b) begin(t_a + 1, 0);
 
             // One iteration.  HN: tile t + 1 exists.
             auto iter = [&](int t, auto hn, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
@@ -317,8 +308,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     if constexpr (HN) __builtin_amdgcn_sched_barrier(0);
                 }
                 st_.add(sum);
-                // B
+                // B, ahead of the other block's waves: their exponentials fill the slots between its MFMAs (3% at head_dim 128)
                 float mx = -INFINITY;
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int f = 0; f < NB; ++f) {
                     const int ks = f / OB, ob = f % OB;
@@ -327,21 +319,24 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     if constexpr (HN) {
 #pragma unroll
                         for (int x = f * EB; x < (f + 1) * EB; ++x) mx = fmaxf(mx, sn[x >> 4][x & 15]);
+                        if constexpr (E4) {
+                            // unit t + 1 from registers (past the last tile stale codes, which nobody reads)
+                            constexpr int EVERY = NB / (2 * NU);
+                            if (f % EVERY == EVERY - 1) {
+                                const int j = f / EVERY;
+                                if (j < NU) put_unit(ck, j, sm[st ^ 1]);
+                                else put_unit(cv, j - NU, sm[st ^ 1] + TILE);
+                            }
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if constexpr (HN) st_.absorb(mx, a.c);
                 wait_lds();
                 if constexpr (!E4) wait_vmcnt<0>();  // unit t + 1
                 __builtin_amdgcn_s_barrier();        // everyone is done with unit t's stage; unit t + 1 is visible
-                if (t + 2 < t_b) {
-                    if constexpr (E4) {
-                        finish(t + 2, st);
-                        if (t + 3 < t_b) begin(t + 3, st);
-                    } else {
-                        begin(t + 2, st);
-                    }
-                }
+                if (t + 2 < t_b) begin(t + 2, st);
             };
             using T1 = std::true_type;
             using F0 = std::false_type;

@@ -25,14 +25,11 @@ def e4m3_encode(x):
     table = e4m3_values()
     fine = np.isfinite(x)
     top = np.where(fine, np.abs(x), 0).max(-1)
-    e = np.zeros(top.shape, np.int64)
-    it = np.nditer(top, flags=["multi_index"])
-    for a in it:
-        if a > 0:
-            k = -126
-            while a > 448.0 * 2.0 ** k:
-                k += 1
-            e[it.multi_index] = k
+    with np.errstate(divide="ignore"):
+        e = np.where(top > 0, np.ceil(np.log2(top / 448.0)), 0).astype(np.int64)
+    e = np.where(top > 0, np.maximum(e, -126), 0)
+    for _ in range(2):  # log2's last bit: the least e that holds top
+        e = np.where(top > 448.0 * 2.0 ** e, e + 1, np.where((top > 0) & (e > -126) & (top <= 448.0 * 2.0 ** (e - 1)), e - 1, e))
     y = np.where(fine, np.abs(x), 0) * 2.0 ** -e[..., None].astype(np.float64)
     hi = np.clip(np.searchsorted(table, y), 0, 126)
     lo = np.maximum(hi - 1, 0)
