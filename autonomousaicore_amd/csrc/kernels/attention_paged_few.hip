@@ -88,6 +88,56 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     __shared__ int at_b;
     __shared__ Steps at_x;
     __shared__ int64_t at_before;
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    // what is left once the sequence is known
+    auto within = [&](bool by_group, int64_t share, int64_t in, double begin, double total) {
+        if (by_group) {
+            const int part = same(static_cast<int>(in)), n = parts_of(x.steps, share);
+            const int gi = same(part / n), i = part - gi * n;
+            // (32 bits hold steps * n: at most 2^24 steps in as many parts as there are shares)
+            const uint32_t steps = static_cast<uint32_t>(x.steps), parts = static_cast<uint32_t>(n);
+            const int u0 = same(static_cast<int>(steps * static_cast<uint32_t>(i) / parts));
+            const int u1 = same(static_cast<int>(steps * static_cast<uint32_t>(i + 1) / parts));
+            before = static_cast<int64_t>(gi) * x.steps + u0;
+            count = u1 - u0;
+        } else {
+            before = in;
+            count = min(share, static_cast<int64_t>(total - begin));
+        }
+    };
+    if (f.a.B <= 64) {
+        // a lane per sequence, every wave for itself
+        const int lane = threadIdx.x & 63;
+        Steps own{};
+        if (lane < f.a.B) own = steps_of(f, sequence(f.a, lane));
+        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * f.a.kv.Hkv : 0.0;
+        auto sum = [](double p, double q) { return p + q; };
+        double size = own.steps * groups, total = wave_all(size, sum);
+        const double pairs = wave_all(groups, sum);
+        const bool by_group = pairs * 4 <= f.shares;
+        const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
+        const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
+        if (by_group) {
+            size = lane < f.a.B ? parts_of(own.steps, share) * groups : 0.0;
+            total = wave_all(size, sum);
+        }
+        const double start = wave_running_sum(size) - size, begin = by_group ? g : static_cast<double>(g) * share;
+        if (g == 0 && threadIdx.x < f.a.B) f.plan[lane] = static_cast<int64_t>(start);
+        if (g == 0 && threadIdx.x == 0) f.plan[f.a.B] = by_group ? -share : share;
+        const uint64_t here = __ballot(begin >= start && begin < start + size);
+        if (!here) return false;
+        b = __builtin_ctzll(here);
+        auto at = [&](int v) { return __builtin_amdgcn_readlane(v, b); };
+        const uint64_t row0 = static_cast<uint64_t>(own.sq.row0), in = static_cast<uint64_t>(static_cast<int64_t>(begin - start));
+        auto at64 = [&](uint64_t v) {
+            return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(at(static_cast<int>(v >> 32)))) << 32 |
+                                        static_cast<uint32_t>(at(static_cast<int>(v))));
+        };
+        x.sq = {at64(row0), at(own.sq.n), at(own.sq.len)};
+        x.lo = at(own.lo), x.steps = at(own.steps), x.groups = at(own.groups);
+        within(by_group, share, at64(in), begin, total);
+        return true;
+    }
     const int per = (f.a.B + 255) / 256, tid = threadIdx.x;
     const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
     Steps own;  // the last of this thread's sequences: its only one in batches of up to 256
@@ -132,29 +182,19 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     if (g == 0 && tid == 0) f.plan[f.a.B] = by_group ? -share : share;
     if (begin >= total) return false;
     __syncthreads();
-    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     b = same(at_b);
     x.sq = {at_x.sq.row0, same(at_x.sq.n), same(at_x.sq.len)};
     x.lo = same(at_x.lo), x.steps = same(at_x.steps), x.groups = same(at_x.groups);
-    if (by_group) {
-        const int part = same(static_cast<int>(at_before)), n = parts_of(x.steps, share);
-        const int gi = same(part / n), i = part - gi * n;
-        const int u0 = same(static_cast<int>(static_cast<int64_t>(x.steps) * i / n)), u1 = same(static_cast<int>(static_cast<int64_t>(x.steps) * (i + 1) / n));
-        before = static_cast<int64_t>(gi) * x.steps + u0;
-        count = u1 - u0;
-    } else {
-        before = at_before;
-        count = min(share, static_cast<int64_t>(total - begin));
-    }
+    within(by_group, share, at_before, begin, total);
     return true;
 }
 
-template <int HD, bool E4>
+template <int HD, bool E4, int NW>
 struct FewLds {
     static constexpr int TILE = 32 * HD * (E4 ? 1 : 2);          // bytes of a tile of K or V
     static constexpr int STAGE = 2 * TILE + (E4 ? 256 : 0);      // and the exponents of 32 keys of K, then of V, a word each
     static constexpr int WAVE = 2 * STAGE;
-    static constexpr int BYTES = 4 * WAVE > 4 * 32 * HD * 4 ? 4 * WAVE : 4 * 32 * HD * 4;  // also the waves' O at the end
+    static constexpr int BYTES = NW * WAVE > NW * 32 * HD * 4 ? NW * WAVE : NW * 32 * HD * 4;  // also the waves' O at the end
     static constexpr int COPIES = 2 * (TILE / 1024) + (E4 ? 1 : 0);  // of a stage
 };
 
@@ -204,15 +244,17 @@ struct Frags8 {
     }
 };
 
-template <int HD, bool E4>
-__global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_k(FewArgs f) {
-    using L = FewLds<HD, E4>;
+// NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
+// else is divided and a block is alone on its CU.
+template <int HD, bool E4, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+    using L = FewLds<HD, E4, NW>;
     const PagedArgs& a = f.a;
     constexpr int KS = HD / 16, OB = HD / 32;
     constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int ids[kIds];
-    __shared__ float2 mls[4][32];
+    __shared__ float2 mls[NW][32];
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
@@ -231,7 +273,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
     int b;
     Steps x;
     int64_t before, count;
-    if (f.shares > 0) {
+    if (NW == 4 && f.shares > 0) {
         if (!find_share(f, static_cast<int>(blockIdx.x), b, x, before, count)) return;
     } else {
         b = static_cast<int>(blockIdx.x) / Hkv;
@@ -377,12 +419,12 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
             for (int w0 = k_lo; w0 < k_hi; w0 += window_keys) {
                 const int w1 = min(k_hi, w0 + window_keys), p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
                 __syncthreads();
-                for (int i = threadIdx.x; i < np; i += 256) {
+                for (int i = threadIdx.x; i < np; i += NW * 64) {
                     const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
                     ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
                 }
                 __syncthreads();
-                const int first = w0 + 32 * wave, nt = first < w1 ? (w1 - first + 127) / 128 : 0;  // this wave's tiles
+                const int first = w0 + 32 * wave, nt = first < w1 ? (w1 - first + 32 * NW - 1) / (32 * NW) : 0;  // this wave's tiles
                 // byte offset of key's row in the pools, negative without a page; keys past the last as the last
                 auto row_at = [&](int key) -> int64_t {
                     key = min(key, w1 - 1);
@@ -392,7 +434,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 };
                 auto issue = [&](int t) {
                     char* dst = mine + (t & 1) * L::STAGE;
-                    const int k0 = first + 128 * t;
+                    const int k0 = first + 32 * NW * t;
                     if (paged && k0 + 32 <= w1) {
                         // each half of the tile lies in one page: uniform bases, offsets per lane made once
                         const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
@@ -432,7 +474,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                 for (int t = 0; t < nt; ++t) {
                     if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
                     else wait_vmcnt<0>();
-                    compute(mine + (t & 1) * L::STAGE, first + 128 * t);
+                    compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t);
                     wait_lds();  // the tile has been read
                     if (t + 2 < nt) issue(t + 2);
                 }
@@ -445,10 +487,10 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
         const int q = lane & 31;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][q].x);
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][q].x);
         const float base = M == -INFINITY ? 0.0f : M;
         const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
-        float* os = reinterpret_cast<float*>(lds);  // [4][32][HD], 16-byte groups swizzled by row
+        float* os = reinterpret_cast<float*>(lds);  // [NW][32][HD], 16-byte groups swizzled by row
 #pragma unroll
         for (int ob = 0; ob < OB; ++ob)
 #pragma unroll
@@ -459,7 +501,7 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
                                 st_.o[ob][4 * g + 3] * factor);
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 32 * (HD / 4); i += 256) {
+        for (int i = threadIdx.x; i < 32 * (HD / 4); i += NW * 64) {
             const int qr = i / (HD / 4), c4 = i % (HD / 4), rr = r0 + qr;
             if (rr >= rows) break;
             const int tk = rr / a.G, hd_ = kvh * a.G + rr % a.G, h2 = sq.len - sq.n + tk;
@@ -467,16 +509,16 @@ __global__ __launch_bounds__(256, HD == 128 && !E4 ? 1 : 2) void attn_paged_few_
             const bool empty = h2 < 0 || max(l2, k_lo) > min(h2, k_hi - 1);
             float mm = -INFINITY, l = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mls[w][qr].x);
+            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, mls[w][qr].x);
             const float bs = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float2 ml = mls[w][qr];
                 l = fmaf(__builtin_amdgcn_exp2f((ml.x - bs) * a.c), ml.y, l);
             }
             float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float4 y = *reinterpret_cast<const float4*>(os + (w * 32 + qr) * HD + ((c4 ^ (qr & 7)) << 2));
                 v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
             }
@@ -582,22 +624,33 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
 // Blocks that are resident at once on 256 CUs: LDS holds one of bf16 at head_dim 128, two of the others.
 int64_t resident(int64_t head_dim, bool e4m3) { return head_dim == 128 && !e4m3 ? 256 : 512; }
 
-template <int HD, bool E4>
-void launch(const FewArgs& f, hipStream_t s) {
-    constexpr int bytes = FewLds<HD, E4>::BYTES;
+template <int HD, bool E4, int NW>
+void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
+    constexpr int bytes = FewLds<HD, E4, NW>::BYTES;
     static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     AIC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
-        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4>),
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4, NW>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) allowed[dev].store(true);
     }
+    attn_paged_few_k<HD, E4, NW><<<static_cast<unsigned>(blocks), NW * 64, bytes, s>>>(f);
+    AIC_LAUNCH_CHECK("attn_paged");
+}
+
+template <int HD, bool E4>
+void launch(const FewArgs& f, hipStream_t s) {
     const int64_t pairs = static_cast<int64_t>(f.a.kv.Hkv) * f.a.B;
     AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
-    attn_paged_few_k<HD, E4><<<static_cast<unsigned>(f.shares > 0 ? f.shares : pairs), 256, bytes, s>>>(f);
-    AIC_LAUNCH_CHECK("attn_paged");
-    if (f.shares == 0) return;
+    if (f.shares == 0) {
+        // eight waves' stages are beyond the LDS for bf16 at head_dim 128; with more blocks than CUs four waves keep two of them there
+        if constexpr (HD < 128 || E4) {
+            if (pairs <= 256) return launch<HD, E4, 8>(f, pairs, s);
+        }
+        return launch<HD, E4, 4>(f, pairs, s);
+    }
+    launch<HD, E4, 4>(f, f.shares, s);
     attn_paged_few_join_k<HD><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>((f.group + 3) / 4)), 256, 0, s>>>(f);
     AIC_LAUNCH_CHECK("attn_paged join");
 }
