@@ -301,11 +301,12 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
 int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H) {
     check_sizes(c, B, T, max_q, max_len, H);
     if (B == 0 || T == 0) return 0;
+    max_q = std::min(max_q, T);
     // the cache's type does not tell the queries' (e4m3 serves both): room for either
     int64_t n = 0;
     const int64_t G = H / c.kv_heads;
     if (c.type != DType::Float32 && few_rows(max_q, G))
-        n = few_workspace(B, max_q, max_len, G, c.head_dim, c.type == DType::UInt8);
+        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, c.type == DType::UInt8);
     if (c.type != DType::Float32 && !few_rows(max_q, G))
         n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
@@ -328,6 +329,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     AIC_CHECK(workspace_bytes >= 0, InvalidArgument, "attn_paged: negative workspace size");
     if (B == 0 || T == 0) return;
     AIC_CHECK(q && o && offsets && lens, InvalidArgument, "attn_paged: null pointer");
+    max_q = std::min(max_q, T);
 
     const int64_t size = static_cast<int64_t>(dtype_size(dt));
     PagedArgs a{};
@@ -354,7 +356,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     if (need == 0) workspace = nullptr;
     if (few) {
         const bool e4m3 = c.type == DType::UInt8;  // need may be the other kernel's alone
-        const bool shares = few_workspace(B, max_q, max_len, a.G, c.head_dim, e4m3) > 0;
+        const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, e4m3) > 0;
         attn_paged_few(a, max_q, e4m3, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;
     }

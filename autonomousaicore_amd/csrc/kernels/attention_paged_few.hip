@@ -36,10 +36,6 @@ namespace {
 constexpr int kIds = 512;    // page ids in LDS at a time
 constexpr int kStep = 128;   // keys: a tile for each wave
 constexpr int kLeast = 4;    // steps of a share at least: a part costs a block about as much as three steps
-// Longest cache whose groups are not divided: finding shares and joining them cost about 7 us, and a step of an
-// undivided group about 1 us (one 512-token sequence of 12 heads of 64: 9.6 us whole, 16.8 us in shares).
-constexpr int kWhole = 1024;
-
 struct FewArgs {
     PagedArgs a;
     int group;         // query rows of a group, at most 32
@@ -657,12 +653,18 @@ void launch(const FewArgs& f, hipStream_t s) {
 
 int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * G, 1, 32); }
 
+// Longest cache whose groups are not divided: finding shares and joining them cost about 7 us, and 128 keys of an
+// undivided group 0.3 us (head_dim 64) to 0.7 us (128).  One sequence of 1600 tokens, shares and whole: 13.3 and
+// 11.9 us with 12 heads of 64, 15.9 and 20.8 us with 8 of 128; of 2048: 13.3 and 13.9, 16.1 and 23.9 us.  With a group
+// for most CUs nothing is won by dividing up to 2048: 32 sequences with 8 heads of 128, 47.6 and 42.8 us.
+int64_t whole_len(int64_t pairs, int64_t head_dim) { return pairs >= 192 ? 2048 : head_dim < 128 ? 1536 : 1024; }
+
 }  // namespace
 
 bool few_rows(int64_t max_q, int64_t G) { return max_q * G <= 32; }
 
-int64_t few_workspace(int64_t B, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3) {
-    if (max_len <= kWhole) return 0;
+int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3) {
+    if (max_len <= whole_len(B * Hkv, head_dim)) return 0;
     return (2 * resident(head_dim, e4m3) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
 }
 
