@@ -24,19 +24,24 @@ namespace aic::hip {
 namespace {
 
 // ----------------------------------------------------------------------- the fp32 kernel
-// Blocks of 4 waves x 32 query rows over tiles of 32 keys, or (SHARE) of 32 query rows over tiles of 128 keys that the
-// waves share, 32 each, their states joined at the end: four times as many blocks with a quarter of the
-// steps, for batches that do not fill the card with the first kind.  Tiles are staged through registers: the
-// next one's loads are in flight during this one's products.  Bound by the fp32 matrix pipe (64 cycles per
+// Blocks of four waves: 4 / SH sets of 32 query rows, over tiles of 32 SH keys that the SH waves of a set share, 32 each,
+// their states joined at the end.  SH = 1 where the batch fills the card with blocks of 128 rows; otherwise more and
+// smaller blocks with fewer steps (SH = 4, or 2 at head_dim 128, where tiles of 128 keys would leave one block per
+// CU).  Tiles are staged through registers: the next one's loads are in flight during this one's products; the
+// page ids come from LDS, since loads that wait for ids from memory would stop the wave in the middle of its
+// products (859 rows of 16 heads of 64: 54.5 us so).  Bound by the fp32 matrix pipe (64 cycles per
 // v_mfma_f32_32x32x2_f32).
-template <typename CT, int HD, bool SHARE>
+constexpr int kIds = 512;  // page ids in LDS at a time
+
+template <typename CT, int HD, int SH>
 __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
-    constexpr int R = SHARE ? 32 : 128, KT = SHARE ? 128 : 32, OB = HD / 32;
+    constexpr int SETS = 4 / SH, R = 32 * SETS, KT = 32 * SH, OB = HD / 32;
     constexpr int UPR = HD * sizeof(CT) / 16;   // 16-byte units of a cached row
     constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
     constexpr bool E4 = sizeof(CT) == 1;
     constexpr int TILE = KT * HD * 4;
     __shared__ __attribute__((aligned(16))) char tiles[2 * TILE];
+    __shared__ int ids[kIds];
     char *ks = tiles, *vs = tiles + TILE;
 
     const int Hkv = a.kv.Hkv;
@@ -47,8 +52,8 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     if (!find_tile<R>(a, tile, b, local)) return;
     const Seq sq = wave_sequence(a, b);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
-    const int sub = SHARE ? 32 * wave : 0;  // this wave's keys of a tile
-    const int rows = sq.n * a.G, r0 = local * R, r = r0 + (SHARE ? 0 : wave * 32) + (lane & 31);
+    const int set = wave % SETS, share = wave / SETS, sub = 32 * share;  // this wave's rows of the block and keys of a tile
+    const int rows = sq.n * a.G, r0 = local * R, r = r0 + set * 32 + (lane & 31);
     const bool real = r < rows;
     const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
     const int64_t t = sq.row0 + tok;
@@ -61,6 +66,10 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
     k_lo &= ~63;
     part_of_keys(k_lo, k_hi, split, a.nsplit);
+    // keys of this wave's rows: those of the set, none behind the sequence's last row
+    const int set_r0 = r0 + set * 32, set_first = sq.len - sq.n + set_r0 / a.G;
+    const int set_hi = set_r0 < rows ? min(k_hi, sq.len - sq.n + (min(set_r0 + 32, rows) - 1) / a.G + 1) : 0;
+    const int set_lo = a.window > 0 ? set_first - a.window + 1 : 0;
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));  // keys from lo on that it sees here
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;                          // of this split
 
@@ -79,20 +88,21 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
         uint4 rk[NU], rv[NU];
         [[maybe_unused]] uint32_t xk[NU], xv[NU];  // exponent bytes
         const int32_t* tr = a.kv.table + b * a.kv.ld_table;
+        int w1 = 0, p0 = 0;  // end and first page of the keys whose page ids are in LDS
         auto load = [&](int k0) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int u = i * 256 + static_cast<int>(threadIdx.x);
                 // keys past the last are read as the last one: hidden below
-                const int key = min(k0 + min(u / UPR, KT - 1), k_hi - 1);
-                const int64_t row = a.kv.row(tr, key, kvh);
+                const int key = min(k0 + min(u / UPR, KT - 1), w1 - 1), pi = a.kv.page_index(key), page = ids[pi - p0];
+                const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * a.kv.ps + (key - pi * a.kv.ps);
                 const int64_t at = row * (UPR * 16) + (u % UPR) * 16;
                 const char* none = reinterpret_cast<const char*>(&kNoPage);
-                rk[i] = *reinterpret_cast<const uint4*>(row >= 0 ? a.kv.kp + at : none);
-                rv[i] = *reinterpret_cast<const uint4*>(row >= 0 ? a.kv.vp + at : none);
+                rk[i] = *reinterpret_cast<const uint4*>(page >= 0 ? a.kv.kp + at : none);
+                rv[i] = *reinterpret_cast<const uint4*>(page >= 0 ? a.kv.vp + at : none);
                 if constexpr (E4) {
-                    xk[i] = row >= 0 ? a.kv.ke[row] : 127;
-                    xv[i] = row >= 0 ? a.kv.ve[row] : 127;
+                    xk[i] = page >= 0 ? a.kv.ke[row] : 127;
+                    xv[i] = page >= 0 ? a.kv.ve[row] : 127;
                 }
             }
         };
@@ -118,8 +128,19 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
             return bad != 0;
         };
 
-        load(k_lo);
+        const int window_keys = min((kIds - 1) * a.kv.ps, 1 << 20) & ~127;  // keys whose page ids fit: at least 384
         for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
+            if (k0 >= w1) {  // the next page ids
+                __syncthreads();
+                w1 = min(k_hi, k0 + window_keys);
+                p0 = a.kv.page_index(k0);
+                for (int i = threadIdx.x; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
+                    const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
+                    ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
+                }
+                __syncthreads();
+                load(k0);
+            }
             // every row of the block sees every key of the tile?
             const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
             const int poison = __syncthreads_or(!open && bad_v());  // also: everyone is done with the last tile
@@ -132,8 +153,8 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
                 }
             }
             __syncthreads();
-            if (k0 + KT < k_hi) load(k0 + KT);
-            if (SHARE && k0 + sub >= k_hi) continue;  // nothing of this tile for this wave
+            if (k0 + KT < w1) load(k0 + KT);
+            if (k0 + sub >= set_hi || k0 + sub + 31 < set_lo) continue;  // nothing of this tile for this wave
 
             f32x16 sc[1];
             zero(sc[0]);
@@ -175,38 +196,39 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
             }
         }
     }
-    if constexpr (SHARE) {
-        // wave 0 takes the others' states: M = max m_w, o = sum 2^((m_w - M) c) o_w, l alike
-        float* os = reinterpret_cast<float*>(tiles);
+    if constexpr (SH > 1) {
+        // each set's first wave takes the others' states: M = max m_w, o = sum 2^((m_w - M) c) o_w, l alike
+        float* os = reinterpret_cast<float*>(tiles);  // [SETS][SH - 1][OB * 16][64]
         __shared__ float2 mls[4][32];
         __syncthreads();  // the tiles have been read
         if (hl == 0) mls[wave][lane] = make_float2(st_.m, st_.l);
         __syncthreads();
         float M = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][lane & 31].x);
+        for (int w = 0; w < SH; ++w) M = fmaxf(M, mls[set + w * SETS][lane & 31].x);
         const float base = M == -INFINITY ? 0.0f : M;
         const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 ml = mls[w][lane & 31];
+        for (int w = 0; w < SH; ++w) {
+            const float2 ml = mls[set + w * SETS][lane & 31];
             l = fmaf(__builtin_amdgcn_exp2f((ml.x - base) * a.c), ml.y, l);
         }
+        auto at = [&](int w, int i) { return ((set * (SH - 1) + w - 1) * OB * 16 + i) * 64 + lane; };
 #pragma unroll
         for (int ob = 0; ob < OB; ++ob)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 st_.o[ob][e] *= factor;
-                if (wave > 0) os[((wave - 1) * OB * 16 + ob * 16 + e) * 64 + lane] = st_.o[ob][e];
+                if (share > 0) os[at(share, ob * 16 + e)] = st_.o[ob][e];
             }
         __syncthreads();
-        if (wave > 0) return;
+        if (share > 0) return;
 #pragma unroll
         for (int ob = 0; ob < OB; ++ob)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
 #pragma unroll
-                for (int w = 0; w < 3; ++w) st_.o[ob][e] += os[(w * OB * 16 + ob * 16 + e) * 64 + lane];
+                for (int w = 1; w < SH; ++w) st_.o[ob][e] += os[at(w, ob * 16 + e)];
         st_.m = M;
         st_.l = l;
     }
@@ -281,8 +303,10 @@ Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
-// fp32: blocks of 32 rows where blocks of 128 rows are fewer than two per CU.
-int64_t f32_rows(int64_t B, int64_t T, int64_t H, int64_t Hkv) { return tile_bound(T, H / Hkv, B, 128) * Hkv < 512 ? 32 : 128; }
+// fp32: query rows of a block, fewer where blocks of 128 rows are fewer than two per CU.
+int64_t f32_rows(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd) {
+    return tile_bound(T, H / Hkv, B, 128) * Hkv >= 512 ? 128 : hd == 128 ? 64 : 32;
+}
 int64_t plan_bytes(const Plan& p, int64_t T, int64_t H, int64_t hd) {
     return p.nsplit <= 1 ? 0 : p.nsplit * T * H * (hd + 2) * 4;
 }
@@ -310,7 +334,7 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     if (c.type != DType::Float32 && !few_rows(max_q, G))
         n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, H, c.kv_heads)), T, H, c.head_dim));
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
     return n;
 }
 
@@ -344,7 +368,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
     const bool few = dt == DType::BFloat16 && few_rows(max_q, a.G);
-    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, H, c.kv_heads);
+    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, H, c.kv_heads, c.head_dim);
     Plan p = plan(B, T, max_len, H, c.kv_heads, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
@@ -375,8 +399,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
             attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
         } else {
             const auto grid = static_cast<unsigned>(blocks);
-            if (R == 32) attn_paged_f32_k<decltype(ct), D, true><<<grid, 256, 0, s>>>(a);
-            else attn_paged_f32_k<decltype(ct), D, false><<<grid, 256, 0, s>>>(a);
+            if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
+            else attn_paged_f32_k<decltype(ct), D, D == 128 ? 2 : 4><<<grid, 256, 0, s>>>(a);
             AIC_LAUNCH_CHECK("attn_paged");
         }
         if (a.nsplit > 1) {
