@@ -24,13 +24,14 @@ namespace aic::hip {
 namespace {
 
 // ----------------------------------------------------------------------- the fp32 kernel
-// Blocks of four waves: 4 / SH sets of 32 query rows, over tiles of 32 SH keys that the SH waves of a set share, 32 each,
-// their states joined at the end.  SH = 1 where the batch fills the card with blocks of 128 rows; otherwise more and
-// smaller blocks with fewer steps (SH = 4, or 2 at head_dim 128, where tiles of 128 keys would leave one block per
-// CU).  Tiles are staged through registers: the next one's loads are in flight during this one's products; the
-// page ids come from LDS, since loads that wait for ids from memory would stop the wave in the middle of its
-// products (859 rows of 16 heads of 64: 54.5 us so).  Bound by the fp32 matrix pipe (64 cycles per
-// v_mfma_f32_32x32x2_f32).
+// Blocks of four waves: 4 / SH sets of 32 query rows, over tiles of 32 SH keys that the SH waves of a set
+// share, 32 each, their states joined at the end.  SH = 1 where the batch fills the card with blocks of
+// 128 rows; otherwise more and smaller blocks with fewer steps (SH = 4, or 2 at head_dim 128, where tiles of
+// 128 keys would leave one block per CU).  Tiles are staged through registers: the next one's loads are in
+// flight during this one's products; the page ids come from LDS, since loads that wait for ids from memory
+// stop the wave in the middle of its products (859 rows of 16 heads of 64: 54.5 us so, 43.6 us from LDS;
+// 1000 rows on 2000 keys of 128, 16 heads over 2: 326 us, 210 us, 58 TFLOP/s).  Bound by the fp32 matrix
+// pipe (64 cycles per v_mfma_f32_32x32x2_f32) and the staging between its runs.
 constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <typename CT, int HD, int SH>
@@ -298,13 +299,15 @@ struct Plan {
 // R: query rows of a block.
 Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t R) {
     Plan p{tile_bound(T, H / Hkv, B, R), 1};
-    const int64_t twice = (2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;  // two times the blocks there probably are
+    // two times the blocks there probably are; tiles of up to 8 rows hold a sequence each
+    const int64_t twice = (R <= 8 ? 2 * std::min(B, T) : 2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;
     const int64_t most = std::max<int64_t>(std::min<int64_t>(4, max_len / 256), max_len / 448);
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
 // fp32: query rows of a block, fewer where blocks of 128 rows are fewer than two per CU.
-int64_t f32_rows(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t hd) {
+int64_t f32_rows(int64_t B, int64_t T, int64_t max_q, int64_t H, int64_t Hkv, int64_t hd) {
+    if (const int few = f32_few_rows(max_q, H / Hkv)) return few;
     return tile_bound(T, H / Hkv, B, 128) * Hkv >= 512 ? 128 : hd == 128 ? 64 : 32;
 }
 int64_t plan_bytes(const Plan& p, int64_t T, int64_t H, int64_t hd) {
@@ -334,7 +337,7 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     if (c.type != DType::Float32 && !few_rows(max_q, G))
         n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
     return n;
 }
 
@@ -368,7 +371,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
     const bool few = dt == DType::BFloat16 && few_rows(max_q, a.G);
-    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, H, c.kv_heads, c.head_dim);
+    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim);
     Plan p = plan(B, T, max_len, H, c.kv_heads, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
@@ -399,7 +402,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
             attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
         } else {
             const auto grid = static_cast<unsigned>(blocks);
-            if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
+            if (R <= 8) attn_paged_f32_few(a, static_cast<int>(R), sizeof(ct) == 1, D, grid, s);
+            else if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
             else attn_paged_f32_k<decltype(ct), D, D == 128 ? 2 : 4><<<grid, 256, 0, s>>>(a);
             AIC_LAUNCH_CHECK("attn_paged");
         }
