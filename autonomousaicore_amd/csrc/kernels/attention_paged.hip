@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     // keys of this wave's rows: those of the set, none behind the sequence's last row
     const int set_r0 = r0 + set * 32, set_first = sq.len - sq.n + set_r0 / a.G;
     const int set_hi = set_r0 < rows ? min(k_hi, sq.len - sq.n + (min(set_r0 + 32, rows) - 1) / a.G + 1) : 0;
-    const int set_lo = a.window > 0 ? set_first - a.window + 1 : 0;
+    const int set_lo = a.window > 0 ? max(set_first, 0) - a.window + 1 : 0;
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));  // keys from lo on that it sees here
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;                          // of this split
 
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
         for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
             if (k0 >= w1) {  // the next page ids
                 __syncthreads();
-                w1 = min(k_hi, k0 + window_keys);
+                w1 = k0 + min(k_hi - k0, window_keys);
                 p0 = a.kv.page_index(k0);
                 for (int i = threadIdx.x; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
                     const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
@@ -351,7 +351,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     const PageView pv = page_view(c, "attn_paged");
     AIC_CHECK(ld_q >= H * c.head_dim && ld_o >= H * c.head_dim, InvalidArgument,
               "attn_paged: leading dimension below heads * head_dim");
-    AIC_CHECK(std::isfinite(scale) && scale > 0.0f, InvalidArgument, "attn_paged: scale must be positive and finite, got ", scale);
+    AIC_CHECK(std::isfinite(scale * kLog2e) && scale > 0.0f, InvalidArgument, "attn_paged: scale must be positive and below 2.3e38, got ", scale);
     AIC_CHECK(window >= 0, InvalidArgument, "attn_paged: window must not be negative, got ", window);
     AIC_CHECK(workspace_bytes >= 0, InvalidArgument, "attn_paged: negative workspace size");
     if (B == 0 || T == 0) return;

@@ -90,10 +90,10 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
         if (by_group) {
             const int part = same(static_cast<int>(in)), n = parts_of(x.steps, share);
             const int gi = same(part / n), i = part - gi * n;
-            // (32 bits hold steps * n: at most 2^24 steps in as many parts as there are shares)
-            const uint32_t steps = static_cast<uint32_t>(x.steps), parts = static_cast<uint32_t>(n);
-            const int u0 = same(static_cast<int>(steps * static_cast<uint32_t>(i) / parts));
-            const int u1 = same(static_cast<int>(steps * static_cast<uint32_t>(i + 1) / parts));
+            // floor(steps i / n), in 32 bits also for 2^24 steps in 512 parts
+            const uint32_t steps = static_cast<uint32_t>(x.steps), parts = static_cast<uint32_t>(n), each = steps / parts, rest = steps % parts;
+            auto upto = [&](uint32_t k) { return same(static_cast<int>(each * k + rest * k / parts)); };
+            const int u0 = upto(static_cast<uint32_t>(i)), u1 = upto(static_cast<uint32_t>(i) + 1);
             before = static_cast<int64_t>(gi) * x.steps + u0;
             count = u1 - u0;
         } else {
@@ -412,8 +412,9 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
             };
 
             const int window_keys = min((kIds - 1) * ps, 1 << 20) & ~31;  // keys whose page ids fit
-            for (int w0 = k_lo; w0 < k_hi; w0 += window_keys) {
-                const int w1 = min(k_hi, w0 + window_keys), p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
+            for (int w0 = k_lo, w1; w0 < k_hi; w0 = w1) {
+                w1 = w0 + min(k_hi - w0, window_keys);
+                const int p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
                 __syncthreads();
                 for (int i = threadIdx.x; i < np; i += NW * 64) {
                     const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;

@@ -84,8 +84,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
         const char* none = reinterpret_cast<const char*>(&kNoPage);
 
         const int window_keys = min((kIds - 1) * ps, 1 << 20) & ~63;  // keys whose page ids fit: at least 448
-        for (int w0 = k_lo; w0 < k_hi; w0 += window_keys) {
-            const int w1 = min(k_hi, w0 + window_keys), p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
+        for (int w0 = k_lo, w1; w0 < k_hi; w0 = w1) {
+            w1 = w0 + min(k_hi - w0, window_keys);
+            const int p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
             __syncthreads();
             for (int i = threadIdx.x; i < np; i += 256) {
                 const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;

@@ -33,7 +33,7 @@ constexpr int kPart = kWave * kPer;  // logits of a part: one wave's
 constexpr int kStatWaves = 4;        // waves of a block: statistics
 constexpr int kWaves = 8;            // decision: rows looked at side by side
 // Logits per lane and per wave of the residual: few, for the weights are straight-line code that each launch
-// fetches anew (16 per lane measured 12.4 us for one sequence, 4 per lane the time in DESIGN).
+// fetches anew (16 per lane: 12.4 us for one sequence, 4 per lane: 7.0 us).
 constexpr int kFew = 4;
 constexpr int kRun = kWave * kFew;
 
@@ -281,9 +281,11 @@ __device__ __forceinline__ Pair<PER> load_pair(const DraftArgs& a, const Decisio
     if (d.minus) load_logits<T, PER>(static_cast<const T*>(a.y) + d.row * a.ldy, i0, a.V, a.vec_y, x.y);
     return x;
 }
-// Their residual weights max(0, p - d).
+// Their residual weights max(0, p - d), both rounded before they are taken off: where p and d are equal nothing is
+// left (an fma would leave p's rounding error).
 template <typename T, int PER>
 __device__ __forceinline__ void residual(const DraftArgs& a, const Decision& d, int i0, const Pair<PER>& x, double (&r)[PER]) {
+#pragma clang fp contract(off)
     const double ip = d.p.max > -INFINITY ? 1.0 / d.p.sum : 0.0, iq = d.minus && d.d.max > -INFINITY ? 1.0 / d.d.sum : 0.0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) r[j] = weight(x.z[j], d.p.max, a.c) * ip;
@@ -328,29 +330,47 @@ __global__ __launch_bounds__(kWave) void draft_pick_k(DraftArgs a) {
     constexpr int W = vec_width<T, kFew>;
     static_assert(W == kFew, "a lane's logits of a run are neighbours");
     const int b = static_cast<int>(blockIdx.x), lane = threadIdx.x;
-    const double* left = a.left + static_cast<int64_t>(b) * a.runs;
-    const Decision d = a.decided[b];
+    double* left = a.left + static_cast<int64_t>(b) * a.runs;
+    Decision d = a.decided[b];
     int64_t token = -1;
     if (d.n > 0 && d.p.max > -INFINITY) {
         if (a.c == 0.0) {
             token = d.p.best;
         } else {
-            double total = 0.0;
-            for (int i = lane; i < a.runs; i += kWave) total += left[i];
-            const double target = wave_all(total, Sum{}) * static_cast<double>(a.u_next[b]);
             int run = -1;  // runs of weight zero hold no token
-            double below = 0.0, sofar = 0.0;
-            for (int i0 = 0; i0 < a.runs; i0 += kWave) {
-                const double w = i0 + lane < a.runs ? left[i0 + lane] : 0.0;
-                const double upto = sofar + wave_running_sum(w);
-                const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && upto > target);
-                if (some) {
-                    const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-                    run = i0 + l;
-                    below = __shfl(upto - w, l, kWave);
+            double below = 0.0, target = 0.0;
+            // once; and again where p - d left nothing in 64 bits, which then tell p from d nowhere: from p
+#pragma unroll 1
+            for (int again = 0; again < 2 && run < 0; ++again) {
+                if (again) {
+                    d.minus = 0;
+                    d.off = -1;
+                    for (int i = 0; i < a.runs; ++i) {
+                        double r[kFew], sum = 0.0;
+                        residual<T, kFew>(a, d, i * kRun, load_pair<T, kFew>(a, d, i * kRun), r);
+#pragma unroll
+                        for (int j = 0; j < kFew; ++j) sum += r[j];
+                        sum = wave_all(sum, Sum{});
+                        if (lane == 0) left[i] = sum;
+                    }
+                    __syncthreads();
                 }
-                if (past) break;
-                sofar = __shfl(upto, kWave - 1, kWave);
+                double total = 0.0;
+                for (int i = lane; i < a.runs; i += kWave) total += left[i];
+                target = wave_all(total, Sum{}) * static_cast<double>(a.u_next[b]);
+                double sofar = 0.0;
+                for (int i0 = 0; i0 < a.runs; i0 += kWave) {
+                    const double w = i0 + lane < a.runs ? left[i0 + lane] : 0.0;
+                    const double upto = sofar + wave_running_sum(w);
+                    const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && upto > target);
+                    if (some) {
+                        const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+                        run = i0 + l;
+                        below = __shfl(upto - w, l, kWave);
+                    }
+                    if (past) break;
+                    sofar = __shfl(upto, kWave - 1, kWave);
+                }
             }
             if (run >= 0) {
                 double r[kFew], mine = 0.0;
@@ -435,7 +455,7 @@ void verify_drafts(const void* logits, int64_t ld, const void* draft, int64_t ld
     a.T = T, a.max_q = max_q;
     a.c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temperature);
     a.reach = 1000.0f * temperature * 0.6931f;  // under 1000 / c: 2^-999.9
-    a.plain_top = std::min(a.reach * 0x1p20f, 1e30f);
+    a.plain_top = a.reach < 1e30f ? std::min(a.reach * 0x1p20f, 1e30f) : 0.0f;
     a.tokens = tokens, a.counts = counts, a.new_lens = new_lens;
     a.sz = static_cast<Stat*>(workspace);
     a.sy = a.sz + T * parts;

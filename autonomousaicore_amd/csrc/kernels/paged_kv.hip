@@ -4,8 +4,9 @@
 // positions of its lens[b] cached tokens.  A block takes a few rows, finds their places once, and its
 // threads then carry 16-byte units of the cache, up to four each with all loads in flight together: a
 // thread that went from the offsets to the page table to its row by itself waited for four loads one
-// after the other (DESIGN has the times of both).  A head's amax is an exchange among its hd / 16
-// lanes.  Bound by memory.
+// after the other (prompts of 8 x 2048 rows of 8 heads of 128 into e4m3: 24.1 us so, 16.4 us; 16 x 4096 rows
+// back: 101 us, 58.8 us).  A head's amax is an exchange among its hd / 16 lanes.  Bound by memory: 4.0 TB/s
+// and 4.3 TB/s there, a large copy's 5.0.
 #include <algorithm>
 #include <type_traits>
 

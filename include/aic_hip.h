@@ -256,7 +256,8 @@ int aic_hip_attn_bwd_qk(const void* q, int64_t ld_q, const void* k, const void* 
  * from 1 to 65536), and position j of sequence b is slot j % page_size of page
  * page_table[b * ld_table + j / page_size] (device memory; several sequences may read one page).
  * type: AIC_F32, AIC_BF16, or AIC_U8 for e4m3 codes (4 exponent, 3 mantissa bits, largest 448):
- * a row's head is code * 2^(byte - 127), byte in k_exps / v_exps [n_pages][kv_heads][page_size].
+ * a row's head is code * 2^(byte - 127), byte (1 .. 254) in k_exps / v_exps
+ * [n_pages][kv_heads][page_size].
  *
  * The calls below share a ragged batch's description, in device memory: offsets [B + 1] and lens [B]
  * (int64).  Sequence b's packed rows offsets[b] .. offsets[b + 1] - 1 are the last ones of its
@@ -309,12 +310,13 @@ int aic_hip_attn_paged(const aic_kv_pages* cache, const void* q, int64_t ld_q, v
                        int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
 /* Speculative sampling's verification.  Sequence b's rows are its newest token and the drafted ones
  * behind it, ids [T] (int64); logits [T, V] (dtype dt F32 or BF16, leading dimension ld) are the target's
- * after each of them, draft_logits (nullable, the same layout, ld_draft; a sequence's last row is not
- * used) those that the next id was drawn from.  With p = softmax(logits[t] / temperature) and d =
+ * after each of them, draft_logits (nullable, the same layout with T rows, ld_draft; a sequence's last row is
+ * not used) those that the next id was drawn from.  With p = softmax(logits[t] / temperature) and d =
  * softmax(draft_logits[t] / temperature) (NULL: all on ids[t + 1]), ids[t + 1] is kept where
  * u[t] d < p (u [T] fp32 in [0, 1)).  The first that is not kept is replaced by a draw from
- * max(0, p - d); if all are, one token more is drawn from the last row's p.  The draw is the first
- * token whose running sum passes u_next[b] (fp32 in [0, 1)) times the whole; sums in 64 bits.
+ * max(0, p - d), or from p where that leaves nothing in 64 bits; if all are, one token more is drawn
+ * from the last row's p.  The draw is the first token whose running sum passes u_next[b] (fp32 in
+ * [0, 1)) times the whole; sums in 64 bits.
  * temperature <= 0.001: greedy, as aic_lm_generate (a draft is kept if it is the largest logit, the
  * lowest index of equal ones; draft_logits, u and u_next are not used).  A NaN logit counts as
  * -infinity; where no logit is above -infinity the token is -1.

@@ -221,6 +221,8 @@ def drafts(logits, draft, ids, u, u_next, offs, lens, max_q, V, temperature):
             else:
                 left = p if greedy else np.maximum(p - d, 0.0)
                 break
+        if not left.any():  # p - d is nothing in 64 bits: from p
+            left = p
         run = np.cumsum(left)
         pos = np.flatnonzero(left > 0)
         if len(pos) == 0:

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 from autonomousaicore_amd import _lib  # noqa: E402
 from tests.gpu_util import call, host, ptr, stream  # noqa: E402
-from tests.paged_ref import CODE, TORCH, Paged, check_attention  # noqa: E402
+from tests.paged_ref import CODE, HALF, TORCH, Paged, attention, check_attention, e4m3_decode, e4m3_encode  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -356,3 +356,48 @@ def test_many_rows_and_heads_fill_the_card(dt, cache):
         some.k, some.v, some.Hkv = p.k[:, h // 2:h // 2 + 1], p.v[:, h // 2:h // 2 + 1], 1
         got = host(a.o.contiguous()).reshape(a.T, 32, 32)[:, h:h + 1]
         check_attention(got, None, some, q[:, h:h + 1], 1, 0, a.scale, dt)
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 62])
+@pytest.mark.parametrize("n,L", [(3, 1), (40, 20), (300, 220), (5, 0)])
+def test_windows_up_to_the_largest(dt, cache, window, n, L):
+    """More rows than cached tokens: the first ones stand before position 0."""
+    p = Paged([n, 2], [L, 50], 1, 32, 16, cache, seed=n)
+    Call(p, 1, dt, window).run().check()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("n", [1, 40])
+def test_the_longest_cache(dt, cache, n):
+    """2^31 - 4096 positions: a page, the same page over and over, and a last one cut short.  The keys of the middle lie
+    40 below the others in the scores: together they weigh less than 2^31 e^-35 = 1.4e-6 of the others, whose
+    scores differ by less than 5, and as much is added to the tolerance."""
+    ps, L = 65536, 2 ** 31 - 4096
+    p = Paged([n], [3 * ps], 1, 32, ps, cache, seed=n)
+    (first, mid, last), p.width, p.lens = p.table[0, :3].tolist(), 2 ** 15, [L]
+    p.table = np.full((1, p.width), mid, np.int32)
+    p.table[0, 0], p.table[0, -1] = first, last
+    k = p.k * 0.125
+    k[..., 0] = 0.0
+    k[mid, ..., 0] = -40.0
+    if cache == "e4m3":
+        codes, exps = e4m3_encode(k)
+        p.pool["k"], p.k = (torch.from_numpy(codes).cuda(), torch.from_numpy(exps).cuda()), e4m3_decode(codes, exps)
+    else:
+        t = torch.from_numpy(k).to(TORCH[cache])
+        p.pool["k"], p.k = (t.cuda(), None), t.double().numpy()
+    q = torch.from_numpy(np.random.default_rng(n).standard_normal((n + 3, 32)).clip(-2, 2))
+    q[:, 0] = 32.0 ** 0.5
+    a = Call(p, 1, dt, q=q).run()
+    torch.cuda.synchronize()
+    short = Paged.__new__(Paged)  # without the middle
+    short.__dict__.update(p.__dict__)
+    short.table, short.width, short.lens = np.array([[first, last]], np.int32), 2, [2 * ps - 4096]
+    q = a.q.double().cpu().numpy().reshape(a.T, 1, 32)
+    o, lse, ab, sb = attention(short, q, 1, 0, a.scale)
+    got, got_lse = host(a.o).reshape(a.T, 1, 32).astype(np.float64), host(a.lse).astype(np.float64)
+    mass = 2.0 ** 31 * math.exp(-35)
+    tol = (4 * sb[:n, :, None] + 2.0 ** -18) * ab[:n] + (HALF[dt] * np.abs(o[:n]) + (HALF["bf16"] * ab[:n] if dt == "bf16" else 0)) * 1.01
+    assert (np.abs(got - o)[:n] <= tol + 2 * mass * np.abs(p.v).max()).all()
+    assert (np.abs(got_lse - lse)[:n] <= 2 * sb[:n] + 2.0 ** -17 + 2.0 ** -22 * np.abs(lse[:n]) + mass).all()

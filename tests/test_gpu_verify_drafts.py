@@ -182,3 +182,25 @@ def test_workspaces_capture_and_lengths_in_place():
 def test_no_rows_at_all():
     b = Batch([0, 0], 10, "f32", 1.0, seed=1).device().launch().check()
     assert (b.tokens == -1).all() and (b.counts == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [1e30, 1e36, 3e38])
+def test_temperatures_up_to_the_largest(dt, temperature):
+    """Nearly equal weights of all logits but the shut out ones."""
+    b = Batch([3, 2, 1], 3000, dt, temperature, seed=11)
+    b.z[:, 5:2900] = float("-inf")
+    b.z[1, 7] = float("nan")
+    b.device().launch().check()
+
+
+@pytest.mark.parametrize("u", [0.9375, 1.0])
+def test_a_residual_that_is_nothing_in_64_bits(u):
+    """p and d differ at one token of weight 1e-26 alone, which no sum holds: the new token is p's."""
+    b = Batch([2, 2], 3000, "f32", 1.0, seed=12, near=0.0)
+    for row, seq in ((0, 0), (2, 1)):
+        b.z[row, 40], b.y[row, 40] = -61.0, -60.0
+        b.ids[row + 1] = 40
+    b.u[:] = u
+    b.device().launch().check()
+    assert (b.counts == 1).all() and (b.tokens[:, 0] >= 0).all()

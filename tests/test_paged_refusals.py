@@ -80,6 +80,7 @@ def test_attention():
     bad(INVALID, "scale", scale=0.0)
     bad(INVALID, "scale", scale=float("nan"))
     bad(INVALID, "scale", scale=float("inf"))
+    bad(INVALID, "scale", scale=3e38)  # infinite in units of log 2
     bad(INVALID, "window", window=-1)
     bad(INVALID, "max_len", max_len=1 << 31)
     bad(INVALID, "max_q", max_q=-1)
