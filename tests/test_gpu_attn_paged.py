@@ -401,3 +401,21 @@ def test_the_longest_cache(dt, cache, n):
     tol = (4 * sb[:n, :, None] + 2.0 ** -18) * ab[:n] + (HALF[dt] * np.abs(o[:n]) + (HALF["bf16"] * ab[:n] if dt == "bf16" else 0)) * 1.01
     assert (np.abs(got - o)[:n] <= tol + 2 * mass * np.abs(p.v).max()).all()
     assert (np.abs(got_lse - lse)[:n] <= 2 * sb[:n] + 2.0 ** -17 + 2.0 ** -22 * np.abs(lse[:n]) + mass).all()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("B,Hkv", [(64, 1), (70, 1), (128, 1), (129, 1), (257, 2), (700, 1)])
+def test_large_batches_with_a_few_long_caches(dt, cache, B, Hkv):
+    """One to three rows of each sequence, some without rows or without a cache, a few of them long enough to be divided."""
+    rng = np.random.default_rng(B)
+    ns = rng.integers(0, 4, B)
+    lens = np.where(rng.random(B) < 0.1, 0, ns + rng.integers(0, 90, B))
+    for b, n in ((0, 2300), (B // 2, 4100), (B - 1, 3000)):
+        ns[b], lens[b] = 2, n
+    p = Paged(ns.tolist(), lens.tolist(), Hkv, 32, 16, cache, seed=B)
+    a = Call(p, 2, dt).run()
+    a.check()
+    first = a.o.clone(), a.lse.clone()
+    a.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first[0], a.o) and torch.equal(first[1], a.lse)
