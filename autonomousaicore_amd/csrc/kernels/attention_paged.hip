@@ -12,6 +12,9 @@
 // O^T += V^T P^T from the accumulator registers.  fp32 runs v_mfma_f32_32x32x2_f32 and keeps P in
 // fp32; bf16 runs v_mfma_f32_32x32x16_bf16 with P rounded to bf16 (each weight off by at most 2^-8 of
 // itself, as an output is by its own rounding; the sum l adds them unrounded).
+//
+// bf16 queries: attention_paged_tiles.hip, or attention_paged_few.hip for up to 32 rows per key/value head.  fp32
+// queries: here, or attention_paged_f32_few.hip for up to 8.  Also here: the plan, the join and the launch.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -238,6 +241,7 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
 
 // ------------------------------------------------------------------------- joining splits
 // One wave per (token, head): M = max m_s, o = sum_s 2^((m_s - M) c) o_s / sum_s 2^((m_s - M) c) l_s.
+// Bound by reading the parts: 12 us for two of 2048 rows of 16 heads of 128 (34 MB read, 8 MB written: 3.5 TB/s).
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);

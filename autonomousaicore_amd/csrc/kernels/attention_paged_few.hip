@@ -15,6 +15,10 @@
 // a share: a block that ends one group and begins another waits twice for its first tile, which is then
 // most of its time.  Every block finds its part from offsets and lens by itself.
 //
+// 32 single tokens on e4m3 caches of up to 8000 tokens, 16 heads of 128 over 2: 29.7 us, 84 MB at 2.8 TB/s (the kernel
+// 24 us, of which 7 before the first tile, and 5 for the join); on bf16 caches of up to 16384, 16 over 8: 242 us,
+// 5.7 TB/s of the 6.5 that reading alone reaches; one token of 12 heads of 64 on 513: 8.6 us, a chain of latencies.
+//
 // Tiles arrive by direct global -> LDS copies, two stages per wave: 32 KB per wave at head_dim 128 in bf16 (one
 // block and up to 128 KB in flight per CU), 16 KB in e4m3 (two blocks).
 //

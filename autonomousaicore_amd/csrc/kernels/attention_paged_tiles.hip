@@ -13,6 +13,9 @@
 // converted once per block as they are stored (converted by each wave as it reads them, the
 // conversions would be four times as many, about as much as the softmax).
 //
+// 2048 rows of 16 heads of 128 over 2, behind 6144 cached tokens: 136 us, 883 TFLOP/s with the join of its two parts
+// per tile (124 us and 12 us); two blocks per CU, for their products fill each other's softmax.
+//
 // Tiles that some row does not see whole (the chunk's own keys, a window's edge: two or three per block) run first, in a
 // plain loop that masks and looks for non-finite v: the order of the keys is free, and the pipelined loop keeps
 // its registers (with masks in it, it spilled, and a reload waits for the copies in flight).
