@@ -419,3 +419,76 @@ def test_large_batches_with_a_few_long_caches(dt, cache, B, Hkv):
     a.run()
     torch.cuda.synchronize()
     assert torch.equal(first[0], a.o) and torch.equal(first[1], a.lse)
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("ns,lens", [([1, 2], [700, 1300]), ([40, 150], [700, 300])])
+def test_pools_past_four_gigabytes_in_every_form(dt, cache, ns, lens):
+    """The first pages at the far end of pools of 6 GB."""
+    hd, Hkv, ps = 64, 4, 64
+    p = Paged(ns, lens, Hkv, hd, ps, cache, seed=sum(ns))
+    small, n_pages = p.n_pages, 6 * 2 ** 30 // (ps * Hkv * hd * TORCH[cache].itemsize)
+    at = np.linspace(n_pages - 1, 0, small).astype(np.int64)
+    for name in "kv":
+        pair = []
+        for t in p.pool[name]:
+            big = None
+            if t is not None:
+                big = torch.empty((n_pages, *t.shape[1:]), dtype=t.dtype, device="cuda")
+                big[torch.from_numpy(at).cuda()] = t
+            pair.append(big)
+        p.pool[name] = tuple(pair)
+    table = p.table
+    p.table = np.where(table < small, at[np.minimum(table, small - 1)], 2 ** 31 - 7).astype(np.int32)
+    p.n_pages = n_pages
+    a = Call(p, 4, dt).run()
+    torch.cuda.synchronize()
+    p.table, p.n_pages = table, small
+    a.check()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("max_q,max_len", [(1, 1), (1, 5000), (7, 64)])
+def test_larger_than_promised_in_every_form(dt, cache, max_q, max_len):
+    p = Paged([20, 1, 90, 0, 9], [900, 2300, 95, 40, 700], 2, 32, 16, cache, seed=max_q)
+    a = Call(p, 4, dt)
+    a.sizes = lambda: (p.B, a.T, max_q, max_len)
+    a.run().check()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("n", [1, 3, 40, 200])
+@pytest.mark.parametrize("own", [True, False])
+def test_replays_of_every_form(dt, cache, n, own):
+    """With a workspace and without: three replays between eager calls on other queries and lengths, equal to the eager
+    result on the same."""
+    p = Paged([n, 1], [1700, 900], 2, 64, 16, cache, seed=n)
+    a = Call(p, 2, dt)
+    ws = torch.empty(max(a.bytes(), 16), dtype=torch.uint8, device="cuda") if own else None
+    c = p.struct()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def launch():
+        call("aic_hip_attn_paged", c, ptr(a.q), a.ld, ptr(a.o), a.ld, ptr(a.lse), ptr(p.dev_offs), ptr(p.dev_lens), *a.sizes(), a.H, 0, a.scale,
+             ptr(ws), 0 if ws is None else ws.numel(), CODE[dt], s.cuda_stream)
+
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        launch()
+    sizes = a.sizes()
+    a.sizes = lambda: sizes
+    for turn in range(3):
+        a.q.copy_(torch.randn(a.q.shape, generator=torch.Generator().manual_seed(turn)))
+        p.lens = [1700 - 200 * turn, 900 - turn]
+        p.dev_lens.copy_(torch.tensor(p.lens))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        torch.cuda.synchronize()
+        a.check()
+        a.buf.fill_(7.0)
+        a.lse.fill_(7.0)
+        launch()
+        torch.cuda.synchronize()
+        a.check()
+    _lib.call("aic_hip_mem_release_stream", s.cuda_stream)
