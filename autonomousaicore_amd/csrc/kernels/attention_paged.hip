@@ -13,7 +13,7 @@
 // fp32; bf16 runs v_mfma_f32_32x32x16_bf16 with P rounded to bf16 (each weight off by at most 2^-8 of
 // itself, as an output is by its own rounding; the sum l adds them unrounded).
 //
-// bf16 queries: attention_paged_tiles.hip, or attention_paged_few.hip for up to 32 rows per key/value head.  fp32
+// bf16 queries: attention_paged_tiles.hip, or attention_paged_few.hip for few rows per key/value head.  fp32
 // queries: here, or attention_paged_f32_few.hip for up to 8.  Also here: the plan, the join and the launch.
 #include <algorithm>
 #include <cmath>
@@ -336,9 +336,10 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     // the cache's type does not tell the queries' (e4m3 serves both): room for either
     int64_t n = 0;
     const int64_t G = H / c.kv_heads;
-    if (c.type != DType::Float32 && few_rows(max_q, G))
-        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, c.type == DType::UInt8);
-    if (c.type != DType::Float32 && !few_rows(max_q, G))
+    const bool e4m3 = c.type == DType::UInt8, few = few_rows(max_q, G, c.head_dim, e4m3);
+    if (c.type != DType::Float32 && few)
+        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, e4m3);
+    if (c.type != DType::Float32 && !few)
         n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
         n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
@@ -374,7 +375,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_q = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q * size % 16 == 0;
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
-    const bool few = dt == DType::BFloat16 && few_rows(max_q, a.G);
+    const bool e4m3 = c.type == DType::UInt8, few = dt == DType::BFloat16 && few_rows(max_q, a.G, c.head_dim, e4m3);
     const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim);
     Plan p = plan(B, T, max_len, H, c.kv_heads, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
@@ -386,7 +387,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         workspace = stream_scratch(static_cast<size_t>(need), s);
     if (need == 0) workspace = nullptr;
     if (few) {
-        const bool e4m3 = c.type == DType::UInt8;  // need may be the other kernel's alone
+        // need may be the other kernel's alone
         const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, e4m3) > 0;
         attn_paged_few(a, max_q, e4m3, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;

@@ -261,7 +261,7 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, const Rows<HD / 32
 
 // Few query rows per key/value head, bf16 queries (attention_paged_few.hip): row groups of `group` rows; with a
 // workspace the batch's keys are cut into equal shares, one per resident block.
-bool few_rows(int64_t max_q, int64_t G);
+bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, bool e4m3);
 int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3);
 void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s);
 

@@ -492,3 +492,12 @@ def test_replays_of_every_form(dt, cache, n, own):
         torch.cuda.synchronize()
         a.check()
     _lib.call("aic_hip_mem_release_stream", s.cuda_stream)
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("ns,lens,H,Hkv,window", [([8, 5, 1], [2600, 1500, 40], 8, 1, 0), ([33, 64], [1400, 70], 1, 1, 0), ([64, 2], [500, 300], 2, 2, 90),
+                                                  ([65], [1300], 1, 1, 0)])
+def test_two_groups_of_rows(dt, cache, ns, lens, H, Hkv, window):
+    """33 to 65 rows per key/value head of 128."""
+    p = Paged(ns, lens, Hkv, 128, 16, cache, seed=len(ns))
+    Call(p, H, dt, window).run().check()
