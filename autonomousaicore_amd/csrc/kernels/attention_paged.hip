@@ -299,13 +299,17 @@ struct Plan {
 };
 // Parts of the keys where the query tiles alone do not fill the card: as many as make one round of about 512 blocks (two
 // per CU; 2048 rows of 16 heads twice: 52.6 us in 464 blocks, 73.6 us in 928), of at least 448 keys where
-// there are more than four (256 rows on 4096 keys: 26.2 us in 8 parts, 30.5 us in 16, 33.0 us in 4).
-// R: query rows of a block.
-Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, int64_t Hkv, int64_t R) {
+// there are more than four (256 rows on 4096 keys: 26.2 us in 8 parts, 30.5 us in 16, 33.0 us in 4).  Where the parts'
+// rows are little to join (4 MB), of 128 keys from 512 on: 8 rows of 16 heads of 128 over 2 on 2000 keys, 19.6 us in 4
+// parts and 15.5 us in 15; one row in fp32 on 1000, 42.0 us in 3 and 26.7 us in 7; but 40 of 12 heads of 64 on 300,
+// 10.7 us in one and 12.2 us in 2.  R: query rows of a block.
+Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, const KVPages& c, int64_t R) {
+    const int64_t Hkv = c.kv_heads;
     Plan p{tile_bound(T, H / Hkv, B, R), 1};
     // two times the blocks there probably are; tiles of up to 8 rows hold a sequence each
     const int64_t twice = (R <= 8 ? 2 * std::min(B, T) : 2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;
-    const int64_t most = std::max<int64_t>(std::min<int64_t>(4, max_len / 256), max_len / 448);
+    int64_t most = std::max<int64_t>(std::min<int64_t>(4, max_len / 256), max_len / 448);
+    if (max_len >= 512) most = std::max(most, std::min(max_len / 128, (int64_t{4} << 20) / (T * H * (c.head_dim + 2) * 4)));
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
@@ -340,9 +344,9 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     if (c.type != DType::Float32 && few)
         n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, e4m3);
     if (c.type != DType::Float32 && !few)
-        n = plan_bytes(plan(B, T, max_len, H, c.kv_heads, 128), T, H, c.head_dim);
+        n = plan_bytes(plan(B, T, max_len, H, c, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c.kv_heads, f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c, f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
     return n;
 }
 
@@ -377,7 +381,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
 
     const bool e4m3 = c.type == DType::UInt8, few = dt == DType::BFloat16 && few_rows(max_q, a.G, c.head_dim, e4m3);
     const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim);
-    Plan p = plan(B, T, max_len, H, c.kv_heads, R);
+    Plan p = plan(B, T, max_len, H, c, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
     if (workspace)
