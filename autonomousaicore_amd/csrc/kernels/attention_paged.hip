@@ -29,16 +29,19 @@ namespace {
 // ----------------------------------------------------------------------- the fp32 kernel
 // Blocks of four waves: 4 / SH sets of 32 query rows, over tiles of 32 SH keys that the SH waves of a set
 // share, 32 each, their states joined at the end.  SH = 1 where the batch fills the card with blocks of
-// 128 rows; otherwise more and smaller blocks with fewer steps (SH = 4, or 2 at head_dim 128, where tiles of
-// 128 keys would leave one block per CU).  Tiles are staged through registers: the next one's loads are in
-// flight during this one's products; the page ids come from LDS, since loads that wait for ids from memory
-// stop the wave in the middle of its products (859 rows of 16 heads of 64: 54.5 us so, 43.6 us from LDS;
-// 1000 rows on 2000 keys of 128, 16 heads over 2: 326 us, 210 us, 58 TFLOP/s).  Bound by the fp32 matrix
-// pipe (64 cycles per v_mfma_f32_32x32x2_f32) and the staging between its runs.
+// 128 rows; otherwise more and smaller blocks with fewer steps (f32_rows).
+//
+// One tile of K and one of V are in LDS: the next K is on its way while this V is multiplied, the next V while that K
+// is, so nothing is staged twice and no copy is waited for.  The copies go straight to LDS (codes through registers)
+// from page ids in LDS, and fragments are read a group of four products ahead from addresses made anew for each
+// tile, so that two blocks of head_dim 128 keep their registers on one CU.  Bound by the fp32 matrix pipe (64 cycles
+// per v_mfma_f32_32x32x2_f32): 4000 rows of 16 heads of 128, 809 us, 81 TFLOP/s of 154; 1000 on 2000 keys, 16 heads
+// over 2, 158 us, 78 TFLOP/s (through registers, one block per CU: 210 us; from page ids in memory: 326 us); 856 of 16
+// heads of 64, 43 us, whose longest block takes most of it.
 constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <typename CT, int HD, int SH>
-__global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
     constexpr int SETS = 4 / SH, R = 32 * SETS, KT = 32 * SH, OB = HD / 32;
     constexpr int UPR = HD * sizeof(CT) / 16;   // 16-byte units of a cached row
     constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
@@ -71,8 +74,8 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
     k_lo &= ~63;
     part_of_keys(k_lo, k_hi, split, a.nsplit);
     // keys of this wave's rows: those of the set, none behind the sequence's last row
-    const int set_r0 = r0 + set * 32, set_first = sq.len - sq.n + set_r0 / a.G;
-    const int set_hi = set_r0 < rows ? min(k_hi, sq.len - sq.n + (min(set_r0 + 32, rows) - 1) / a.G + 1) : 0;
+    const int set_r0 = r0 + set * 32, set_first = sq.len - sq.n + set_r0 / a.G, set_last = sq.len - sq.n + (min(set_r0 + 32, rows) - 1) / a.G;
+    const int set_hi = set_r0 < rows ? min(k_hi, set_last + 1) : 0;
     const int set_lo = a.window > 0 ? max(set_first, 0) - a.window + 1 : 0;
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));  // keys from lo on that it sees here
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;                          // of this split
@@ -89,114 +92,173 @@ __global__ __launch_bounds__(256) void attn_paged_f32_k(PagedArgs a) {
             qf[cc] = !real ? make_float4(0, 0, 0, 0) : a.vec_q ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
         }
 
-        uint4 rk[NU], rv[NU];
-        [[maybe_unused]] uint32_t xk[NU], xv[NU];  // exponent bytes
+        // Where this lane's fragments lie, in bytes: K row sub + lane % 32, chunk 2 c + h; V row sub + 8 (e >> 2) + 4 h + (e & 3),
+        // column 32 ob + lane % 32.  The swizzles are exclusive-ors of a lane's part and constants.
+        const int lr = lane & 31;
+        const int k_lane = (sub + lr) * HD * 4 + ((hl ^ (HD == 32 ? (lr >> 1) & 7 : lr & 15)) << 4);
+        const int v_lane = (sub + 4 * hl) * HD * 4 + (((lr >> 2) ^ (HD == 32 ? 2 * hl : 4 * hl)) << 4) + (lr & 3) * 4;
+        auto k_at = [&](int lane_part, int c) { return (lane_part ^ ((2 * c & 15) << 4)) + ((2 * c & 16) << 4); };
+        auto v_at = [&](int lane_part, int e, int ob) {
+            const int g = (e >> 2) & 1, row = (8 * (e >> 2) + (e & 3)) * HD * 4;
+            if constexpr (HD == 32) return (lane_part ^ (((e & 3) >> 1 | g << 2) << 4)) + row;
+            else return (lane_part ^ ((e & 3) << 4)) + row + (ob ^ g) * 128;
+        };
+        // Copies of K and V of a tile: in fp32 straight to LDS, 1 KB per wave's instruction; codes through registers.
+        struct Codes {
+            uint4 w[NU];
+            uint32_t e[NU];
+        };
+        [[maybe_unused]] Codes codes;
         const int32_t* tr = a.kv.table + b * a.kv.ld_table;
-        int w1 = 0, p0 = 0;  // end and first page of the keys whose page ids are in LDS
-        auto load = [&](int k0) {
-#pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                const int u = i * 256 + static_cast<int>(threadIdx.x);
-                // keys past the last are read as the last one: hidden below
-                const int key = min(k0 + min(u / UPR, KT - 1), w1 - 1), pi = a.kv.page_index(key), page = ids[pi - p0];
-                const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * a.kv.ps + (key - pi * a.kv.ps);
-                const int64_t at = row * (UPR * 16) + (u % UPR) * 16;
-                const char* none = reinterpret_cast<const char*>(&kNoPage);
-                rk[i] = *reinterpret_cast<const uint4*>(page >= 0 ? a.kv.kp + at : none);
-                rv[i] = *reinterpret_cast<const uint4*>(page >= 0 ? a.kv.vp + at : none);
-                if constexpr (E4) {
-                    xk[i] = page >= 0 ? a.kv.ke[row] : 127;
-                    xv[i] = page >= 0 ? a.kv.ve[row] : 127;
-                }
-            }
-        };
-        auto put = [&](char* tile, int row, int c, uint4 x, [[maybe_unused]] uint32_t xe) {
-            if constexpr (!E4) {
-                *reinterpret_cast<uint4*>(tile + chunk_at<float, HD>(row, c)) = x;
-            } else {
-                const float s = exp_scale(xe);
-                const uint2 w[2] = {make_uint2(x.x, x.y), make_uint2(x.z, x.w)};
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float y[8];
-                    e4m3_floats(w[j], s, y);
-                    *reinterpret_cast<float4*>(tile + chunk_at<float, HD>(row, 4 * c + 2 * j)) = make_float4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<float4*>(tile + chunk_at<float, HD>(row, 4 * c + 2 * j + 1)) = make_float4(y[4], y[5], y[6], y[7]);
-                }
-            }
-        };
-        auto bad_v = [&] {  // this thread's part of the V tile in registers holds an infinity or NaN
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < NU; ++i) bad |= non_finite_bits<CT>(rv[i]);
-            return bad != 0;
-        };
-
         const int window_keys = min((kIds - 1) * a.kv.ps, 1 << 20) & ~127;  // keys whose page ids fit: at least 384
-        for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
-            if (k0 >= w1) {  // the next page ids
-                __syncthreads();
-                w1 = k0 + min(k_hi - k0, window_keys);
-                p0 = a.kv.page_index(k0);
-                for (int i = threadIdx.x; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
-                    const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
-                    ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
-                }
-                __syncthreads();
-                load(k0);
-            }
-            // every row of the block sees every key of the tile?
-            const bool open = k0 + KT - 1 <= first_pos && k0 + KT <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
-            const int poison = __syncthreads_or(!open && bad_v());  // also: everyone is done with the last tile
-#pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                const int u = i * 256 + static_cast<int>(threadIdx.x);
-                if (KT * UPR % 256 == 0 || u < KT * UPR) {
-                    put(ks, u / UPR, u % UPR, rk[i], E4 ? xk[i] : 0);
-                    put(vs, u / UPR, u % UPR, rv[i], E4 ? xv[i] : 0);
-                }
+        for (int w0 = k_lo, w1; w0 < k_hi; w0 = w1) {
+            w1 = w0 + min(k_hi - w0, window_keys);
+            const int p0 = a.kv.page_index(w0), nt = (w1 - w0 + KT - 1) / KT;
+            __syncthreads();
+            for (int i = threadIdx.x; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
+                const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
+                ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
             }
             __syncthreads();
-            if (k0 + KT < w1) load(k0 + KT);
-            if (k0 + sub >= set_hi || k0 + sub + 31 < set_lo) continue;  // nothing of this tile for this wave
-
-            f32x16 sc[1];
-            zero(sc[0]);
+            auto row_at = [&](int key) -> int64_t {  // row in the pools, negative without a page; past the last key: the last
+                key = min(key, w1 - 1);
+                const int pi = a.kv.page_index(key), page = ids[pi - p0];
+                const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * a.kv.ps + (key - pi * a.kv.ps);
+                return page < 0 ? -1 : row;
+            };
+            const char* none = reinterpret_cast<const char*>(&kNoPage);
+            auto fetch = [&](const char* pool, [[maybe_unused]] const uint8_t* exps, int t, [[maybe_unused]] char* dst) {
+                if constexpr (E4) {
 #pragma unroll
-            for (int cc = 0; cc < KF; ++cc) {
-                const float4 x = *reinterpret_cast<const float4*>(ks + chunk_at<float, HD>(sub + (lane & 31), 2 * cc + hl));
-                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, qf[cc].x, sc[0], 0, 0, 0);
-                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, qf[cc].y, sc[0], 0, 0, 0);
-                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, qf[cc].z, sc[0], 0, 0, 0);
-                sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, qf[cc].w, sc[0], 0, 0, 0);
-            }
-            auto seen = [&](int j) { return static_cast<uint32_t>(k0 + sub + j - lo) < span; };
-            if (!open)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
-            st_.absorb(mx, a.c);
-            const float off = st_.offset(a.c);
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[0][e] = weight<float>(sc[0][e], a.c, off);
-                sum += sc[0][e];
-            }
-            st_.add(sum);
-            if (poison) {
-                add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<float, HD>(vs, sub + key, d); }, seen);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-#pragma unroll
-                    for (int ob = 0; ob < OB; ++ob) {
-                        const int d = 32 * ob + (lane & 31), row = sub + 8 * (e >> 2) + 4 * hl + (e & 3);
-                        const float x = *reinterpret_cast<const float*>(vs + chunk_at<float, HD>(row, d >> 2) + (d & 3) * 4);
-                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, sc[0][e], st_.o[ob], 0, 0, 0);
+                    for (int i = 0; i < NU; ++i) {
+                        const int u = i * 256 + static_cast<int>(threadIdx.x);
+                        const int64_t row = row_at(w0 + t * KT + min(u / UPR, KT - 1));
+                        codes.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * HD + (u % UPR) * 16 : none);
+                        codes.e[i] = row >= 0 ? exps[row] : 127;
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < TILE / 4096; ++i) {
+                        const int at = (4 * i + wave) * 1024, rr = (at + lane * 16) / (HD * 4), ch = lane % (HD / 4);
+                        const int64_t row = row_at(w0 + t * KT + rr);
+                        dma16(row >= 0 ? pool + row * (HD * 4) + ((ch ^ (HD == 32 ? (rr >> 1) & 7 : rr & 15)) << 4) : none, dst + at);
+                    }
+                }
+            };
+            auto put = [&]([[maybe_unused]] char* dst) {  // codes to LDS
+                if constexpr (E4) {
+#pragma unroll
+                    for (int i = 0; i < NU; ++i) {
+                        const int u = i * 256 + static_cast<int>(threadIdx.x), row = u / UPR, c = u % UPR;
+                        if (KT * UPR % 256 != 0 && u >= KT * UPR) continue;
+                        const float s = exp_scale(codes.e[i]);
+                        const uint2 w[2] = {make_uint2(codes.w[i].x, codes.w[i].y), make_uint2(codes.w[i].z, codes.w[i].w)};
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            float y[8];
+                            e4m3_floats(w[j], s, y);
+                            *reinterpret_cast<float4*>(dst + chunk_at<float, HD>(row, 4 * c + 2 * j)) = make_float4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<float4*>(dst + chunk_at<float, HD>(row, 4 * c + 2 * j + 1)) = make_float4(y[4], y[5], y[6], y[7]);
+                        }
+                    }
+                }
+            };
+            auto meet = [&] {  // what this wave brought is there and what it read is read; then everyone's
+                wait_lds();
+                if constexpr (!E4) wait_vmcnt<0>();
+                __builtin_amdgcn_s_barrier();
+            };
+            fetch(a.kv.kp, a.kv.ke, 0, ks);
+            put(ks);
+            meet();
+            fetch(a.kv.vp, a.kv.ve, 0, vs);
+            put(vs);
+            for (int t = 0; t < nt; ++t) {
+                const int k0 = w0 + t * KT;
+                const bool next = t + 1 < nt, mine = k0 + sub < set_hi && k0 + sub + 31 >= set_lo;  // else no row of this wave sees a key of its
+                // made anew for each tile: dozens of addresses kept through the loop would take the registers of a second block
+                int kl = k_lane, vl = v_lane;
+                asm volatile("" : "+v"(kl), "+v"(vl));
+                f32x16 sc[1];
+                if (E4 && next) fetch(a.kv.kp, a.kv.ke, t + 1, ks);
+                if (mine) {
+                    zero(sc[0]);
+                    // fragments are read one group of four products ahead, no further
+                    float4 kx[2];
+                    kx[0] = *reinterpret_cast<const float4*>(ks + k_at(kl, 0));
+#pragma unroll
+                    for (int cc = 0; cc < KF; ++cc) {
+                        if (cc + 1 < KF) kx[(cc + 1) & 1] = *reinterpret_cast<const float4*>(ks + k_at(kl, cc + 1));
+                        const float4 x = kx[cc & 1];
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, qf[cc].x, sc[0], 0, 0, 0);
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, qf[cc].y, sc[0], 0, 0, 0);
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, qf[cc].z, sc[0], 0, 0, 0);
+                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, qf[cc].w, sc[0], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                meet();  // V is there, K has been read
+                if (next) {
+                    if constexpr (E4) {
+                        put(ks);
+                        fetch(a.kv.vp, a.kv.ve, t + 1, vs);
+                    } else {
+                        fetch(a.kv.kp, a.kv.ke, t + 1, ks);
+                    }
+                }
+                if (mine) {
+                    const int kw = k0 + sub;  // this wave's first key of the tile
+                    // every row of the set sees every one of them?
+                    const bool open = kw + 31 <= set_first && kw + 32 <= k_hi && (a.window <= 0 || kw > set_last - a.window);
+                    auto seen = [&](int j) { return static_cast<uint32_t>(kw + j - lo) < span; };
+                    bool poison = false;  // a hidden key beside a non-finite v
+                    if (!open) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
+                        uint32_t bits = 0;
+#pragma unroll 4
+                        for (int i = 0; i < HD / 8; ++i)
+                            bits |= non_finite_bits<float>(*reinterpret_cast<const uint4*>(vs + sub * HD * 4 + i * 1024 + lane * 16));
+                        poison = __any(bits != 0);
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
+                    st_.absorb(mx, a.c);
+                    const float off = st_.offset(a.c);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        sc[0][e] = weight<float>(sc[0][e], a.c, off);
+                        sum += sc[0][e];
+                    }
+                    st_.add(sum);
+                    if (poison) {
+                        add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<float, HD>(vs, sub + key, d); }, seen);
+                    } else {
+                        float vx[2][4];
+                        auto read = [&](int g, float (&x)[4]) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const float*>(vs + v_at(vl, (4 * g + j) / OB, (4 * g + j) % OB));
+                        };
+                        read(0, vx[0]);
+#pragma unroll
+                        for (int g = 0; g < 4 * OB; ++g) {
+                            if (g + 1 < 4 * OB) read(g + 1, vx[(g + 1) & 1]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int e = (4 * g + j) / OB, ob = (4 * g + j) % OB;
+                                st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[g & 1][j], sc[0][e], st_.o[ob], 0, 0, 0);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+                meet();  // K of the next tile is there, V has been read
+                if (next) {
+                    if constexpr (E4) put(vs);
+                    else fetch(a.kv.vp, a.kv.ve, t + 1, vs);
+                }
             }
         }
     }
@@ -313,10 +375,13 @@ Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, const KVPages& c, in
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
-// fp32: query rows of a block, fewer where blocks of 128 rows are fewer than two per CU.
-int64_t f32_rows(int64_t B, int64_t T, int64_t max_q, int64_t H, int64_t Hkv, int64_t hd) {
+// fp32: query rows of a block: fewer than 128 where such blocks are fewer than two per CU; at head_dim 128 then 64, two
+// blocks to a CU, or 32 where a block is alone there and the keys are not divided: 300 rows of 16 heads on 300 keys,
+// 33.9 us in 32 and 39.7 us in 64; on 452 rows and 554 keys, in two parts, 59.0 and 48.4 us.
+int64_t f32_rows(int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t Hkv, int64_t hd) {
     if (const int few = f32_few_rows(max_q, H / Hkv)) return few;
-    return tile_bound(T, H / Hkv, B, 128) * Hkv >= 512 ? 128 : hd == 128 ? 64 : 32;
+    if (tile_bound(T, H / Hkv, B, 128) * Hkv >= 512) return 128;
+    return hd == 128 && (max_len >= 512 || tile_bound(T, H / Hkv, B, 32) * Hkv > 256) ? 64 : 32;
 }
 int64_t plan_bytes(const Plan& p, int64_t T, int64_t H, int64_t hd) {
     return p.nsplit <= 1 ? 0 : p.nsplit * T * H * (hd + 2) * 4;
@@ -346,7 +411,7 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     if (c.type != DType::Float32 && !few)
         n = plan_bytes(plan(B, T, max_len, H, c, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c, f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c, f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
     return n;
 }
 
@@ -380,7 +445,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
 
     const bool e4m3 = c.type == DType::UInt8, few = dt == DType::BFloat16 && few_rows(max_q, a.G, c.head_dim, e4m3);
-    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, H, c.kv_heads, c.head_dim);
+    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim);
     Plan p = plan(B, T, max_len, H, c, R);
     const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
     const StreamScratchUse use(s);
@@ -413,7 +478,8 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
             const auto grid = static_cast<unsigned>(blocks);
             if (R <= 8) attn_paged_f32_few(a, static_cast<int>(R), sizeof(ct) == 1, D, grid, s);
             else if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
-            else attn_paged_f32_k<decltype(ct), D, D == 128 ? 2 : 4><<<grid, 256, 0, s>>>(a);
+            else if (R == 64) attn_paged_f32_k<decltype(ct), D, 2><<<grid, 256, 0, s>>>(a);
+            else attn_paged_f32_k<decltype(ct), D, 4><<<grid, 256, 0, s>>>(a);
             AIC_LAUNCH_CHECK("attn_paged");
         }
         if (a.nsplit > 1) {
