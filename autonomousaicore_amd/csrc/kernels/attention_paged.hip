@@ -14,7 +14,7 @@
 // itself, as an output is by its own rounding; the sum l adds them unrounded).
 //
 // bf16 queries: attention_paged_tiles.hip, or attention_paged_few.hip for few rows per key/value head.  fp32
-// queries: here, or attention_paged_f32_few.hip for up to 8.  Also here: the plan, the join and the launch.
+// queries: here, or attention_paged_f32_few.hip for up to 4.  Also here: the plan, the join and the launch.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -363,13 +363,12 @@ struct Plan {
 // per CU; 2048 rows of 16 heads twice: 52.6 us in 464 blocks, 73.6 us in 928), of at least 448 keys where
 // there are more than four (256 rows on 4096 keys: 26.2 us in 8 parts, 30.5 us in 16, 33.0 us in 4).  Where the parts'
 // rows are little to join (4 MB), of 128 keys from 512 on: 8 rows of 16 heads of 128 over 2 on 2000 keys, 19.6 us in 4
-// parts and 15.5 us in 15; one row in fp32 on 1000, 42.0 us in 3 and 26.7 us in 7; but 40 of 12 heads of 64 on 300,
-// 10.7 us in one and 12.2 us in 2.  R: query rows of a block.
+// parts and 15.5 us in 15; but 40 rows of 12 heads of 64 on 300, 10.7 us in one and 12.2 us in 2.  R: query rows of a block.
 Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, const KVPages& c, int64_t R) {
     const int64_t Hkv = c.kv_heads;
     Plan p{tile_bound(T, H / Hkv, B, R), 1};
-    // two times the blocks there probably are; tiles of up to 8 rows hold a sequence each
-    const int64_t twice = (R <= 8 ? 2 * std::min(B, T) : 2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;
+    // two times the blocks there probably are; tiles of up to 4 rows hold a sequence each
+    const int64_t twice = (R <= 4 ? 2 * std::min(B, T) : 2 * T * (H / Hkv) / R + std::min(B, T)) * Hkv;
     int64_t most = std::max<int64_t>(std::min<int64_t>(4, max_len / 256), max_len / 448);
     if (max_len >= 512) most = std::max(most, std::min(max_len / 128, (int64_t{4} << 20) / (T * H * (c.head_dim + 2) * 4)));
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
@@ -476,7 +475,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
             attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
         } else {
             const auto grid = static_cast<unsigned>(blocks);
-            if (R <= 8) attn_paged_f32_few(a, static_cast<int>(R), sizeof(ct) == 1, D, grid, s);
+            if (R <= 4) attn_paged_f32_few(a, static_cast<int>(R), sizeof(ct) == 1, D, grid, s);
             else if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
             else if (R == 64) attn_paged_f32_k<decltype(ct), D, 2><<<grid, 256, 0, s>>>(a);
             else attn_paged_f32_k<decltype(ct), D, 4><<<grid, 256, 0, s>>>(a);

@@ -265,7 +265,7 @@ bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, bool e4m3);
 int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3);
 void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s);
 
-// Up to 8 query rows per key/value head, fp32 queries (attention_paged_f32_few.hip): tiles of so many rows, 0 for
+// Up to 4 query rows per key/value head, fp32 queries (attention_paged_f32_few.hip): tiles of so many rows, 0 for
 // more of them; tiles x splits x key/value heads blocks.
 int f32_few_rows(int64_t max_q, int64_t G);
 void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, unsigned blocks, hipStream_t s);

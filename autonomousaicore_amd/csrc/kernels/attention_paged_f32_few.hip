@@ -1,17 +1,16 @@
-// Attention over the paged cache, fp32 queries: up to 8 query rows per key/value head (single tokens,
+// Attention over the paged cache, fp32 queries: up to 4 query rows per key/value head (single tokens, a few
 // drafted ones).
 //
 // The formulas are attention_paged.hip's.  A tile of the matrix pipe has 32 rows: with one row in it,
-// 64 steps of 64 cycles per 32 keys of 128 cost more than the keys' bytes (30 single tokens of 16
-// heads of 128 on 1000 keys: 205 us).  Here hd / 4 lanes hold one key's four values each, q alike; a
+// 128 steps of 64 cycles per 32 keys of 128 cost more than the keys' bytes.  Here hd / 4 lanes hold one key's four values each, q alike; a
 // score is four products and a sum over those lanes, which leaves it in all of them, so that the same
 // lanes weigh their four values of v without an exchange.  Each group of lanes keeps maximum, sum and
 // output of its own keys; they are joined once at the end.  The waves of a block take batches of keys in
 // turn and share nothing until then; 8 loads of 1 KB of K and of V per wave are in flight, with enough waves
-// per CU to cover them (16 loads: 71 us for that case, 8: 66 us, which is 4.8 TB/s).  Bound by the bytes of
-// the cache for one and two rows, by the vector instructions behind them: a tile of 8 rows takes as long as
-// the matrix pipe's (26 us and 22 us at 30 tokens of 16 heads of 64 over 2, 46 us and 54 us at heads of
-// 128), two of them longer (16 rows of 128: 68 us and 55 us).
+// per CU to cover them (30 single tokens of 16 heads of 128 on 1000 keys: 66 us, 4.8 TB/s; 16 loads: 71 us).  Bound by the bytes of
+// the cache for one and two rows, by the vector instructions behind them; tiles of 8 rows would take 24.5 us for 30
+// tokens of 16 heads of 64 over 2 on 1000 keys, and the matrix pipe 20.9 us (59 and 52 us for 30 sequences of 7
+// rows of 12 heads; the other way round, 26 and 30 us, for 10 of them).
 #include <type_traits>
 
 #include "attention_paged.hpp"
@@ -181,10 +180,10 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
 
 }  // namespace
 
-// Row tiles of 1, 2, 4 or 8 rows for up to 8 rows, 0: for the matrix pipe.
+// Row tiles of 1, 2 or 4 rows for up to 4 rows, 0: for the matrix pipe.
 int f32_few_rows(int64_t max_q, int64_t G) {
     const int64_t rows = max_q * G;
-    return rows > 8 ? 0 : rows > 4 ? 8 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
+    return rows > 4 ? 0 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
 }
 
 void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, unsigned blocks, hipStream_t s) {
@@ -193,8 +192,7 @@ void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, u
         constexpr int D = decltype(hd)::value;
         if (rows == 1) attn_paged_f32_few_k<C, D, 1><<<blocks, 256, 0, s>>>(a);
         else if (rows == 2) attn_paged_f32_few_k<C, D, 2><<<blocks, 256, 0, s>>>(a);
-        else if (rows == 4) attn_paged_f32_few_k<C, D, 4><<<blocks, 256, 0, s>>>(a);
-        else attn_paged_f32_few_k<C, D, 8><<<blocks, 256, 0, s>>>(a);
+        else attn_paged_f32_few_k<C, D, 4><<<blocks, 256, 0, s>>>(a);
         AIC_LAUNCH_CHECK("attn_paged few, fp32");
     };
     auto type = [&](auto hd) { e4m3 ? run(uint8_t{}, hd) : run(float{}, hd); };
