@@ -119,8 +119,10 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
                     if (!open) s[i] = static_cast<uint32_t>(k0 + i * KI + grp - lo[r]) < span[r] ? s[i] : -INFINITY;
                     mx = fmaxf(mx, s[i]);
                 }
-                // keys that this group's row has seen only scores of -infinity from count from zero
-                const float off = mx == -INFINITY ? 0.0f : -mx * a.c, alpha = __builtin_amdgcn_exp2f(fmaf(m[r], a.c, off));
+                // keys that this group's row has seen only scores of -infinity from count from zero; alpha is 1 exactly where the
+                // maximum stands (an fma with off would leave off's rounding error in it, once per batch of keys)
+                const float off = mx == -INFINITY ? 0.0f : -mx * a.c;
+                const float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[r] - mx) * a.c);
                 m[r] = mx;
                 l[r] *= alpha;
                 o[r].x *= alpha, o[r].y *= alpha, o[r].z *= alpha, o[r].w *= alpha;
