@@ -70,7 +70,7 @@ struct DraftArgs {
     int B, V, parts, runs;
     int64_t T, max_q;
     double c;  // log2(e) / temperature; 0: greedy
-    // logits below the maximum less reach weigh under 2^-1000, and fp32 tells them from a maximum under plain_top
+    // logits below the maximum less reach weigh under 2^-1000; maxima under plain_top, 8 reaches, times c are below 2^13
     float reach, plain_top;
     int64_t *tokens, *counts, *new_lens;
     Stat *sz, *sy;       // [T][parts]
@@ -171,7 +171,10 @@ __global__ __launch_bounds__(kStatWaves * kWave) void draft_stats_k(DraftArgs a)
             st.best = wave_all(best, Min{});
         } else {
             double sum = 0.0;
-            if (fabsf(mx) < a.plain_top) {  // 2^-1000 of the maximum is a step that fp32 resolves: clamped there, also NaN
+            // Clamped at 2^-1000 of the maximum, also NaN.  One product with mx * c rounded beforehand: that rounding, 2^-41
+            // for maxima up to 8 reaches, moves all weights of the part by 3e-13 of themselves.  It would be 1e-7 for the largest
+            // maxima, and another one in p than in d: those take the exact difference.
+            if (fabsf(mx) < a.plain_top) {
                 const float low = mx - a.reach;
                 const double top = -static_cast<double>(mx) * a.c;
 #pragma unroll
@@ -460,7 +463,7 @@ void verify_drafts(const void* logits, int64_t ld, const void* draft, int64_t ld
     a.T = T, a.max_q = max_q;
     a.c = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(temperature);
     a.reach = 1000.0f * temperature * 0.6931f;  // under 1000 / c: 2^-999.9
-    a.plain_top = a.reach < 1e30f ? std::min(a.reach * 0x1p20f, 1e30f) : 0.0f;
+    a.plain_top = a.reach < 1e30f ? a.reach * 8.0f : 0.0f;
     a.tokens = tokens, a.counts = counts, a.new_lens = new_lens;
     a.sz = static_cast<Stat*>(workspace);
     a.sy = a.sz + T * parts;
