@@ -41,7 +41,7 @@ namespace {
 constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <typename CT, int HD, int SH>
-__global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
+__device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block, float down) {
     constexpr int SETS = 4 / SH, R = 32 * SETS, KT = 32 * SH, OB = HD / 32;
     constexpr int UPR = HD * sizeof(CT) / 16;   // 16-byte units of a cached row
     constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
@@ -52,13 +52,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
     char *ks = tiles, *vs = tiles + TILE;
 
     const int Hkv = a.kv.Hkv;
-    const int kvh = static_cast<int>(blockIdx.x) % Hkv;
-    const int rest = static_cast<int>(blockIdx.x) / Hkv;
+    const int kvh = block % Hkv;
+    const int rest = block / Hkv;
     const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
-    if (!find_tile<R>(a, tile, b, local)) return;
+    if (!find_tile<R>(a, tile, b, local)) return false;
     const Seq sq = wave_sequence(a, b);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     const int set = wave % SETS, share = wave / SETS, sub = 32 * share;  // this wave's rows of the block and keys of a tile
     const int rows = sq.n * a.G, r0 = local * R, r = r0 + set * 32 + (lane & 31);
     const bool real = r < rows;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
             w1 = w0 + min(k_hi - w0, window_keys);
             const int p0 = a.kv.page_index(w0), nt = (w1 - w0 + KT - 1) / KT;
             __syncthreads();
-            for (int i = threadIdx.x; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
+            for (int i = tid; i <= a.kv.page_index(w1 - 1) - p0; i += 256) {
                 const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
                 ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
             }
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
                 if constexpr (E4) {
 #pragma unroll
                     for (int i = 0; i < NU; ++i) {
-                        const int u = i * 256 + static_cast<int>(threadIdx.x);
+                        const int u = i * 256 + tid;
                         const int64_t row = row_at(w0 + t * KT + min(u / UPR, KT - 1));
                         codes.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * HD + (u % UPR) * 16 : none);
                         codes.e[i] = row >= 0 ? exps[row] : 127;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
                 if constexpr (E4) {
 #pragma unroll
                     for (int i = 0; i < NU; ++i) {
-                        const int u = i * 256 + static_cast<int>(threadIdx.x), row = u / UPR, c = u % UPR;
+                        const int u = i * 256 + tid, row = u / UPR, c = u % UPR;
                         if (KT * UPR % 256 != 0 && u >= KT * UPR) continue;
                         const float s = exp_scale(codes.e[i]);
                         const uint2 w[2] = {make_uint2(codes.w[i].x, codes.w[i].y), make_uint2(codes.w[i].z, codes.w[i].w)};
@@ -225,11 +225,11 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
                     st_.absorb(mx, a.c);
-                    const float off = st_.offset(a.c);
+                    const float off = st_.offset(a.c, down);
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        sc[0][e] = weight<float>(sc[0][e], a.c, off);
+                        sc[0][e] = weight(sc[0][e], a.c, off);
                         sum += sc[0][e];
                     }
                     st_.add(sum);
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
                 if (share > 0) os[at(share, ob * 16 + e)] = st_.o[ob][e];
             }
         __syncthreads();
-        if (share > 0) return;
+        if (share > 0) return false;
 #pragma unroll
         for (int ob = 0; ob < OB; ++ob)
 #pragma unroll
@@ -298,11 +298,16 @@ __global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
         st_.m = M;
         st_.l = l;
     }
-    if (real) store_row<float, HD>(a, st_, t, head, empty, split);
+    return real && store_row<float, HD>(a, st_, t, head, empty, split, down > 0.0f);
+}
+
+template <typename CT, int HD, int SH>
+__global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
+    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return f32_pass<CT, HD, SH>(args, tid, block, down); });
 }
 
 // ------------------------------------------------------------------------- joining splits
-// One wave per (token, head): M = max m_s, o = sum_s 2^((m_s - M) c) o_s / sum_s 2^((m_s - M) c) l_s.
+// One wave per (token, head): M = max m_s, w_s = 2^((m_s - M) c) l_s, o = sum_s w_s o_s / sum_s w_s; o_s is divided by l_s.
 // Bound by reading the parts: 12 us for two of 2048 rows of 16 heads of 128 (34 MB read, 8 MB written: 3.5 TB/s).
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
@@ -318,8 +323,9 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
     const float M = wave_all(ml.y != 0.0f ? ml.x : -INFINITY, [](float x, float y) { return fmaxf(x, y); });
     const float base = M == -INFINITY ? 0.0f : M;
     const bool some = ml.y != 0.0f && ml.y != -1.0f;
-    const float w = some ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) : 0.0f;
-    const float l = wave_all(some ? w * ml.y : 0.0f, [](float x, float y) { return x + y; });
+    const float own = some ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) * ml.y : 0.0f;
+    const float l = wave_all(own, [](float x, float y) { return x + y; });
+    const float w = own * (1.0f / l);  // of a part's row, which is divided by its own sum
     constexpr int PL = HD >= 64 ? HD / 64 : 1;
     float o[PL] = {};
     uint64_t left = __ballot(some);  // their partial rows, four at a time
@@ -344,11 +350,10 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
 #pragma unroll
             for (int u = 0; u < PL; ++u) o[u] = live[j] ? fmaf(ws[j], x[j][u], o[u]) : o[u];
     }
-    const float inv = any ? 1.0f / l : 0.0f;
     T* op = static_cast<T*>(a.o) + t * a.ldo + (i % a.H) * HD;
 #pragma unroll
     for (int u = 0; u < PL; ++u)
-        if (lane * PL < HD) st(op, lane * PL + u, o[u] * inv);
+        if (lane * PL < HD) st(op, lane * PL + u, any && l == 0.0f ? NAN : o[u]);  // only scores of -infinity: NaN
     if (a.lse && lane == 0) a.lse[i] = any ? log_sum(base, l, a.c) : -INFINITY;
 }
 

@@ -31,17 +31,58 @@ __device__ const uint4 kNoPage = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xfffff
 
 constexpr int64_t kMaxLen = INT32_MAX - 4095;  // positions and a tile past them fit in 32 bits
 
-// Weights are held times 2^-40: at most 2^8 2^-40 each, so that the sums over 2^31 keys stay below
-// the largest v, and a finite v never overflows before the division by l.  Exact, and it costs weights
-// below 2^-86 of the maximum.  bf16 takes it in exp2's argument, whose last bits (2^-19 there) are far below
-// the weight's rounding; fp32 multiplies.
+// Weights are at most 2^8 of the maximum's, and sums of many of them times values near the largest number can leave fp32's
+// range where the output does not.  A block that ends with such a sum goes over its keys again with the weights times 2^-40
+// (2^31 of them stay below the largest v then) and replaces the elements that had left the range, only those: so small, weights
+// cost values below 2^-86 their digits.  down: 0, then kDown.  An infinity or NaN in a v that is seen takes the second pass too.
 constexpr float kDown = 40.0f;
+__device__ __forceinline__ float weight(float s, float c, float off) { return __builtin_amdgcn_exp2f(fmaf(s, c, off)); }
+__device__ __forceinline__ float log_sum(float m, float l, float c) { return (m * c + log2f(l)) * kLn2; }
+// Whether some sums have left the range: are not finite, and not by the scores, whose weights' sum l shows theirs.
+struct Range {
+    float none = 0.0f;  // NaN once one of them is not finite
+    __device__ __forceinline__ void look(float o) { none = fmaf(o, 0.0f, none); }
+    __device__ __forceinline__ bool left(float l) const { return none != 0.0f && l > 0.0f && l < INFINITY; }
+};
+
+// x, with its origin hidden (fresh_uniform: one for the whole wave); and the kernel's only argument, loaded anew.  A second pass made
+// of them alone shares nothing with the first that the first one's loops would have to carry in registers (both as one loop:
+// 2048 rows behind 6144 tokens 143.6 us for 135.9, 256 rows on 4096 keys 32.6 for 30.3, fp32 1000 rows on 2000 keys 178 for 159).
 template <typename T>
-__device__ __forceinline__ float weight(float s, float c, float off) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(fmaf(s, c, off - kDown));
-    else return __builtin_amdgcn_exp2f(fmaf(s, c, off)) * 0x1p-40f;
+__device__ __forceinline__ T fresh(T x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
-__device__ __forceinline__ float log_sum(float m, float l, float c) { return (m * c + log2f(l * 0x1p40f)) * kLn2; }
+__device__ __forceinline__ int fresh_uniform(int x) { return __builtin_amdgcn_readfirstlane(fresh(x)); }
+template <typename A>
+__device__ __forceinline__ A fresh_argument() {
+    typedef const __attribute__((address_space(4))) uint32_t* words_t;
+    struct Words {
+        uint32_t w[sizeof(A) / 4];
+    } x;
+    words_t p = (words_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+#pragma unroll
+    for (size_t i = 0; i < sizeof(A) / 4; ++i) x.w[i] = p[i];
+    return __builtin_bit_cast(A, x);
+}
+// A barrier for what is in LDS: stores to memory are not waited for.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// A block's first pass and, where a sum has left the range, its second.  pass(argument, thread, block, down): all of a thread's work,
+// true where a sum has left the range, with a barrier before its first true.
+template <typename A, typename F>
+__device__ __forceinline__ void one_or_two_passes(const A& a, F pass) {
+    __shared__ int past;
+    if (threadIdx.x == 0) past = 0;
+    if (pass(a, static_cast<int>(threadIdx.x), static_cast<int>(blockIdx.x), 0.0f)) past = 1;
+    lds_barrier();
+    if (__builtin_expect(past, 0))
+        pass(fresh_argument<A>(), fresh(static_cast<int>(threadIdx.x)), fresh_uniform(static_cast<int>(blockIdx.x)), kDown);
+}
 
 struct Seq {
     int64_t row0;  // first packed row
@@ -156,8 +197,10 @@ __device__ __forceinline__ float4 v4_at(const char* tile, int row, int d0) {
 template <int OB>
 struct Rows {
     f32x16 o[OB];
-    float m = -INFINITY, l = 0.0f;
+    float m, l;
     __device__ __forceinline__ void init() {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
         for (int i = 0; i < OB; ++i) zero(o[i]);
     }
@@ -178,8 +221,8 @@ struct Rows {
     }
     // A tile's weights of this half of the wave join the sum.
     __device__ __forceinline__ void add(float sum) { l += facing_op<32>(sum, [](float x, float y) { return x + y; }); }
-    // -m in log2 units; a row that has seen only scores of -infinity counts from zero
-    __device__ __forceinline__ float offset(float c) const { return m == -INFINITY ? 0.0f : -m * c; }
+    // -m in log2 units, less down; a row that has seen only scores of -infinity counts from zero
+    __device__ __forceinline__ float offset(float c, float down) const { return m == -INFINITY ? -down : fmaf(-m, c, -down); }
 };
 
 // o += sum over the tile's keys of p v, key by key and only where the row sees the key: a hidden key has
@@ -213,48 +256,55 @@ __device__ __forceinline__ void add_seen_rows(f32x16 (&o)[HD / 32], const f32x16
         }
 }
 
-// Output of one query row: the lane's half of the head dimension.
+// Four neighbouring elements of a row of outputs or parts.  again: those that stand there and are finite stay.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 x, bool vec, bool again) {
+    float y[4] = {x.x, x.y, x.z, x.w};
+    if (__builtin_expect(again, 0)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float old = static_cast<float>(p[u]);
+            y[u] = fabsf(old) < INFINITY ? old : y[u];
+        }
+    }
+    if (__builtin_expect(!vec, 0)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) st(p, u, y[u]);
+    } else if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    } else {
+        *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+    }
+}
+
+// Output of one query row, the lane's half of the head dimension; or of its part, divided by the part's own sum of weights, so
+// that parts join without leaving the range.  True where a sum has left it.  again: with the weights' down.
 template <typename T, int HD>
-__device__ __forceinline__ void store_row(const PagedArgs& a, const Rows<HD / 32>& r, int64_t t, int head, bool empty,
-                                          int split) {
+__device__ __forceinline__ bool store_row(const PagedArgs& a, const Rows<HD / 32>& r, int64_t t, int head, bool empty,
+                                          int split, bool again) {
     constexpr int OB = HD / 32;
     const int h = (threadIdx.x & 63) >> 5;
-    if (a.nsplit > 1) {
-        const int64_t i = (static_cast<int64_t>(split) * a.T + t) * a.H + head;
-        if (h == 0) a.part_ml[i] = make_float2(r.m, empty ? 0.0f : r.l == 0.0f ? -1.0f : r.l);
-        if (empty) return;
-        float* p = a.part_o + i * HD;
-#pragma unroll
-        for (int ob = 0; ob < OB; ++ob)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4*>(p + ob * 32 + 8 * g + 4 * h) =
-                    make_float4(r.o[ob][4 * g], r.o[ob][4 * g + 1], r.o[ob][4 * g + 2], r.o[ob][4 * g + 3]);
-        return;
-    }
     const float inv = empty ? 0.0f : 1.0f / r.l;  // l == 0: only scores of -infinity, 0 / 0 = NaN below
+    const int64_t part = (static_cast<int64_t>(split) * a.T + t) * a.H + head;
+    if (h == 0 && !again) {
+        if (a.nsplit > 1) a.part_ml[part] = make_float2(r.m, empty ? 0.0f : r.l == 0.0f ? -1.0f : r.l);
+        else if (a.lse) a.lse[t * a.H + head] = empty ? -INFINITY : log_sum(r.m, r.l, a.c);
+    }
+    if (empty && a.nsplit > 1) return false;
     T* op = static_cast<T*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD;
+    Range range;
 #pragma unroll
-    for (int ob = 0; ob < OB; ++ob) {
-        if constexpr (sizeof(T) == 2) {
-            if (a.vec_o) {
-                store_t(op, r.o[ob], ob, inv);
-                continue;
-            }
-        }
+    for (int ob = 0; ob < OB; ++ob)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int d0 = ob * 32 + 8 * g + 4 * h;
-            if (sizeof(T) == 4 && a.vec_o) {
-                *reinterpret_cast<float4*>(op + d0) = make_float4(r.o[ob][4 * g] * inv, r.o[ob][4 * g + 1] * inv,
-                                                                  r.o[ob][4 * g + 2] * inv, r.o[ob][4 * g + 3] * inv);
-            } else {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) st(op, d0 + u, r.o[ob][4 * g + u] * inv);
-            }
+            for (int u = 0; u < 4; ++u) range.look(r.o[ob][4 * g + u]);
+            const float4 x = make_float4(r.o[ob][4 * g] * inv, r.o[ob][4 * g + 1] * inv, r.o[ob][4 * g + 2] * inv, r.o[ob][4 * g + 3] * inv);
+            if (a.nsplit > 1) store4(a.part_o + part * HD + d0, x, true, again);
+            else store4(op + d0, x, a.vec_o, again);
         }
-    }
-    if (a.lse && h == 0) a.lse[t * a.H + head] = empty ? -INFINITY : log_sum(r.m, r.l, a.c);
+    return range.left(r.l) && !empty;
 }
 
 }  // namespace

@@ -48,18 +48,18 @@ __device__ __forceinline__ float4 floats(uint32_t x, uint32_t e) {
 
 // RM: rows of a tile.
 template <typename CT, int HD, int RM>
-__global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
+__device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int block, float down) {
     constexpr int L = HD / 4, KI = 64 / L, NI = 8, KB = NI * KI;  // a batch: NI loads of KI keys
     static_assert(KB <= 64, "a lane per key looks its page up");
     __shared__ float2 mls[4][RM];
     __shared__ float os[4][RM][HD];
     const int Hkv = a.kv.Hkv;
-    const int kvh = static_cast<int>(blockIdx.x) % Hkv, rest = static_cast<int>(blockIdx.x) / Hkv;
+    const int kvh = block % Hkv, rest = block / Hkv;
     const int split = rest % a.nsplit, tile = rest / a.nsplit;
     int b, local;
-    if (!find_tile<RM>(a, tile, b, local)) return;
+    if (!find_tile<RM>(a, tile, b, local)) return false;
     const Seq sq = wave_sequence(a, b);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = lane / L, d0 = 4 * (lane % L);
     const int rows = sq.n * a.G, r0 = local * RM;
 
@@ -121,14 +121,14 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
                 }
                 // keys that this group's row has seen only scores of -infinity from count from zero; alpha is 1 exactly where the
                 // maximum stands (an fma with off would leave off's rounding error in it, once per batch of keys)
-                const float off = mx == -INFINITY ? 0.0f : -mx * a.c;
+                const float off = mx == -INFINITY ? -down : fmaf(-mx, a.c, -down);
                 const float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[r] - mx) * a.c);
                 m[r] = mx;
                 l[r] *= alpha;
                 o[r].x *= alpha, o[r].y *= alpha, o[r].z *= alpha, o[r].w *= alpha;
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    const float w = weight<float>(s[i], a.c, off);
+                    const float w = weight(s[i], a.c, off);
                     const float4 v = floats(vx[i], ve[i]);
                     l[r] += w;
                     const float4 y = make_float4(fmaf(w, v.x, o[r].x), fmaf(w, v.y, o[r].y), fmaf(w, v.z, o[r].z), fmaf(w, v.w, o[r].w));
@@ -139,7 +139,10 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
             }
         }
     }
-    // the groups of a wave, then the waves: M = max m_i, o = sum 2^((m_i - M) c) o_i, l alike
+    // the groups of a wave, then the waves: M = max m_i, o = sum 2^((m_i - M) c) o_i, l alike.  True where a sum of this thread's has
+    // left fp32's range.
+    const bool again = down > 0.0f;
+    bool over = false;
     auto add = [](float x, float y) { return x + y; };
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
         if (lane < L) *reinterpret_cast<float4*>(&os[wave][r][d0]) = x;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < RM * HD; i += 256) {
+    for (int i = tid; i < RM * HD; i += 256) {
         const int r = i / HD, d = i % HD;
         if (r0 + r >= rows) break;
         const int tok = (r0 + r) / a.G, head = kvh * a.G + (r0 + r) % a.G, pos = sq.len - sq.n + tok;
@@ -168,16 +171,27 @@ __global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
             lw = fmaf(f, mls[w][r].y, lw);
             x = fmaf(f, os[w][r][d], x);
         }
+        Range range;
+        range.look(x);
+        over |= !empty && range.left(lw);
+        const float y = empty ? 0.0f : x * (1.0f / lw);  // lw == 0: only scores of -infinity, 0 / 0 = NaN
+        float* to;
         if (a.nsplit > 1) {
             const int64_t at = (static_cast<int64_t>(split) * a.T + t) * a.H + head;
-            if (d == 0) a.part_ml[at] = make_float2(M, empty ? 0.0f : lw == 0.0f ? -1.0f : lw);
-            if (!empty) a.part_o[at * HD + d] = x;
+            if (d == 0 && !again) a.part_ml[at] = make_float2(M, empty ? 0.0f : lw == 0.0f ? -1.0f : lw);
+            to = a.part_o + at * HD + d;
         } else {
-            // lw == 0: only scores of -infinity, 0 / 0 = NaN
-            static_cast<float*>(a.o)[t * a.ldo + static_cast<int64_t>(head) * HD + d] = empty ? 0.0f : x * (1.0f / lw);
-            if (a.lse && d == 0) a.lse[t * a.H + head] = empty ? -INFINITY : log_sum(M, lw, a.c);
+            if (a.lse && d == 0 && !again) a.lse[t * a.H + head] = empty ? -INFINITY : log_sum(M, lw, a.c);
+            to = static_cast<float*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD + d;
         }
+        if (!again || !(fabsf(*to) < INFINITY)) *to = y;
     }
+    return over;
+}
+
+template <typename CT, int HD, int RM>
+__global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
+    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return f32_few_pass<CT, HD, RM>(args, tid, block, down); });
 }
 
 }  // namespace

@@ -228,8 +228,8 @@ typedef __attribute__((address_space(3))) v2i_t lds_v2i_t;
 template <int HD>
 struct Frags8 {
     int k_off[HD / 32], v_off[HD / 32];
-    __device__ __forceinline__ void init() {
-        const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
+    __device__ __forceinline__ void init(int lane) {
+        const int h = lane >> 5, r = lane & 31;
         const int g = lane >> 4, j = (lane & 15) >> 1, p = lane & 1, row = (j & 3) + 8 * (j >> 2) + 4 * h;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
@@ -244,31 +244,299 @@ struct Frags8 {
     }
 };
 
-// NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
-// else is divided and a block is alone on its CU.
+// What a thread knows of the tiles: where its copies and fragments lie.
+template <int HD, bool E4>
+struct FewLane {
+    static constexpr int TILE = FewLds<HD, E4, 1>::TILE;
+    static constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
+    uint32_t voff[TILE / 1024];
+    std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
+    __device__ __forceinline__ void init(int lane) {
+#pragma unroll
+        for (int i = 0; i < TILE / 1024; ++i) {
+            const int rr = i * RPS + lane / NC;
+            const int ch = (lane % NC) ^ (E4 ? swz8<HD>(rr) : swz<HD>(rr));
+            voff[i] = static_cast<uint32_t>((rr - (i * RPS >= 16 ? 16 : 0)) * RB + ch * 16);
+        }
+        F.init(lane);
+    }
+};
+// A group's keys, or a block's share of them; one for the whole block.
+struct Part {
+    Seq sq;
+    int b, kvh, r0;  // the group's sequence, key/value head and first row
+    int first, end;  // keys
+    int slot;        // of its state in the workspace
+    int whole;       // all of the group's keys
+};
+
+// The work on one part: true where a sum of this thread's has left fp32's range.
 template <int HD, bool E4, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, E4>& me, float down) {
     using L = FewLds<HD, E4, NW>;
     const PagedArgs& a = f.a;
     constexpr int KS = HD / 16, OB = HD / 32;
-    constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
+    constexpr int RB = FewLane<HD, E4>::RB, NC = FewLane<HD, E4>::NC, RPS = FewLane<HD, E4>::RPS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int ids[kIds];
     __shared__ float2 mls[NW][32];
 
-    const int Hkv = a.kv.Hkv, ps = a.kv.ps;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+    const Seq sq = pt.sq;
+    const int Hkv = a.kv.Hkv, ps = a.kv.ps, kvh = pt.kvh, r0 = pt.r0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     char* mine = lds + wave * L::WAVE;
     const bool paged = ps % (RPS > 16 ? RPS : 16) == 0;  // halves of tiles (whole ones where one copy spans both) do not leave a page
-    uint32_t voff[L::TILE / 1024];
+
+    const int32_t* tr = a.kv.table + pt.b * a.kv.ld_table;
+    const int rows = min(sq.n * a.G, r0 + f.group);
+    const int r = r0 + (lane & 31);
+    const bool real = r < rows;
+    const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
+    const int hi = real ? sq.len - sq.n + tok : -1;
+    const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
+    const int first_pos = sq.len - sq.n + r0 / a.G, last_pos = sq.len - sq.n + (rows - 1) / a.G;
+    // keys of this part that the group sees
+    int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0;
+    k_lo = max(k_lo & ~31, pt.first);
+    const int k_hi = min(last_pos + 1, pt.end);
+    const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));
+
+    Rows<OB> st_;
+    st_.init();
+    if (k_lo < k_hi) {
+        bf16x8 qb[KS];
+        const bf16* qp = static_cast<const bf16*>(a.q) + (sq.row0 + tok) * a.ldq + static_cast<int64_t>(head) * HD;
 #pragma unroll
-    for (int i = 0; i < L::TILE / 1024; ++i) {
-        const int rr = i * RPS + lane / NC;
-        const int ch = (lane % NC) ^ (E4 ? swz8<HD>(rr) : swz<HD>(rr));
-        voff[i] = static_cast<uint32_t>((rr - (i * RPS >= 16 ? 16 : 0)) * RB + ch * 16);
+        for (int kk = 0; kk < KS; ++kk) {
+            const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : 16 * kk + 8 * hl;
+            if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + col, real));
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[col + j] : f2bf(0.0f);
+        }
+
+        // one tile's products, from the stage it arrived in
+        auto compute = [&](const char* kt, int k0) {
+            const char* vt = kt + L::TILE;
+            [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
+            f32x16 sc[1];
+            zero(sc[0]);
+            [[maybe_unused]] int e_max = 0;
+            bool one_by_one = false;
+            if constexpr (E4) {
+                const float sk = exp_scale(ex[lane & 31]);
+                const int ev = static_cast<int>(ex[32 + (lane & 31)]);
+                e_max = wave_all(ev, [](int x, int y) { return max(x, y); });
+                one_by_one = __any(e_max - ev > 40);
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) {
+                    const uint4 x = me.F.k(kt, j);
+                    sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.x, x.y), sk)),
+                                                                    qb[2 * j], sc[0], 0, 0, 0);
+                    sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.z, x.w), sk)),
+                                                                    qb[2 * j + 1], sc[0], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk)
+                    sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(me.F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
+            }
+            // every row sees every key of the tile?
+            const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
+            auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
+            if (!open) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
+                uint32_t bits = 0;  // a hidden key and a non-finite v
+#pragma unroll
+                for (int i = 0; i < L::TILE / 1024; ++i)
+                    bits |= non_finite_bits<std::conditional_t<E4, uint8_t, bf16>>(*reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16));
+                one_by_one |= __any(bits != 0) != 0;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
+            st_.absorb(mx, a.c);
+            const float off = st_.offset(a.c, down);
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[0][e] = weight(sc[0][e], a.c, off);
+                sum += sc[0][e];
+            }
+            st_.add(sum);
+            if (one_by_one) {
+                if constexpr (E4)
+                    add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + key * HD + (((d >> 4) ^ swz8<HD>(key)) << 4) + (d & 15));
+                        const float s = exp_scale(ex[32 + key]);
+                        const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
+                        return make_float4(x[0], x[1], y[0], y[1]);
+                    }, seen);
+                else add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<bf16, HD>(vt, key, d); }, seen);
+                return;
+            }
+            if constexpr (E4) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(ex + 32 + 8 * g + 4 * hl);
+                    const uint32_t ev[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) sc[0][4 * g + u] = __builtin_amdgcn_ldexpf(sc[0][4 * g + u], static_cast<int>(ev[u]) - e_max);
+                }
+            }
+            [[maybe_unused]] const float sv = exp_scale(static_cast<uint32_t>(e_max));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8 p = pack_bf16x8(sc[0], 8 * s);
+#pragma unroll
+                for (int ob = 0; ob < OB; ++ob) {
+                    bf16x8 v;
+                    if constexpr (E4) v = __builtin_bit_cast(bf16x8, e4m3_bf16(me.F.v(vt, ob, s), sv));
+                    else v = me.F.tr(vt, ob, s);
+                    st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, st_.o[ob], 0, 0, 0);
+                }
+            }
+        };
+
+        const int window_keys = min((kIds - 1) * ps, 1 << 20) & ~31;  // keys whose page ids fit
+        for (int w0 = k_lo, w1; w0 < k_hi; w0 = w1) {
+            w1 = w0 + min(k_hi - w0, window_keys);
+            const int p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
+            __syncthreads();
+            for (int i = tid; i < np; i += NW * 64) {
+                const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
+                ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
+            }
+            __syncthreads();
+            const int first = w0 + 32 * wave, nt = first < w1 ? (w1 - first + 32 * NW - 1) / (32 * NW) : 0;  // this wave's tiles
+            // byte offset of key's row in the pools, negative without a page; keys past the last as the last
+            auto row_at = [&](int key) -> int64_t {
+                key = min(key, w1 - 1);
+                const int pi = a.kv.page_index(key), page = ids[pi - p0];
+                const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * ps + (key - pi * ps);
+                return page < 0 ? -1 : row;
+            };
+            auto issue = [&](int t) {
+                char* dst = mine + (t & 1) * L::STAGE;
+                const int k0 = first + 32 * NW * t;
+                if (paged && k0 + 32 <= w1) {
+                    // each half of the tile lies in one page: uniform bases, offsets per lane made once
+                    const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
+                    const int page0 = __builtin_amdgcn_readfirstlane(ids[pi - p0]), page1 = __builtin_amdgcn_readfirstlane(ids[pj - p0]);
+                    if (page0 >= 0 && page1 >= 0) {
+                        const int64_t row[2] = {(static_cast<int64_t>(page0) * Hkv + kvh) * ps + (k0 - pi * ps),
+                                                (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps)};
+#pragma unroll
+                        for (int i = 0; i < L::TILE / 1024; ++i) {
+                            const int64_t at = row[i * RPS >= 16 ? 1 : 0] * RB;
+                            dma16s(a.kv.kp + at, me.voff[i], dst + i * 1024);
+                            dma16s(a.kv.vp + at, me.voff[i], dst + L::TILE + i * 1024);
+                        }
+                        if constexpr (E4)
+                            dma_byte((hl ? a.kv.ve : a.kv.ke) + (lane & 16 ? row[1] : row[0]) + (lane & 15), dst + 2 * L::TILE);
+                        return;
+                    }
+                }
+                const char* none = reinterpret_cast<const char*>(&kNoPage);
+#pragma unroll
+                for (int i = 0; i < L::TILE / 1024; ++i) {
+                    const int rr = i * RPS + lane / NC;
+                    int ch = lane % NC;
+                    if constexpr (E4) ch ^= swz8<HD>(rr);
+                    else ch ^= swz<HD>(rr);
+                    const int64_t row = row_at(k0 + rr), at = row * RB + ch * 16;
+                    dma16(row >= 0 ? a.kv.kp + at : none, dst + i * 1024);
+                    dma16(row >= 0 ? a.kv.vp + at : none, dst + L::TILE + i * 1024);
+                }
+                if constexpr (E4) {
+                    const int64_t row = row_at(k0 + (lane & 31));
+                    dma_byte(row >= 0 ? (hl ? a.kv.ve : a.kv.ke) + row : &kNoExponent, dst + 2 * L::TILE);
+                }
+            };
+            if (nt > 0) issue(0);
+            if (nt > 1) issue(1);
+            for (int t = 0; t < nt; ++t) {
+                if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
+                else wait_vmcnt<0>();
+                compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t);
+                wait_lds();  // the tile has been read
+                if (t + 2 < nt) issue(t + 2);
+            }
+        }
     }
-    std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
-    F.init();
+
+    // The waves' states joined: everyone's factor against the common maximum, then the sums over the waves.
+    bool over = false;
+    if (hl == 0) mls[wave][lane] = make_float2(st_.m, st_.l);
+    __syncthreads();  // also: the tiles have been read
+    const int q = lane & 31;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][q].x);
+    const float base = M == -INFINITY ? 0.0f : M;
+    const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
+    float* os = reinterpret_cast<float*>(lds);  // [NW][32][HD], 16-byte groups swizzled by row
+#pragma unroll
+    for (int ob = 0; ob < OB; ++ob)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c4 = (ob * 32 + 8 * g + 4 * hl) / 4;
+            *reinterpret_cast<float4*>(os + (wave * 32 + q) * HD + ((c4 ^ (q & 7)) << 2)) =
+                make_float4(st_.o[ob][4 * g] * factor, st_.o[ob][4 * g + 1] * factor, st_.o[ob][4 * g + 2] * factor,
+                            st_.o[ob][4 * g + 3] * factor);
+        }
+    __syncthreads();
+    for (int i = tid; i < 32 * (HD / 4); i += NW * 64) {
+        const int qr = i / (HD / 4), c4 = i % (HD / 4), rr = r0 + qr;
+        if (rr >= rows) break;
+        const int tk = rr / a.G, hd_ = kvh * a.G + rr % a.G, h2 = sq.len - sq.n + tk;
+        const int l2 = a.window > 0 ? max(0, max(h2, 0) - a.window + 1) : 0;
+        const bool empty = h2 < 0 || max(l2, k_lo) > min(h2, k_hi - 1);
+        float mm = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, mls[w][qr].x);
+        const float bs = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float2 ml = mls[w][qr];
+            l = fmaf(__builtin_amdgcn_exp2f((ml.x - bs) * a.c), ml.y, l);
+        }
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(os + (w * 32 + qr) * HD + ((c4 ^ (qr & 7)) << 2));
+            v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+        }
+        Range range;
+        range.look(v.x), range.look(v.y), range.look(v.z), range.look(v.w);
+        over |= !empty && range.left(l);
+        const float inv = empty ? 0.0f : 1.0f / l;
+        const float4 y = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        const int64_t t = sq.row0 + tk;
+        if (!pt.whole) {
+            const int64_t at = static_cast<int64_t>(pt.slot) * f.group + qr;
+            if (c4 == 0 && !(down > 0.0f)) f.part_ml[at] = make_float2(mm, empty ? 0.0f : l == 0.0f ? -1.0f : l);
+            if (!empty) store4(f.part_o + at * HD + c4 * 4, y, true, down > 0.0f);
+            continue;
+        }
+        bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(hd_) * HD + c4 * 4;
+        store4(op, y, a.vec_o, down > 0.0f);
+        if (a.lse && c4 == 0 && !(down > 0.0f)) a.lse[t * a.H + hd_] = empty ? -INFINITY : log_sum(bs, l, a.c);
+    }
+    return over;
+}
+
+// NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
+// else is divided and a block is alone on its CU.
+template <int HD, bool E4, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+    const PagedArgs& a = f.a;
+    __shared__ int past;
+    const int Hkv = a.kv.Hkv;
+    FewLane<HD, E4> me;
+    me.init(threadIdx.x & 63);
+    if (threadIdx.x == 0) past = 0;
 
     int b;
     Steps x;
@@ -297,249 +565,23 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
         const int u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
         const int u1 = static_cast<int>(min(static_cast<int64_t>(x.steps), u0 + min(count, int64_t{1} << 30)));
         const int kvh = f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv, r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
-        const bool whole = u0 == 0 && u1 == x.steps;
-        const int slot = 2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1);
+        const Part pt{sq, b, kvh, r0, x.lo + u0 * kStep, u1 < x.steps ? x.lo + u1 * kStep : INT32_MAX,
+                      2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1), u0 == 0 && u1 == x.steps};
         first_part = false;
         before += u1 - u0;
         count -= u1 - u0;
 
-        const int32_t* tr = a.kv.table + b * a.kv.ld_table;
-        const int rows = min(sq.n * a.G, r0 + f.group);
-        const int r = r0 + (lane & 31);
-        const bool real = r < rows;
-        const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
-        const int hi = real ? sq.len - sq.n + tok : -1;
-        const int lo = a.window > 0 ? max(0, max(hi, 0) - a.window + 1) : 0;
-        const int first_pos = sq.len - sq.n + r0 / a.G, last_pos = sq.len - sq.n + (rows - 1) / a.G;
-        // keys of this part that the group sees
-        int k_lo = a.window > 0 ? max(0, max(first_pos, 0) - a.window + 1) : 0, k_hi = last_pos + 1;
-        k_lo = max(k_lo & ~31, x.lo + u0 * kStep);
-        if (u1 < x.steps) k_hi = min(k_hi, x.lo + u1 * kStep);
-        const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));
-
-        Rows<OB> st_;
-        st_.init();
-        if (k_lo < k_hi) {
-            bf16x8 qb[KS];
-            const bf16* qp = static_cast<const bf16*>(a.q) + (sq.row0 + tok) * a.ldq + static_cast<int64_t>(head) * HD;
-#pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : 16 * kk + 8 * hl;
-                if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + col, real));
-                else
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[col + j] : f2bf(0.0f);
+        bool again = false;
+        do {
+            const bool over = few_part<HD, E4, NW>(f, pt, me, again ? kDown : 0.0f);
+            if (over && !again) past = 1;
+            lds_barrier();  // also: before the next part's tiles
+            again = !again && past;
+            if (__builtin_expect(again, 0)) {
+                lds_barrier();
+                if (threadIdx.x == 0) past = 0;
             }
-
-            // one tile's products, from the stage it arrived in
-            auto compute = [&](const char* kt, int k0) {
-                const char* vt = kt + L::TILE;
-                [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
-                f32x16 sc[1];
-                zero(sc[0]);
-                [[maybe_unused]] int e_max = 0;
-                bool one_by_one = false;
-                if constexpr (E4) {
-                    const float sk = exp_scale(ex[lane & 31]);
-                    const int ev = static_cast<int>(ex[32 + (lane & 31)]);
-                    e_max = wave_all(ev, [](int x, int y) { return max(x, y); });
-                    one_by_one = __any(e_max - ev > 40);
-#pragma unroll
-                    for (int j = 0; j < HD / 32; ++j) {
-                        const uint4 x = F.k(kt, j);
-                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.x, x.y), sk)),
-                                                                        qb[2 * j], sc[0], 0, 0, 0);
-                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.z, x.w), sk)),
-                                                                        qb[2 * j + 1], sc[0], 0, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int kk = 0; kk < KS; ++kk)
-                        sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
-                }
-                // every row sees every key of the tile?
-                const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
-                auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
-                if (!open) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[0][e] = seen(8 * (e >> 2) + 4 * hl + (e & 3)) ? sc[0][e] : -INFINITY;
-                    uint32_t bits = 0;  // a hidden key and a non-finite v
-#pragma unroll
-                    for (int i = 0; i < L::TILE / 1024; ++i)
-                        bits |= non_finite_bits<std::conditional_t<E4, uint8_t, bf16>>(*reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16));
-                    one_by_one |= __any(bits != 0) != 0;
-                }
-                float mx = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[0][e]);
-                st_.absorb(mx, a.c);
-                const float off = st_.offset(a.c);
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[0][e] = weight<bf16>(sc[0][e], a.c, off);
-                    sum += sc[0][e];
-                }
-                st_.add(sum);
-                if (one_by_one) {
-                    if constexpr (E4)
-                        add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + key * HD + (((d >> 4) ^ swz8<HD>(key)) << 4) + (d & 15));
-                            const float s = exp_scale(ex[32 + key]);
-                            const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
-                            return make_float4(x[0], x[1], y[0], y[1]);
-                        }, seen);
-                    else add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) { return v4_at<bf16, HD>(vt, key, d); }, seen);
-                    return;
-                }
-                if constexpr (E4) {
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(ex + 32 + 8 * g + 4 * hl);
-                        const uint32_t ev[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) sc[0][4 * g + u] = __builtin_amdgcn_ldexpf(sc[0][4 * g + u], static_cast<int>(ev[u]) - e_max);
-                    }
-                }
-                [[maybe_unused]] const float sv = exp_scale(static_cast<uint32_t>(e_max));
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const bf16x8 p = pack_bf16x8(sc[0], 8 * s);
-#pragma unroll
-                    for (int ob = 0; ob < OB; ++ob) {
-                        bf16x8 v;
-                        if constexpr (E4) v = __builtin_bit_cast(bf16x8, e4m3_bf16(F.v(vt, ob, s), sv));
-                        else v = F.tr(vt, ob, s);
-                        st_.o[ob] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, st_.o[ob], 0, 0, 0);
-                    }
-                }
-            };
-
-            const int window_keys = min((kIds - 1) * ps, 1 << 20) & ~31;  // keys whose page ids fit
-            for (int w0 = k_lo, w1; w0 < k_hi; w0 = w1) {
-                w1 = w0 + min(k_hi - w0, window_keys);
-                const int p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
-                __syncthreads();
-                for (int i = threadIdx.x; i < np; i += NW * 64) {
-                    const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
-                    ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
-                }
-                __syncthreads();
-                const int first = w0 + 32 * wave, nt = first < w1 ? (w1 - first + 32 * NW - 1) / (32 * NW) : 0;  // this wave's tiles
-                // byte offset of key's row in the pools, negative without a page; keys past the last as the last
-                auto row_at = [&](int key) -> int64_t {
-                    key = min(key, w1 - 1);
-                    const int pi = a.kv.page_index(key), page = ids[pi - p0];
-                    const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * ps + (key - pi * ps);
-                    return page < 0 ? -1 : row;
-                };
-                auto issue = [&](int t) {
-                    char* dst = mine + (t & 1) * L::STAGE;
-                    const int k0 = first + 32 * NW * t;
-                    if (paged && k0 + 32 <= w1) {
-                        // each half of the tile lies in one page: uniform bases, offsets per lane made once
-                        const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
-                        const int page0 = __builtin_amdgcn_readfirstlane(ids[pi - p0]), page1 = __builtin_amdgcn_readfirstlane(ids[pj - p0]);
-                        if (page0 >= 0 && page1 >= 0) {
-                            const int64_t row[2] = {(static_cast<int64_t>(page0) * Hkv + kvh) * ps + (k0 - pi * ps),
-                                                    (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps)};
-#pragma unroll
-                            for (int i = 0; i < L::TILE / 1024; ++i) {
-                                const int64_t at = row[i * RPS >= 16 ? 1 : 0] * RB;
-                                dma16s(a.kv.kp + at, voff[i], dst + i * 1024);
-                                dma16s(a.kv.vp + at, voff[i], dst + L::TILE + i * 1024);
-                            }
-                            if constexpr (E4)
-                                dma_byte((hl ? a.kv.ve : a.kv.ke) + (lane & 16 ? row[1] : row[0]) + (lane & 15), dst + 2 * L::TILE);
-                            return;
-                        }
-                    }
-                    const char* none = reinterpret_cast<const char*>(&kNoPage);
-#pragma unroll
-                    for (int i = 0; i < L::TILE / 1024; ++i) {
-                        const int rr = i * RPS + lane / NC;
-                        int ch = lane % NC;
-                        if constexpr (E4) ch ^= swz8<HD>(rr);
-                        else ch ^= swz<HD>(rr);
-                        const int64_t row = row_at(k0 + rr), at = row * RB + ch * 16;
-                        dma16(row >= 0 ? a.kv.kp + at : none, dst + i * 1024);
-                        dma16(row >= 0 ? a.kv.vp + at : none, dst + L::TILE + i * 1024);
-                    }
-                    if constexpr (E4) {
-                        const int64_t row = row_at(k0 + (lane & 31));
-                        dma_byte(row >= 0 ? (hl ? a.kv.ve : a.kv.ke) + row : &kNoExponent, dst + 2 * L::TILE);
-                    }
-                };
-                if (nt > 0) issue(0);
-                if (nt > 1) issue(1);
-                for (int t = 0; t < nt; ++t) {
-                    if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
-                    else wait_vmcnt<0>();
-                    compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t);
-                    wait_lds();  // the tile has been read
-                    if (t + 2 < nt) issue(t + 2);
-                }
-            }
-        }
-
-        // The waves' states joined: everyone's factor against the common maximum, then the sums over the waves.
-        if (hl == 0) mls[wave][lane] = make_float2(st_.m, st_.l);
-        __syncthreads();  // also: the tiles have been read
-        const int q = lane & 31;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, mls[w][q].x);
-        const float base = M == -INFINITY ? 0.0f : M;
-        const float factor = __builtin_amdgcn_exp2f((st_.m - base) * a.c);
-        float* os = reinterpret_cast<float*>(lds);  // [NW][32][HD], 16-byte groups swizzled by row
-#pragma unroll
-        for (int ob = 0; ob < OB; ++ob)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int c4 = (ob * 32 + 8 * g + 4 * hl) / 4;
-                *reinterpret_cast<float4*>(os + (wave * 32 + q) * HD + ((c4 ^ (q & 7)) << 2)) =
-                    make_float4(st_.o[ob][4 * g] * factor, st_.o[ob][4 * g + 1] * factor, st_.o[ob][4 * g + 2] * factor,
-                                st_.o[ob][4 * g + 3] * factor);
-            }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 32 * (HD / 4); i += NW * 64) {
-            const int qr = i / (HD / 4), c4 = i % (HD / 4), rr = r0 + qr;
-            if (rr >= rows) break;
-            const int tk = rr / a.G, hd_ = kvh * a.G + rr % a.G, h2 = sq.len - sq.n + tk;
-            const int l2 = a.window > 0 ? max(0, max(h2, 0) - a.window + 1) : 0;
-            const bool empty = h2 < 0 || max(l2, k_lo) > min(h2, k_hi - 1);
-            float mm = -INFINITY, l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, mls[w][qr].x);
-            const float bs = mm == -INFINITY ? 0.0f : mm;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float2 ml = mls[w][qr];
-                l = fmaf(__builtin_amdgcn_exp2f((ml.x - bs) * a.c), ml.y, l);
-            }
-            float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float4 y = *reinterpret_cast<const float4*>(os + (w * 32 + qr) * HD + ((c4 ^ (qr & 7)) << 2));
-                v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-            }
-            const int64_t t = sq.row0 + tk;
-            if (!whole) {
-                const int64_t at = static_cast<int64_t>(slot) * f.group + qr;
-                if (c4 == 0) f.part_ml[at] = make_float2(mm, empty ? 0.0f : l == 0.0f ? -1.0f : l);
-                if (!empty) *reinterpret_cast<float4*>(f.part_o + at * HD + c4 * 4) = v;
-                continue;
-            }
-            const float inv = empty ? 0.0f : 1.0f / l;
-            bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(hd_) * HD + c4 * 4;
-            if (a.vec_o) {
-                *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
-            } else {
-                op[0] = f2bf(v.x * inv), op[1] = f2bf(v.y * inv), op[2] = f2bf(v.z * inv), op[3] = f2bf(v.w * inv);
-            }
-            if (a.lse && c4 == 0) a.lse[t * a.H + hd_] = empty ? -INFINITY : log_sum(bs, l, a.c);
-        }
-        __syncthreads();  // before the next group's tiles
+        } while (__builtin_expect(again, 0));
     }
 }
 
@@ -571,10 +613,12 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
         }
         if (parts == 1) continue;  // undivided: written already
         auto at = [&](int i) { return (2 * (s0 + i) + (i == 0 ? first_slot : 0)) * f.group + qr; };
-        float M = -INFINITY;
-        bool any = false;
-        for (int i = lane; i < parts; i += 64) {
-            const float2 ml = f.part_ml[at(i)];
+        auto state = [&](int i) { return i < parts ? f.part_ml[at(i)] : make_float2(-INFINITY, 0.0f); };
+        const float2 first = state(lane);
+        float M = first.y != 0.0f ? first.x : -INFINITY;
+        bool any = first.y != 0.0f;
+        for (int i = lane + 64; i < parts; i += 64) {
+            const float2 ml = state(i);
             any |= ml.y != 0.0f;
             M = ml.y != 0.0f ? fmaxf(M, ml.x) : M;
         }
@@ -582,13 +626,16 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
         M = wave_all(M, [](float p, float q) { return fmaxf(p, q); });
         const float base = M == -INFINITY ? 0.0f : M;
         constexpr int PL = HD >= 64 ? HD / 64 : 1;
-        float o[PL] = {}, l = 0.0f;
+        // a part's weight, of its row divided by its own sum
+        auto weigh = [&](float2 ml) { return ml.y != 0.0f && ml.y != -1.0f ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) * ml.y : 0.0f; };
+        float own = weigh(first), o[PL] = {}, l = own;
+        for (int i = lane + 64; i < parts; i += 64) l += weigh(state(i));
+        l = wave_all(l, [](float p, float q) { return p + q; });
+        const float inv = 1.0f / l;
         for (int i0 = 0; i0 < parts; i0 += 64) {
-            const float2 ml = i0 + lane < parts ? f.part_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.0f);
-            const bool some = ml.y != 0.0f && ml.y != -1.0f;
-            const float w = some ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) : 0.0f;
-            l += wave_all(some ? w * ml.y : 0.0f, [](float p, float q) { return p + q; });
-            uint64_t left = __ballot(some);
+            if (i0 > 0) own = weigh(state(i0 + lane));
+            const float w = own * inv;
+            uint64_t left = __ballot(own != 0.0f);
             while (left) {  // four parts' rows at a time
                 int j[4];
                 float v[4][PL], ws[4];
@@ -613,11 +660,10 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
         }
         const int64_t t = x.sq.row0 + r / a.G;
         const int head = kvh * a.G + r % a.G;
-        const float inv = any ? 1.0f / l : 0.0f;
         bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD;
 #pragma unroll
         for (int u = 0; u < PL; ++u)
-            if (lane * PL < HD) st(op, lane * PL + u, o[u] * inv);
+            if (lane * PL < HD) st(op, lane * PL + u, any && l == 0.0f ? NAN : o[u]);  // only scores of -infinity: NaN
         if (a.lse && lane == 0) a.lse[t * a.H + head] = any ? log_sum(base, l, a.c) : -INFINITY;
     }
 }

@@ -30,7 +30,7 @@ namespace {
 constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <int HD, bool E4>
-__global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
+__device__ __forceinline__ bool tiles_pass(const PagedArgs& a, int tid, int block, float down) {
     constexpr int KS = HD / 16, OB = HD / 32, TILE = 64 * HD;  // elements of a tile
     constexpr int NA = 2 * KS, NB = 4 * OB;                   // MFMAs of groups A and B
     constexpr int EA = 32 / NA, EB = 32 / NB;                 // elements per slot
@@ -41,12 +41,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
     __shared__ int ids[kIds];
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
-    const int kvh = static_cast<int>(blockIdx.x) % Hkv, rest = static_cast<int>(blockIdx.x) / Hkv;
+    const int kvh = block % Hkv, rest = block / Hkv;
     const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
-    if (!find_tile<128>(a, tile, b, local)) return;
+    if (!find_tile<128>(a, tile, b, local)) return false;
     const Seq sq = wave_sequence(a, b);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hl = lane >> 5;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     const int rows = sq.n * a.G, r0 = local * 128, r = r0 + wave * 32 + (lane & 31);
     const bool real = r < rows;
     const int tok = real ? r / a.G : 0, head = kvh * a.G + (real ? r % a.G : 0);
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                 for (int j = 0; j < 8; ++j) qf[kk][j] = real ? qp[16 * kk + j] : f2bf(0.0f);
         }
         Frags<HD> F;
-        F.init();
+        F.init(lane);
         [[maybe_unused]] uint32_t voff[PW];
         if constexpr (!E4) {
 #pragma unroll
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             w1 = w0 + min(k_hi - w0, window_keys);
             const int p0 = a.kv.page_index(w0), np = a.kv.page_index(w1 - 1) - p0 + 1;
             __syncthreads();
-            for (int i = threadIdx.x; i < np; i += 256) {
+            for (int i = tid; i < np; i += 256) {
                 const int page = p0 + i < a.kv.ld_table ? tr[p0 + i] : -1;
                 ids[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages) ? page : -1;
             }
@@ -133,14 +133,14 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             auto fetch = [&](const char* pool, const uint8_t* exps, int t, Codes& c) {
 #pragma unroll
                 for (int i = 0; i < NU; ++i) {
-                    const int u = i * 256 + static_cast<int>(threadIdx.x);
+                    const int u = i * 256 + tid;
                     const int64_t row = row_at(w0 + 64 * t + min(u / UPR, 63));
                     c.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * HD + (u % UPR) * 16 : none);
                     c.e[i] = row >= 0 ? exps[row] : 127;
                 }
             };
             auto put_unit = [&](const Codes& c, int i, bf16* dst) {
-                const int u = i * 256 + static_cast<int>(threadIdx.x);
+                const int u = i * 256 + tid;
                 if (UNITS % 256 != 0 && u >= UNITS) return;
                 const float s = exp_scale(c.e[i]);
                 char* tile = reinterpret_cast<char*>(dst);
@@ -203,13 +203,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                     }
                 }
                 st_.absorb(mx, a.c);
-                const float off = st_.offset(a.c);
+                const float off = st_.offset(a.c, down);
                 float sum = 0.0f;
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        sc[jb][e] = weight<bf16>(sc[jb][e], a.c, off);
+                        sc[jb][e] = weight(sc[jb][e], a.c, off);
                         sum += sc[jb][e];
                     }
                 st_.add(sum);
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
                 const int st = (t - t_a + 1) & 1;
                 const char* Kb = reinterpret_cast<const char*>(sm[st]);
                 const char* Vb = reinterpret_cast<const char*>(sm[st] + TILE);
-                const float off = st_.offset(a.c) - kDown;
+                const float off = st_.offset(a.c, down);
                 bf16x8 rk[KR], tv[NR], pf[4];
                 auto rd_k = [&](int g) { rk[g % KR] = F.row(Kb, 32 * (g / KS), g % KS); };
                 auto rd_v = [&](int f) { tv[f % NR] = F.tr(Vb, f % OB, f / OB); };
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
 #pragma unroll
                     for (int x = i * EA; x < (i + 1) * EA; ++x) {
                         const int jb = x >> 4, e = x & 15;
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[jb][e], a.c, off));
+                        const float p = weight(sc[jb][e], a.c, off);
                         sc[jb][e] = p;
                         sum += p;
                         if ((e & 7) == 7) pf[2 * jb + (e >> 3)] = pack_bf16x8(sc[jb], e - 7);
@@ -357,7 +357,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
             }
         }
     }
-    if (real) store_row<bf16, HD>(a, st_, trow, head, empty, split);
+    return real && store_row<bf16, HD>(a, st_, trow, head, empty, split, down > 0.0f);
+}
+
+template <int HD, bool E4>
+__global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
+    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return tiles_pass<HD, E4>(args, tid, block, down); });
 }
 
 template <int HD, bool E4>

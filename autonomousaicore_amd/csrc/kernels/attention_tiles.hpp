@@ -50,8 +50,7 @@ struct Frags {
     static constexpr int KS = HD / 16, OB = HD / 32, RB = HD * 2;  // RB: bytes per row
     int row_off[KS];
     int tr_off[OB][2];
-    __device__ __forceinline__ void init() {
-        const int lane = threadIdx.x & 63;
+    __device__ __forceinline__ void init(int lane = threadIdx.x & 63) {
         const int h = lane >> 5, r = lane & 31;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) row_off[kk] = r * RB + (((2 * kk + h) ^ swz<HD>(r)) << 4);
