@@ -152,6 +152,7 @@ __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block,
                         const int u = i * 256 + tid, row = u / UPR, c = u % UPR;
                         if (KT * UPR % 256 != 0 && u >= KT * UPR) continue;
                         const float s = exp_scale(codes.e[i]);
+                        if (__builtin_expect(codes.e[i] >= kTopByte, 0)) codes.w[i] = e4m3_in_range(codes.w[i], codes.e[i]);
                         const uint2 w[2] = {make_uint2(codes.w[i].x, codes.w[i].y), make_uint2(codes.w[i].z, codes.w[i].w)};
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {

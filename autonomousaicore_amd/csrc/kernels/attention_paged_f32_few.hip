@@ -108,6 +108,18 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
                 }
             }
             row = row_of(k0 + 4 * KB);
+            if constexpr (sizeof(CT) == 1) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) most = max(most, max(ke[i], ve[i]));
+                if (__builtin_expect(most >= kTopByte, 0)) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+                        if (ke[i] >= kTopByte) kx[i] = e4m3_in_range(kx[i], ke[i]);
+                        if (ve[i] >= kTopByte) vx[i] = e4m3_in_range(vx[i], ve[i]);
+                    }
+                }
+            }
             const bool open = k0 + KB - 1 <= first_pos && k0 + KB <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
 #pragma unroll
             for (int r = 0; r < RM; ++r) {

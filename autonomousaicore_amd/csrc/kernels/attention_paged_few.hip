@@ -26,7 +26,8 @@
 // and so one power of two; V fragments (transposed reads) hold eight keys, so they are converted with
 // the tile's largest power 2^E, and the weights take 2^(e - E).  That loses what is below 2^-86 of
 // the tile's largest: where the tile's powers differ by more than 2^40, its keys are added one by one instead,
-// so that a hidden key's large v costs a visible one nothing.
+// so that a hidden key's large v costs a visible one nothing; and
+// from power kTopByte on, where other rows' codes with that power would be past the range.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -316,7 +317,7 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
         }
 
         // one tile's products, from the stage it arrived in
-        auto compute = [&](const char* kt, int k0) {
+        auto compute = [&](char* kt, int k0) {
             const char* vt = kt + L::TILE;
             [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
             f32x16 sc[1];
@@ -324,10 +325,18 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
             [[maybe_unused]] int e_max = 0;
             bool one_by_one = false;
             if constexpr (E4) {
-                const float sk = exp_scale(ex[lane & 31]);
+                const uint32_t ek = ex[lane & 31];
+                const float sk = exp_scale(ek);
+                if (__builtin_expect(__any(ek >= kTopByte), 0)) {  // each lane what it reads
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) {
+                        uint4* x = reinterpret_cast<uint4*>(kt + me.F.k_off[j]);
+                        if (ek >= kTopByte) *x = e4m3_in_range(*x, ek);
+                    }
+                }
                 const int ev = static_cast<int>(ex[32 + (lane & 31)]);
                 e_max = wave_all(ev, [](int x, int y) { return max(x, y); });
-                one_by_one = __any(e_max - ev > 40);
+                one_by_one = __any(e_max - ev > 40) || e_max >= static_cast<int>(kTopByte);
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
                     const uint4 x = me.F.k(kt, j);
@@ -368,7 +377,8 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
             if (one_by_one) {
                 if constexpr (E4)
                     add_seen_rows<HD, 1>(st_.o, sc, [&](int key, int d) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(vt + key * HD + (((d >> 4) ^ swz8<HD>(key)) << 4) + (d & 15));
+                        uint32_t w = *reinterpret_cast<const uint32_t*>(vt + key * HD + (((d >> 4) ^ swz8<HD>(key)) << 4) + (d & 15));
+                        if (ex[32 + key] >= kTopByte) w = e4m3_in_range(w, ex[32 + key]);
                         const float s = exp_scale(ex[32 + key]);
                         const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
                         return make_float4(x[0], x[1], y[0], y[1]);

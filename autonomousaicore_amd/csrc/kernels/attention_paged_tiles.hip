@@ -29,22 +29,33 @@ namespace {
 
 constexpr int kIds = 512;  // page ids in LDS at a time
 
-template <int HD, bool E4>
-__device__ __forceinline__ bool tiles_pass(const PagedArgs& a, int tid, int block, float down) {
+// What a pass has found.  kTop: a row whose codes can be past the range (e4m3_in_range): looked for in the first pass only, and kept
+// in the range by the other one, for a branch between the products costs 4% at head_dim 128.
+constexpr int kPast = 1, kTop = 2;
+
+template <int HD>
+struct TilesLds {
+    __attribute__((aligned(16))) bf16 sm[2][2 * 64 * HD];
+    int ids[kIds];
+    int past, top;
+};
+
+template <int HD, bool E4, bool SECOND>
+__device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a, int tid, int block, float down) {
     constexpr int KS = HD / 16, OB = HD / 32, TILE = 64 * HD;  // elements of a tile
     constexpr int NA = 2 * KS, NB = 4 * OB;                   // MFMAs of groups A and B
     constexpr int EA = 32 / NA, EB = 32 / NB;                 // elements per slot
     constexpr int NR = OB + 1, KR = 3;                        // fragment rings
     constexpr int RB = HD * 2, NC = RB / 16, RPS = 1024 / RB, PW = 16 / RPS;  // bf16 copies: of a wave's 16 rows
     constexpr int UPR = HD / 16, UNITS = 64 * UPR, NU = (UNITS + 255) / 256;  // e4m3: 16-byte units of a tile
-    __shared__ __attribute__((aligned(16))) bf16 sm[2][2 * TILE];
-    __shared__ int ids[kIds];
+    auto& sm = lds.sm;
+    auto& ids = lds.ids;
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
     const int kvh = block % Hkv, rest = block / Hkv;
     const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
-    if (!find_tile<128>(a, tile, b, local)) return false;
+    if (!find_tile<128>(a, tile, b, local)) return 0;
     const Seq sq = wave_sequence(a, b);
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     const int rows = sq.n * a.G, r0 = local * 128, r = r0 + wave * 32 + (lane & 31);
@@ -61,6 +72,7 @@ __device__ __forceinline__ bool tiles_pass(const PagedArgs& a, int tid, int bloc
     const uint32_t span = static_cast<uint32_t>(max(min(hi, k_hi - 1) - lo + 1, 0));
     const bool empty = span == 0 || min(hi, k_hi - 1) < k_lo;
 
+    [[maybe_unused]] uint64_t top = 0;  // lanes, in scalar registers
     Rows<OB> st_;
     st_.init();
     if (k_lo < k_hi) {
@@ -142,11 +154,17 @@ __device__ __forceinline__ bool tiles_pass(const PagedArgs& a, int tid, int bloc
             auto put_unit = [&](const Codes& c, int i, bf16* dst) {
                 const int u = i * 256 + tid;
                 if (UNITS % 256 != 0 && u >= UNITS) return;
+                uint4 w = c.w[i];
+                if constexpr (SECOND) {
+                    if (c.e[i] >= kTopByte) w = e4m3_in_range(w, c.e[i]);
+                } else {
+                    top |= __ballot(c.e[i] >= kTopByte);
+                }
                 const float s = exp_scale(c.e[i]);
                 char* tile = reinterpret_cast<char*>(dst);
                 const int rr = u / UPR, ch = 2 * (u % UPR);
-                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch)) = e4m3_bf16(make_uint2(c.w[i].x, c.w[i].y), s);
-                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + 1)) = e4m3_bf16(make_uint2(c.w[i].z, c.w[i].w), s);
+                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch)) = e4m3_bf16(make_uint2(w.x, w.y), s);
+                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + 1)) = e4m3_bf16(make_uint2(w.z, w.w), s);
             };
             auto put = [&](const Codes& c, bf16* dst) {
 #pragma unroll
@@ -357,12 +375,32 @@ __device__ __forceinline__ bool tiles_pass(const PagedArgs& a, int tid, int bloc
             }
         }
     }
-    return real && store_row<bf16, HD>(a, st_, trow, head, empty, split, down > 0.0f);
+    const int past = real && store_row<bf16, HD>(a, st_, trow, head, empty, split, down > 0.0f) ? kPast : 0;
+    return past | (top ? kTop : 0);
 }
 
 template <int HD, bool E4>
 __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
-    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return tiles_pass<HD, E4>(args, tid, block, down); });
+    // as one_or_two_passes; where a row of the largest powers was found, the second pass is anew from the start, and there may be a third
+    __shared__ TilesLds<HD> lds;
+    const int tid = threadIdx.x;
+    if (tid == 0) lds.past = 0, lds.top = 0;
+    const int found = tiles_pass<HD, E4, false>(lds, a, tid, static_cast<int>(blockIdx.x), 0.0f);
+    if (found & kPast) lds.past = 1;
+    if (E4 && found & kTop) lds.top = 1;
+    lds_barrier();
+    if (__builtin_expect(lds.past || (E4 && lds.top), 0)) {
+#pragma unroll 1
+        for (float down = E4 && lds.top ? 0.0f : kDown;; down = kDown) {
+            lds_barrier();
+            if (threadIdx.x == 0) lds.past = 0;
+            const int again = tiles_pass<HD, E4, true>(lds, fresh_argument<PagedArgs>(), fresh(tid), fresh_uniform(static_cast<int>(blockIdx.x)), down);
+            lds_barrier();  // (a tile without keys has none)
+            if (again & kPast) lds.past = 1;
+            lds_barrier();
+            if (down > 0.0f || !lds.past) return;
+        }
+    }
 }
 
 template <int HD, bool E4>

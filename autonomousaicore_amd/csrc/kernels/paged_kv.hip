@@ -231,6 +231,7 @@ __global__ __launch_bounds__(kBlock) void kv_read_k(PageView pv, Cut c, T* __res
         float x[EPU];
         if constexpr (sizeof(CT) == 1) {
             const float s = exp_scale(ex[i]);
+            if (__builtin_expect(ex[i] >= kTopByte, 0)) raw[i] = e4m3_in_range(raw[i], ex[i]);
             float a[8], b[8];
             e4m3_floats(make_uint2(raw[i].x, raw[i].y), s, a);
             e4m3_floats(make_uint2(raw[i].z, raw[i].w), s, b);

@@ -10,7 +10,8 @@ namespace aic::hip {
 // of a head that one block reads are whole runs of ps * hd elements.  e4m3 pools carry one byte per
 // (page, head, slot): the row is code * 2^(byte - 127).  Powers of two cost no precision that the
 // codes have (e4m3 is a floating format: moving a row by up to one binade leaves its relative steps),
-// make the values exact in bf16, and go through the hardware's scaled conversion for free.
+// make the values exact in bf16 (from 2^-124 on, where the codes' last digit meets bf16's), and go through the hardware's
+// scaled conversion for free.
 struct PageView {
     char *kp, *vp;
     uint8_t *ke, *ve;
@@ -57,12 +58,28 @@ __device__ __forceinline__ void e4m3_floats(uint2 w, float s, float (&v)[8]) {
     const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w.y, s, true);
     v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
 }
-// The same as bf16, where code * s is exact.
+// The same as bf16, to nearest even where code * s has bits below 2^-133.
 __device__ __forceinline__ uint4 e4m3_bf16(uint2 w, float s) {
     return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, false)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, true)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, false)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, true)));
+}
+// The largest number that codes and both types share is 240 * 2^120.  From exponent byte kTopByte (2^120) on, a row's larger codes
+// are past it: 256 * 2^120 is 2^128, the code nearest to numbers past 248 * 2^120.  They are read as 240 * 2^120, so that finite
+// numbers stay finite.  Four codes of a row with such a byte, brought into the range; NaN stays.
+constexpr uint32_t kTopByte = 247;
+__device__ __forceinline__ uint32_t e4m3_in_range(uint32_t w, uint32_t byte) {
+    const uint32_t top = 0x77u - 8u * (min(byte, 254u) - kTopByte);  // 8 codes to a binade
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        const uint32_t c = w >> i & 0x7fu;
+        w = c > top && c != 0x7fu ? (w & ~(0x7fu << i)) | top << i : w;
+    }
+    return w;
+}
+__device__ __forceinline__ uint4 e4m3_in_range(uint4 w, uint32_t byte) {
+    return make_uint4(e4m3_in_range(w.x, byte), e4m3_in_range(w.y, byte), e4m3_in_range(w.z, byte), e4m3_in_range(w.w, byte));
 }
 // 2^(b - 127) of a stored exponent byte (1 .. 254; 0 and 255 cannot be written and read as 2^-126, 2^127).
 __device__ __forceinline__ float exp_scale(uint32_t b) {

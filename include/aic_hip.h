@@ -257,7 +257,9 @@ int aic_hip_attn_bwd_qk(const void* q, int64_t ld_q, const void* k, const void* 
  * page_table[b * ld_table + j / page_size] (device memory; several sequences may read one page).
  * type: AIC_F32, AIC_BF16, or AIC_U8 for e4m3 codes (4 exponent, 3 mantissa bits, largest 448):
  * a row's head is code * 2^(byte - 127), byte (1 .. 254) in k_exps / v_exps
- * [n_pages][kv_heads][page_size].
+ * [n_pages][kv_heads][page_size]; what would be past 240 * 2^120, the largest number that codes and the
+ * types share, counts as that number (codes from 256 * 2^120 on, which stand for numbers past 248 * 2^120), so finite
+ * numbers stay finite.
  *
  * The calls below share a ragged batch's description, in device memory: offsets [B + 1] and lens [B]
  * (int64).  Sequence b's packed rows offsets[b] .. offsets[b + 1] - 1 are the last ones of its
@@ -285,7 +287,7 @@ typedef struct {
 int aic_hip_kv_write(const aic_kv_pages* cache, const void* k, const void* v, int64_t ld, const int64_t* offsets,
                      const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
 /* The other way: the cached rows at the batch's positions to k, v [T, kv_heads * head_dim] (e4m3 to
- * bf16 is exact); rows without a place are zero. */
+ * bf16 is exact but for bits below 2^-133, bf16's least number); rows without a place are zero. */
 int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, const int64_t* offsets,
                     const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
 /* Attention of the batch's rows over the cache, for chunks of a prompt, drafted tokens and single tokens
