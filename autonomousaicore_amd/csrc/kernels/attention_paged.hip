@@ -398,6 +398,7 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
               "attn_paged: max_q must not be negative and max_len must be 0 .. ", kMaxLen);
     AIC_CHECK(c.kv_heads >= 1 && H >= 1 && H % c.kv_heads == 0, ShapeMismatch, "attn_paged: ", H, " query heads over ", c.kv_heads,
               " key/value heads");
+    AIC_CHECK(H <= INT32_MAX, InvalidArgument, "attn_paged: more than 2^31 - 1 query heads");  // the products below stay in 64 bits
     AIC_CHECK(T * (H / c.kv_heads) <= kMaxLen, OutOfRange, "attn_paged: more than ", kMaxLen, " query rows per key/value head");
 }
 
@@ -405,6 +406,7 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
 
 int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H) {
     check_sizes(c, B, T, max_q, max_len, H);
+    check_cache_shape(c, "attn_paged");
     if (B == 0 || T == 0) return 0;
     max_q = std::min(max_q, T);
     // the cache's type does not tell the queries' (e4m3 serves both): room for either

@@ -15,13 +15,17 @@
 
 namespace aic::hip {
 
-PageView page_view(const KVPages& c, const char* what) {
+void check_cache_shape(const KVPages& c, const char* what) {
     AIC_CHECK(c.type == DType::Float32 || c.type == DType::BFloat16 || c.type == DType::UInt8, DTypeMismatch, what,
               ": a cache holds float32, bfloat16 or e4m3 (uint8)");
     AIC_CHECK(c.head_dim == 32 || c.head_dim == 64 || c.head_dim == 128, InvalidArgument, what,
               ": head_dim must be 32, 64 or 128, got ", c.head_dim);
     AIC_CHECK(c.kv_heads >= 1 && c.kv_heads <= 4096, InvalidArgument, what, ": kv_heads must be 1 .. 4096, got ",
               c.kv_heads);
+}
+
+PageView page_view(const KVPages& c, const char* what) {
+    check_cache_shape(c, what);
     AIC_CHECK(c.page_size >= 1 && c.page_size <= 65536, InvalidArgument, what, ": page_size must be 1 .. 65536, got ",
               c.page_size);
     AIC_CHECK(c.n_pages >= 1 && c.n_pages <= INT32_MAX, InvalidArgument, what, ": n_pages must be 1 .. 2^31 - 1, got ",

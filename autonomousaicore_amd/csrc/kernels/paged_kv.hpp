@@ -34,7 +34,9 @@ struct PageView {
     }
 };
 
-// Arguments checked, and the view made of them.  `what` names the entry in the messages.
+// Type, heads and head_dim checked: what sizes are made of.  `what` names the entry in the messages.
+void check_cache_shape(const KVPages& c, const char* what);
+// All arguments checked, and the view made of them.
 PageView page_view(const KVPages& c, const char* what);
 
 constexpr int kBlock = 256;
