@@ -461,6 +461,7 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
                   "attn_paged: the workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
     else if (need > 0 && stream_scratch_ready(s))
         workspace = stream_scratch(static_cast<size_t>(need), s);
+    AIC_CHECK(q != o, InvalidArgument, "attn_paged: q and o must not overlap");  // a second pass reads q anew
     if (need == 0) workspace = nullptr;
     if (few) {
         // need may be the other kernel's alone

@@ -292,7 +292,7 @@ int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, con
                     const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
 /* Attention of the batch's rows over the cache, for chunks of a prompt, drafted tokens and single tokens
  * alike.  q and o are [T, H * head_dim] (leading dimensions ld_q, ld_o; dtype dt: the cache's, or
- * either with an e4m3 cache); query head h reads key/value head h / (H / kv_heads).  The row at
+ * either with an e4m3 cache; they must not overlap); query head h reads key/value head h / (H / kv_heads).  The row at
  * position pos sees the cached positions j <= pos, with window > 0 only those above pos - window:
  *   o = sum_j softmax_j(scale q . k_j) v_j,   lse[t * H + h] = log sum_j exp(scale q . k_j)
  * (lse fp32, nullable).  A row that sees nothing (position before 0) has o = 0 and lse = -infinity.  A

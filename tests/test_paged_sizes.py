@@ -46,3 +46,7 @@ def test_a_query_size_without_a_place_for_the_cache():
     """The size is asked before the pools are there."""
     c = cache(k_pages=None, v_pages=None, page_table=None)
     assert _lib.load().aic_hip_attn_paged_workspace(c, 1, 1, 1, 100000, 4) > 0
+
+
+def test_output_in_the_place_of_the_queries():
+    refused(INVALID, "overlap", "aic_hip_attn_paged", *attention(cache(), o=P))
