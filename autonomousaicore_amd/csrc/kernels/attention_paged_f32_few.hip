@@ -136,18 +136,21 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
                 const float off = mx == -INFINITY ? -down : fmaf(-mx, a.c, -down);
                 const float alpha = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[r] - mx) * a.c);
                 m[r] = mx;
-                l[r] *= alpha;
-                o[r].x *= alpha, o[r].y *= alpha, o[r].z *= alpha, o[r].w *= alpha;
+                // the batch by itself first: added one by one, keys lighter than half a step of the sum would all be lost
+                float lb = 0.0f;
+                float4 ob = make_float4(0, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
                     const float w = weight(s[i], a.c, off);
                     const float4 v = floats(vx[i], ve[i]);
-                    l[r] += w;
-                    const float4 y = make_float4(fmaf(w, v.x, o[r].x), fmaf(w, v.y, o[r].y), fmaf(w, v.z, o[r].z), fmaf(w, v.w, o[r].w));
+                    lb += w;
+                    const float4 y = make_float4(fmaf(w, v.x, ob.x), fmaf(w, v.y, ob.y), fmaf(w, v.z, ob.z), fmaf(w, v.w, ob.w));
                     // a hidden key adds nothing, also where its v is an infinity or NaN
                     const bool seen = open || static_cast<uint32_t>(k0 + i * KI + grp - lo[r]) < span[r];
-                    o[r].x = seen ? y.x : o[r].x, o[r].y = seen ? y.y : o[r].y, o[r].z = seen ? y.z : o[r].z, o[r].w = seen ? y.w : o[r].w;
+                    ob.x = seen ? y.x : ob.x, ob.y = seen ? y.y : ob.y, ob.z = seen ? y.z : ob.z, ob.w = seen ? y.w : ob.w;
                 }
+                l[r] = fmaf(l[r], alpha, lb);
+                o[r] = make_float4(fmaf(o[r].x, alpha, ob.x), fmaf(o[r].y, alpha, ob.y), fmaf(o[r].z, alpha, ob.z), fmaf(o[r].w, alpha, ob.w));
             }
         }
     }
