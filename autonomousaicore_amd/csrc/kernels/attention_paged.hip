@@ -35,10 +35,10 @@ namespace {
 // is, so nothing is staged twice and no copy is waited for.  The copies go straight to LDS (codes through registers)
 // from page ids in LDS, and fragments are read a group of four products ahead from addresses made anew for each
 // tile, so that two blocks of head_dim 128 keep their registers on one CU.  Bound by the fp32 matrix pipe (64 cycles
-// per v_mfma_f32_32x32x2_f32) and by how evenly one round of blocks fills the card: 4000 rows of 16 heads of 128, 809 us, 81 TFLOP/s
-// of 154, the pipe busy 51% of the time; behind 16000 cached tokens, where tiles are even, 117 TFLOP/s; 1000 on 2000 keys, 16 heads
-// over 2, 158 us, 78 TFLOP/s (through registers, one block per CU: 210 us; from page ids in memory: 326 us); 856 of 16
-// heads of 64, 43 us, whose longest block takes most of it.
+// per v_mfma_f32_32x32x2_f32) and by how evenly one round of blocks fills the card: 4000 rows of 16 heads of 128, 809 us,
+// 81 TFLOP/s of 154, the pipe busy 51% of the time; behind 16000 cached tokens, where tiles are even, 117 TFLOP/s; 1000 on
+// 2000 keys, 16 heads over 2, 158 us, 78 TFLOP/s (through registers, one block per CU: 210 us; from page ids in memory:
+// 326 us); 856 of 16 heads of 64, 43 us, whose longest block takes most of it.
 constexpr int kIds = 512;  // page ids in LDS at a time
 
 template <typename CT, int HD, int SH>

@@ -56,6 +56,7 @@ __device__ __forceinline__ T fresh(T x) {
 __device__ __forceinline__ int fresh_uniform(int x) { return __builtin_amdgcn_readfirstlane(fresh(x)); }
 template <typename A>
 __device__ __forceinline__ A fresh_argument() {
+    static_assert(sizeof(A) % 4 == 0);
     typedef const __attribute__((address_space(4))) uint32_t* words_t;
     struct Words {
         uint32_t w[sizeof(A) / 4];

@@ -8,10 +8,10 @@
 // output of its own keys; they are joined once at the end.  The waves of a block take batches of keys in
 // turn and share nothing until then; 8 loads of 1 KB of K and of V per wave are in flight, with enough waves
 // per CU to cover them (30 single tokens of 16 heads of 128 on 1000 keys: 66 us, 4.8 TB/s; 16 loads: 71 us; on e4m3
-// caches of 4000, where each value is converted, 148 us).  Bound by the bytes of
-// the cache for one and two rows, by the vector instructions behind them; tiles of 8 rows would take 24.5 us for 30
-// tokens of 16 heads of 64 over 2 on 1000 keys, and the matrix pipe 20.9 us (59 and 52 us for 30 sequences of 7
-// rows of 12 heads; the other way round, 26 and 30 us, for 10 of them).
+// caches of 4000, where each value is converted, 148 us).  Bound by the bytes of the cache for one and two rows, by the
+// vector instructions behind them; tiles of 8 rows would take 24.5 us for 30 tokens of 16 heads of 64 over 2 on 1000
+// keys, and the matrix pipe 20.9 us (59 and 52 us for 30 sequences of 7 rows of 12 heads; the other way round, 26 and
+// 30 us, for 10 of them).
 #include <type_traits>
 
 #include "attention_paged.hpp"

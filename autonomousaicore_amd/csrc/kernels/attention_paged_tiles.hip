@@ -382,7 +382,8 @@ __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a,
 
 template <int HD, bool E4>
 __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
-    // as one_or_two_passes; where a row of the largest powers was found, the second pass is anew from the start, and there may be a third
+    // as one_or_two_passes; where a row of the largest powers was found, the second pass is anew from the start, and there
+    // may be a third
     __shared__ TilesLds<HD> lds;
     const int tid = threadIdx.x;
     if (tid == 0) lds.past = 0, lds.top = 0;

@@ -18,9 +18,9 @@
 // Nothing is returned to the host.  (Two launches, the draw by the last block of a sequence, came to the same:
 // 33.3 us for 33.6, for the counting is another trip to memory.)
 //
-// 64 sequences of up to 7 drafts, 32000 fp32 logits: 33.6 us; statistics 19.5 us (75 MB at 3.8 TB/s, and as long for
-// bf16 logits: 64-bit products, vector units busy about 60% of the time and waves waiting for issue half of theirs), residual 11.7 us, draw 4.9 us.  One sequence of 4 drafts: 14.2 us, three chains
-// of latencies of 3.8, 6.9 and 4.4 us.
+// 64 sequences of up to 7 drafts, 32000 fp32 logits: 33.6 us; statistics 19.5 us (75 MB at 3.8 TB/s, and as long for bf16
+// logits: 64-bit products, vector units busy about 60% of the time and waves waiting for issue half of theirs),
+// residual 11.7 us, draw 4.9 us.  One sequence of 4 drafts: 14.2 us, three chains of latencies of 3.8, 6.9 and 4.4 us.
 #include <algorithm>
 #include <cmath>
 

@@ -32,7 +32,7 @@ def test_size_queries_refuse_what_the_call_refuses(kw, code):
     H = kw.get("kv_heads", 2) * 2
     for max_len in (9, 600, 100000):
         assert _lib.load().aic_hip_attn_paged_workspace(c, 4, 8, 2, max_len, H) == -code
-    refused(code, "", "aic_hip_attn_paged", *attention(c, H=H))
+    refused(code, "head|cache", "aic_hip_attn_paged", *attention(c, H=H))
 
 
 def test_cache_sizes_of_rows():
