@@ -7,8 +7,9 @@ torch = pytest.importorskip("torch")
 
 pytestmark = pytest.mark.gpu
 
-from tests.gpu_util import host  # noqa: E402
-from tests.paged_ref import HALF, TORCH, Paged, attention  # noqa: E402
+from autonomousaicore_amd import _lib  # noqa: E402
+from tests.gpu_util import call, host, ptr  # noqa: E402
+from tests.paged_ref import CODE, HALF, TORCH, Paged, attention  # noqa: E402
 from tests.test_gpu_attn_paged import TYPES, Call  # noqa: E402
 
 
@@ -117,3 +118,41 @@ def test_large_values_in_rows_of_odd_strides(dt, cache, n, L):
     inside = np.zeros(a.buf.numel(), bool)
     inside[a.shift:a.shift + a.T * a.ld].reshape(a.T, a.ld)[p.offs[0]:p.offs[-1], :a.w] = True
     assert np.all(host(a.buf)[~inside] == 7.0) and np.all(host(a.lse)[p.offs[-1]:] == 7.0)
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("n,L", [(1, 300), (1, 2100), (40, 300), (200, 700)])
+def test_replays_over_values_that_change_their_size(dt, cache, n, L):
+    """One graph over normal, large, normal and small values in turn, between eager calls: each replay equals the eager call bit for
+    bit, so no replay leaves anything to the next."""
+    p = Paged([n], [L], 2, 64, 16, cache, seed=n + L)
+    a, e = Call(p, 4, dt), Call(p, 4, dt)
+    ws = [torch.empty(max(a.bytes(), 16), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    c = p.struct()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def launch(x, w):
+        call("aic_hip_attn_paged", c, ptr(x.q), x.ld, ptr(x.o), x.ld, ptr(x.lse), ptr(p.dev_offs), ptr(p.dev_lens), *x.sizes(), x.H, 0, x.scale,
+             ptr(w), w.numel(), CODE[dt], s.cuda_stream)
+
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        launch(a, ws[0])
+    pool, exps = p.pool["v"]
+    normal = pool.clone(), None if exps is None else exps.clone()
+    plain = p.v
+    for by in (0, 125, 0, -100):
+        if exps is None:
+            pool.copy_((normal[0].double() * 2.0 ** by).to(pool.dtype))
+        else:
+            exps.copy_(normal[1].int() + by)
+        p.v = plain * 2.0 ** by
+        a.buf.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        launch(e, ws[1])
+        torch.cuda.synchronize()
+        assert torch.equal(a.o, e.o) and torch.equal(a.lse, e.lse)
+        _check(a, dt)
+    _lib.call("aic_hip_mem_release_stream", s.cuda_stream)
