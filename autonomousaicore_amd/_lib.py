@@ -11,7 +11,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaic_hip.so")
 
-AIC_F32, AIC_F16, AIC_BF16, AIC_I32, AIC_I64, AIC_U8, AIC_U16 = 0, 1, 2, 3, 4, 5, 6
+AIC_F32, AIC_F16, AIC_BF16, AIC_I32, AIC_I64, AIC_U8, AIC_U16, AIC_U4 = 0, 1, 2, 3, 4, 5, 6, 7
 
 vp = C.c_void_p
 i64 = C.c_int64
@@ -109,6 +109,13 @@ SIGNATURES = {
                                     vp, vp, i32, vp]),
     "aic_hip_kv_write": (i32, [C.POINTER(KVPages), vp, vp, i64, vp, vp, i64, i64, i32, vp]),
     "aic_hip_kv_read": (i32, [C.POINTER(KVPages), vp, vp, i64, vp, vp, i64, i64, i32, vp]),
+    "aic_hip_kv_append": (i32, [C.POINTER(KVPages), vp, i64, vp, i64, i64, vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i32, vp]),
+    "aic_hip_kv_bounds": (i32, [C.POINTER(KVPages), vp, vp, vp, i64, i64, vp]),
+    "aic_hip_kv_select_workspace": (i64, [C.POINTER(KVPages), i64, i64]),
+    "aic_hip_kv_select": (i32, [C.POINTER(KVPages), vp, vp, i64, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, vp, vp, vp, i64, i32,
+                                vp]),
+    "aic_hip_attn_paged_selected_workspace": (i64, [C.POINTER(KVPages), i64, i64, i64]),
+    "aic_hip_attn_paged_selected": (i32, [C.POINTER(KVPages), vp, i64, vp, i64, vp, vp, vp, i64, i64, i64, f32, vp, i64, i32, vp]),
     "aic_hip_attn_paged_workspace": (i64, [C.POINTER(KVPages), i64, i64, i64, i64, i64]),
     "aic_hip_attn_paged": (i32, [C.POINTER(KVPages), vp, i64, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, i64, f32,
                                  vp, i64, i32, vp]),

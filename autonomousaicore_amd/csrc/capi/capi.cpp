@@ -54,6 +54,7 @@ const char* dtype_name(DType d) noexcept {
         case DType::Int64: return "int64";
         case DType::UInt8: return "uint8";
         case DType::UInt16: return "uint16";
+        case DType::UInt4: return "uint4";
     }
     return "unknown";
 }
@@ -264,6 +265,47 @@ int aic_hip_kv_write(const aic_kv_pages* cache, const void* k, const void* v, in
 int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, const int64_t* offsets,
                     const int64_t* lens, int64_t B, int64_t T, aic_dtype d, aic_stream stream) {
     return guard([&] { aic::hip::kv_read(pages(cache), k, v, ld, offsets, lens, B, T, dt(d), st(stream)); });
+}
+
+int aic_hip_kv_append(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* q_out, int64_t ld_qo, int64_t H, const void* k,
+                      const void* v, int64_t ld_kv, const float* cos_t, const float* sin_t, int64_t n_pos, const int64_t* offsets,
+                      const int64_t* lens, int64_t B, int64_t T, aic_dtype d, aic_stream stream) {
+    return guard([&] {
+        aic::hip::kv_append_rope(pages(cache), q, ld_q, q_out, ld_qo, H, k, v, ld_kv, cos_t, sin_t, n_pos, offsets, lens, B, T, dt(d),
+                                 st(stream));
+    });
+}
+
+int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T,
+                      aic_stream stream) {
+    return guard([&] { aic::hip::kv_bounds(pages(cache), bounds, offsets, lens, B, T, st(stream)); });
+}
+
+int64_t aic_hip_kv_select_workspace(const aic_kv_pages* cache, int64_t T, int64_t max_len) {
+    return guard_size([&] { return aic::hip::kv_select_workspace(pages(cache), T, max_len); });
+}
+
+int aic_hip_kv_select(const aic_kv_pages* cache, const void* bounds, const void* q, int64_t ld_q, const int64_t* offsets,
+                      const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t first, int64_t last,
+                      int64_t n_sel, int32_t* picked, int64_t* picked_lens, void* workspace, int64_t workspace_bytes, aic_dtype d,
+                      aic_stream stream) {
+    return guard([&] {
+        aic::hip::kv_select(pages(cache), bounds, q, ld_q, offsets, lens, B, T, max_q, max_len, H, first, last, n_sel, picked,
+                            picked_lens, workspace, workspace_bytes, dt(d), st(stream));
+    });
+}
+
+int64_t aic_hip_attn_paged_selected_workspace(const aic_kv_pages* cache, int64_t T, int64_t n_sel, int64_t H) {
+    return guard_size([&] { return aic::hip::attn_paged_selected_workspace(pages(cache), T, n_sel, H); });
+}
+
+int aic_hip_attn_paged_selected(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse,
+                                const int32_t* picked, const int64_t* picked_lens, int64_t T, int64_t n_sel, int64_t H, float scale,
+                                void* workspace, int64_t workspace_bytes, aic_dtype d, aic_stream stream) {
+    return guard([&] {
+        aic::hip::attn_paged_selected(pages(cache), q, ld_q, o, ld_o, lse, picked, picked_lens, T, n_sel, H, scale, workspace,
+                                      workspace_bytes, dt(d), st(stream));
+    });
 }
 
 int64_t aic_hip_attn_paged_workspace(const aic_kv_pages* cache, int64_t B, int64_t T, int64_t max_q, int64_t max_len,

@@ -44,21 +44,22 @@ constexpr int kIds = 512;  // page ids in LDS at a time
 template <typename CT, int HD, int SH>
 __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block, float down) {
     constexpr int SETS = 4 / SH, R = 32 * SETS, KT = 32 * SH, OB = HD / 32;
-    constexpr int UPR = HD * sizeof(CT) / 16;   // 16-byte units of a cached row
+    constexpr int UPR = HD / kPer16<CT>;        // 16-byte units of a cached row
     constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
-    constexpr bool E4 = sizeof(CT) == 1;
+    constexpr bool E4 = kE4<CT> || kE2<CT>;     // codes
     constexpr int TILE = KT * HD * 4;
     __shared__ __attribute__((aligned(16))) char tiles[2 * TILE];
     __shared__ int ids[kIds];
     char *ks = tiles, *vs = tiles + TILE;
 
     const int Hkv = a.kv.Hkv;
-    const int kvh = block % Hkv;
-    const int rest = block / Hkv;
-    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
+    const int rest = block / a.heads;
+    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (a.heads * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
     if (!find_tile<R>(a, tile, b, local)) return false;
+    const int kvh = kv_head(a, b, block % a.heads);
     const Seq sq = wave_sequence(a, b);
+    if (sq.n == 0) return false;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     const int set = wave % SETS, share = wave / SETS, sub = 32 * share;  // this wave's rows of the block and keys of a tile
     const int rows = sq.n * a.G, r0 = local * R, r = r0 + set * 32 + (lane & 31);
@@ -134,8 +135,9 @@ __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block,
                     for (int i = 0; i < NU; ++i) {
                         const int u = i * 256 + tid;
                         const int64_t row = row_at(w0 + t * KT + min(u / UPR, KT - 1));
-                        codes.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * HD + (u % UPR) * 16 : none);
-                        codes.e[i] = row >= 0 ? exps[row] : 127;
+                        codes.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * kRowBytes<CT, HD> + (u % UPR) * 16 : none);
+                        if constexpr (kE2<CT>) codes.e[i] = row >= 0 ? exps[row * UPR + u % UPR] : kNanGroup;
+                        else codes.e[i] = row >= 0 ? exps[row] : 127;
                     }
                 } else {
 #pragma unroll
@@ -153,6 +155,20 @@ __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block,
                         const int u = i * 256 + tid, row = u / UPR, c = u % UPR;
                         if (KT * UPR % 256 != 0 && u >= KT * UPR) continue;
                         const float s = exp_scale(codes.e[i]);
+                        if constexpr (kE2<CT>) {
+                            const uint32_t w[4] = {codes.w[i].x, codes.w[i].y, codes.w[i].z, codes.w[i].w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                float y[8];
+                                e2m1_floats(w[j], s, y);
+                                if (__builtin_expect(codes.e[i] == kNanGroup, 0))
+#pragma unroll
+                                    for (int x = 0; x < 8; ++x) y[x] = NAN;
+                                *reinterpret_cast<float4*>(dst + chunk_at<float, HD>(row, 8 * c + 2 * j)) = make_float4(y[0], y[1], y[2], y[3]);
+                                *reinterpret_cast<float4*>(dst + chunk_at<float, HD>(row, 8 * c + 2 * j + 1)) = make_float4(y[4], y[5], y[6], y[7]);
+                            }
+                            continue;
+                        }
                         if (__builtin_expect(codes.e[i] >= kTopByte, 0)) codes.w[i] = e4m3_in_range(codes.w[i], codes.e[i]);
                         const uint2 w[2] = {make_uint2(codes.w[i].x, codes.w[i].y), make_uint2(codes.w[i].z, codes.w[i].w)};
 #pragma unroll
@@ -316,7 +332,8 @@ __global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (i >= a.T * a.H) return;
     const int64_t t = i / a.H;
-    if (t < a.offsets[0] || t >= a.offsets[a.B]) return;  // rows of no sequence stay as they are
+    // rows of no sequence stay as they are
+    if (a.picked ? a.lens[t * a.kv.Hkv + i % a.H / a.G] < 0 : t < a.offsets[0] || t >= a.offsets[a.B]) return;
     const int lane = threadIdx.x & 63;
     const int64_t step = a.T * a.H;
     // a lane per split: the splits of one launch are at most kMaxSplits
@@ -405,17 +422,21 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
 
 }  // namespace
 
-int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H) {
+// Bytes of the parts of a call's sizes; picked: of rows with pages of their own, a sequence each (bf16 queries then always go to the
+// few rows' kernel).
+namespace {
+
+int64_t parts_bytes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, bool picked) {
     check_sizes(c, B, T, max_q, max_len, H);
     check_cache_shape(c, "attn_paged");
     if (B == 0 || T == 0) return 0;
     max_q = std::min(max_q, T);
-    // the cache's type does not tell the queries' (e4m3 serves both): room for either
+    // the cache's type does not tell the queries' (codes serve both): room for either
     int64_t n = 0;
     const int64_t G = H / c.kv_heads;
-    const bool e4m3 = c.type == DType::UInt8, few = few_rows(max_q, G, c.head_dim, e4m3);
+    const bool few = picked || few_rows(max_q, G, c.head_dim, c.type);
     if (c.type != DType::Float32 && few)
-        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, e4m3);
+        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, c.type);
     if (c.type != DType::Float32 && !few)
         n = plan_bytes(plan(B, T, max_len, H, c, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
@@ -423,51 +444,37 @@ int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max
     return n;
 }
 
-void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int64_t* offsets,
-                const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t window,
-                float scale, void* workspace, int64_t workspace_bytes, DType dt, hipStream_t s) {
-    check_sizes(c, B, T, max_q, max_len, H);
-    AIC_CHECK(dt == DType::Float32 || dt == DType::BFloat16, DTypeMismatch, "attn_paged: queries are float32 or bfloat16");
-    AIC_CHECK(c.type == dt || c.type == DType::UInt8, DTypeMismatch, "attn_paged: queries of ", dtype_name(dt),
-              " with a cache of ", dtype_name(c.type));
-    const PageView pv = page_view(c, "attn_paged");
-    AIC_CHECK(ld_q >= H * c.head_dim && ld_o >= H * c.head_dim, InvalidArgument,
-              "attn_paged: leading dimension below heads * head_dim");
-    AIC_CHECK(std::isfinite(scale * kLog2e) && scale > 0.0f, InvalidArgument, "attn_paged: scale must be positive and below 2.3e38, got ", scale);
-    AIC_CHECK(window >= 0, InvalidArgument, "attn_paged: window must not be negative, got ", window);
-    AIC_CHECK(workspace_bytes >= 0, InvalidArgument, "attn_paged: negative workspace size");
-    if (B == 0 || T == 0) return;
-    AIC_CHECK(q && o && offsets && lens, InvalidArgument, "attn_paged: null pointer");
+struct Workspace {
+    void* at;
+    int64_t bytes;
+};
+
+// a: pointers, strides, T, H, G and the batch; the rest follows from the sizes, which are those of the sequences that the blocks see.
+void attend(PagedArgs& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, float scale, Workspace w,
+            DType dt, hipStream_t s) {
     max_q = std::min(max_q, T);
-
     const int64_t size = static_cast<int64_t>(dtype_size(dt));
-    PagedArgs a{};
-    a.kv = pv;
-    a.q = q, a.o = o, a.lse = lse;
-    a.ldq = ld_q, a.ldo = ld_o, a.T = T;
-    a.offsets = offsets, a.lens = lens;
-    a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.G = static_cast<int>(H / c.kv_heads);
-    a.window = static_cast<int>(std::min<int64_t>(window, INT32_MAX));
     a.c = scale * kLog2e;
-    a.vec_q = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q * size % 16 == 0;
-    a.vec_o = reinterpret_cast<uintptr_t>(o) % 16 == 0 && ld_o * size % 16 == 0;
+    a.vec_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq * size % 16 == 0;
+    a.vec_o = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.ldo * size % 16 == 0;
 
-    const bool e4m3 = c.type == DType::UInt8, few = dt == DType::BFloat16 && few_rows(max_q, a.G, c.head_dim, e4m3);
+    const bool few = dt == DType::BFloat16 && (a.picked || few_rows(max_q, a.G, c.head_dim, c.type));
     const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim);
     Plan p = plan(B, T, max_len, H, c, R);
-    const int64_t need = attn_paged_workspace(c, B, T, max_q, max_len, H);
+    const int64_t need = parts_bytes(c, B, T, max_q, max_len, H, a.picked);
     const StreamScratchUse use(s);
+    void* workspace = w.at;
     if (workspace)
-        AIC_CHECK(workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
-                  "attn_paged: the workspace must be 16-byte aligned and hold ", need, " bytes, got ", workspace_bytes);
+        AIC_CHECK(w.bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
+                  "attn_paged: the workspace must be 16-byte aligned and hold ", need, " bytes, got ", w.bytes);
     else if (need > 0 && stream_scratch_ready(s))
         workspace = stream_scratch(static_cast<size_t>(need), s);
-    AIC_CHECK(q != o, InvalidArgument, "attn_paged: q and o must not overlap");  // a second pass reads q anew
+    AIC_CHECK(a.q != a.o, InvalidArgument, "attn_paged: q and o must not overlap");  // a second pass reads q anew
     if (need == 0) workspace = nullptr;
     if (few) {
         // need may be the other kernel's alone
-        const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, e4m3) > 0;
-        attn_paged_few(a, max_q, e4m3, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
+        const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, c.type) > 0;
+        attn_paged_few(a, max_q, c.type, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;
     }
     if (!workspace) p.nsplit = 1;  // nothing to split, or captured without a workspace of its own
@@ -478,17 +485,21 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     }
     const int64_t blocks = p.tiles * c.kv_heads * p.nsplit;
     AIC_CHECK(blocks <= INT32_MAX, OutOfRange, "attn_paged: too many rows in one call");
-    auto run = [&](auto t, auto ct, auto hd) {
+    auto run = [&](auto t, auto hd) {
         using X = decltype(t);
         constexpr int D = decltype(hd)::value;
+        const auto grid = static_cast<unsigned>(blocks);
         if constexpr (sizeof(X) == 2) {
-            attn_paged_tiles(a, sizeof(ct) == 1, D, static_cast<unsigned>(blocks), s);
+            attn_paged_tiles(a, c.type, D, grid, s);
+        } else if (R <= 4) {
+            attn_paged_f32_few(a, static_cast<int>(R), c.type, D, grid, s);
         } else {
-            const auto grid = static_cast<unsigned>(blocks);
-            if (R <= 4) attn_paged_f32_few(a, static_cast<int>(R), sizeof(ct) == 1, D, grid, s);
-            else if (R == 128) attn_paged_f32_k<decltype(ct), D, 1><<<grid, 256, 0, s>>>(a);
-            else if (R == 64) attn_paged_f32_k<decltype(ct), D, 2><<<grid, 256, 0, s>>>(a);
-            else attn_paged_f32_k<decltype(ct), D, 4><<<grid, 256, 0, s>>>(a);
+            by_cache_type<float>(c.type, [&](auto ct) {
+                using CT = decltype(ct);
+                if (R == 128) attn_paged_f32_k<CT, D, 1><<<grid, 256, 0, s>>>(a);
+                else if (R == 64) attn_paged_f32_k<CT, D, 2><<<grid, 256, 0, s>>>(a);
+                else attn_paged_f32_k<CT, D, 4><<<grid, 256, 0, s>>>(a);
+            });
             AIC_LAUNCH_CHECK("attn_paged");
         }
         if (a.nsplit > 1) {
@@ -499,14 +510,104 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
         }
     };
     auto types = [&](auto hd) {
-        if (dt == DType::Float32 && c.type == DType::Float32) run(float{}, float{}, hd);
-        else if (dt == DType::Float32) run(float{}, uint8_t{}, hd);
-        else if (c.type == DType::BFloat16) run(bf16{}, bf16{}, hd);
-        else run(bf16{}, uint8_t{}, hd);
+        if (dt == DType::Float32) run(float{}, hd);
+        else run(bf16{}, hd);
     };
     if (c.head_dim == 32) types(std::integral_constant<int, 32>{});
     else if (c.head_dim == 64) types(std::integral_constant<int, 64>{});
     else types(std::integral_constant<int, 128>{});
+}
+
+void check_call(const KVPages& c, int64_t ld_q, int64_t ld_o, int64_t H, float scale, int64_t workspace_bytes, DType dt) {
+    AIC_CHECK(ld_q >= H * c.head_dim && ld_o >= H * c.head_dim, InvalidArgument,
+              "attn_paged: leading dimension below heads * head_dim");
+    AIC_CHECK(std::isfinite(scale * kLog2e) && scale > 0.0f, InvalidArgument, "attn_paged: scale must be positive and below 2.3e38, got ", scale);
+    AIC_CHECK(workspace_bytes >= 0, InvalidArgument, "attn_paged: negative workspace size");
+}
+
+void check_types(const KVPages& c, DType dt) {
+    AIC_CHECK(dt == DType::Float32 || dt == DType::BFloat16, DTypeMismatch, "attn_paged: queries are float32 or bfloat16");
+    AIC_CHECK(c.type == dt || holds_codes(c.type), DTypeMismatch, "attn_paged: queries of ", dtype_name(dt),
+              " with a cache of ", dtype_name(c.type));
+}
+
+// The cache as its (row, key/value head) pairs see it: sequences of one head.
+KVPages one_head(const KVPages& c) {
+    AIC_CHECK(c.kv_heads >= 1 && c.kv_heads <= 4096, InvalidArgument, "attn_paged: kv_heads must be 1 .. 4096, got ", c.kv_heads);
+    KVPages x = c;
+    x.kv_heads = 1;
+    return x;
+}
+
+// Sizes of attn_paged_selected: keys of a row.
+int64_t check_picked(const KVPages& c, int64_t T, int64_t n_sel, int64_t H) {
+    check_cache_shape(c, "attn_paged");
+    AIC_CHECK(T >= 0 && T <= INT32_MAX, InvalidArgument, "attn_paged: T must be 0 .. 2^31 - 1");
+    AIC_CHECK(H >= 1 && H % c.kv_heads == 0, ShapeMismatch, "attn_paged: ", H, " query heads over ", c.kv_heads, " key/value heads");
+    AIC_CHECK(T * c.kv_heads <= INT32_MAX, OutOfRange, "attn_paged: more than 2^31 - 1 pairs of rows and key/value heads");
+    AIC_CHECK(c.page_size >= 1 && c.page_size <= 65536, InvalidArgument, "attn_paged: page_size must be 1 .. 65536, got ", c.page_size);
+    AIC_CHECK(n_sel >= 1 && n_sel <= kMaxLen / c.page_size, InvalidArgument, "attn_paged: n_sel must be 1 .. ", kMaxLen / c.page_size, ", got ",
+              n_sel);
+    return n_sel * c.page_size;
+}
+
+}  // namespace
+
+int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H) {
+    return parts_bytes(c, B, T, max_q, max_len, H, false);
+}
+
+void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int64_t* offsets,
+                const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t window,
+                float scale, void* workspace, int64_t workspace_bytes, DType dt, hipStream_t s) {
+    check_sizes(c, B, T, max_q, max_len, H);
+    check_types(c, dt);
+    const PageView pv = page_view(c, "attn_paged");
+    check_call(c, ld_q, ld_o, H, scale, workspace_bytes, dt);
+    AIC_CHECK(window >= 0, InvalidArgument, "attn_paged: window must not be negative, got ", window);
+    if (B == 0 || T == 0) return;
+    AIC_CHECK(q && o && offsets && lens, InvalidArgument, "attn_paged: null pointer");
+    PagedArgs a{};
+    a.kv = pv;
+    a.q = q, a.o = o, a.lse = lse;
+    a.ldq = ld_q, a.ldo = ld_o, a.T = T;
+    a.offsets = offsets, a.lens = lens;
+    a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.G = static_cast<int>(H / c.kv_heads);
+    a.window = static_cast<int>(std::min<int64_t>(window, INT32_MAX));
+    a.heads = static_cast<int>(c.kv_heads);
+    attend(a, c, B, T, max_q, max_len, H, scale, {workspace, workspace_bytes}, dt, s);
+}
+
+int64_t attn_paged_selected_workspace(const KVPages& c, int64_t T, int64_t n_sel, int64_t H) {
+    const int64_t len = check_picked(c, T, n_sel, H), rows = T * c.kv_heads;
+    return parts_bytes(one_head(c), rows, rows, 1, len, H / c.kv_heads, true);
+}
+
+void attn_paged_selected(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int32_t* picked,
+                         const int64_t* picked_lens, int64_t T, int64_t n_sel, int64_t H, float scale, void* workspace,
+                         int64_t workspace_bytes, DType dt, hipStream_t s) {
+    const int64_t len = check_picked(c, T, n_sel, H), rows = T * c.kv_heads, G = H / c.kv_heads;
+    const KVPages one = one_head(c);
+    check_sizes(one, rows, rows, 1, len, G);
+    check_types(c, dt);
+    KVPages view = c;
+    view.page_table = picked;
+    view.ld_table = n_sel;
+    if (T > 0) AIC_CHECK(picked && picked_lens, InvalidArgument, "attn_paged: null pointer");
+    else view.page_table = reinterpret_cast<const int32_t*>(c.k_pages);  // nothing is read
+    const PageView pv = page_view(view, "attn_paged");
+    check_call(c, ld_q, ld_o, H, scale, workspace_bytes, dt);
+    if (T == 0) return;
+    AIC_CHECK(q && o, InvalidArgument, "attn_paged: null pointer");
+    PagedArgs a{};
+    a.kv = pv;
+    a.q = q, a.o = o, a.lse = lse;
+    a.ldq = ld_q, a.ldo = ld_o, a.T = T;
+    a.lens = picked_lens;
+    a.B = static_cast<int>(rows), a.H = static_cast<int>(H), a.G = static_cast<int>(G);
+    a.heads = 1;
+    a.picked = true;
+    attend(a, one, rows, rows, 1, len, G, scale, {workspace, workspace_bytes}, dt, s);
 }
 
 }  // namespace aic::hip

@@ -21,6 +21,10 @@ struct PagedArgs {
     float2* part_ml;  // [nsplit][T][H]: maximum, sum (-1: only scores of -infinity)
     float* part_o;    // [nsplit][T][H][hd]
     bool vec_q, vec_o;
+    // key/value heads that a launch's blocks go over beside the sequences: all of them, or one where each (row, head) is a
+    // sequence of its own with the pages picked for it as its page table
+    int heads;
+    bool picked;
 };
 
 namespace {
@@ -90,8 +94,17 @@ struct Seq {
     int n, len;    // queries, cached keys
 };
 __device__ __forceinline__ Seq sequence(const PagedArgs& a, int b) {
+    if (a.picked) {  // its one row stands behind the picked positions; length -1: nobody's row, left as it is
+        const int64_t len = a.lens[b];
+        return {static_cast<uint32_t>(b) / static_cast<uint32_t>(a.kv.Hkv), len >= 0, static_cast<int>(min(max(len, int64_t{0}), kMaxLen))};
+    }
     const int64_t lo = min(max(a.offsets[b], int64_t{0}), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
     return {lo, static_cast<int>(hi - lo), static_cast<int>(min(max(a.lens[b], int64_t{0}), kMaxLen))};
+}
+
+// The key/value head of sequence b's blocks numbered h.
+__device__ __forceinline__ int kv_head(const PagedArgs& a, int b, int h) {
+    return a.picked ? static_cast<int>(static_cast<uint32_t>(b) % static_cast<uint32_t>(a.kv.Hkv)) : h;
 }
 
 // The same for a b that is one for the whole wave, in scalar registers.
@@ -108,6 +121,12 @@ __device__ __forceinline__ Seq wave_sequence(const PagedArgs& a, int b) {
 // Every wave finds it by itself: 64 sequences per step, their tile counts added up across lanes.
 template <int R>
 __device__ __forceinline__ bool find_tile(const PagedArgs& a, int tile, int& b, int& local) {
+    if (a.picked) {  // all have as many tiles
+        const uint32_t per = static_cast<uint32_t>((a.G + R - 1) / R);
+        b = static_cast<int>(static_cast<uint32_t>(tile) / per);
+        local = tile - b * static_cast<int>(per);
+        return b < a.B;
+    }
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int tiles = 0;
@@ -310,18 +329,26 @@ __device__ __forceinline__ bool store_row(const PagedArgs& a, const Rows<HD / 32
 
 }  // namespace
 
+// f(cache type) of a cache that bf16 or fp32 (T) queries read.
+template <typename T, typename F>
+void by_cache_type(DType type, F&& f) {
+    if (type == DType::UInt8) f(uint8_t{});
+    else if (type == DType::UInt4) f(e2m1x2{});
+    else f(T{});
+}
+
 // Few query rows per key/value head, bf16 queries (attention_paged_few.hip): row groups of `group` rows; with a
 // workspace the batch's keys are cut into equal shares, one per resident block.
-bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, bool e4m3);
-int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3);
-void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s);
+bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, DType type);
+int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type);
+void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s);
 
 // Up to 4 query rows per key/value head, fp32 queries (attention_paged_f32_few.hip): tiles of so many rows, 0 for
 // more of them; tiles x splits x key/value heads blocks.
 int f32_few_rows(int64_t max_q, int64_t G);
-void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, unsigned blocks, hipStream_t s);
+void attn_paged_f32_few(const PagedArgs& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s);
 
 // Many query rows per key/value head, bf16 queries (attention_paged_tiles.hip): tiles x splits x key/value heads blocks.
-void attn_paged_tiles(const PagedArgs& a, bool e4m3, int head_dim, unsigned blocks, hipStream_t s);
+void attn_paged_tiles(const PagedArgs& a, DType type, int head_dim, unsigned blocks, hipStream_t s);
 
 }  // namespace aic::hip

@@ -38,8 +38,16 @@ __device__ __forceinline__ float across_groups(float x, F f) {
     return facing_op<32>(x, f);
 }
 
-template <typename CT> using Quad = std::conditional_t<sizeof(CT) == 1, uint32_t, float4>;
+// Four neighbouring elements of a cached row.
+template <typename CT> using Quad = std::conditional_t<kE2<CT>, uint16_t, std::conditional_t<kE4<CT>, uint32_t, float4>>;
 __device__ __forceinline__ float4 floats(float4 x, uint32_t) { return x; }
+__device__ __forceinline__ float4 floats(uint16_t x, uint32_t e) {
+    const float s = exp_scale(e);
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, s, 0);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, s, 1);
+    const bool none = e == kNanGroup;
+    return make_float4(none ? NAN : a[0], none ? NAN : a[1], none ? NAN : b[0], none ? NAN : b[1]);
+}
 __device__ __forceinline__ float4 floats(uint32_t x, uint32_t e) {
     const float s = exp_scale(e);
     const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, s, false);
@@ -54,12 +62,13 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
     static_assert(KB <= 64, "a lane per key looks its page up");
     __shared__ float2 mls[4][RM];
     __shared__ float os[4][RM][HD];
-    const int Hkv = a.kv.Hkv;
-    const int kvh = block % Hkv, rest = block / Hkv;
+    const int rest = block / a.heads;
     const int split = rest % a.nsplit, tile = rest / a.nsplit;
     int b, local;
     if (!find_tile<RM>(a, tile, b, local)) return false;
+    const int kvh = kv_head(a, b, block % a.heads);
     const Seq sq = wave_sequence(a, b);
+    if (sq.n == 0) return false;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = lane / L, d0 = 4 * (lane % L);
     const int rows = sq.n * a.G, r0 = local * RM;
@@ -98,10 +107,13 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
             for (int i = 0; i < NI; ++i) {
                 const int64_t at = __shfl(row, i * KI + grp, 64);
                 const char* none = reinterpret_cast<const char*>(&kNoPage);
-                const int64_t byte = (at * HD + d0) * static_cast<int64_t>(sizeof(CT));
+                const int64_t byte = at * kRowBytes<CT, HD> + d0 * 16 / kPer16<CT>;
                 kx[i] = *reinterpret_cast<const Quad<CT>*>(at >= 0 ? a.kv.kp + byte : none);
                 vx[i] = *reinterpret_cast<const Quad<CT>*>(at >= 0 ? a.kv.vp + byte : none);
-                if constexpr (sizeof(CT) == 1) {
+                if constexpr (kE2<CT>) {
+                    ke[i] = at >= 0 ? a.kv.ke[at * (HD / kGroup) + d0 / kGroup] : kNanGroup;
+                    ve[i] = at >= 0 ? a.kv.ve[at * (HD / kGroup) + d0 / kGroup] : kNanGroup;
+                } else if constexpr (kE4<CT>) {
                     ke[i] = at >= 0 ? a.kv.ke[at] : 127;
                     ve[i] = at >= 0 ? a.kv.ve[at] : 127;
                 } else {
@@ -109,7 +121,7 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
                 }
             }
             row = row_of(k0 + 4 * KB);
-            if constexpr (sizeof(CT) == 1) {
+            if constexpr (kE4<CT>) {
                 uint32_t most = 0;
 #pragma unroll
                 for (int i = 0; i < NI; ++i) most = max(most, max(ke[i], ve[i]));
@@ -218,7 +230,7 @@ int f32_few_rows(int64_t max_q, int64_t G) {
     return rows > 4 ? 0 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
 }
 
-void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, unsigned blocks, hipStream_t s) {
+void attn_paged_f32_few(const PagedArgs& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s) {
     auto run = [&](auto ct, auto hd) {
         using C = decltype(ct);
         constexpr int D = decltype(hd)::value;
@@ -227,10 +239,11 @@ void attn_paged_f32_few(const PagedArgs& a, int rows, bool e4m3, int head_dim, u
         else attn_paged_f32_few_k<C, D, 4><<<blocks, 256, 0, s>>>(a);
         AIC_LAUNCH_CHECK("attn_paged few, fp32");
     };
-    auto type = [&](auto hd) { e4m3 ? run(uint8_t{}, hd) : run(float{}, hd); };
-    if (head_dim == 32) type(std::integral_constant<int, 32>{});
-    else if (head_dim == 64) type(std::integral_constant<int, 64>{});
-    else type(std::integral_constant<int, 128>{});
+    by_cache_type<float>(type, [&](auto ct) {
+        if (head_dim == 32) run(ct, std::integral_constant<int, 32>{});
+        else if (head_dim == 64) run(ct, std::integral_constant<int, 64>{});
+        else run(ct, std::integral_constant<int, 128>{});
+    });
 }
 
 }  // namespace aic::hip

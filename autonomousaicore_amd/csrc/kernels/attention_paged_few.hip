@@ -111,7 +111,7 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
         const int lane = threadIdx.x & 63;
         Steps own{};
         if (lane < f.a.B) own = steps_of(f, sequence(f.a, lane));
-        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * f.a.kv.Hkv : 0.0;
+        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * f.a.heads : 0.0;
         auto sum = [](double p, double q) { return p + q; };
         double size = own.steps * groups, total = wave_all(size, sum);
         const double pairs = wave_all(groups, sum);
@@ -146,7 +146,7 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     auto load = [&](int i) {
         if (per > 1) own = steps_of(f, sequence(f.a, i));
     };
-    auto groups = [&] { return static_cast<double>(own.groups) * f.a.kv.Hkv; };
+    auto groups = [&] { return static_cast<double>(own.groups) * f.a.heads; };
     double mine = 0.0, mine_pairs = 0.0, start, pairs_start, total, pairs;
     for (int i = first; i < last; ++i) {
         load(i);
@@ -190,11 +190,12 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     return true;
 }
 
-template <int HD, bool E4, int NW>
+template <int HD, typename CT, int NW>
 struct FewLds {
+    static constexpr bool E4 = kE4<CT>;
     static constexpr int TILE = 32 * HD * (E4 ? 1 : 2);          // bytes of a tile of K or V
     static constexpr int STAGE = 2 * TILE + (E4 ? 256 : 0);      // and the exponents of 32 keys of K, then of V, a word each
-    static constexpr int WAVE = 2 * STAGE;
+    static constexpr int WAVE = kE2<CT> ? TILE : 2 * STAGE;      // e2m1: one tile of V, as bf16
     static constexpr int BYTES = NW * WAVE > NW * 32 * HD * 4 ? NW * WAVE : NW * 32 * HD * 4;  // also the waves' O at the end
     static constexpr int COPIES = 2 * (TILE / 1024) + (E4 ? 1 : 0);  // of a stage
 };
@@ -246,9 +247,10 @@ struct Frags8 {
 };
 
 // What a thread knows of the tiles: where its copies and fragments lie.
-template <int HD, bool E4>
+template <int HD, typename CT>
 struct FewLane {
-    static constexpr int TILE = FewLds<HD, E4, 1>::TILE;
+    static constexpr bool E4 = kE4<CT>;
+    static constexpr int TILE = FewLds<HD, CT, 1>::TILE;
     static constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
     uint32_t voff[TILE / 1024];
     std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
@@ -262,6 +264,69 @@ struct FewLane {
         F.init(lane);
     }
 };
+
+// e2m1: a tile's codes in registers, two tiles ahead.  K's are fragments as they come: half h of the wave holds half h of each key's
+// columns (the order of the columns is free, as long as Q's is the same); V's are 16-byte units of 32 columns, for LDS.
+template <int HD>
+struct Codes4 {
+    static constexpr int KW = HD / 16;                  // words of a lane's half of a key
+    static constexpr int KE = HD / 64 > 0 ? HD / 64 : 1;  // its exponents
+    static constexpr int UPR = HD / kGroup, NV = HD / 64 > 0 ? HD / 64 : 1;  // units of a row of V, of a lane (head_dim 32: of half the lanes)
+    uint32_t k[KW], ke[KE], ve[NV];
+    uint4 v[NV];
+    // rows: of the lane's key and of its units, in the pools; negative: without a page
+    __device__ __forceinline__ void load(const PageView& kv, int64_t key, const int64_t (&row)[NV], int lane) {
+        const int h = lane >> 5;
+        const char* none = reinterpret_cast<const char*>(&kNoPage);
+        const char* kp = key >= 0 ? kv.kp + key * (HD / 2) + h * (HD / 4) : none;
+        if constexpr (KW == 8) {
+            const uint4 x = reinterpret_cast<const uint4*>(kp)[0], y = *reinterpret_cast<const uint4*>(key >= 0 ? kp + 16 : none);
+            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w, k[4] = y.x, k[5] = y.y, k[6] = y.z, k[7] = y.w;
+            const uint32_t e = key >= 0 ? reinterpret_cast<const uint16_t*>(kv.ke)[key * 2 + h] : 0xffffu;
+            ke[0] = e & 255u, ke[1] = e >> 8;
+        } else if constexpr (KW == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(kp);
+            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+            ke[0] = key >= 0 ? kv.ke[key * 2 + h] : kNanGroup;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(kp);
+            k[0] = x.x, k[1] = x.y;
+            ke[0] = key >= 0 ? kv.ke[key] : kNanGroup;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t at = row[i] * UPR + (i * 64 + lane) % UPR;
+            v[i] = *reinterpret_cast<const uint4*>(row[i] >= 0 ? kv.vp + at * 16 : none);
+            ve[i] = row[i] >= 0 ? kv.ve[at] : kNanGroup;
+        }
+    }
+    __device__ static __forceinline__ int v_row(int i, int lane) { return min((i * 64 + lane) / UPR, 31); }
+    // V to LDS as bf16, for the products' transposed reads.
+    __device__ __forceinline__ void put_v(char* tile, int lane) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (HD < 64 && lane >= 32) break;
+            const int u = i * 64 + lane, rr = u / UPR, ch = u % UPR * 4;
+            const float s = exp_scale(ve[i]);
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            const uint32_t nan = ve[i] == kNanGroup ? 0x7fff7fffu : 0u;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint4 x = e2m1_bf16(w[c], s);
+                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + c)) = make_uint4(x.x | nan, x.y | nan, x.z | nan, x.w | nan);
+            }
+        }
+    }
+    // Eight columns of the lane's key.
+    __device__ __forceinline__ bf16x8 k_frag(int kk) const {
+        const uint32_t e = ke[kk * KE / KW];
+        const uint4 x = e2m1_bf16(k[kk], exp_scale(e));
+        const uint32_t nan = e == kNanGroup ? 0x7fff7fffu : 0u;
+        return __builtin_bit_cast(bf16x8, make_uint4(x.x | nan, x.y | nan, x.z | nan, x.w | nan));
+    }
+};
+// What lanes have stored to LDS, for other lanes of the wave: LDS works in order, so this is for the compiler alone.
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
 // A group's keys, or a block's share of them; one for the whole block.
 struct Part {
     Seq sq;
@@ -272,12 +337,13 @@ struct Part {
 };
 
 // The work on one part: true where a sum of this thread's has left fp32's range.
-template <int HD, bool E4, int NW>
-__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, E4>& me, float down) {
-    using L = FewLds<HD, E4, NW>;
+template <int HD, typename CT, int NW>
+__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, CT>& me, float down) {
+    using L = FewLds<HD, CT, NW>;
     const PagedArgs& a = f.a;
+    constexpr bool E4 = kE4<CT>, E2 = kE2<CT>;
     constexpr int KS = HD / 16, OB = HD / 32;
-    constexpr int RB = FewLane<HD, E4>::RB, NC = FewLane<HD, E4>::NC, RPS = FewLane<HD, E4>::RPS;
+    constexpr int RB = FewLane<HD, CT>::RB, NC = FewLane<HD, CT>::NC, RPS = FewLane<HD, CT>::RPS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int ids[kIds];
     __shared__ float2 mls[NW][32];
@@ -309,16 +375,16 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
         const bf16* qp = static_cast<const bf16*>(a.q) + (sq.row0 + tok) * a.ldq + static_cast<int64_t>(head) * HD;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
-            const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : 16 * kk + 8 * hl;
+            const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : E2 ? HD / 2 * hl + 8 * kk : 16 * kk + 8 * hl;
             if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + col, real));
             else
 #pragma unroll
                 for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[col + j] : f2bf(0.0f);
         }
 
-        // one tile's products, from the stage it arrived in
-        auto compute = [&](char* kt, int k0) {
-            const char* vt = kt + L::TILE;
+        // one tile's products, from the stage it arrived in; e2m1: from V's tile, and the registers c, which `loaded` then fills anew
+        auto compute = [&](char* kt, int k0, [[maybe_unused]] const Codes4<HD>* c, auto loaded) {
+            const char* vt = kt + (E2 ? 0 : L::TILE);
             [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
             f32x16 sc[1];
             zero(sc[0]);
@@ -345,11 +411,15 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
                     sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.z, x.w), sk)),
                                                                     qb[2 * j + 1], sc[0], 0, 0, 0);
                 }
+            } else if constexpr (E2) {
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c->k_frag(kk), qb[kk], sc[0], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
                     sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(me.F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
             }
+            loaded();
             // every row sees every key of the tile?
             const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
             auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
@@ -427,6 +497,44 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
                 const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * ps + (key - pi * ps);
                 return page < 0 ? -1 : row;
             };
+            if constexpr (E2) {
+                // page ids of the halves of a tile, or of each row
+                auto load = [&](int t, Codes4<HD>& c) {
+                    const int k0 = first + 32 * NW * t;
+                    int64_t key, row[Codes4<HD>::NV];
+                    if (paged && k0 + 32 <= w1) {
+                        const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
+                        const int page0 = __builtin_amdgcn_readfirstlane(ids[pi - p0]), page1 = __builtin_amdgcn_readfirstlane(ids[pj - p0]);
+                        const int64_t row0 = (static_cast<int64_t>(page0) * Hkv + kvh) * ps + (k0 - pi * ps);
+                        const int64_t row1 = (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps);
+                        auto at = [&](int r) { return (r & 16 ? page1 : page0) < 0 ? -1 : (r & 16 ? row1 : row0) + (r & 15); };
+                        key = at(lane & 31);
+#pragma unroll
+                        for (int i = 0; i < Codes4<HD>::NV; ++i) row[i] = at(Codes4<HD>::v_row(i, lane));
+                    } else {
+                        key = row_at(k0 + (lane & 31));
+#pragma unroll
+                        for (int i = 0; i < Codes4<HD>::NV; ++i) row[i] = row_at(k0 + Codes4<HD>::v_row(i, lane));
+                    }
+                    c.load(a.kv, key, row, lane);
+                };
+                Codes4<HD> even, odd;
+                if (nt > 0) load(0, even);
+                if (nt > 1) load(1, odd);
+                auto step = [&](int t, Codes4<HD>& c) {
+                    c.put_v(mine, lane);
+                    wave_lds_fence();
+                    compute(mine, first + 32 * NW * t, &c, [&] {
+                        if (t + 2 < nt) load(t + 2, c);
+                    });
+                    wave_lds_fence();
+                };
+                for (int t = 0; t < nt; t += 2) {
+                    step(t, even);
+                    if (t + 1 < nt) step(t + 1, odd);
+                }
+                continue;
+            }
             auto issue = [&](int t) {
                 char* dst = mine + (t & 1) * L::STAGE;
                 const int k0 = first + 32 * NW * t;
@@ -469,7 +577,7 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
             for (int t = 0; t < nt; ++t) {
                 if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
                 else wait_vmcnt<0>();
-                compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t);
+                compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t, nullptr, [] {});
                 wait_lds();  // the tile has been read
                 if (t + 2 < nt) issue(t + 2);
             }
@@ -539,12 +647,12 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
 
 // NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
 // else is divided and a block is alone on its CU.
-template <int HD, bool E4, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+template <int HD, typename CT, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && sizeof(CT) > 1) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
     const PagedArgs& a = f.a;
     __shared__ int past;
-    const int Hkv = a.kv.Hkv;
-    FewLane<HD, E4> me;
+    const int Hkv = a.heads;
+    FewLane<HD, CT> me;
     me.init(threadIdx.x & 63);
     if (threadIdx.x == 0) past = 0;
 
@@ -574,7 +682,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
                                     : __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(before) / static_cast<uint32_t>(x.steps)));
         const int u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
         const int u1 = static_cast<int>(min(static_cast<int64_t>(x.steps), u0 + min(count, int64_t{1} << 30)));
-        const int kvh = f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv, r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
+        const int kvh = kv_head(a, b, f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv), r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
         const Part pt{sq, b, kvh, r0, x.lo + u0 * kStep, u1 < x.steps ? x.lo + u1 * kStep : INT32_MAX,
                       2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1), u0 == 0 && u1 == x.steps};
         first_part = false;
@@ -583,7 +691,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
 
         bool again = false;
         do {
-            const bool over = few_part<HD, E4, NW>(f, pt, me, again ? kDown : 0.0f);
+            const bool over = few_part<HD, CT, NW>(f, pt, me, again ? kDown : 0.0f);
             if (over && !again) past = 1;
             lds_barrier();  // also: before the next part's tiles
             again = !again && past;
@@ -599,7 +707,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
     const PagedArgs& a = f.a;
-    const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv;
+    const int Hkv = a.heads, grid_head = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv, kvh = kv_head(a, b, grid_head);
     const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
     if (qr >= f.group) return;
     const int64_t planned = f.plan[a.B], share = planned < 0 ? -planned : planned, base_step = f.plan[b];
@@ -609,7 +717,7 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
         const int r = g * f.group + qr;
         if (r >= x.sq.n * a.G) return;
         // the group's first block and its parts; a block's second slot holds a group that begins behind its own begin
-        const int64_t group = static_cast<int64_t>(g) * Hkv + kvh;
+        const int64_t group = static_cast<int64_t>(g) * Hkv + grid_head;
         int64_t s0;
         int parts, first_slot = 0;
         if (by_group) {
@@ -679,35 +787,35 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
 }
 
 // Blocks that are resident at once on 256 CUs: LDS holds one of bf16 at head_dim 128, two of the others.
-int64_t resident(int64_t head_dim, bool e4m3) { return head_dim == 128 && !e4m3 ? 256 : 512; }
+int64_t resident(int64_t head_dim, DType type) { return head_dim == 128 && !holds_codes(type) ? 256 : 512; }
 
-template <int HD, bool E4, int NW>
+template <int HD, typename CT, int NW>
 void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
-    constexpr int bytes = FewLds<HD, E4, NW>::BYTES;
+    constexpr int bytes = FewLds<HD, CT, NW>::BYTES;
     static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     AIC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
-        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4, NW>),
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, CT, NW>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) allowed[dev].store(true);
     }
-    attn_paged_few_k<HD, E4, NW><<<static_cast<unsigned>(blocks), NW * 64, bytes, s>>>(f);
+    attn_paged_few_k<HD, CT, NW><<<static_cast<unsigned>(blocks), NW * 64, bytes, s>>>(f);
     AIC_LAUNCH_CHECK("attn_paged");
 }
 
-template <int HD, bool E4>
+template <int HD, typename CT>
 void launch(const FewArgs& f, hipStream_t s) {
-    const int64_t pairs = static_cast<int64_t>(f.a.kv.Hkv) * f.a.B;
+    const int64_t pairs = static_cast<int64_t>(f.a.heads) * f.a.B;
     AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
     if (f.shares == 0) {
         // eight waves' stages are beyond the LDS for bf16 at head_dim 128; with more blocks than CUs four waves keep two of them there
-        if constexpr (HD < 128 || E4) {
-            if (pairs <= 256) return launch<HD, E4, 8>(f, pairs, s);
+        if constexpr (HD < 128 || sizeof(CT) == 1) {
+            if (pairs <= 256) return launch<HD, CT, 8>(f, pairs, s);
         }
-        return launch<HD, E4, 4>(f, pairs, s);
+        return launch<HD, CT, 4>(f, pairs, s);
     }
-    launch<HD, E4, 4>(f, f.shares, s);
+    launch<HD, CT, 4>(f, f.shares, s);
     attn_paged_few_join_k<HD><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>((f.group + 3) / 4)), 256, 0, s>>>(f);
     AIC_LAUNCH_CHECK("attn_paged join");
 }
@@ -725,24 +833,27 @@ int64_t whole_len(int64_t pairs, int64_t head_dim) { return pairs >= 192 ? 2048 
 // One group; or two where the cache is e4m3 and head_dim 128, whose tiles of 128 rows go through registers: 30 sequences of
 // up to 8000 tokens, 16 heads over 2, 64 rows: 41.6 us so, 66.6 us there; one sequence: 22.5 and 26.7 us; 96 rows on
 // up to 4000: 41.1 and 39.1 us.  bf16, 64 rows: 61.6 and 55.5 us; head_dim 64 25.0 and 22.7 us in e4m3.
-bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, bool e4m3) { return max_q * G <= (e4m3 && head_dim == 128 ? 64 : 32); }
+bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, DType type) { return max_q * G <= (holds_codes(type) && head_dim == 128 ? 64 : 32); }
 
-int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, bool e4m3) {
+int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type) {
     if (max_len <= whole_len(B * Hkv, head_dim)) return 0;
-    return (2 * resident(head_dim, e4m3) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
+    return (2 * resident(head_dim, type) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
 }
 
-void attn_paged_few(const PagedArgs& a, int64_t max_q, bool e4m3, int head_dim, void* workspace, hipStream_t s) {
+void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s) {
     FewArgs f{a, static_cast<int>(group_of(max_q, a.G)), 0, nullptr, nullptr, nullptr};
     if (workspace) {
-        f.shares = static_cast<int>(resident(head_dim, e4m3));
+        f.shares = static_cast<int>(resident(head_dim, type));
         f.part_o = static_cast<float*>(workspace);
         f.part_ml = reinterpret_cast<float2*>(f.part_o + 2LL * f.shares * f.group * head_dim);
         f.plan = reinterpret_cast<int64_t*>(f.part_ml + 2LL * f.shares * f.group);
     }
-    if (head_dim == 32) e4m3 ? launch<32, true>(f, s) : launch<32, false>(f, s);
-    else if (head_dim == 64) e4m3 ? launch<64, true>(f, s) : launch<64, false>(f, s);
-    else e4m3 ? launch<128, true>(f, s) : launch<128, false>(f, s);
+    by_cache_type<bf16>(type, [&](auto ct) {
+        using CT = decltype(ct);
+        if (head_dim == 32) launch<32, CT>(f, s);
+        else if (head_dim == 64) launch<64, CT>(f, s);
+        else launch<128, CT>(f, s);
+    });
 }
 
 }  // namespace aic::hip

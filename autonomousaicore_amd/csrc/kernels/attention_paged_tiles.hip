@@ -30,8 +30,8 @@ namespace {
 
 constexpr int kIds = 512;  // page ids in LDS at a time
 
-// What a pass has found.  kTop: a row whose codes can be past the range (e4m3_in_range): looked for in the first pass only, and kept
-// in the range by the other one, for a branch between the products costs 4% at head_dim 128.
+// What a pass has found.  kTop: a row whose codes can be past the range (e4m3_in_range), or a group that is NaN (e2m1): looked for
+// in the first pass only, and minded by the other one, for a branch between the products costs 4% at head_dim 128.
 constexpr int kPast = 1, kTop = 2;
 
 template <int HD>
@@ -41,19 +41,20 @@ struct TilesLds {
     int past, top;
 };
 
-template <int HD, bool E4, bool SECOND>
+template <int HD, typename CT, bool SECOND>
 __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a, int tid, int block, float down) {
     constexpr int KS = HD / 16, OB = HD / 32, TILE = 64 * HD;  // elements of a tile
     constexpr int NA = 2 * KS, NB = 4 * OB;                   // MFMAs of groups A and B
     constexpr int EA = 32 / NA, EB = 32 / NB;                 // elements per slot
     constexpr int NR = OB + 1, KR = 3;                        // fragment rings
     constexpr int RB = HD * 2, NC = RB / 16, RPS = 1024 / RB, PW = 16 / RPS;  // bf16 copies: of a wave's 16 rows
-    constexpr int UPR = HD / 16, UNITS = 64 * UPR, NU = (UNITS + 255) / 256;  // e4m3: 16-byte units of a tile
+    constexpr bool E4 = kE4<CT> || kE2<CT>;                   // codes
+    constexpr int UPR = E4 ? HD / kPer16<CT> : 1, UNITS = 64 * UPR, NU = (UNITS + 255) / 256;  // 16-byte units of a tile of codes
     auto& sm = lds.sm;
     auto& ids = lds.ids;
 
     const int Hkv = a.kv.Hkv, ps = a.kv.ps;
-    const int kvh = block % Hkv, rest = block / Hkv;
+    const int kvh = block % Hkv, rest = block / Hkv;  // (picked pages are the few rows' kernel's)
     const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (Hkv * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
     if (!find_tile<128>(a, tile, b, local)) return 0;
@@ -138,7 +139,7 @@ __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a,
                     dma16(row >= 0 ? pool + row * RB + (((l % NC) ^ swz<HD>(rr)) << 4) : none, dst + i * 512);
                 }
             };
-            // e4m3: units of tile t of a pool in registers, and into dst
+            // codes: units of tile t of a pool in registers, and into dst
             struct Codes {
                 uint4 w[NU];
                 uint32_t e[NU];
@@ -148,14 +149,28 @@ __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a,
                 for (int i = 0; i < NU; ++i) {
                     const int u = i * 256 + tid;
                     const int64_t row = row_at(w0 + 64 * t + min(u / UPR, 63));
-                    c.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * HD + (u % UPR) * 16 : none);
-                    c.e[i] = row >= 0 ? exps[row] : 127;
+                    c.w[i] = *reinterpret_cast<const uint4*>(row >= 0 ? pool + row * kRowBytes<CT, HD> + (u % UPR) * 16 : none);
+                    if constexpr (kE2<CT>) c.e[i] = row >= 0 ? exps[row * UPR + u % UPR] : kNanGroup;
+                    else c.e[i] = row >= 0 ? exps[row] : 127;
                 }
             };
             auto put_unit = [&](const Codes& c, int i, bf16* dst) {
                 const int u = i * 256 + tid;
                 if (UNITS % 256 != 0 && u >= UNITS) return;
                 uint4 w = c.w[i];
+                if constexpr (kE2<CT>) {
+                    const float s = exp_scale(c.e[i]);
+                    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+                    const uint32_t nan = SECOND && c.e[i] == kNanGroup ? 0x7fff7fffu : 0u;
+                    if constexpr (!SECOND) top |= __ballot(c.e[i] == kNanGroup);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 x = e2m1_bf16(q[j], s);
+                        *reinterpret_cast<uint4*>(reinterpret_cast<char*>(dst) + chunk_at<bf16, HD>(u / UPR, 4 * (u % UPR) + j)) =
+                            make_uint4(x.x | nan, x.y | nan, x.z | nan, x.w | nan);
+                    }
+                    return;
+                }
                 if constexpr (SECOND) {
                     if (c.e[i] >= kTopByte) w = e4m3_in_range(w, c.e[i]);
                 } else {
@@ -249,7 +264,7 @@ __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a,
             __builtin_amdgcn_s_barrier();  // the stages are free
 
             // The pipelined loop over tiles t_a .. t_b - 1; stage of unit t: (t - t_a + 1) & 1
-            // unit t on its way (bf16: into stage st; e4m3: to registers, into the stage by iteration t - 1)
+            // unit t on its way (bf16: into stage st; codes: to registers, into the stage by iteration t - 1)
             auto begin = [&](int t, [[maybe_unused]] int st) {
                 if constexpr (E4) {
                     if (t + 1 < t_b) fetch(a.kv.kp, a.kv.ke, t + 1, ck);
@@ -380,14 +395,15 @@ __device__ __forceinline__ int tiles_pass(TilesLds<HD>& lds, const PagedArgs& a,
     return past | (top ? kTop : 0);
 }
 
-template <int HD, bool E4>
+template <int HD, typename CT>
 __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
+    constexpr bool E4 = kE4<CT> || kE2<CT>;
     // as one_or_two_passes; where a row of the largest powers was found, the second pass is anew from the start, and there
     // may be a third
     __shared__ TilesLds<HD> lds;
     const int tid = threadIdx.x;
     if (tid == 0) lds.past = 0, lds.top = 0;
-    const int found = tiles_pass<HD, E4, false>(lds, a, tid, static_cast<int>(blockIdx.x), 0.0f);
+    const int found = tiles_pass<HD, CT, false>(lds, a, tid, static_cast<int>(blockIdx.x), 0.0f);
     if (found & kPast) lds.past = 1;
     if (E4 && found & kTop) lds.top = 1;
     lds_barrier();
@@ -396,7 +412,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
         for (float down = E4 && lds.top ? 0.0f : kDown;; down = kDown) {
             lds_barrier();
             if (threadIdx.x == 0) lds.past = 0;
-            const int again = tiles_pass<HD, E4, true>(lds, fresh_argument<PagedArgs>(), fresh(tid), fresh_uniform(static_cast<int>(blockIdx.x)), down);
+            const int again = tiles_pass<HD, CT, true>(lds, fresh_argument<PagedArgs>(), fresh(tid), fresh_uniform(static_cast<int>(blockIdx.x)), down);
             lds_barrier();  // (a tile without keys has none)
             if (again & kPast) lds.past = 1;
             lds_barrier();
@@ -405,18 +421,21 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tiles_k(PagedArgs a) {
     }
 }
 
-template <int HD, bool E4>
+template <int HD, typename CT>
 void launch(const PagedArgs& a, unsigned blocks, hipStream_t s) {
-    attn_paged_tiles_k<HD, E4><<<blocks, 256, 0, s>>>(a);
+    attn_paged_tiles_k<HD, CT><<<blocks, 256, 0, s>>>(a);
     AIC_LAUNCH_CHECK("attn_paged");
 }
 
 }  // namespace
 
-void attn_paged_tiles(const PagedArgs& a, bool e4m3, int head_dim, unsigned blocks, hipStream_t s) {
-    if (head_dim == 32) e4m3 ? launch<32, true>(a, blocks, s) : launch<32, false>(a, blocks, s);
-    else if (head_dim == 64) e4m3 ? launch<64, true>(a, blocks, s) : launch<64, false>(a, blocks, s);
-    else e4m3 ? launch<128, true>(a, blocks, s) : launch<128, false>(a, blocks, s);
+void attn_paged_tiles(const PagedArgs& a, DType type, int head_dim, unsigned blocks, hipStream_t s) {
+    by_cache_type<bf16>(type, [&](auto ct) {
+        using CT = decltype(ct);
+        if (head_dim == 32) launch<32, CT>(a, blocks, s);
+        else if (head_dim == 64) launch<64, CT>(a, blocks, s);
+        else launch<128, CT>(a, blocks, s);
+    });
 }
 
 }  // namespace aic::hip

@@ -162,8 +162,8 @@ void kv_append(const void* qkv, void* kc, void* vc, int64_t B, int64_t S, int64_
                int64_t start_pos, DType dt, hipStream_t s);
 
 // The paged key/value cache (paged_kv.hip): pools [n_pages][kv_heads][page_size][head_dim] of type
-// (UInt8: e4m3 codes with an exponent byte per [n_pages][kv_heads][page_size]) and the sequences' page
-// ids.  Sequence b's rows offsets[b] .. offsets[b + 1] are the last of its lens[b] cached tokens.
+// (UInt8: e4m3 codes with an exponent byte per [n_pages][kv_heads][page_size]; UInt4: e2m1 codes, two a byte, with an
+// exponent byte per 32 of a row's head_dim) and the sequences' page ids.  Sequence b's rows offsets[b] .. offsets[b + 1] are the last of its lens[b] cached tokens.
 struct KVPages {
     void *k_pages = nullptr, *v_pages = nullptr;
     uint8_t *k_exps = nullptr, *v_exps = nullptr;
@@ -175,6 +175,22 @@ void kv_write(const KVPages& c, const void* k, const void* v, int64_t ld, const 
               int64_t B, int64_t T, DType dt, hipStream_t s);
 void kv_read(const KVPages& c, void* k, void* v, int64_t ld, const int64_t* offsets, const int64_t* lens, int64_t B,
              int64_t T, DType dt, hipStream_t s);
+// kv_write of k and v with q (to q_out) and k turned to their positions on the way.
+void kv_append_rope(const KVPages& c, const void* q, int64_t ld_q, void* q_out, int64_t ld_qo, int64_t H, const void* k, const void* v,
+                    int64_t ld_kv, const float* cos_t, const float* sin_t, int64_t n_pos, const int64_t* offsets, const int64_t* lens,
+                    int64_t B, int64_t T, DType dt, hipStream_t s);
+// Pages chosen for each row by bounds of their keys (paged_select.hip): bounds [n_pages][kv_heads][2][head_dim] (fp32 for an
+// fp32 cache, else bf16); picked [T][kv_heads][n_sel] page ids, picked_lens [T][kv_heads].
+void kv_bounds(const KVPages& c, void* bounds, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, hipStream_t s);
+int64_t kv_select_workspace(const KVPages& c, int64_t T, int64_t max_len);
+void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q, const int64_t* offsets, const int64_t* lens, int64_t B,
+               int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t first, int64_t last, int64_t n_sel, int32_t* picked,
+               int64_t* picked_lens, void* workspace, int64_t workspace_bytes, DType dt, hipStream_t s);
+// Attention of each row over its picked pages (attention_paged.hip).
+int64_t attn_paged_selected_workspace(const KVPages& c, int64_t T, int64_t n_sel, int64_t H);
+void attn_paged_selected(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse, const int32_t* picked,
+                         const int64_t* picked_lens, int64_t T, int64_t n_sel, int64_t H, float scale, void* workspace,
+                         int64_t workspace_bytes, DType dt, hipStream_t s);
 // Attention over it (attention_paged.hip).  workspace null: the stream's scratch, or no split of the
 // keys where the call is captured.
 int64_t attn_paged_workspace(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H);

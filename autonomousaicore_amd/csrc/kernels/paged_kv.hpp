@@ -1,6 +1,8 @@
 // The paged key/value cache as its kernels see it (paged_kv.hip, attention_paged.hip).
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -12,6 +14,23 @@ namespace aic::hip {
 // codes have (e4m3 is a floating format: moving a row by up to one binade leaves its relative steps),
 // make the values exact in bf16 (from 2^-124 on, where the codes' last digit meets bf16's), and go through the hardware's
 // scaled conversion for free.
+//
+// 4-bit pools hold e2m1 codes, two a byte (the first element in the low bits), and a power of two per 32 neighbouring elements of a
+// row's head: 32 codes are 16 bytes.  e2m1 has one mantissa bit and a range of 12, so a power for a whole head would leave most of
+// a head with a few loud elements at zero; a power per 32 costs 6% of the codes' bytes.  Code times power is exact in bf16,
+// and e2m1 has no NaN: byte kNanGroup marks 32 elements of which one was an infinity or NaN.
+struct e2m1x2 {
+    uint8_t codes;
+};
+template <typename CT> constexpr bool kE4 = std::is_same_v<CT, uint8_t>;
+template <typename CT> constexpr bool kE2 = std::is_same_v<CT, e2m1x2>;
+constexpr int kGroup = 32;
+constexpr uint32_t kNanGroup = 255;
+// Elements in 16 bytes of a pool; bytes and exponents of a head's row.
+template <typename CT> constexpr int kPer16 = kE2<CT> ? 32 : 16 / static_cast<int>(sizeof(CT));
+template <typename CT, int HD> constexpr int kRowBytes = HD * 16 / kPer16<CT>;
+template <typename CT, int HD> constexpr int kRowExps = kE2<CT> ? HD / kGroup : 1;
+
 struct PageView {
     char *kp, *vp;
     uint8_t *ke, *ve;
@@ -34,6 +53,7 @@ struct PageView {
     }
 };
 
+inline bool holds_codes(DType t) { return t == DType::UInt8 || t == DType::UInt4; }
 // Type, heads and head_dim checked: what sizes are made of.  `what` names the entry in the messages.
 void check_cache_shape(const KVPages& c, const char* what);
 // All arguments checked, and the view made of them.
@@ -86,6 +106,40 @@ __device__ __forceinline__ uint4 e4m3_in_range(uint4 w, uint32_t byte) {
 // 2^(b - 127) of a stored exponent byte (1 .. 254; 0 and 255 cannot be written and read as 2^-126, 2^127).
 __device__ __forceinline__ float exp_scale(uint32_t b) {
     return __uint_as_float(min(max(b, 1u), 254u) << 23);
+}
+
+// The eight e2m1 codes of w times the power of two s, as floats and as bf16, both exact: element j in bits 4 j.
+__device__ __forceinline__ void e2m1_floats(uint32_t w, float s, float (&v)[8]) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
+    const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
+}
+__device__ __forceinline__ uint4 e2m1_bf16(uint32_t w, float s) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3)));
+}
+// The power of 32 elements whose largest |x| has these bits: the least 2^e with 6 2^e >= it, -126 <= e <= 125 (6 2^126 is past
+// fp32: what is past 6 2^125 counts as that); 0 for zeros.  6 = 1.5 2^2.  An infinity or NaN: kNanGroup.
+__device__ __forceinline__ uint32_t group_byte(uint32_t amax) {
+    if (amax >= 0x7f800000u) return kNanGroup;
+    const int e = static_cast<int>(amax >> 23) - 129 + ((amax & 0x7fffffu) > 0x400000u ? 1 : 0);
+    return amax == 0 ? 127u : static_cast<uint32_t>(min(max(e, -126), 125) + 127);
+}
+// Eight elements as codes of that power: one rounding, to nearest, ties to the even code.
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], uint32_t byte) {
+    if (byte == kNanGroup) return 0;
+    const float inv = __uint_as_float((254u - byte) << 23);  // byte 1 .. 252: a normal number
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = __builtin_amdgcn_fmed3f(x[j] * inv, -6.0f, 6.0f);
+    uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
 }
 
 }  // namespace aic::hip

@@ -1,5 +1,6 @@
 // Element types.  The numeric values are those of the reference's aic::DType
-// (include/core/dtype.hpp:18-26), which is also what its .aic checkpoints store.
+// (include/core/dtype.hpp:18-26), which is also what its .aic checkpoints store; UInt4 (two codes a byte) is
+// a key/value cache's alone and not the reference's.
 #pragma once
 
 #include <cstddef>
@@ -14,7 +15,8 @@ enum class DType : std::uint8_t {
     Int32 = 3,
     Int64 = 4,
     UInt8 = 5,
-    UInt16 = 6
+    UInt16 = 6,
+    UInt4 = 7
 };
 
 constexpr std::size_t dtype_size(DType d) noexcept {
@@ -26,6 +28,7 @@ constexpr std::size_t dtype_size(DType d) noexcept {
         case DType::Int64: return 8;
         case DType::UInt8: return 1;
         case DType::UInt16: return 2;
+        case DType::UInt4: return 0;  // no whole number of bytes
     }
     return 0;
 }

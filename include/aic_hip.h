@@ -34,7 +34,8 @@ typedef enum {
     AIC_I32 = 3,
     AIC_I64 = 4,
     AIC_U8 = 5,
-    AIC_U16 = 6
+    AIC_U16 = 6,
+    AIC_U4 = 7 /* 4-bit codes, two per byte: paged key/value caches only; not the reference's */
 } aic_dtype;
 
 typedef void* aic_stream; /* hipStream_t */
@@ -259,7 +260,10 @@ int aic_hip_attn_bwd_qk(const void* q, int64_t ld_q, const void* k, const void* 
  * a row's head is code * 2^(byte - 127), byte (1 .. 254) in k_exps / v_exps
  * [n_pages][kv_heads][page_size]; what would be past 240 * 2^120, the largest number that codes and the
  * types share, counts as that number (codes from 256 * 2^120 on, which stand for numbers past 248 * 2^120), so finite
- * numbers stay finite.
+ * numbers stay finite.  AIC_U4: pools [n_pages][kv_heads][page_size][head_dim / 2] of e2m1 codes (the numbers 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives), two a byte with the first element in the low bits; 32 neighbouring elements of a row's head are
+ * code * 2^(byte - 127), byte (1 .. 252; 255: all 32 are NaN) in k_exps / v_exps [n_pages][kv_heads][page_size][head_dim / 32]
+ * (4-byte aligned).
  *
  * The calls below share a ragged batch's description, in device memory: offsets [B + 1] and lens [B]
  * (int64).  Sequence b's packed rows offsets[b] .. offsets[b + 1] - 1 are the last ones of its
@@ -273,7 +277,7 @@ int aic_hip_attn_bwd_qk(const void* q, int64_t ld_q, const void* k, const void* 
 typedef struct {
     void* k_pages;
     void* v_pages;
-    uint8_t* k_exps; /* AIC_U8 only */
+    uint8_t* k_exps; /* AIC_U8 and AIC_U4 only */
     uint8_t* v_exps;
     const int32_t* page_table;
     int64_t ld_table, n_pages, page_size, kv_heads, head_dim;
@@ -282,17 +286,29 @@ typedef struct {
 /* The new rows k, v [T, kv_heads * head_dim] (leading dimension ld, dtype dt F32 or BF16) into their
  * places.  A cache of dt takes them as they are.  An e4m3 cache takes each row's head with the least
  * power of two 2^e >= max|x| / 448 (e >= -126), codes rounded to nearest, ties to even; an
- * infinity or NaN is held as NaN.  Rows without a place are not written.  Two rows of one call must
- * not share a place. */
+ * infinity or NaN is held as NaN.  An e2m1 cache takes 32 elements with the least 2^e >= max|x| / 6 (-126 <= e <= 125; what is past
+ * 6 * 2^125 counts as that), codes rounded alike; an infinity or NaN among them makes all 32 NaN.  Rows without a place are not written.
+ * Two rows of one call must not share a place. */
 int aic_hip_kv_write(const aic_kv_pages* cache, const void* k, const void* v, int64_t ld, const int64_t* offsets,
                      const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
 /* The other way: the cached rows at the batch's positions to k, v [T, kv_heads * head_dim] (e4m3 to
  * bf16 is exact but for bits below 2^-133, bf16's least number); rows without a place are zero. */
 int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, const int64_t* offsets,
                     const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
+/* aic_hip_kv_write with the rotary embedding on the way: q [T, H * head_dim] (leading dimension ld_q) goes to q_out (ld_qo; q
+ * itself with the same leading dimension, or memory that does not overlap; H 0: no q) and k into the cache turned to their rows'
+ * positions, v as it is.  cos_t, sin_t: fp32 [n_pos, head_dim / 2] as aic_hip_rope_tables builds them; with x1, x2 the elements i and
+ * i + head_dim / 2 of a head, y1 = x1 c - x2 s, y2 = x1 s + x2 c in fp32, each product and sum rounded, then one rounding to the
+ * type, or the cache's codes.  Rows without a place in the cache: q is turned, k and v are not written.  Rows at a position before 0
+ * are left as they are; at positions from n_pos on q_out is NaN, and k and v are not written.
+ * Replaces: RotaryPositionEmbedding::forward with its start position (include/nn/rope.hpp:23-112) and the cache's append
+ * (include/nn/attention.hpp:49-120), which know one position for all sequences. */
+int aic_hip_kv_append(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* q_out, int64_t ld_qo, int64_t H, const void* k,
+                      const void* v, int64_t ld_kv, const float* cos_t, const float* sin_t, int64_t n_pos, const int64_t* offsets,
+                      const int64_t* lens, int64_t B, int64_t T, aic_dtype dt, aic_stream stream);
 /* Attention of the batch's rows over the cache, for chunks of a prompt, drafted tokens and single tokens
  * alike.  q and o are [T, H * head_dim] (leading dimensions ld_q, ld_o; dtype dt: the cache's, or
- * either with an e4m3 cache; they must not overlap); query head h reads key/value head h / (H / kv_heads).  The row at
+ * either with a cache of codes; they must not overlap); query head h reads key/value head h / (H / kv_heads).  The row at
  * position pos sees the cached positions j <= pos, with window > 0 only those above pos - window:
  *   o = sum_j softmax_j(scale q . k_j) v_j,   lse[t * H + h] = log sum_j exp(scale q . k_j)
  * (lse fp32, nullable).  A row that sees nothing (position before 0) has o = 0 and lse = -infinity.  A
@@ -313,6 +329,38 @@ int aic_hip_attn_paged(const aic_kv_pages* cache, const void* q, int64_t ld_q, v
                        const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, int64_t max_q,
                        int64_t max_len, int64_t H, int64_t window, float scale, void* workspace,
                        int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
+/* Attention over chosen pages of long caches, in three calls.
+ *
+ * Bounds: bounds [n_pages][kv_heads][2][head_dim] (16-byte aligned; fp32 for an fp32 cache, otherwise bf16, which holds every cached value) gets,
+ * for every page that the batch's rows stand in, the least and the greatest of each element over the page's keys
+ * at positions below lens[b]; NaN where one of them is.  Other pages' bounds stay as they are: call it after each
+ * aic_hip_kv_write or aic_hip_kv_append of a batch, with the same offsets and lens.  Rows of two sequences must not stand in
+ * one page (full pages may be shared).  Pages without a place are left out. */
+int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T,
+                      aic_stream stream);
+/* The choice: a row at position pos has P = pos / page_size + 1 pages and takes, for each key/value head, all of them if they are at
+ * most n_sel, and otherwise the first `first` and the last `last` (at least 1: its own) ones and the n_sel - first - last others of the
+ * greatest
+ *   score = max over the head's query heads of sum_d max(q_d lo_d, q_d hi_d)
+ * which no q . k of the page's keys exceeds; sums in 64 bits, a NaN counts as infinity, ties go to the lower position.
+ * q as in aic_hip_attn_paged.  picked [T][kv_heads][n_sel]: the pages' ids in order of position, then -1;
+ * picked_lens [T][kv_heads]: the positions in them that the row sees, all but the last page whole.  A row of no sequence:
+ * ids -1, length -1; at a position before 0: length 0; past max_len: id -1, length 1.  A page id outside [0, n_pages) is chosen as it is.
+ * max_q: for the choice of forms.  max_len: the longest lens[b].  workspace: as aic_hip_attn_paged,
+ * aic_hip_kv_select_workspace(cache, T, max_len) bytes; a captured call must bring one (InvalidState). */
+int64_t aic_hip_kv_select_workspace(const aic_kv_pages* cache, int64_t T, int64_t max_len); /* negative: -(error code) */
+int aic_hip_kv_select(const aic_kv_pages* cache, const void* bounds, const void* q, int64_t ld_q, const int64_t* offsets,
+                      const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t first, int64_t last,
+                      int64_t n_sel, int32_t* picked, int64_t* picked_lens, void* workspace, int64_t workspace_bytes, aic_dtype dt,
+                      aic_stream stream);
+/* The attention: as aic_hip_attn_paged without a window, where row t's query heads of key/value head h see the first picked_lens[t][h]
+ * positions of the pages picked[t][h][0 ..] (from aic_hip_kv_select, or the caller's own choice; the cache's page_table is not
+ * used).  Length 0: o = 0 and lse = -infinity; a negative length: the row's heads are left as they are; lengths past n_sel * page_size
+ * read positions without a place.  workspace: as aic_hip_attn_paged, aic_hip_attn_paged_selected_workspace(...) bytes. */
+int64_t aic_hip_attn_paged_selected_workspace(const aic_kv_pages* cache, int64_t T, int64_t n_sel, int64_t H); /* negative: -(error code) */
+int aic_hip_attn_paged_selected(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* o, int64_t ld_o, float* lse,
+                                const int32_t* picked, const int64_t* picked_lens, int64_t T, int64_t n_sel, int64_t H, float scale,
+                                void* workspace, int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
 /* Speculative sampling's verification.  Sequence b's rows are its newest token and the drafted ones
  * behind it, ids [T] (int64); logits [T, V] (dtype dt F32 or BF16, leading dimension ld) are the target's
  * after each of them, draft_logits (nullable, the same layout with T rows, ld_draft; a sequence's last row is
