@@ -46,6 +46,7 @@ def _obj(src: str) -> str:
 FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_general.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+              "attention_paged_e2m1.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_paged_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "attention_paged_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 

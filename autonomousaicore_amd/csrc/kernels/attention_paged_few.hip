@@ -32,170 +32,17 @@
 #include <atomic>
 #include <type_traits>
 
-#include "attention_paged.hpp"
+#include "attention_paged_shares.hpp"
 
 namespace aic::hip {
 
 namespace {
 
-constexpr int kIds = 512;    // page ids in LDS at a time
-constexpr int kStep = 128;   // keys: a tile for each wave
-constexpr int kLeast = 4;    // steps of a share at least: a part costs a block about as much as three steps
-struct FewArgs {
-    PagedArgs a;
-    int group;         // query rows of a group, at most 32
-    int shares;        // 0: a block per sequence and key/value head, nothing divided
-    int64_t* plan;     // [B + 1], as find_share leaves it
-    float2* part_ml;   // [2 shares][group]: a share's first group's, then its last one's
-    float* part_o;     // [2 shares][group][hd]
-};
-// A sequence's place in the list of steps.
-struct Steps {
-    Seq sq;
-    int lo, steps, groups;  // first key (a multiple of kStep), steps over its keys, row groups
-};
-__device__ __forceinline__ Steps steps_of(const FewArgs& f, const Seq& sq) {
-    Steps x;
-    x.sq = sq;
-    const int first = max(x.sq.len - x.sq.n, 0);
-    x.lo = f.a.window > 0 ? max(0, first - f.a.window + 1) & ~(kStep - 1) : 0;
-    x.steps = max(1, (x.sq.len - x.lo + kStep - 1) / kStep);  // also of a sequence without keys: its rows are zeros
-    x.groups = (x.sq.n * f.a.G + f.group - 1) / f.group;
-    return x;
-}
-// Parts of a group of `steps` steps that is cut by itself.
-__device__ __forceinline__ int parts_of(int steps, int64_t share) {
-    return share >= steps ? 1 : (steps + static_cast<int>(share) - 1) / static_cast<int>(share);
-}
-// Whole numbers below 2^53, added over the block's threads: what comes before each, and all of them.
-__device__ __forceinline__ void block_scan(double mine, double (&sums)[4], double& before, double& total) {
-    const int wave = threadIdx.x >> 6;
-    const double upto = wave_running_sum(mine);
-    if ((threadIdx.x & 63) == 63) sums[wave] = upto;
-    __syncthreads();
-    before = upto - mine;
-    total = 0.0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        before += w < wave ? sums[w] : 0.0;
-        total += sums[w];
-    }
-}
-// The part of block g: its sequence, the steps before it there and its own.  False: nothing is left for it.
-// plan: for each sequence the steps (or, where groups are cut by themselves, the blocks) before it; behind
-// them a share's steps, negative in the second case.
-__device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Steps& x, int64_t& before, int64_t& count) {
-    __shared__ double sums[2][4], pair_sums[4];
-    __shared__ int at_b;
-    __shared__ Steps at_x;
-    __shared__ int64_t at_before;
-    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    // what is left once the sequence is known
-    auto within = [&](bool by_group, int64_t share, int64_t in, double begin, double total) {
-        if (by_group) {
-            const int part = same(static_cast<int>(in)), n = parts_of(x.steps, share);
-            const int gi = same(part / n), i = part - gi * n;
-            // floor(steps i / n), in 32 bits also for 2^24 steps in 512 parts
-            const uint32_t steps = static_cast<uint32_t>(x.steps), parts = static_cast<uint32_t>(n), each = steps / parts, rest = steps % parts;
-            auto upto = [&](uint32_t k) { return same(static_cast<int>(each * k + rest * k / parts)); };
-            const int u0 = upto(static_cast<uint32_t>(i)), u1 = upto(static_cast<uint32_t>(i) + 1);
-            before = static_cast<int64_t>(gi) * x.steps + u0;
-            count = u1 - u0;
-        } else {
-            before = in;
-            count = min(share, static_cast<int64_t>(total - begin));
-        }
-    };
-    if (f.a.B <= 64) {
-        // a lane per sequence, every wave for itself
-        const int lane = threadIdx.x & 63;
-        Steps own{};
-        if (lane < f.a.B) own = steps_of(f, sequence(f.a, lane));
-        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * f.a.heads : 0.0;
-        auto sum = [](double p, double q) { return p + q; };
-        double size = own.steps * groups, total = wave_all(size, sum);
-        const double pairs = wave_all(groups, sum);
-        const bool by_group = pairs * 4 <= f.shares;
-        const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
-        const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
-        if (by_group) {
-            size = lane < f.a.B ? parts_of(own.steps, share) * groups : 0.0;
-            total = wave_all(size, sum);
-        }
-        const double start = wave_running_sum(size) - size, begin = by_group ? g : static_cast<double>(g) * share;
-        if (g == 0 && threadIdx.x < f.a.B) f.plan[lane] = static_cast<int64_t>(start);
-        if (g == 0 && threadIdx.x == 0) f.plan[f.a.B] = by_group ? -share : share;
-        const uint64_t here = __ballot(begin >= start && begin < start + size);
-        if (!here) return false;
-        b = __builtin_ctzll(here);
-        auto at = [&](int v) { return __builtin_amdgcn_readlane(v, b); };
-        const uint64_t row0 = static_cast<uint64_t>(own.sq.row0), in = static_cast<uint64_t>(static_cast<int64_t>(begin - start));
-        auto at64 = [&](uint64_t v) {
-            return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(at(static_cast<int>(v >> 32)))) << 32 |
-                                        static_cast<uint32_t>(at(static_cast<int>(v))));
-        };
-        x.sq = {at64(row0), at(own.sq.n), at(own.sq.len)};
-        x.lo = at(own.lo), x.steps = at(own.steps), x.groups = at(own.groups);
-        within(by_group, share, at64(in), begin, total);
-        return true;
-    }
-    const int per = (f.a.B + 255) / 256, tid = threadIdx.x;
-    const int first = min(tid * per, f.a.B), last = min(first + per, f.a.B);
-    Steps own;  // the last of this thread's sequences: its only one in batches of up to 256
-    if (first < last) own = steps_of(f, sequence(f.a, first));
-    auto load = [&](int i) {
-        if (per > 1) own = steps_of(f, sequence(f.a, i));
-    };
-    auto groups = [&] { return static_cast<double>(own.groups) * f.a.heads; };
-    double mine = 0.0, mine_pairs = 0.0, start, pairs_start, total, pairs;
-    for (int i = first; i < last; ++i) {
-        load(i);
-        mine += own.steps * groups();
-        mine_pairs += groups();
-    }
-    block_scan(mine_pairs, pair_sums, pairs_start, pairs);
-    block_scan(mine, sums[0], start, total);
-    const bool by_group = pairs * 4 <= f.shares;
-    const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
-    const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
-    auto size = [&] { return (by_group ? parts_of(own.steps, share) : own.steps) * groups(); };
-    if (by_group) {
-        mine = 0.0;
-        for (int i = first; i < last; ++i) {
-            load(i);
-            mine += size();
-        }
-        block_scan(mine, sums[1], start, total);
-    }
-    const double begin = by_group ? g : static_cast<double>(g) * share;
-    double s = start;
-    for (int i = first; i < last; ++i) {
-        load(i);
-        const double n = size();
-        if (g == 0) f.plan[i] = static_cast<int64_t>(s);
-        if (begin >= s && begin < s + n) {
-            at_b = i;
-            at_x = own;
-            at_before = static_cast<int64_t>(begin - s);
-        }
-        s += n;
-    }
-    if (g == 0 && tid == 0) f.plan[f.a.B] = by_group ? -share : share;
-    if (begin >= total) return false;
-    __syncthreads();
-    b = same(at_b);
-    x.sq = {at_x.sq.row0, same(at_x.sq.n), same(at_x.sq.len)};
-    x.lo = same(at_x.lo), x.steps = same(at_x.steps), x.groups = same(at_x.groups);
-    within(by_group, share, at_before, begin, total);
-    return true;
-}
-
-template <int HD, typename CT, int NW>
+template <int HD, bool E4, int NW>
 struct FewLds {
-    static constexpr bool E4 = kE4<CT>;
     static constexpr int TILE = 32 * HD * (E4 ? 1 : 2);          // bytes of a tile of K or V
     static constexpr int STAGE = 2 * TILE + (E4 ? 256 : 0);      // and the exponents of 32 keys of K, then of V, a word each
-    static constexpr int WAVE = kE2<CT> ? TILE : 2 * STAGE;      // e2m1: one tile of V, as bf16
+    static constexpr int WAVE = 2 * STAGE;
     static constexpr int BYTES = NW * WAVE > NW * 32 * HD * 4 ? NW * WAVE : NW * 32 * HD * 4;  // also the waves' O at the end
     static constexpr int COPIES = 2 * (TILE / 1024) + (E4 ? 1 : 0);  // of a stage
 };
@@ -247,10 +94,9 @@ struct Frags8 {
 };
 
 // What a thread knows of the tiles: where its copies and fragments lie.
-template <int HD, typename CT>
+template <int HD, bool E4>
 struct FewLane {
-    static constexpr bool E4 = kE4<CT>;
-    static constexpr int TILE = FewLds<HD, CT, 1>::TILE;
+    static constexpr int TILE = FewLds<HD, E4, 1>::TILE;
     static constexpr int RB = HD * (E4 ? 1 : 2), NC = RB / 16, RPS = 1024 / RB;  // bytes and chunks of a row, rows of a 1 KB copy
     uint32_t voff[TILE / 1024];
     std::conditional_t<E4, Frags8<HD>, Frags<HD>> F;
@@ -264,86 +110,13 @@ struct FewLane {
         F.init(lane);
     }
 };
-
-// e2m1: a tile's codes in registers, two tiles ahead.  K's are fragments as they come: half h of the wave holds half h of each key's
-// columns (the order of the columns is free, as long as Q's is the same); V's are 16-byte units of 32 columns, for LDS.
-template <int HD>
-struct Codes4 {
-    static constexpr int KW = HD / 16;                  // words of a lane's half of a key
-    static constexpr int KE = HD / 64 > 0 ? HD / 64 : 1;  // its exponents
-    static constexpr int UPR = HD / kGroup, NV = HD / 64 > 0 ? HD / 64 : 1;  // units of a row of V, of a lane (head_dim 32: of half the lanes)
-    uint32_t k[KW], ke[KE], ve[NV];
-    uint4 v[NV];
-    // rows: of the lane's key and of its units, in the pools; negative: without a page
-    __device__ __forceinline__ void load(const PageView& kv, int64_t key, const int64_t (&row)[NV], int lane) {
-        const int h = lane >> 5;
-        const char* none = reinterpret_cast<const char*>(&kNoPage);
-        const char* kp = key >= 0 ? kv.kp + key * (HD / 2) + h * (HD / 4) : none;
-        if constexpr (KW == 8) {
-            const uint4 x = reinterpret_cast<const uint4*>(kp)[0], y = *reinterpret_cast<const uint4*>(key >= 0 ? kp + 16 : none);
-            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w, k[4] = y.x, k[5] = y.y, k[6] = y.z, k[7] = y.w;
-            const uint32_t e = key >= 0 ? reinterpret_cast<const uint16_t*>(kv.ke)[key * 2 + h] : 0xffffu;
-            ke[0] = e & 255u, ke[1] = e >> 8;
-        } else if constexpr (KW == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kp);
-            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
-            ke[0] = key >= 0 ? kv.ke[key * 2 + h] : kNanGroup;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(kp);
-            k[0] = x.x, k[1] = x.y;
-            ke[0] = key >= 0 ? kv.ke[key] : kNanGroup;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t at = row[i] * UPR + (i * 64 + lane) % UPR;
-            v[i] = *reinterpret_cast<const uint4*>(row[i] >= 0 ? kv.vp + at * 16 : none);
-            ve[i] = row[i] >= 0 ? kv.ve[at] : kNanGroup;
-        }
-    }
-    __device__ static __forceinline__ int v_row(int i, int lane) { return min((i * 64 + lane) / UPR, 31); }
-    // V to LDS as bf16, for the products' transposed reads.
-    __device__ __forceinline__ void put_v(char* tile, int lane) const {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (HD < 64 && lane >= 32) break;
-            const int u = i * 64 + lane, rr = u / UPR, ch = u % UPR * 4;
-            const float s = exp_scale(ve[i]);
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-            const uint32_t nan = ve[i] == kNanGroup ? 0x7fff7fffu : 0u;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint4 x = e2m1_bf16(w[c], s);
-                *reinterpret_cast<uint4*>(tile + chunk_at<bf16, HD>(rr, ch + c)) = make_uint4(x.x | nan, x.y | nan, x.z | nan, x.w | nan);
-            }
-        }
-    }
-    // Eight columns of the lane's key.
-    __device__ __forceinline__ bf16x8 k_frag(int kk) const {
-        const uint32_t e = ke[kk * KE / KW];
-        const uint4 x = e2m1_bf16(k[kk], exp_scale(e));
-        const uint32_t nan = e == kNanGroup ? 0x7fff7fffu : 0u;
-        return __builtin_bit_cast(bf16x8, make_uint4(x.x | nan, x.y | nan, x.z | nan, x.w | nan));
-    }
-};
-// What lanes have stored to LDS, for other lanes of the wave: LDS works in order, so this is for the compiler alone.
-__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
-// A group's keys, or a block's share of them; one for the whole block.
-struct Part {
-    Seq sq;
-    int b, kvh, r0;  // the group's sequence, key/value head and first row
-    int first, end;  // keys
-    int slot;        // of its state in the workspace
-    int whole;       // all of the group's keys
-};
-
 // The work on one part: true where a sum of this thread's has left fp32's range.
-template <int HD, typename CT, int NW>
-__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, CT>& me, float down) {
-    using L = FewLds<HD, CT, NW>;
+template <int HD, bool E4, int NW>
+__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, E4>& me, float down) {
+    using L = FewLds<HD, E4, NW>;
     const PagedArgs& a = f.a;
-    constexpr bool E4 = kE4<CT>, E2 = kE2<CT>;
     constexpr int KS = HD / 16, OB = HD / 32;
-    constexpr int RB = FewLane<HD, CT>::RB, NC = FewLane<HD, CT>::NC, RPS = FewLane<HD, CT>::RPS;
+    constexpr int RB = FewLane<HD, E4>::RB, NC = FewLane<HD, E4>::NC, RPS = FewLane<HD, E4>::RPS;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int ids[kIds];
     __shared__ float2 mls[NW][32];
@@ -375,16 +148,16 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
         const bf16* qp = static_cast<const bf16*>(a.q) + (sq.row0 + tok) * a.ldq + static_cast<int64_t>(head) * HD;
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
-            const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : E2 ? HD / 2 * hl + 8 * kk : 16 * kk + 8 * hl;
+            const int col = E4 ? 32 * (kk >> 1) + 16 * hl + 8 * (kk & 1) : 16 * kk + 8 * hl;
             if (a.vec_q) qb[kk] = __builtin_bit_cast(bf16x8, ldg16(qp + col, real));
             else
 #pragma unroll
                 for (int j = 0; j < 8; ++j) qb[kk][j] = real ? qp[col + j] : f2bf(0.0f);
         }
 
-        // one tile's products, from the stage it arrived in; e2m1: from V's tile, and the registers c, which `loaded` then fills anew
-        auto compute = [&](char* kt, int k0, [[maybe_unused]] const Codes4<HD>* c, auto loaded) {
-            const char* vt = kt + (E2 ? 0 : L::TILE);
+        // one tile's products, from the stage it arrived in
+        auto compute = [&](char* kt, int k0) {
+            const char* vt = kt + L::TILE;
             [[maybe_unused]] const uint32_t* ex = reinterpret_cast<const uint32_t*>(vt + L::TILE);
             f32x16 sc[1];
             zero(sc[0]);
@@ -411,15 +184,11 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
                     sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, e4m3_bf16(make_uint2(x.z, x.w), sk)),
                                                                     qb[2 * j + 1], sc[0], 0, 0, 0);
                 }
-            } else if constexpr (E2) {
-#pragma unroll
-                for (int kk = 0; kk < KS; ++kk) sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c->k_frag(kk), qb[kk], sc[0], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk)
                     sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(me.F.row(kt, 0, kk), qb[kk], sc[0], 0, 0, 0);
             }
-            loaded();
             // every row sees every key of the tile?
             const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
             auto seen = [&](int j) { return static_cast<uint32_t>(k0 + j - lo) < span; };
@@ -497,44 +266,6 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
                 const int64_t row = (static_cast<int64_t>(page) * Hkv + kvh) * ps + (key - pi * ps);
                 return page < 0 ? -1 : row;
             };
-            if constexpr (E2) {
-                // page ids of the halves of a tile, or of each row
-                auto load = [&](int t, Codes4<HD>& c) {
-                    const int k0 = first + 32 * NW * t;
-                    int64_t key, row[Codes4<HD>::NV];
-                    if (paged && k0 + 32 <= w1) {
-                        const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
-                        const int page0 = __builtin_amdgcn_readfirstlane(ids[pi - p0]), page1 = __builtin_amdgcn_readfirstlane(ids[pj - p0]);
-                        const int64_t row0 = (static_cast<int64_t>(page0) * Hkv + kvh) * ps + (k0 - pi * ps);
-                        const int64_t row1 = (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps);
-                        auto at = [&](int r) { return (r & 16 ? page1 : page0) < 0 ? -1 : (r & 16 ? row1 : row0) + (r & 15); };
-                        key = at(lane & 31);
-#pragma unroll
-                        for (int i = 0; i < Codes4<HD>::NV; ++i) row[i] = at(Codes4<HD>::v_row(i, lane));
-                    } else {
-                        key = row_at(k0 + (lane & 31));
-#pragma unroll
-                        for (int i = 0; i < Codes4<HD>::NV; ++i) row[i] = row_at(k0 + Codes4<HD>::v_row(i, lane));
-                    }
-                    c.load(a.kv, key, row, lane);
-                };
-                Codes4<HD> even, odd;
-                if (nt > 0) load(0, even);
-                if (nt > 1) load(1, odd);
-                auto step = [&](int t, Codes4<HD>& c) {
-                    c.put_v(mine, lane);
-                    wave_lds_fence();
-                    compute(mine, first + 32 * NW * t, &c, [&] {
-                        if (t + 2 < nt) load(t + 2, c);
-                    });
-                    wave_lds_fence();
-                };
-                for (int t = 0; t < nt; t += 2) {
-                    step(t, even);
-                    if (t + 1 < nt) step(t + 1, odd);
-                }
-                continue;
-            }
             auto issue = [&](int t) {
                 char* dst = mine + (t & 1) * L::STAGE;
                 const int k0 = first + 32 * NW * t;
@@ -577,7 +308,7 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
             for (int t = 0; t < nt; ++t) {
                 if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
                 else wait_vmcnt<0>();
-                compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t, nullptr, [] {});
+                compute(mine + (t & 1) * L::STAGE, first + 32 * NW * t);
                 wait_lds();  // the tile has been read
                 if (t + 2 < nt) issue(t + 2);
             }
@@ -647,175 +378,43 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
 
 // NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
 // else is divided and a block is alone on its CU.
-template <int HD, typename CT, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && sizeof(CT) > 1) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
-    const PagedArgs& a = f.a;
-    __shared__ int past;
-    const int Hkv = a.heads;
-    FewLane<HD, CT> me;
+template <int HD, bool E4, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+    FewLane<HD, E4> me;
     me.init(threadIdx.x & 63);
-    if (threadIdx.x == 0) past = 0;
-
-    int b;
-    Steps x;
-    int64_t before, count;
-    if (NW == 4 && f.shares > 0) {
-        if (!find_share(f, static_cast<int>(blockIdx.x), b, x, before, count)) return;
-    } else {
-        b = static_cast<int>(blockIdx.x) / Hkv;
-        x = steps_of(f, wave_sequence(f.a, b));
-        before = 0;
-        count = INT64_MAX;
-    }
-    for (bool first_part = true; count > 0 && b < a.B;) {
-        const Seq sq = x.sq;
-        // groups of a sequence: all of them (shares), or those of the block's head
-        const int64_t groups = static_cast<int64_t>(x.groups) * (f.shares > 0 ? Hkv : 1);
-        if (before >= groups * x.steps) {
-            if (f.shares == 0) return;
-            before -= groups * x.steps;
-            if (++b < a.B) x = steps_of(f, wave_sequence(f.a, b));
-            continue;
-        }
-        // (a 64-bit division takes a microsecond's worth of instructions)
-        const int gi = before >> 31 ? static_cast<int>(before / x.steps)
-                                    : __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(before) / static_cast<uint32_t>(x.steps)));
-        const int u0 = static_cast<int>(before - static_cast<int64_t>(gi) * x.steps);
-        const int u1 = static_cast<int>(min(static_cast<int64_t>(x.steps), u0 + min(count, int64_t{1} << 30)));
-        const int kvh = kv_head(a, b, f.shares > 0 ? gi % Hkv : static_cast<int>(blockIdx.x) % Hkv), r0 = (f.shares > 0 ? gi / Hkv : gi) * f.group;
-        const Part pt{sq, b, kvh, r0, x.lo + u0 * kStep, u1 < x.steps ? x.lo + u1 * kStep : INT32_MAX,
-                      2 * static_cast<int>(blockIdx.x) + (first_part ? 0 : 1), u0 == 0 && u1 == x.steps};
-        first_part = false;
-        before += u1 - u0;
-        count -= u1 - u0;
-
-        bool again = false;
-        do {
-            const bool over = few_part<HD, CT, NW>(f, pt, me, again ? kDown : 0.0f);
-            if (over && !again) past = 1;
-            lds_barrier();  // also: before the next part's tiles
-            again = !again && past;
-            if (__builtin_expect(again, 0)) {
-                lds_barrier();
-                if (threadIdx.x == 0) past = 0;
-            }
-        } while (__builtin_expect(again, 0));
-    }
-}
-
-// The groups that shares divided: one wave per row adds the parts of its group.
-template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
-    const PagedArgs& a = f.a;
-    const int Hkv = a.heads, grid_head = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv, kvh = kv_head(a, b, grid_head);
-    const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
-    if (qr >= f.group) return;
-    const int64_t planned = f.plan[a.B], share = planned < 0 ? -planned : planned, base_step = f.plan[b];
-    const bool by_group = planned < 0;
-    const Steps x = steps_of(f, wave_sequence(f.a, b));
-    for (int g = 0; g < x.groups; ++g) {
-        const int r = g * f.group + qr;
-        if (r >= x.sq.n * a.G) return;
-        // the group's first block and its parts; a block's second slot holds a group that begins behind its own begin
-        const int64_t group = static_cast<int64_t>(g) * Hkv + grid_head;
-        int64_t s0;
-        int parts, first_slot = 0;
-        if (by_group) {
-            parts = parts_of(x.steps, share);
-            s0 = base_step + group * parts;
-        } else {
-            const int64_t from = base_step + group * x.steps;
-            s0 = from / share;
-            parts = static_cast<int>((from + x.steps - 1) / share - s0) + 1;
-            first_slot = from != s0 * share;
-        }
-        if (parts == 1) continue;  // undivided: written already
-        auto at = [&](int i) { return (2 * (s0 + i) + (i == 0 ? first_slot : 0)) * f.group + qr; };
-        auto state = [&](int i) { return i < parts ? f.part_ml[at(i)] : make_float2(-INFINITY, 0.0f); };
-        const float2 first = state(lane);
-        float M = first.y != 0.0f ? first.x : -INFINITY;
-        bool any = first.y != 0.0f;
-        for (int i = lane + 64; i < parts; i += 64) {
-            const float2 ml = state(i);
-            any |= ml.y != 0.0f;
-            M = ml.y != 0.0f ? fmaxf(M, ml.x) : M;
-        }
-        any = __any(any);
-        M = wave_all(M, [](float p, float q) { return fmaxf(p, q); });
-        const float base = M == -INFINITY ? 0.0f : M;
-        constexpr int PL = HD >= 64 ? HD / 64 : 1;
-        // a part's weight, of its row divided by its own sum
-        auto weigh = [&](float2 ml) { return ml.y != 0.0f && ml.y != -1.0f ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) * ml.y : 0.0f; };
-        float own = weigh(first), o[PL] = {}, l = own;
-        for (int i = lane + 64; i < parts; i += 64) l += weigh(state(i));
-        l = wave_all(l, [](float p, float q) { return p + q; });
-        const float inv = 1.0f / l;
-        for (int i0 = 0; i0 < parts; i0 += 64) {
-            if (i0 > 0) own = weigh(state(i0 + lane));
-            const float w = own * inv;
-            uint64_t left = __ballot(own != 0.0f);
-            while (left) {  // four parts' rows at a time
-                int j[4];
-                float v[4][PL], ws[4];
-                bool live[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    live[k] = left != 0;
-                    j[k] = live[k] ? __builtin_ctzll(left) : j[k > 0 ? k - 1 : 0];
-                    ws[k] = __shfl(w, j[k], 64);
-                    left &= left - 1;
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int u = 0; u < PL; ++u)
-                        if (lane * PL < HD) v[k][u] = f.part_o[at(i0 + j[k]) * HD + lane * PL + u];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int u = 0; u < PL; ++u) o[u] = live[k] ? fmaf(ws[k], v[k][u], o[u]) : o[u];
-            }
-        }
-        const int64_t t = x.sq.row0 + r / a.G;
-        const int head = kvh * a.G + r % a.G;
-        bf16* op = static_cast<bf16*>(a.o) + t * a.ldo + static_cast<int64_t>(head) * HD;
-#pragma unroll
-        for (int u = 0; u < PL; ++u)
-            if (lane * PL < HD) st(op, lane * PL + u, any && l == 0.0f ? NAN : o[u]);  // only scores of -infinity: NaN
-        if (a.lse && lane == 0) a.lse[t * a.H + head] = any ? log_sum(base, l, a.c) : -INFINITY;
-    }
+    work_on_parts<NW == 4>(f, [&](const Part& pt, float down) { return few_part<HD, E4, NW>(f, pt, me, down); });
 }
 
 // Blocks that are resident at once on 256 CUs: LDS holds one of bf16 at head_dim 128, two of the others.
 int64_t resident(int64_t head_dim, DType type) { return head_dim == 128 && !holds_codes(type) ? 256 : 512; }
 
-template <int HD, typename CT, int NW>
+template <int HD, bool E4, int NW>
 void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
-    constexpr int bytes = FewLds<HD, CT, NW>::BYTES;
+    constexpr int bytes = FewLds<HD, E4, NW>::BYTES;
     static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     AIC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
-        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, CT, NW>),
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4, NW>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) allowed[dev].store(true);
     }
-    attn_paged_few_k<HD, CT, NW><<<static_cast<unsigned>(blocks), NW * 64, bytes, s>>>(f);
+    attn_paged_few_k<HD, E4, NW><<<static_cast<unsigned>(blocks), NW * 64, bytes, s>>>(f);
     AIC_LAUNCH_CHECK("attn_paged");
 }
 
-template <int HD, typename CT>
+template <int HD, bool E4>
 void launch(const FewArgs& f, hipStream_t s) {
     const int64_t pairs = static_cast<int64_t>(f.a.heads) * f.a.B;
     AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
     if (f.shares == 0) {
         // eight waves' stages are beyond the LDS for bf16 at head_dim 128; with more blocks than CUs four waves keep two of them there
-        if constexpr (HD < 128 || sizeof(CT) == 1) {
-            if (pairs <= 256) return launch<HD, CT, 8>(f, pairs, s);
+        if constexpr (HD < 128 || E4) {
+            if (pairs <= 256) return launch<HD, E4, 8>(f, pairs, s);
         }
-        return launch<HD, CT, 4>(f, pairs, s);
+        return launch<HD, E4, 4>(f, pairs, s);
     }
-    launch<HD, CT, 4>(f, f.shares, s);
+    launch<HD, E4, 4>(f, f.shares, s);
     attn_paged_few_join_k<HD><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>((f.group + 3) / 4)), 256, 0, s>>>(f);
     AIC_LAUNCH_CHECK("attn_paged join");
 }
@@ -848,12 +447,11 @@ void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim,
         f.part_ml = reinterpret_cast<float2*>(f.part_o + 2LL * f.shares * f.group * head_dim);
         f.plan = reinterpret_cast<int64_t*>(f.part_ml + 2LL * f.shares * f.group);
     }
-    by_cache_type<bf16>(type, [&](auto ct) {
-        using CT = decltype(ct);
-        if (head_dim == 32) launch<32, CT>(f, s);
-        else if (head_dim == 64) launch<64, CT>(f, s);
-        else launch<128, CT>(f, s);
-    });
+    if (type == DType::UInt4) return attn_paged_e2m1_few(f, head_dim, s);
+    const bool e4m3 = type == DType::UInt8;
+    if (head_dim == 32) e4m3 ? launch<32, true>(f, s) : launch<32, false>(f, s);
+    else if (head_dim == 64) e4m3 ? launch<64, true>(f, s) : launch<64, false>(f, s);
+    else e4m3 ? launch<128, true>(f, s) : launch<128, false>(f, s);
 }
 
 }  // namespace aic::hip
