@@ -41,8 +41,8 @@ namespace {
 // 326 us); 856 of 16 heads of 64, 43 us, whose longest block takes most of it.
 constexpr int kIds = 512;  // page ids in LDS at a time
 
-template <typename CT, int HD, int SH>
-__device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block, float down) {
+template <typename CT, int HD, int SH, typename A>
+__device__ __forceinline__ bool f32_pass(const A& a, int tid, int block, float down) {
     constexpr int SETS = 4 / SH, R = 32 * SETS, KT = 32 * SH, OB = HD / 32;
     constexpr int UPR = HD / kPer16<CT>;        // 16-byte units of a cached row
     constexpr int NU = (KT * UPR + 255) / 256;  // units of a tile per thread
@@ -53,13 +53,13 @@ __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block,
     char *ks = tiles, *vs = tiles + TILE;
 
     const int Hkv = a.kv.Hkv;
-    const int rest = block / a.heads;
-    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (a.heads * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
+    const int rest = block / grid_heads(a);
+    const int split = rest % a.nsplit, tile = static_cast<int>(gridDim.x) / (grid_heads(a) * a.nsplit) - 1 - rest / a.nsplit;  // long ones first
     int b, local;
     if (!find_tile<R>(a, tile, b, local)) return false;
-    const int kvh = kv_head(a, b, block % a.heads);
+    const int kvh = kv_head(a, b, block % grid_heads(a));
     const Seq sq = wave_sequence(a, b);
-    if (sq.n == 0) return false;
+    if (std::is_same_v<A, PickedArgs> && sq.n == 0) return false;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hl = lane >> 5;
     const int set = wave % SETS, share = wave / SETS, sub = 32 * share;  // this wave's rows of the block and keys of a tile
     const int rows = sq.n * a.G, r0 = local * R, r = r0 + set * 32 + (lane & 31);
@@ -319,21 +319,25 @@ __device__ __forceinline__ bool f32_pass(const PagedArgs& a, int tid, int block,
     return real && store_row<float, HD>(a, st_, t, head, empty, split, down > 0.0f);
 }
 
-template <typename CT, int HD, int SH>
-__global__ __launch_bounds__(256, 2) void attn_paged_f32_k(PagedArgs a) {
-    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return f32_pass<CT, HD, SH>(args, tid, block, down); });
+template <typename CT, int HD, int SH, typename A>
+__global__ __launch_bounds__(256, 2) void attn_paged_f32_k(A a) {
+    one_or_two_passes(a, [](const A& args, int tid, int block, float down) { return f32_pass<CT, HD, SH>(args, tid, block, down); });
 }
 
 // ------------------------------------------------------------------------- joining splits
 // One wave per (token, head): M = max m_s, w_s = 2^((m_s - M) c) l_s, o = sum_s w_s o_s / sum_s w_s; o_s is divided by l_s.
 // Bound by reading the parts: 12 us for two of 2048 rows of 16 heads of 128 (34 MB read, 8 MB written: 3.5 TB/s).
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_paged_join_k(PagedArgs a) {
+template <typename T, int HD, typename A>
+__global__ __launch_bounds__(256) void attn_paged_join_k(A a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (i >= a.T * a.H) return;
     const int64_t t = i / a.H;
     // rows of no sequence stay as they are
-    if (a.picked ? a.lens[t * a.kv.Hkv + i % a.H / a.G] < 0 : t < a.offsets[0] || t >= a.offsets[a.B]) return;
+    if constexpr (std::is_same_v<A, PickedArgs>) {
+        if (a.lens[t * a.kv.Hkv + i % a.H / a.G] < 0) return;
+    } else {
+        if (t < a.offsets[0] || t >= a.offsets[a.B]) return;
+    }
     const int lane = threadIdx.x & 63;
     const int64_t step = a.T * a.H;
     // a lane per split: the splits of one launch are at most kMaxSplits
@@ -398,11 +402,12 @@ Plan plan(int64_t B, int64_t T, int64_t max_len, int64_t H, const KVPages& c, in
     p.nsplit = std::clamp<int64_t>((1024 + twice / 2) / std::max<int64_t>(twice, 1), 1, std::clamp<int64_t>(most, 1, kMaxSplits));
     return p;
 }
-// fp32: query rows of a block: fewer than 128 where such blocks are fewer than two per CU; at head_dim 128 then 64, two
+// fp32: query rows of a block: 32 where rows have pages of their own, a group each; otherwise fewer than 128 where such blocks are fewer than two per CU; at head_dim 128 then 64, two
 // blocks to a CU, or 32 where a block is alone there and the keys are not divided: 300 rows of 16 heads on 300 keys,
 // 33.9 us in 32 and 39.7 us in 64; on 452 rows and 554 keys, in two parts, 59.0 and 48.4 us.
-int64_t f32_rows(int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t Hkv, int64_t hd) {
+int64_t f32_rows(int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t Hkv, int64_t hd, bool picked) {
     if (const int few = f32_few_rows(max_q, H / Hkv)) return few;
+    if (picked) return 32;
     if (tile_bound(T, H / Hkv, B, 128) * Hkv >= 512) return 128;
     return hd == 128 && (max_len >= 512 || tile_bound(T, H / Hkv, B, 32) * Hkv > 256) ? 64 : 32;
 }
@@ -440,7 +445,7 @@ int64_t parts_bytes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64
     if (c.type != DType::Float32 && !few)
         n = plan_bytes(plan(B, T, max_len, H, c, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
-        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c, f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim)), T, H, c.head_dim));
+        n = std::max(n, plan_bytes(plan(B, T, max_len, H, c, f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim, picked)), T, H, c.head_dim));
     return n;
 }
 
@@ -450,18 +455,20 @@ struct Workspace {
 };
 
 // a: pointers, strides, T, H, G and the batch; the rest follows from the sizes, which are those of the sequences that the blocks see.
-void attend(PagedArgs& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, float scale, Workspace w,
+template <typename A>
+void attend(A& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, float scale, Workspace w,
             DType dt, hipStream_t s) {
+    constexpr bool picked = std::is_same_v<A, PickedArgs>;
     max_q = std::min(max_q, T);
     const int64_t size = static_cast<int64_t>(dtype_size(dt));
     a.c = scale * kLog2e;
     a.vec_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq * size % 16 == 0;
     a.vec_o = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.ldo * size % 16 == 0;
 
-    const bool few = dt == DType::BFloat16 && (a.picked || few_rows(max_q, a.G, c.head_dim, c.type));
-    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim);
+    const bool few = dt == DType::BFloat16 && (picked || few_rows(max_q, a.G, c.head_dim, c.type));
+    const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim, picked);
     Plan p = plan(B, T, max_len, H, c, R);
-    const int64_t need = parts_bytes(c, B, T, max_q, max_len, H, a.picked);
+    const int64_t need = parts_bytes(c, B, T, max_q, max_len, H, picked);
     const StreamScratchUse use(s);
     void* workspace = w.at;
     if (workspace)
@@ -490,15 +497,17 @@ void attend(PagedArgs& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q,
         constexpr int D = decltype(hd)::value;
         const auto grid = static_cast<unsigned>(blocks);
         if constexpr (sizeof(X) == 2) {
-            attn_paged_tiles(a, c.type, D, grid, s);
+            if constexpr (!picked) attn_paged_tiles(a, c.type, D, grid, s);
         } else if (R <= 4) {
             attn_paged_f32_few(a, static_cast<int>(R), c.type, D, grid, s);
         } else {
             by_cache_type<float>(c.type, [&](auto ct) {
                 using CT = decltype(ct);
-                if (R == 128) attn_paged_f32_k<CT, D, 1><<<grid, 256, 0, s>>>(a);
-                else if (R == 64) attn_paged_f32_k<CT, D, 2><<<grid, 256, 0, s>>>(a);
-                else attn_paged_f32_k<CT, D, 4><<<grid, 256, 0, s>>>(a);
+                if constexpr (!picked) {
+                    if (R == 128) return attn_paged_f32_k<CT, D, 1><<<grid, 256, 0, s>>>(a);
+                    if (R == 64) return attn_paged_f32_k<CT, D, 2><<<grid, 256, 0, s>>>(a);
+                }
+                attn_paged_f32_k<CT, D, 4><<<grid, 256, 0, s>>>(a);
             });
             AIC_LAUNCH_CHECK("attn_paged");
         }
@@ -574,7 +583,6 @@ void attn_paged(const KVPages& c, const void* q, int64_t ld_q, void* o, int64_t 
     a.offsets = offsets, a.lens = lens;
     a.B = static_cast<int>(B), a.H = static_cast<int>(H), a.G = static_cast<int>(H / c.kv_heads);
     a.window = static_cast<int>(std::min<int64_t>(window, INT32_MAX));
-    a.heads = static_cast<int>(c.kv_heads);
     attend(a, c, B, T, max_q, max_len, H, scale, {workspace, workspace_bytes}, dt, s);
 }
 
@@ -599,14 +607,12 @@ void attn_paged_selected(const KVPages& c, const void* q, int64_t ld_q, void* o,
     check_call(c, ld_q, ld_o, H, scale, workspace_bytes, dt);
     if (T == 0) return;
     AIC_CHECK(q && o, InvalidArgument, "attn_paged: null pointer");
-    PagedArgs a{};
+    PickedArgs a{};
     a.kv = pv;
     a.q = q, a.o = o, a.lse = lse;
     a.ldq = ld_q, a.ldo = ld_o, a.T = T;
     a.lens = picked_lens;
     a.B = static_cast<int>(rows), a.H = static_cast<int>(H), a.G = static_cast<int>(G);
-    a.heads = 1;
-    a.picked = true;
     attend(a, one, rows, rows, 1, len, G, scale, {workspace, workspace_bytes}, dt, s);
 }
 

@@ -21,11 +21,10 @@ struct PagedArgs {
     float2* part_ml;  // [nsplit][T][H]: maximum, sum (-1: only scores of -infinity)
     float* part_o;    // [nsplit][T][H][hd]
     bool vec_q, vec_o;
-    // key/value heads that a launch's blocks go over beside the sequences: all of them, or one where each (row, head) is a
-    // sequence of its own with the pages picked for it as its page table
-    int heads;
-    bool picked;
 };
+// The same for rows that have pages picked for them: each (row, key/value head) is a sequence of its own, its pages the page table's row.
+// A type, not a flag, which would cost the calls without it (one token of 12 heads on 513 keys 0.2 us).
+struct PickedArgs : PagedArgs {};
 
 namespace {
 
@@ -93,22 +92,27 @@ struct Seq {
     int64_t row0;  // first packed row
     int n, len;    // queries, cached keys
 };
+// A picked row stands behind its pages' positions; length -1: nobody's row, left as it is.
+__device__ __forceinline__ Seq sequence(const PickedArgs& a, int b) {
+    const int64_t len = a.lens[b];
+    return {static_cast<uint32_t>(b) / static_cast<uint32_t>(a.kv.Hkv), len >= 0, static_cast<int>(min(max(len, int64_t{0}), kMaxLen))};
+}
 __device__ __forceinline__ Seq sequence(const PagedArgs& a, int b) {
-    if (a.picked) {  // its one row stands behind the picked positions; length -1: nobody's row, left as it is
-        const int64_t len = a.lens[b];
-        return {static_cast<uint32_t>(b) / static_cast<uint32_t>(a.kv.Hkv), len >= 0, static_cast<int>(min(max(len, int64_t{0}), kMaxLen))};
-    }
     const int64_t lo = min(max(a.offsets[b], int64_t{0}), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
     return {lo, static_cast<int>(hi - lo), static_cast<int>(min(max(a.lens[b], int64_t{0}), kMaxLen))};
 }
 
-// The key/value head of sequence b's blocks numbered h.
-__device__ __forceinline__ int kv_head(const PagedArgs& a, int b, int h) {
-    return a.picked ? static_cast<int>(static_cast<uint32_t>(b) % static_cast<uint32_t>(a.kv.Hkv)) : h;
+// Key/value heads that a launch's blocks go over beside the sequences; the one of sequence b's blocks numbered h.
+__device__ __forceinline__ int grid_heads(const PagedArgs& a) { return a.kv.Hkv; }
+__device__ __forceinline__ int grid_heads(const PickedArgs&) { return 1; }
+__device__ __forceinline__ int kv_head(const PagedArgs&, int, int h) { return h; }
+__device__ __forceinline__ int kv_head(const PickedArgs& a, int b, int) {
+    return static_cast<int>(static_cast<uint32_t>(b) % static_cast<uint32_t>(a.kv.Hkv));
 }
 
 // The same for a b that is one for the whole wave, in scalar registers.
-__device__ __forceinline__ Seq wave_sequence(const PagedArgs& a, int b) {
+template <typename A>
+__device__ __forceinline__ Seq wave_sequence(const A& a, int b) {
     const Seq x = sequence(a, b);
     const uint64_t r = static_cast<uint64_t>(x.row0);
     const uint32_t r_lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(r)));
@@ -121,12 +125,6 @@ __device__ __forceinline__ Seq wave_sequence(const PagedArgs& a, int b) {
 // Every wave finds it by itself: 64 sequences per step, their tile counts added up across lanes.
 template <int R>
 __device__ __forceinline__ bool find_tile(const PagedArgs& a, int tile, int& b, int& local) {
-    if (a.picked) {  // all have as many tiles
-        const uint32_t per = static_cast<uint32_t>((a.G + R - 1) / R);
-        b = static_cast<int>(static_cast<uint32_t>(tile) / per);
-        local = tile - b * static_cast<int>(per);
-        return b < a.B;
-    }
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int tiles = 0;
@@ -147,6 +145,14 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& a, int tile, int& b, 
         tile -= __shfl(upto, 63, 64);
     }
     return false;
+}
+
+template <int R>
+__device__ __forceinline__ bool find_tile(const PickedArgs& a, int tile, int& b, int& local) {  // all have as many tiles
+    const uint32_t per = static_cast<uint32_t>((a.G + R - 1) / R);
+    b = static_cast<int>(static_cast<uint32_t>(tile) / per);
+    local = tile - b * static_cast<int>(per);
+    return b < a.B;
 }
 
 // The keys [k_lo, k_hi) of part `split` of a query tile's, k_lo a multiple of 64: equal parts of whole tiles of 64, by
@@ -346,12 +352,14 @@ void by_cache_type(DType type, F&& f) {
 // workspace the batch's keys are cut into equal shares, one per resident block.
 bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, DType type);
 int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type);
-void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s);
+template <typename A>
+void attn_paged_few(const A& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s);
 
 // Up to 4 query rows per key/value head, fp32 queries (attention_paged_f32_few.hip): tiles of so many rows, 0 for
 // more of them; tiles x splits x key/value heads blocks.
 int f32_few_rows(int64_t max_q, int64_t G);
-void attn_paged_f32_few(const PagedArgs& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s);
+template <typename A>
+void attn_paged_f32_few(const A& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s);
 
 // Many query rows per key/value head, bf16 queries (attention_paged_tiles.hip): tiles x splits x key/value heads blocks.
 void attn_paged_tiles(const PagedArgs& a, DType type, int head_dim, unsigned blocks, hipStream_t s);

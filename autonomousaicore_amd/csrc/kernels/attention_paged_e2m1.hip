@@ -206,8 +206,8 @@ __device__ __forceinline__ void add_seen(State<HD, R>& st_, const float (&p)[Sta
 }
 
 // The work on one part: true where a sum of this thread's has left fp32's range.
-template <int HD, int NW, int R>
-__device__ __forceinline__ bool few4_part(const FewArgs& f, const Part& pt, float down) {
+template <int HD, int NW, int R, typename A>
+__device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, float down) {
     using L = Lds4<HD, NW, R>;
     using P = Lane4<HD, R>;
     using S = State<HD, R>;
@@ -399,6 +399,7 @@ __device__ __forceinline__ bool few4_part(const FewArgs& f, const Part& pt, floa
                 const int64_t row = row_at(k0 + (fl & 31));
                 dma_exps<HD>(row >= 0 ? reinterpret_cast<const char*>(fl >> 5 ? a.kv.ve : a.kv.ke) + row * NC : none, dst + 2 * L::CODES);
             };
+            wait_vmcnt<0>();  // Q is there: left to the compiler, which does not count the copies, it would be waited for with all of them, at every tile
             if (nt > 0) issue(0);
             if (nt > 1) issue(1);
             float sc[S::NS], mx;
@@ -488,19 +489,19 @@ __device__ __forceinline__ bool few4_part(const FewArgs& f, const Part& pt, floa
     return over;
 }
 
-template <int HD, int NW, int R>
-__global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void attn_paged_e2m1_k(FewArgs f) {
+template <int HD, int NW, int R, typename A>
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) void attn_paged_e2m1_k(FewArgs<A> f) {
     work_on_parts<NW == 4>(f, [&](const Part& pt, float down) { return few4_part<HD, NW, R>(f, pt, down); });
 }
 
-template <int HD, int NW, int R>
-void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
+template <int HD, int NW, int R, typename A>
+void launch(const FewArgs<A>& f, int64_t blocks, hipStream_t s) {
     constexpr int bytes = Lds4<HD, NW, R>::BYTES;
     static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     AIC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
-        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_e2m1_k<HD, NW, R>),
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_e2m1_k<HD, NW, R, A>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) allowed[dev].store(true);
     }
@@ -508,9 +509,9 @@ void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
     AIC_LAUNCH_CHECK("attn_paged");
 }
 
-template <int HD, int R>
-void launch(const FewArgs& f, hipStream_t s) {
-    const int64_t pairs = static_cast<int64_t>(f.a.heads) * f.a.B;
+template <int HD, int R, typename A>
+void launch(const FewArgs<A>& f, hipStream_t s) {
+    const int64_t pairs = (std::is_same_v<A, PickedArgs> ? int64_t{1} : f.a.kv.Hkv) * f.a.B;
     AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
     if (f.shares == 0) return pairs <= 256 ? launch<HD, 8, R>(f, pairs, s) : launch<HD, 4, R>(f, pairs, s);
     launch<HD, 4, R>(f, f.shares, s);
@@ -520,7 +521,8 @@ void launch(const FewArgs& f, hipStream_t s) {
 
 }  // namespace
 
-void attn_paged_e2m1_few(const FewArgs& f, int head_dim, hipStream_t s) {
+template <typename A>
+void attn_paged_e2m1_few(const FewArgs<A>& f, int head_dim, hipStream_t s) {
     auto rows = [&](auto hd) {
         constexpr int D = decltype(hd)::value;
         f.group <= 16 ? launch<D, 16>(f, s) : launch<D, 32>(f, s);
@@ -529,5 +531,8 @@ void attn_paged_e2m1_few(const FewArgs& f, int head_dim, hipStream_t s) {
     else if (head_dim == 64) rows(std::integral_constant<int, 64>{});
     else rows(std::integral_constant<int, 128>{});
 }
+
+template void attn_paged_e2m1_few(const FewArgs<PagedArgs>&, int, hipStream_t);
+template void attn_paged_e2m1_few(const FewArgs<PickedArgs>&, int, hipStream_t);
 
 }  // namespace aic::hip

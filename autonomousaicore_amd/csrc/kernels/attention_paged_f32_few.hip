@@ -56,19 +56,19 @@ __device__ __forceinline__ float4 floats(uint32_t x, uint32_t e) {
 }
 
 // RM: rows of a tile.
-template <typename CT, int HD, int RM>
-__device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int block, float down) {
+template <typename CT, int HD, int RM, typename A>
+__device__ __forceinline__ bool f32_few_pass(const A& a, int tid, int block, float down) {
     constexpr int L = HD / 4, KI = 64 / L, NI = 8, KB = NI * KI;  // a batch: NI loads of KI keys
     static_assert(KB <= 64, "a lane per key looks its page up");
     __shared__ float2 mls[4][RM];
     __shared__ float os[4][RM][HD];
-    const int rest = block / a.heads;
+    const int rest = block / grid_heads(a);
     const int split = rest % a.nsplit, tile = rest / a.nsplit;
     int b, local;
     if (!find_tile<RM>(a, tile, b, local)) return false;
-    const int kvh = kv_head(a, b, block % a.heads);
+    const int kvh = kv_head(a, b, block % grid_heads(a));
     const Seq sq = wave_sequence(a, b);
-    if (sq.n == 0) return false;
+    if (std::is_same_v<A, PickedArgs> && sq.n == 0) return false;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = lane / L, d0 = 4 * (lane % L);
     const int rows = sq.n * a.G, r0 = local * RM;
@@ -217,9 +217,9 @@ __device__ __forceinline__ bool f32_few_pass(const PagedArgs& a, int tid, int bl
     return over;
 }
 
-template <typename CT, int HD, int RM>
-__global__ __launch_bounds__(256) void attn_paged_f32_few_k(PagedArgs a) {
-    one_or_two_passes(a, [](const PagedArgs& args, int tid, int block, float down) { return f32_few_pass<CT, HD, RM>(args, tid, block, down); });
+template <typename CT, int HD, int RM, typename A>
+__global__ __launch_bounds__(256) void attn_paged_f32_few_k(A a) {
+    one_or_two_passes(a, [](const A& args, int tid, int block, float down) { return f32_few_pass<CT, HD, RM>(args, tid, block, down); });
 }
 
 }  // namespace
@@ -230,7 +230,8 @@ int f32_few_rows(int64_t max_q, int64_t G) {
     return rows > 4 ? 0 : rows > 2 ? 4 : rows > 1 ? 2 : 1;
 }
 
-void attn_paged_f32_few(const PagedArgs& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s) {
+template <typename A>
+void attn_paged_f32_few(const A& a, int rows, DType type, int head_dim, unsigned blocks, hipStream_t s) {
     auto run = [&](auto ct, auto hd) {
         using C = decltype(ct);
         constexpr int D = decltype(hd)::value;
@@ -245,5 +246,8 @@ void attn_paged_f32_few(const PagedArgs& a, int rows, DType type, int head_dim, 
         else run(ct, std::integral_constant<int, 128>{});
     });
 }
+
+template void attn_paged_f32_few(const PagedArgs&, int, DType, int, unsigned, hipStream_t);
+template void attn_paged_f32_few(const PickedArgs&, int, DType, int, unsigned, hipStream_t);
 
 }  // namespace aic::hip

@@ -111,8 +111,8 @@ struct FewLane {
     }
 };
 // The work on one part: true where a sum of this thread's has left fp32's range.
-template <int HD, bool E4, int NW>
-__device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const FewLane<HD, E4>& me, float down) {
+template <int HD, bool E4, int NW, typename A>
+__device__ __forceinline__ bool few_part(const FewArgs<A>& f, const Part& pt, const FewLane<HD, E4>& me, float down) {
     using L = FewLds<HD, E4, NW>;
     const PagedArgs& a = f.a;
     constexpr int KS = HD / 16, OB = HD / 32;
@@ -303,6 +303,7 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
                     dma_byte(row >= 0 ? (hl ? a.kv.ve : a.kv.ke) + row : &kNoExponent, dst + 2 * L::TILE);
                 }
             };
+            wait_vmcnt<0>();  // Q is there: left to the compiler, which does not count the copies, it would be waited for with all of them, at every tile
             if (nt > 0) issue(0);
             if (nt > 1) issue(1);
             for (int t = 0; t < nt; ++t) {
@@ -378,8 +379,8 @@ __device__ __forceinline__ bool few_part(const FewArgs& f, const Part& pt, const
 
 // NW waves: four, and two blocks per CU (bf16 at head_dim 128: one); or eight that divide a group among them where nothing
 // else is divided and a block is alone on its CU.
-template <int HD, bool E4, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs f) {
+template <int HD, bool E4, int NW, typename A>
+__global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) void attn_paged_few_k(FewArgs<A> f) {
     FewLane<HD, E4> me;
     me.init(threadIdx.x & 63);
     work_on_parts<NW == 4>(f, [&](const Part& pt, float down) { return few_part<HD, E4, NW>(f, pt, me, down); });
@@ -388,14 +389,14 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || (HD == 128 && !E4) ? 1 : 2) voi
 // Blocks that are resident at once on 256 CUs: LDS holds one of bf16 at head_dim 128, two of the others.
 int64_t resident(int64_t head_dim, DType type) { return head_dim == 128 && !holds_codes(type) ? 256 : 512; }
 
-template <int HD, bool E4, int NW>
-void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
+template <int HD, bool E4, int NW, typename A>
+void launch(const FewArgs<A>& f, int64_t blocks, hipStream_t s) {
     constexpr int bytes = FewLds<HD, E4, NW>::BYTES;
     static std::atomic<bool> allowed[64];  // by device
     int dev = 0;
     AIC_HIP_CHECK(hipGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !allowed[dev].load()) {
-        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4, NW>),
+        AIC_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_few_k<HD, E4, NW, A>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) allowed[dev].store(true);
     }
@@ -403,9 +404,9 @@ void launch(const FewArgs& f, int64_t blocks, hipStream_t s) {
     AIC_LAUNCH_CHECK("attn_paged");
 }
 
-template <int HD, bool E4>
-void launch(const FewArgs& f, hipStream_t s) {
-    const int64_t pairs = static_cast<int64_t>(f.a.heads) * f.a.B;
+template <int HD, bool E4, typename A>
+void launch(const FewArgs<A>& f, hipStream_t s) {
+    const int64_t pairs = (std::is_same_v<A, PickedArgs> ? int64_t{1} : f.a.kv.Hkv) * f.a.B;
     AIC_CHECK(pairs <= INT32_MAX, OutOfRange, "attn_paged: too many sequences in one call");
     if (f.shares == 0) {
         // eight waves' stages are beyond the LDS for bf16 at head_dim 128; with more blocks than CUs four waves keep two of them there
@@ -439,8 +440,9 @@ int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, in
     return (2 * resident(head_dim, type) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
 }
 
-void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s) {
-    FewArgs f{a, static_cast<int>(group_of(max_q, a.G)), 0, nullptr, nullptr, nullptr};
+template <typename A>
+void attn_paged_few(const A& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s) {
+    FewArgs<A> f{a, static_cast<int>(group_of(max_q, a.G)), 0, nullptr, nullptr, nullptr};
     if (workspace) {
         f.shares = static_cast<int>(resident(head_dim, type));
         f.part_o = static_cast<float*>(workspace);
@@ -453,5 +455,8 @@ void attn_paged_few(const PagedArgs& a, int64_t max_q, DType type, int head_dim,
     else if (head_dim == 64) e4m3 ? launch<64, true>(f, s) : launch<64, false>(f, s);
     else e4m3 ? launch<128, true>(f, s) : launch<128, false>(f, s);
 }
+
+template void attn_paged_few(const PagedArgs&, int64_t, DType, int, void*, hipStream_t);
+template void attn_paged_few(const PickedArgs&, int64_t, DType, int, void*, hipStream_t);
 
 }  // namespace aic::hip

@@ -6,8 +6,9 @@
 
 namespace aic::hip {
 
+template <typename A>
 struct FewArgs {
-    PagedArgs a;
+    A a;
     int group;         // query rows of a group, at most 32
     int shares;        // 0: a block per sequence and key/value head, nothing divided
     int64_t* plan;     // [B + 1], as find_share leaves it
@@ -25,7 +26,8 @@ struct Steps {
     Seq sq;
     int lo, steps, groups;  // first key (a multiple of kStep), steps over its keys, row groups
 };
-__device__ __forceinline__ Steps steps_of(const FewArgs& f, const Seq& sq) {
+template <typename A>
+__device__ __forceinline__ Steps steps_of(const FewArgs<A>& f, const Seq& sq) {
     Steps x;
     x.sq = sq;
     const int first = max(x.sq.len - x.sq.n, 0);
@@ -55,7 +57,8 @@ __device__ __forceinline__ void block_scan(double mine, double (&sums)[4], doubl
 // The part of block g: its sequence, the steps before it there and its own.  False: nothing is left for it.
 // plan: for each sequence the steps (or, where groups are cut by themselves, the blocks) before it; behind
 // them a share's steps, negative in the second case.
-__device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Steps& x, int64_t& before, int64_t& count) {
+template <typename A>
+__device__ __forceinline__ bool find_share(const FewArgs<A>& f, int g, int& b, Steps& x, int64_t& before, int64_t& count) {
     __shared__ double sums[2][4], pair_sums[4];
     __shared__ int at_b;
     __shared__ Steps at_x;
@@ -82,7 +85,7 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
         const int lane = threadIdx.x & 63;
         Steps own{};
         if (lane < f.a.B) own = steps_of(f, sequence(f.a, lane));
-        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * f.a.heads : 0.0;
+        const double groups = lane < f.a.B ? static_cast<double>(own.groups) * grid_heads(f.a) : 0.0;
         auto sum = [](double p, double q) { return p + q; };
         double size = own.steps * groups, total = wave_all(size, sum);
         const double pairs = wave_all(groups, sum);
@@ -117,7 +120,7 @@ __device__ __forceinline__ bool find_share(const FewArgs& f, int g, int& b, Step
     auto load = [&](int i) {
         if (per > 1) own = steps_of(f, sequence(f.a, i));
     };
-    auto groups = [&] { return static_cast<double>(own.groups) * f.a.heads; };
+    auto groups = [&] { return static_cast<double>(own.groups) * grid_heads(f.a); };
     double mine = 0.0, mine_pairs = 0.0, start, pairs_start, total, pairs;
     for (int i = first; i < last; ++i) {
         load(i);
@@ -172,11 +175,11 @@ struct Part {
 
 // A block's parts, one after another.  work(part, down): all of a thread's work on one, true where a sum of this thread's has left fp32's
 // range; then once more, with the weights' down.  SHARES: whether the launch may have cut the keys into shares.
-template <bool SHARES, typename F>
-__device__ __forceinline__ void work_on_parts(const FewArgs& f, F work) {
-    const PagedArgs& a = f.a;
+template <bool SHARES, typename A, typename F>
+__device__ __forceinline__ void work_on_parts(const FewArgs<A>& f, F work) {
+    const A& a = f.a;
     __shared__ int past;
-    const int Hkv = a.heads;
+    const int Hkv = grid_heads(a);
     if (threadIdx.x == 0) past = 0;
 
     int b;
@@ -227,10 +230,10 @@ __device__ __forceinline__ void work_on_parts(const FewArgs& f, F work) {
 }
 
 // The groups that shares divided: one wave per row adds the parts of its group.
-template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
-    const PagedArgs& a = f.a;
-    const int Hkv = a.heads, grid_head = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv;
+template <int HD, typename A>
+__global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs<A> f) {
+    const A& a = f.a;
+    const int Hkv = grid_heads(a), grid_head = static_cast<int>(blockIdx.x) % Hkv, b = static_cast<int>(blockIdx.x) / Hkv;
     const int kvh = kv_head(a, b, grid_head);
     const int lane = threadIdx.x & 63, qr = static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x >> 6);
     if (qr >= f.group) return;
@@ -313,6 +316,7 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs f) {
 }  // namespace
 
 // Single tokens and a few drafted ones on e2m1 caches (attention_paged_e2m1.hip).
-void attn_paged_e2m1_few(const FewArgs& f, int head_dim, hipStream_t s);
+template <typename A>
+void attn_paged_e2m1_few(const FewArgs<A>& f, int head_dim, hipStream_t s);
 
 }  // namespace aic::hip
