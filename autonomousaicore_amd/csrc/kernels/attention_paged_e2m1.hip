@@ -49,19 +49,19 @@ struct Lds4 {
     static constexpr int COPIES = (2 * CODES + 1023) / 1024 + 1;          // of a stage
 };
 
-// A lane's places in a tile.  Codes: rows of HD / 32 chunks of 16 bytes, swizzled so that a chunk of 16 neighbouring rows
+// A lane's places in a tile, as bytes.  Codes: rows of HD / 32 chunks of 16 bytes, swizzled so that a chunk of 16 neighbouring rows
 // lies in different banks.  V as bf16: 16-byte chunks swizzled so that the same holds, and that the transposed reads, which take
-// 4 rows per 16 lanes, spread over the banks as well.
+// 4 rows per 16 lanes, spread over the banks as well.  Swizzles go by a row's place among 16, so that what lies 16 rows on is an
+// instruction's offset, and chunks of a row are exclusive-ors of constants.
 template <int HD, int R>
 struct Lane4 {
     static constexpr int RB = HD / 2, NC = RB / 16, NV = HD / 64 > 0 ? HD / 64 : 1;  // bytes and chunks of a row of codes, units of V of a lane
     static constexpr int KL = R == 16 ? 4 : 2, KH = 32 / (64 / KL);  // lanes of a key; keys of a lane
     static constexpr int KW = HD / 8 / KL;                           // words of a key in a lane: 8 columns each
-    int lane;
-    __device__ __forceinline__ explicit Lane4(int l) : lane(l) {}
+    static constexpr int KC = 64 / KL;                               // lanes of a column of keys
+    int k, ke, ke_shift, v, ve, put, frag;
+    uint32_t voff;  // 16 bytes of 16 rows of a pool (head_dim 128)
     __device__ static __forceinline__ int swz4(int r) { return NC == 4 ? (r >> 2) & 3 : NC == 2 ? (r >> 3) & 1 : 0; }
-    // 16 bytes of 16 rows of a pool (head_dim 128)
-    __device__ __forceinline__ uint32_t voff() const { return static_cast<uint32_t>(lane / NC * RB + ((lane % NC ^ swz4(lane / NC)) << 4)); }
     // row of V's bf16 tile, chunk of 8 columns
     __device__ static __forceinline__ int v_swz(int r) {
         if constexpr (R == 32) return swz<HD>(r);
@@ -70,71 +70,68 @@ struct Lane4 {
         else return 2 * ((r >> 2) & 1) | ((r >> 3) & 1);
     }
     __device__ static __forceinline__ int v_chunk(int r, int ch) { return r * HD * 2 + ((ch ^ v_swz(r)) << 4); }
-
+    __device__ __forceinline__ explicit Lane4(int lane) {
+        const int r = lane & (KC - 1), q = lane / KC, at = q * (RB / KL);  // key, its part, the part's byte of a row
+        k = r * RB + ((at >> 4 ^ swz4(r)) << 4) + (at & 15);
+        ke = r * 4;
+        ke_shift = NC == 1 ? 0 : 8 * (q * (HD / KL) / kGroup);
+        // 16 lanes hold a chunk of 16 rows of V each
+        const int vr = NC == 4 ? lane & 15 : lane & 31, g = NC == 4 ? lane >> 4 : NC == 2 ? lane >> 5 : 0;
+        v = vr * RB + ((g ^ swz4(vr)) << 4);
+        ve = vr * 4 + g;
+        put = v_chunk(vr, 4 * g);
+        const int s = lane & 15, fr = 4 * (lane >> 4) + (s >> 2), c = s & 3;
+        frag = v_chunk(fr, c >> 1) + (c & 1) * 8;
+        voff = static_cast<uint32_t>(lane / NC * RB + ((lane % NC ^ swz4(lane / NC)) << 4));
+    }
     // Words of the lane's u-th key; the lane's columns are HD / KL neighbouring ones.
     __device__ __forceinline__ void k_words(const char* t, int u, uint32_t (&w)[KW]) const {
-        const int r = lane % (64 / KL) + (64 / KL) * u, q = lane / (64 / KL), at = q * (RB / KL);  // byte of the row
-        const char* p = t + r * RB;
+        const char* p = t + u * KC * RB;
         if constexpr (KW >= 4) {
 #pragma unroll
             for (int i = 0; i < KW / 4; ++i) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p + (((at >> 4) + i ^ swz4(r)) << 4));
+                const uint4 x = *reinterpret_cast<const uint4*>(p + (k ^ (i << 4)));
                 w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
             }
+        } else if constexpr (KW == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p + k);
+            w[0] = x.x, w[1] = x.y;
         } else {
-            p += ((at >> 4 ^ swz4(r)) << 4) + (at & 15);
-            if constexpr (KW == 2) {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                w[0] = x.x, w[1] = x.y;
-            } else {
-                w[0] = *reinterpret_cast<const uint32_t*>(p);
-            }
+            w[0] = *reinterpret_cast<const uint32_t*>(p + k);
         }
     }
-    __device__ __forceinline__ uint32_t k_exps(const char* exps, int u) const {
-        return *reinterpret_cast<const uint32_t*>(exps + (lane % (64 / KL) + (64 / KL) * u) * 4);
-    }
-    // Power of word i, from the key's word of exponents.
-    __device__ __forceinline__ float k_scale(uint32_t e, int i) const {
-        const int first = lane / (64 / KL) * (HD / KL);  // column
-        return exp_scale(NC == 1 ? e : e >> (8 * (first / kGroup + (HD / KL >= kGroup ? 8 * i / kGroup : 0))) & 255u);
-    }
+    __device__ __forceinline__ uint32_t k_exps(const char* exps, int u) const { return *reinterpret_cast<const uint32_t*>(exps + ke + u * KC * 4); }
+    // Byte of word i's group, from the key's word of them.
+    __device__ __forceinline__ uint32_t k_byte(uint32_t e, int i) const { return e >> (ke_shift + (HD / KL > kGroup ? 8 * (8 * i / kGroup) : 0)) & 255u; }
     __device__ static __forceinline__ bool k_nan(uint32_t e) { return NC == 1 ? e == kNanGroup : any_nan_group(NC == 2 ? e & 0xffffu : e); }
-    // 16 lanes hold a chunk of 16 rows of V each
-    __device__ __forceinline__ int v_row(int i) const { return NC == 4 ? 16 * i + (lane & 15) : lane & 31; }
-    __device__ __forceinline__ int v_group() const { return NC == 4 ? lane >> 4 : NC == 2 ? lane >> 5 : 0; }
-    // V's bf16 tile from codes and words of exponents; true where a lane has met a NaN group.
-    __device__ __forceinline__ bool put_v(const char* codes, const char* exps, char* tile) const {
-        bool nan = false;
-        const int g = v_group();
+    // V's bf16 tile from codes and words of exponents; the largest byte of the lane's groups.
+    __device__ __forceinline__ uint32_t put_v(const char* codes, const char* exps, char* tile, bool mine) const {
+        uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int r = v_row(i);
-            const uint4 x = *reinterpret_cast<const uint4*>(codes + r * RB + ((g ^ swz4(r)) << 4));
-            const uint32_t e = *reinterpret_cast<const uint8_t*>(exps + r * 4 + g);
-            nan |= e == kNanGroup;
-            if (NC == 1 && lane >= 32) break;  // half of the lanes hold all
-            const float s = exp_scale(e);
+            const uint4 x = *reinterpret_cast<const uint4*>(codes + v + i * 16 * RB);
+            const uint32_t e = *reinterpret_cast<const uint8_t*>(exps + ve + i * 64);
+            most = max(most, e);
+            if (NC == 1 && !mine) break;  // half of the lanes hold all
+            const float s = scale_of(e);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(tile + v_chunk(r, 4 * g + c)) = e2m1_bf16(w[c], s);
+            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(tile + (put ^ (c << 4)) + i * 32 * HD) = e2m1_bf16(w[c], s);
         }
-        return nan;
+        return most;
     }
     __device__ __forceinline__ void put_nan(const char* exps, char* tile) const {
-        const int g = v_group();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int r = v_row(i);
-            if (*reinterpret_cast<const uint8_t*>(exps + r * 4 + g) == kNanGroup)
+        for (int i = 0; i < NV; ++i)
+            if (*reinterpret_cast<const uint8_t*>(exps + ve + i * 64) == kNanGroup)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(tile + v_chunk(r, 4 * g + c)) = make_uint4(~0u, ~0u, ~0u, ~0u);
-        }
+                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(tile + (put ^ (c << 4)) + i * 32 * HD) = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
+    // A byte's power; of kNanGroup no number, for what it makes is overwritten.
+    __device__ static __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
     // Operand of O^T += V^T P^T, 8 keys of one column: R 16: column 16 ob + lane % 16, keys 4 q + 0..3 and 16 more, q = lane / 16.
     __device__ __forceinline__ bf16x8 v_frag16(const char* tile, int ob) const {
-        const int s = lane & 15, r = 4 * (lane >> 4) + (s >> 2), c = s & 3;
-        const char* p = tile + r * HD * 2 + ((2 * ob + (c >> 1) ^ v_swz(r)) << 4) + (c & 1) * 8;  // row + 16 has the same swizzle
+        const char* p = tile + (frag ^ (ob << 5));
         const v4i16_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)p);
         const v4i16_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(p + 16 * HD * 2));
         const uint2 a = __builtin_bit_cast(uint2, x), b = __builtin_bit_cast(uint2, y);
@@ -257,16 +254,21 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
         std::conditional_t<R == 32, Frags<HD>, char> F;
         if constexpr (R == 32) F.init(lane);
 
+        // R 32: made anew for each tile, for kept through the loop they would take registers that it does not have
+        [[maybe_unused]] const P own(lane);
+        auto places = [&] {
+            if constexpr (R == 16) return own;
+            else return P(fresh(lane));
+        };
         // A tile's scores and the maximum of the lane's row; one_by_one: where its keys have to be added so.  read() where the stage has
         // been read.
-        auto scores = [&](const char* kt, int k0, float (&sc)[S::NS], bool& one_by_one, auto read) {
-            // made anew for each tile: its addresses kept through the loop would take registers that it does not have
-            const P at(fresh(lane));
+        auto scores = [&](const char* kt, int k0, float (&sc)[S::NS], int& one_by_one, auto read) {
+            const P at = places();
             char* vt = mine + L::V;
             const char* exps = kt + 2 * L::CODES;
             uint32_t ek[KH];
             typename S::acc_t acc[KH];
-            bool nan = at.put_v(kt + L::CODES, exps + 128, vt), nan_k[KH];
+            uint32_t most = at.put_v(kt + L::CODES, exps + 128, vt, lane < 32);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < KH; ++u) {
@@ -277,20 +279,20 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
                 for (int e = 0; e < S::NS / KH; ++e) acc[u][e] = 0.0f;
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) {
-                    const bf16x8 x = __builtin_bit_cast(bf16x8, e2m1_bf16(w[kk], at.k_scale(ek[u], kk)));
+                    const uint32_t byte = at.k_byte(ek[u], kk);
+                    most = max(most, byte);
+                    const bf16x8 x = __builtin_bit_cast(bf16x8, e2m1_bf16(w[kk], P::scale_of(byte)));
                     if constexpr (R == 16) acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qb[kk], acc[u], 0, 0, 0);
                     else acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qb[kk], acc[u], 0, 0, 0);
                 }
-                nan_k[u] = P::k_nan(ek[u]);
-                nan |= nan_k[u];
             }
 #pragma unroll
             for (int e = 0; e < S::NS; ++e) sc[e] = acc[e / (S::NS / KH)][e % (S::NS / KH)];
-            if (__builtin_expect(__ballot(nan) != 0, 0)) {
+            if (__builtin_expect(__ballot(most == kNanGroup) != 0, 0)) {
                 at.put_nan(exps + 128, vt);
                 uint32_t bad = 0;  // by key
 #pragma unroll
-                for (int u = 0; u < KH; ++u) bad |= (static_cast<uint32_t>(__ballot(nan_k[u])) & (R == 16 ? 0xffffu : ~0u)) << (16 * u);
+                for (int u = 0; u < KH; ++u) bad |= (static_cast<uint32_t>(__ballot(P::k_nan(ek[u]))) & (R == 16 ? 0xffffu : ~0u)) << (16 * u);
                 bad >>= 4 * (fresh(lane) / R);
 #pragma unroll
                 for (int e = 0; e < S::NS; ++e) sc[e] = bad & (1u << S::key(e, 0)) ? NAN : sc[e];
@@ -300,7 +302,7 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
             read();
             // every row sees every key of the tile?
             const bool open = k0 + 31 <= first_pos && k0 + 32 <= k_hi && (a.window <= 0 || k0 > last_pos - a.window);
-            one_by_one = false;
+            one_by_one = 0;
             if (!open) {
 #pragma unroll
                 for (int e = 0; e < S::NS; ++e) sc[e] = static_cast<uint32_t>(k0 + S::key(e, lane) - lo) < span ? sc[e] : -INFINITY;
@@ -308,7 +310,7 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
 #pragma unroll
                 for (int i = 0; i < 64 * HD / 1024; ++i)
                     bits |= non_finite_bits<bf16>(*reinterpret_cast<const uint4*>(vt + i * 1024 + lane * 16));
-                one_by_one = __ballot(bits != 0) != 0;
+                one_by_one = __ballot(bits != 0) != 0 ? 1 : 0;
             }
             float mx = sc[0];
 #pragma unroll
@@ -332,7 +334,7 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
                 return;
             }
             if constexpr (R == 16) {
-                const P at(fresh(lane));
+                const P at = places();
                 const bf16x8 p = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16x2(sc[0], sc[1]), pack_bf16x2(sc[2], sc[3]), pack_bf16x2(sc[4], sc[5]),
                                                                        pack_bf16x2(sc[6], sc[7])));
 #pragma unroll
@@ -370,8 +372,8 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
             };
             auto issue = [&](int t) {
                 char* dst = mine + (t & 1) * L::STAGE;
-                const int k0 = first + 32 * NW * t, fl = fresh(lane);
-                const P at(fl);
+                const int k0 = first + 32 * NW * t, fl = R == 16 ? lane : fresh(lane);
+                const P at = places();
                 if (HD == 128 && ps % 16 == 0 && k0 + 32 <= w1) {
                     // each half of the tile lies in one page: uniform bases
                     const int pi = a.kv.page_index(k0), pj = a.kv.page_index(k0 + 16);
@@ -381,8 +383,8 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
                                                 (static_cast<int64_t>(page1) * Hkv + kvh) * ps + (k0 + 16 - pj * ps)};
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            dma16s(a.kv.kp + row[i] * RB, at.voff(), dst + i * 1024);
-                            dma16s(a.kv.vp + row[i] * RB, at.voff(), dst + L::CODES + i * 1024);
+                            dma16s(a.kv.kp + row[i] * RB, at.voff, dst + i * 1024);
+                            dma16s(a.kv.vp + row[i] * RB, at.voff, dst + L::CODES + i * 1024);
                         }
                         dma_exps<HD>((fl >> 5 ? a.kv.ve : a.kv.ke) + ((fl & 16 ? row[1] : row[0]) + (fl & 15)) * NC, dst + 2 * L::CODES);
                         return;
@@ -403,25 +405,25 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
             if (nt > 0) issue(0);
             if (nt > 1) issue(1);
             float sc[S::NS], mx;
-            bool one_by_one;
+            int one_by_one;
             // The tiles whose row maxima stand, which are nearly all, in a loop of their own: with the rescaling in it the sums would be
             // copied from one set of registers to another for every tile.
             for (int t = 0; t < nt; ++t) {
-                bool stands;
+                int turn;  // one for the whole wave, in a scalar register
                 do {
                     if (t + 1 < nt) wait_vmcnt<L::COPIES>();  // tile t has landed; t + 1 may be in flight
                     else wait_vmcnt<0>();
                     mx = scores(mine + (t & 1) * L::STAGE, first + 32 * NW * t, sc, one_by_one, [&] {
                         if (t + 2 < nt) issue(t + 2);
                     });
-                    stands = !one_by_one && !st_.moves(mx, a.c);
-                    if (!stands) break;
+                    turn = same(one_by_one | (st_.moves(mx, a.c) ? 2 : 0));
+                    if (turn) break;
                     add(first + 32 * NW * t, sc, false);
                     wave_lds_fence();
                 } while (++t < nt);
-                if (stands) break;
+                if (!turn) break;
                 st_.absorb(mx, a.c);
-                add(first + 32 * NW * t, sc, one_by_one);
+                add(first + 32 * NW * t, sc, turn & 1);
                 wave_lds_fence();
             }
         }
