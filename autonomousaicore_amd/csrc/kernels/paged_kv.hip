@@ -242,6 +242,10 @@ __global__ __launch_bounds__(kBlock) void kv_write_k(PageView pv, Cut c, const T
     }
 }
 
+// Elements of a unit of kv_read: 16 bytes of the cache, of e2m1 half as many (32 elements, four stores 64 bytes apart, would
+// leave a store's lanes 16 bytes of every 64: 8 x 2048 rows of 8 heads of 128 21.0 us for 14.5, 5.9 TB/s).
+template <typename CT> constexpr int kRead = kE2<CT> ? 16 : kPer16<CT>;
+
 // Appending with the rotation on the way: a unit is 16 elements of a head, i .. i + 7 of its first half and the same of its second,
 // so that a thread holds the pairs that turn together, and the head's hd / 16 lanes hold it whole.  Columns of a row: H heads of
 // q, then Hkv of k, then Hkv of v.
@@ -350,21 +354,22 @@ __global__ __launch_bounds__(kBlock) void kv_append_k(PageView pv, Cut c, Turn a
 
 template <typename T, typename CT, int HD, int U>
 __global__ __launch_bounds__(kBlock) void kv_read_k(PageView pv, Cut c, T* __restrict__ k, T* __restrict__ v, int64_t ld, bool vec) {
-    constexpr int EPU = kPer16<CT>;
+    constexpr int EPU = kRead<CT>;
+    using raw_t = std::conditional_t<EPU == kPer16<CT>, uint4, uint2>;
     __shared__ int64_t at[kMaxRows];
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * c.rows;
     const int u0 = static_cast<int>(blockIdx.y) * (kBlock * U) + static_cast<int>(threadIdx.x);
     block_places(pv, c, t0, at);
-    uint4 raw[U];
+    raw_t raw[U];
     uint32_t ex[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
         const Unit w = unit<HD, EPU>(pv, c, min(u0 + i * kBlock, c.rows * c.ncol - 1));
         const int64_t place = at[w.r], row = place + static_cast<int64_t>(w.h) * pv.ps;
-        raw[i] = make_uint4(0, 0, 0, 0);
+        raw[i] = raw_t{};
         ex[i] = 127;
         if (place >= 0) {
-            raw[i] = *reinterpret_cast<const uint4*>((w.kv ? pv.vp : pv.kp) + row * static_cast<int64_t>(kRowBytes<CT, HD>) + w.d / EPU * 16);
+            raw[i] = *reinterpret_cast<const raw_t*>((w.kv ? pv.vp : pv.kp) + row * static_cast<int64_t>(kRowBytes<CT, HD>) + w.d * 16 / kPer16<CT>);
             if constexpr (kE4<CT>) ex[i] = (w.kv ? pv.ve : pv.ke)[row];
             if constexpr (kE2<CT>) ex[i] = (w.kv ? pv.ve : pv.ke)[row * (HD / kGroup) + w.d / kGroup];
         }
@@ -378,9 +383,8 @@ __global__ __launch_bounds__(kBlock) void kv_read_k(PageView pv, Cut c, T* __res
         float x[EPU];
         if constexpr (kE2<CT>) {
             const float s = exp_scale(ex[i]);
-            const uint32_t q[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) e2m1_floats(q[j], s, reinterpret_cast<float(&)[8]>(x[8 * j]));
+            e2m1_floats(raw[i].x, s, reinterpret_cast<float(&)[8]>(x[0]));
+            e2m1_floats(raw[i].y, s, reinterpret_cast<float(&)[8]>(x[8]));
             if (__builtin_expect(ex[i] == kNanGroup, 0)) {
 #pragma unroll
                 for (int j = 0; j < EPU; ++j) x[j] = NAN;
@@ -447,13 +451,13 @@ void by_types(const KVPages& c, DType dt, F&& f) {
     else f(bf16{}, e2m1x2{});
 }
 
-// Four units of 16 bytes per thread; of 32 codes, whose values take twice the registers, two.
-template <typename F>
+// Four units per thread; of 32 elements, which take twice the registers, two.
+template <bool READ, typename F>
 void launch_rows(const KVPages& c, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T, DType dt, F&& f) {
     by_types(c, dt, [&](auto t, auto ct) {
         using CT = decltype(ct);
-        constexpr int most = kE2<CT> ? 2 : 4;
-        cut_rows(2 * c.kv_heads * (c.head_dim / kPer16<CT>), most, offsets, lens, B, T, [&](const Cut& cut, dim3 grid, bool few) {
+        constexpr int per = READ ? kRead<CT> : kPer16<CT>, most = per == 32 ? 2 : 4;
+        cut_rows(2 * c.kv_heads * (c.head_dim / per), most, offsets, lens, B, T, [&](const Cut& cut, dim3 grid, bool few) {
             by_head_dim(c.head_dim, [&](auto hd) {
                 if (few) f(t, ct, hd, std::integral_constant<int, 1>{}, grid, cut);
                 else f(t, ct, hd, std::integral_constant<int, most>{}, grid, cut);
@@ -470,7 +474,7 @@ void kv_write(const KVPages& c, const void* k, const void* v, int64_t ld, const 
     const PageView pv = page_view(c, "kv_write");
     if (B == 0 || T == 0) return;
     const bool vec = aligned16(k, v, ld, static_cast<int64_t>(dtype_size(dt)));
-    launch_rows(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
+    launch_rows<false>(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
         using X = decltype(t);
         kv_write_k<X, decltype(ct), decltype(hd)::value, decltype(u)::value><<<grid, kBlock, 0, s>>>(
             pv, cut, static_cast<const X*>(k), static_cast<const X*>(v), ld, vec);
@@ -513,7 +517,7 @@ void kv_read(const KVPages& c, void* k, void* v, int64_t ld, const int64_t* offs
     const PageView pv = page_view(c, "kv_read");
     if (B == 0 || T == 0) return;
     const bool vec = aligned16(k, v, ld, static_cast<int64_t>(dtype_size(dt)));
-    launch_rows(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
+    launch_rows<true>(c, offsets, lens, B, T, dt, [&](auto t, auto ct, auto hd, auto u, dim3 grid, const Cut& cut) {
         using X = decltype(t);
         kv_read_k<X, decltype(ct), decltype(hd)::value, decltype(u)::value><<<grid, kBlock, 0, s>>>(
             pv, cut, static_cast<X*>(k), static_cast<X*>(v), ld, vec);
