@@ -7,11 +7,17 @@
 // depend on how the sum is cut.
 //
 // kv_bounds_k: a wave per page and key/value head that the batch's rows touch; lanes hold 16 bytes of a key (8 of codes), the
-// wave's groups of lanes go over the keys in turn and are joined at the end.
+// wave's groups of lanes go over the keys in turn, with several loads in flight, and are joined at the end.  8 x 2048 e2m1 rows
+// of 8 heads of 128: 6.4 us, 2.0 TB/s; 32 rows: 6.5 us with the call, a launch's latency.
 // kv_score_k: tiles of up to 32 (token, head) pairs of one sequence and key/value head, their q in LDS as doubles, over a run of
-// pages; hd / 8 lanes hold a page's bounds in registers and go over the tile's rows.
+// pages; hd / 8 lanes hold a page's bounds in registers, all pages of a wave loaded at once, and go over the tile's rows.
+// Where a query's element is negative it meets the page's least, else the greatest: a choice of bits, one product of
+// 64 bits in place of two.  32 x 512 pages of 8 heads of 128: 16.2 us, 2.6 TB/s (a table entry and a page's bounds read for one
+// step at a time: 24.8); bound by the 64-bit sums' chains and the pages' latency.
 // kv_pick_k: a block per row and key/value head finds the score that separates the chosen pages (10 bits of
-// their order at a time, from the first bit in which they differ) and writes the pages in order of position.
+// their order at a time, from the first bit in which they differ) and writes the pages in order of position.  The scores stay
+// in registers, a thread has neighbouring pages: 64 of 2048 pages 7.5 us (read from memory at each step: 14.6), 32 x 8 rows' 32 of
+// 512 4.8 (9.6): steps of a block that wait for one another.
 #include <algorithm>
 
 #include "../runtime/memory_pool.hpp"
@@ -20,8 +26,6 @@
 namespace aic::hip {
 
 namespace {
-
-template <typename T> using Bound = std::conditional_t<std::is_same_v<T, float>, float, bf16>;
 
 // ------------------------------------------------------------------------------ bounds
 struct BoundArgs {
@@ -42,7 +46,7 @@ __device__ __forceinline__ int touched(const BoundArgs& a, int b, int& first, in
     return n > 0 && len > 0 ? a.kv.page_index(len - 1) - first + 1 : 0;
 }
 
-// EPL neighbouring elements of a key as floats.
+// EPL neighbouring elements of a key as floats; of a NaN group anything, its byte tells.
 template <typename CT, int EPL>
 __device__ __forceinline__ void load_key(const char* p, uint32_t byte, float (&x)[EPL]) {
     if constexpr (kE2<CT>) {
@@ -50,12 +54,9 @@ __device__ __forceinline__ void load_key(const char* p, uint32_t byte, float (&x
         const float s = exp_scale(byte);
         e2m1_floats(w.x, s, reinterpret_cast<float(&)[8]>(x[0]));
         e2m1_floats(w.y, s, reinterpret_cast<float(&)[8]>(x[8]));
-        if (byte == kNanGroup)
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) x[j] = NAN;
     } else if constexpr (kE4<CT>) {
         uint4 w = *reinterpret_cast<const uint4*>(p);
-        if (byte >= kTopByte) w = e4m3_in_range(w, byte);
+        if (__builtin_expect(byte >= kTopByte, 0)) w = e4m3_in_range(w, byte);
         const float s = exp_scale(byte);
         e4m3_floats(make_uint2(w.x, w.y), s, reinterpret_cast<float(&)[8]>(x[0]));
         e4m3_floats(make_uint2(w.z, w.w), s, reinterpret_cast<float(&)[8]>(x[8]));
@@ -67,34 +68,36 @@ __device__ __forceinline__ void load_key(const char* p, uint32_t byte, float (&x
     }
 }
 
-// The first one's NaN or the second's.
-__device__ __forceinline__ float least(float x, float y) { return x < y || x != x ? x : y; }
-__device__ __forceinline__ float most(float x, float y) { return x > y || x != x ? x : y; }
+// f, idempotent, over the lanes that stand at the same place of their groups of L.
+template <int L, typename F>
+__device__ __forceinline__ float across_groups(float x, F f) {
+    if constexpr (L <= 8) x = f(x, dpp<0x128>(x));  // row_ror 8, 4, 2
+    if constexpr (L <= 4) x = f(x, dpp<0x124>(x));
+    if constexpr (L <= 2) x = f(x, dpp<0x122>(x));
+    if constexpr (L <= 16) x = facing_op<16>(x, f);
+    return facing_op<32>(x, f);
+}
 
 template <typename CT, int HD>
 __global__ __launch_bounds__(kBlock) void kv_bounds_k(BoundArgs a) {
-    constexpr int EPL = kE2<CT> ? 16 : kPer16<CT>, L = HD / EPL, RPS = 64 / L;  // lanes of a key, keys of a step
+    constexpr int EPL = kE2<CT> ? 16 : kPer16<CT>, L = HD / EPL, RPS = 64 / L, U = kE2<CT> || kE4<CT> ? 4 : 8;  // lanes of a key, keys of a step, steps at a time
     const int lane = threadIdx.x & 63;
     const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (w >= a.pages * a.kv.Hkv) return;
     const int kvh = static_cast<int>(w % a.kv.Hkv);
-    int64_t left = w / a.kv.Hkv;
+    double left = static_cast<double>(w / a.kv.Hkv);  // whole numbers below 2^53
     int b = -1, pi = 0, len = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {  // 64 sequences per step, their pages added up across lanes
         int first = 0, n = 0, mine = 0;
         if (b0 + lane < a.B) mine = touched(a, b0 + lane, first, n);
-        int64_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
+        const double upto = wave_running_sum(static_cast<double>(mine));
         const uint64_t past = __ballot(left < upto);
         if (past) {
             const int l = __builtin_ctzll(past);
             b = b0 + l;
-            pi = __shfl(first, l, 64) + static_cast<int>(left - (__shfl(upto, l, 64) - __shfl(mine, l, 64)));
-            len = __shfl(n, l, 64);
+            const int before = static_cast<int>(left - (upto - mine));  // in lane l: of its sequence's pages
+            pi = __builtin_amdgcn_readlane(first, l) + __builtin_amdgcn_readlane(before, l);
+            len = __builtin_amdgcn_readlane(n, l);
             break;
         }
         left -= __shfl(upto, 63, 64);
@@ -105,43 +108,50 @@ __global__ __launch_bounds__(kBlock) void kv_bounds_k(BoundArgs a) {
     const int64_t row0 = (static_cast<int64_t>(page) * a.kv.Hkv + kvh) * a.kv.ps;
     const int filled = static_cast<int>(min(static_cast<int64_t>(a.kv.ps), len - static_cast<int64_t>(pi) * a.kv.ps));
     const int grp = lane / L, d0 = lane % L * EPL;
+    auto least = [](float x, float y) { return __builtin_elementwise_minimum(x, y); };  // a NaN stays
+    auto most = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
     float lo[EPL], hi[EPL];
+    uint32_t top_byte = 0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) lo[j] = INFINITY, hi[j] = -INFINITY;
-    for (int r0 = 0; r0 < filled; r0 += 2 * RPS) {
-        // two keys at a time: past the last one, the last one again
-        float x[2][EPL];
+    for (int r0 = 0; r0 < filled; r0 += U * RPS) {
+        float x[U][EPL];
+        uint32_t byte[U];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t row = row0 + min(r0 + i * RPS + grp, filled - 1);
-            uint32_t byte = 127;
-            if constexpr (kE4<CT>) byte = a.kv.ke[row];
-            if constexpr (kE2<CT>) byte = a.kv.ke[row * (HD / kGroup) + d0 / kGroup];
-            load_key<CT, EPL>(a.kv.kp + row * kRowBytes<CT, HD> + d0 * 16 / kPer16<CT>, byte, x[i]);
+        for (int i = 0; i < U; ++i) {
+            const int64_t row = row0 + min(r0 + i * RPS + grp, filled - 1);  // past the last key: the last one again
+            byte[i] = 127;
+            if constexpr (kE4<CT>) byte[i] = a.kv.ke[row];
+            if constexpr (kE2<CT>) byte[i] = a.kv.ke[row * (HD / kGroup) + d0 / kGroup];
+            top_byte = max(top_byte, byte[i]);
+            load_key<CT, EPL>(a.kv.kp + row * kRowBytes<CT, HD> + d0 * 16 / kPer16<CT>, byte[i], x[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < U; i += 2)
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
-                lo[j] = least(lo[j], x[i][j]);
-                hi[j] = most(hi[j], x[i][j]);
+                lo[j] = least(least(lo[j], x[i][j]), x[i + 1][j]);
+                hi[j] = most(most(hi[j], x[i][j]), x[i + 1][j]);
             }
     }
+    if constexpr (kE2<CT>) {
+        if (top_byte == kNanGroup)
 #pragma unroll
-    for (int o = L; o < 64; o <<= 1)
+            for (int j = 0; j < EPL; ++j) lo[j] = hi[j] = NAN;
+    }
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-            const float x = __shfl_xor(lo[j], o, 64), y = __shfl_xor(hi[j], o, 64);
-            lo[j] = least(lo[j], x);
-            hi[j] = most(hi[j], y);
-        }
-    if (grp == 0) {
-        using BT = Bound<CT>;
-        BT* out = static_cast<BT*>(a.bounds) + (static_cast<int64_t>(page) * a.kv.Hkv + kvh) * 2 * HD + d0;
+    for (int j = 0; j < EPL; ++j) lo[j] = across_groups<L>(lo[j], least), hi[j] = across_groups<L>(hi[j], most);
+    if (grp < 2) {  // one group writes the least, the next one the greatest values; exact: each is a cached value
+        using BT = std::conditional_t<std::is_same_v<CT, float>, float, bf16>;
+        BT* out = static_cast<BT*>(a.bounds) + ((static_cast<int64_t>(page) * a.kv.Hkv + kvh) * 2 + grp) * HD + d0;
+        constexpr int W = 16 / sizeof(BT);
+        typedef BT vec_t __attribute__((ext_vector_type(W)));
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) {  // exact: a bound is a cached value
-            st(out, j, lo[j]);
-            st(out, HD + j, hi[j]);
+        for (int j = 0; j < EPL; j += W) {
+            vec_t y;
+#pragma unroll
+            for (int u = 0; u < W; ++u) y[u] = static_cast<BT>(grp == 0 ? lo[j + u] : hi[j + u]);
+            *reinterpret_cast<vec_t*>(out + j) = y;
         }
     }
 }
@@ -156,8 +166,9 @@ struct SelectArgs {
     int32_t* picked;
     int64_t* picked_lens;
 };
-constexpr int kRows = 32;    // (token, head) pairs of a tile
-constexpr int kRun = 32;     // pages of a block
+constexpr int kRows = 32;       // (token, head) pairs of a tile
+constexpr int kWavePages = 16;  // pages of a wave
+constexpr int kRun = 4 * kWavePages;
 
 __device__ __forceinline__ int pages_of(const PageView& kv, int pos) { return pos < 0 ? 0 : kv.page_index(pos) + 1; }
 
@@ -171,10 +182,48 @@ __device__ __forceinline__ double group_sum(double x) {
     return x;
 }
 
+// Eight elements of a page's bounds, and of them those that a query's signs meet: the least where it is negative.
+template <typename BT> struct Bounds8;
+template <> struct Bounds8<bf16> {
+    uint4 lo, hi;
+    __device__ __forceinline__ void load(const bf16* p, int hd) {
+        lo = *reinterpret_cast<const uint4*>(p);
+        hi = *reinterpret_cast<const uint4*>(p + hd);
+    }
+    __device__ __forceinline__ void meet(const uint32_t (&neg)[8], float (&x)[8]) const {
+        const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t m = (neg[2 * i] & 0xffffu) | (neg[2 * i + 1] & 0xffff0000u), w = (l[i] & m) | (h[i] & ~m);
+            x[2 * i] = __uint_as_float(w << 16);
+            x[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+        }
+    }
+};
+template <> struct Bounds8<float> {
+    uint4 lo[2], hi[2];
+    __device__ __forceinline__ void load(const float* p, int hd) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            lo[i] = reinterpret_cast<const uint4*>(p)[i];
+            hi[i] = reinterpret_cast<const uint4*>(p + hd)[i];
+        }
+    }
+    __device__ __forceinline__ void meet(const uint32_t (&neg)[8], float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t l[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, h[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = __uint_as_float((l[j] & neg[4 * i + j]) | (h[j] & ~neg[4 * i + j]));
+        }
+    }
+};
+
 template <typename T, typename BT, int HD>
 __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
-    constexpr int L = HD / 8, PPS = 64 / L;  // lanes of a page, pages of a wave's step
-    __shared__ __attribute__((aligned(16))) double qs[kRows][HD];
+    constexpr int L = HD / 8, PPS = 64 / L, NS = kWavePages / PPS;  // lanes of a page, pages of a step, steps of a wave
+    // [pair][4][L] of two doubles: a lane's eight elements lie L doubles apart, so that its neighbours read other banks
+    extern __shared__ __attribute__((aligned(16))) double2 qs[];
     const PagedArgs& a = s.a;
     const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, tile = static_cast<int>(blockIdx.x) / Hkv;
     int b, local;
@@ -197,41 +246,69 @@ __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
     const int most_pages = static_cast<int>(min(static_cast<int64_t>(pages_of(a.kv, sq.len - sq.n + t0 + nt - 1)), s.n_pages));
     const int first_run = static_cast<int>(blockIdx.y) * kRun;
     if (most_pages <= s.n_sel || first_run >= most_pages - s.last) return;  // nothing to choose here
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / L, d0 = lane % L * 8;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / L, l = lane % L;
     const int32_t* tr = a.kv.table + b * a.kv.ld_table;
 
     // heads of the group, kRows / tokens at a time (one chunk unless the group is larger than kRows)
     const int per = min(a.G, kRows / tokens);
-    for (int g0 = 0; g0 < a.G; g0 += per) {
-        const int ng = min(per, a.G - g0), rows = nt * ng;
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * HD; i += kBlock) {
-            const int r = i / HD, d = i % HD;
-            qs[r][d] = ld(static_cast<const T*>(a.q) + (sq.row0 + t0 + r / ng) * a.ldq + static_cast<int64_t>(kvh * a.G + g0 + r % ng) * HD, d);
+    for (int64_t run = first_run; run < most_pages; run += static_cast<int64_t>(gridDim.y) * kRun) {
+        const int p0 = static_cast<int>(run) + wave * kWavePages;
+        const int own = p0 + lane;
+        const int id = lane < kWavePages && own < most_pages && own < a.kv.ld_table ? tr[own] : -1;
+        Bounds8<BT> bd[NS];
+        bool valid[NS];
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            const int page = __shfl(id, k * PPS + grp, 64);
+            valid[k] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages);
+            bd[k].load(static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid[k] ? page : 0) * Hkv + kvh) * 2 * HD + l * 8, HD);
         }
-        __syncthreads();
-        for (int64_t p0 = first_run; p0 < most_pages; p0 += static_cast<int64_t>(gridDim.y) * kRun)
-        for (int p = static_cast<int>(p0) + wave * PPS + grp; p - grp < min(static_cast<int>(p0) + kRun, most_pages); p += 4 * PPS) {
-            const int page = p < most_pages && p < a.kv.ld_table ? tr[p] : -1;
-            const bool valid = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages);
-            const BT* bp = static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid ? page : 0) * Hkv + kvh) * 2 * HD + d0;
-            double lo[8], hi[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lo[j] = ld(bp, j), hi[j] = ld(bp + HD, j);
-            for (int t = 0; t < nt; ++t) {
-                double best = -INFINITY;
-                for (int g = 0; g < ng; ++g) {
-                    const double* q = &qs[t * ng + g][d0];
-                    double sum = 0.0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum = fma(q[j], q[j] >= 0.0 ? hi[j] : lo[j], sum);
-                    sum = group_sum<L>(sum);
-                    best = sum > best || sum != sum ? sum : best;
+        for (int g0 = 0; g0 < a.G; g0 += per) {
+            const int ng = min(per, a.G - g0), rows = nt * ng;
+            if (run != first_run || g0 > 0) __syncthreads();
+            if (run == first_run || a.G > per) {  // else it is there
+                for (int i = threadIdx.x; i < rows * HD; i += kBlock) {
+                    const int r = i / HD, d = i % HD;
+                    const float x = ld(static_cast<const T*>(a.q) + (sq.row0 + t0 + r / ng) * a.ldq + static_cast<int64_t>(kvh * a.G + g0 + r % ng) * HD, d);
+                    reinterpret_cast<double*>(qs)[r * HD + ((d & 7) >> 1) * (2 * L) + (d >> 3) * 2 + (d & 1)] = x;
                 }
-                if (best != best || !valid) best = INFINITY;  // also a page that is none: chosen, and the row's attention is NaN
-                if (lane % L == 0 && p < most_pages) {
-                    double* out = s.scores + ((sq.row0 + t0 + t) * Hkv + kvh) * s.n_pages + p;
-                    *out = g0 > 0 ? fmax(*out, best) : best;
+                __syncthreads();
+            }
+            if (p0 >= most_pages) continue;
+            for (int t = 0; t < nt; ++t) {
+                double best[NS];
+#pragma unroll
+                for (int k = 0; k < NS; ++k) best[k] = -INFINITY;
+                for (int g = 0; g < ng; ++g) {
+                    double q[8];
+                    uint32_t neg[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const double2 x = qs[(t * ng + g) * (HD / 2) + j * L + l];
+                        q[2 * j] = x.x, q[2 * j + 1] = x.y;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) neg[j] = static_cast<uint32_t>(static_cast<int64_t>(__double_as_longlong(q[j])) >> 63);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) {
+                        float x[8];
+                        bd[k].meet(neg, x);
+                        double sum = 0.0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum = fma(q[j], static_cast<double>(x[j]), sum);
+                        sum = group_sum<L>(sum);
+                        best[k] = sum > best[k] || sum != sum ? sum : best[k];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < NS; ++k) {
+                    // a NaN; a page that is none: chosen, and the row's attention is NaN
+                    if (best[k] != best[k] || !valid[k]) best[k] = INFINITY;
+                    const int p = p0 + k * PPS + grp;
+                    if (l == 0 && p < most_pages) {
+                        double* out = s.scores + ((sq.row0 + t0 + t) * Hkv + kvh) * s.n_pages + p;
+                        *out = g0 > 0 ? fmax(*out, best[k]) : best[k];
+                    }
                 }
             }
         }
@@ -247,22 +324,38 @@ __device__ __forceinline__ uint64_t order(double x) {
 
 constexpr int kBins = 1024;
 
+// K: pages of a thread, neighbouring ones, whose scores it keeps; 0: any number, read from memory each time.
+template <int K>
 __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
     const PagedArgs& a = s.a;
     const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t t = blockIdx.x / static_cast<unsigned>(Hkv), at = t * Hkv + kvh;
-    __shared__ uint32_t bins[kBins];
-    __shared__ uint64_t ends[2][4];
-    __shared__ int sums[2][4];
-    __shared__ int cut_bin, cut_need, cut_count;
+    __shared__ uint4 bins[kBins / 4];
+    __shared__ double ends[2][4];
+    __shared__ int sums[3][4];
+    __shared__ int own_b, own_pos, cut_bin, cut_need, cut_count;
 
-    int b = block_sequence(a.offsets, a.B, t);
-    while (b >= 0 && b < a.B && t >= a.offsets[b + 1]) ++b;
+    const double* scores = s.scores + at * s.n_pages;
+    double kept[K > 0 ? K : 1];
+    if constexpr (K > 0) {  // on their way before the row is known; what lies behind its pages is not used
+#pragma unroll
+        for (int j = 0; j < K; ++j) kept[j] = tid * K + j < s.n_pages ? scores[tid * K + j] : 0.0;
+    }
+    if (tid == 0) own_b = -1, own_pos = -1;
+    __syncthreads();
+    for (int i = tid; i < a.B; i += kBlock) {
+        const int64_t from = a.offsets[i], to = a.offsets[i + 1], len = a.lens[i];
+        if (from <= t && t < to) {
+            const int64_t pos = len - (to - t);
+            own_b = i;
+            own_pos = pos < 0 || pos > kMaxLen ? -1 : static_cast<int>(pos);
+        }
+    }
+    __syncthreads();
+    const bool nobody = own_b < 0;
+    const int pos = own_pos, P = pages_of(a.kv, pos);
     int32_t* out = s.picked + at * s.n_sel;
-    const bool nobody = b < 0 || b >= a.B;
-    const int64_t pos64 = nobody ? -1 : a.lens[b] - (a.offsets[b + 1] - t);
-    const int pos = pos64 < 0 || pos64 > kMaxLen ? -1 : static_cast<int>(pos64), P = pages_of(a.kv, pos);
-    const int32_t* tr = a.kv.table + static_cast<int64_t>(nobody ? 0 : b) * a.kv.ld_table;
+    const int32_t* tr = a.kv.table + static_cast<int64_t>(nobody ? 0 : own_b) * a.kv.ld_table;
     auto id = [&](int p) { return p < a.kv.ld_table ? tr[p] : -1; };
     if (P > s.n_pages) {  // past max_len: a position without a place, so that the row's attention is NaN
         for (int i = tid; i < s.n_sel; i += kBlock) out[i] = -1;
@@ -275,91 +368,104 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
         return;
     }
 
-    const int c0 = s.first, c1 = P - s.last;
-    int need = s.n_sel - s.first - s.last;
-    const double* scores = s.scores + at * s.n_pages;
-    // chosen: order >> shift above `prefix`, and of those at it the first `need`
-    uint64_t lo = ~0ull, hi = 0;
-    for (int p = c0 + tid; p < c1; p += kBlock) {
-        const uint64_t k = order(scores[p]);
-        lo = min(lo, k), hi = max(hi, k);
-    }
+    // a thread's pages [q0, q1), of which those in [c0, c1) are free to choose
+    const int run = K > 0 ? K : (P + kBlock - 1) / kBlock;
+    const int q0 = static_cast<int>(min(static_cast<int64_t>(tid) * run, static_cast<int64_t>(P))), q1 = min(q0 + run, P), c0 = s.first, c1 = P - s.last;
+    [[maybe_unused]] int32_t ids[K > 0 ? K : 1];
+    uint64_t keys[K > 0 ? K : 1];
+    if constexpr (K > 0) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t x = __shfl_xor(static_cast<unsigned long long>(lo), o, 64), y = __shfl_xor(static_cast<unsigned long long>(hi), o, 64);
-        lo = min(lo, x), hi = max(hi, y);
+        for (int j = 0; j < K; ++j) {
+            ids[j] = q0 + j < q1 ? id(q0 + j) : -1;
+            keys[j] = order(kept[j]);
+        }
     }
+    // f(page, its score's order, j) of this thread's pages
+    auto each = [&](auto f) {
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (q0 + j < q1) f(q0 + j, keys[j], j);
+        } else {
+            for (int p = q0; p < q1; ++p) f(p, order(scores[p]), 0);
+        }
+    };
+    auto free = [&](int p) { return p >= c0 && p < c1; };
+
+    // chosen: order >> shift above `prefix`, and of those at it the first `need`
+    int need = s.n_sel - s.first - s.last;
+    double lo = INFINITY, hi = -INFINITY;
+    if constexpr (K > 0) {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            if (q0 + j < q1 && free(q0 + j)) lo = fmin(lo, kept[j]), hi = fmax(hi, kept[j]);
+    } else {
+        for (int p = max(q0, c0); p < min(q1, c1); ++p) lo = fmin(lo, scores[p]), hi = fmax(hi, scores[p]);
+    }
+    lo = wave_all(lo, [](double x, double y) { return fmin(x, y); });
+    hi = wave_all(hi, [](double x, double y) { return fmax(x, y); });
     if (lane == 0) ends[0][wave] = lo, ends[1][wave] = hi;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) lo = min(lo, ends[0][w]), hi = max(hi, ends[1][w]);
-    int shift = lo == hi ? 0 : 64 - __builtin_clzll(lo ^ hi);  // the bits below it differ
-    uint64_t prefix = shift == 64 ? 0 : hi >> shift;
+    for (int w = 0; w < 4; ++w) lo = fmin(lo, ends[0][w]), hi = fmax(hi, ends[1][w]);
+    const uint64_t first_key = order(lo), last_key = order(hi);
+    int shift = first_key == last_key ? 0 : 64 - __builtin_clzll(first_key ^ last_key);  // the bits below it differ
+    uint64_t prefix = shift == 64 ? 0 : last_key >> shift;
     int count = c1 - c0;
     while (shift > 0 && count != need && need > 0) {
         const int next = max(shift - 10, 0), bits = shift - next;
-        for (int i = tid; i < kBins; i += kBlock) bins[i] = 0;
+        bins[tid] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int p = c0 + tid; p < c1; p += kBlock) {
-            const uint64_t k = order(scores[p]);
-            if ((shift == 64 ? 0 : k >> shift) == prefix) atomicAdd(&bins[(k >> next) & ((1u << bits) - 1)], 1u);
-        }
+        each([&](int p, uint64_t k, int) {
+            if (free(p) && (shift == 64 ? 0 : k >> shift) == prefix) atomicAdd(reinterpret_cast<uint32_t*>(bins) + ((k >> next) & ((1u << bits) - 1)), 1u);
+        });
         __syncthreads();
-        if (wave == 0) {
-            // lane l: bins 16 l .. 16 l + 15, from the top
-            uint32_t mine = 0;
+        // from the top: thread i has bins 1023 - 4 i and the three below
+        const uint4 mine = bins[kBins / 4 - 1 - tid];
+        const int total = static_cast<int>(mine.x + mine.y + mine.z + mine.w), upto = wave_running_sum(total);
+        if (lane == 63) sums[2][wave] = upto;
+        __syncthreads();
+        int before = upto - total;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mine += bins[kBins - 1 - (16 * lane + i)];
-            const int upto = wave_running_sum(static_cast<int>(mine)), before = upto - static_cast<int>(mine);
-            if (before < need && need <= upto) {
-                int left = need - before;
-                for (int i = 0; i < 16; ++i) {
-                    const int bin = kBins - 1 - (16 * lane + i), n = static_cast<int>(bins[bin]);
-                    if (left <= n) {
-                        cut_bin = bin, cut_need = left, cut_count = n;
-                        break;
-                    }
-                    left -= n;
-                }
-            }
+        for (int w = 0; w < 3; ++w) before += w < wave ? sums[2][w] : 0;
+        if (before < need && need <= before + total) {
+            const uint32_t n[4] = {mine.w, mine.z, mine.y, mine.x};
+            int left = need - before, i = 0;
+            while (i < 3 && left > static_cast<int>(n[i])) left -= static_cast<int>(n[i++]);
+            cut_bin = kBins - 1 - (4 * tid + i), cut_need = left, cut_count = static_cast<int>(n[i]);
         }
         __syncthreads();
         prefix = shift == 64 ? static_cast<uint64_t>(cut_bin) : prefix << bits | static_cast<uint64_t>(cut_bin);
         need = cut_need, count = cut_count, shift = next;
     }
 
-    // in order of position: a run of pages per thread
-    const int run = (P + kBlock - 1) / kBlock, q0 = min(tid * run, P), q1 = min(q0 + run, P);
-    auto head = [&](int p) { return order(scores[p]) >> shift; };
-    auto free = [&](int p) { return p >= c0 && p < c1; };
+    // in order of position
     int ties = 0, sure = 0;
-    for (int p = q0; p < q1; ++p) {
-        if (!free(p)) {
-            ++sure;
-        } else {
-            const uint64_t h = shift == 64 ? 0 : head(p);
-            ties += h == prefix;
-            sure += h > prefix;
-        }
-    }
+    each([&](int p, uint64_t k, int) {
+        const uint64_t h = shift == 64 ? 0 : k >> shift;
+        ties += free(p) && h == prefix;
+        sure += !free(p) || h > prefix;
+    });
     const int ties_upto = wave_running_sum(ties);
     if (lane == 63) sums[0][wave] = ties_upto;
     __syncthreads();
     int tie = ties_upto - ties;
-    for (int w = 0; w < wave; ++w) tie += sums[0][w];
+#pragma unroll
+    for (int w = 0; w < 3; ++w) tie += w < wave ? sums[0][w] : 0;
     const int mine = sure + min(ties, max(need - tie, 0)), upto = wave_running_sum(mine);
     if (lane == 63) sums[1][wave] = upto;
     __syncthreads();
     int place = upto - mine;
-    for (int w = 0; w < wave; ++w) place += sums[1][w];
-    for (int p = q0; p < q1; ++p) {
+#pragma unroll
+    for (int w = 0; w < 3; ++w) place += w < wave ? sums[1][w] : 0;
+    each([&](int p, uint64_t k, int j) {
         bool take = true;
         if (free(p)) {
-            const uint64_t h = shift == 64 ? 0 : head(p);
+            const uint64_t h = shift == 64 ? 0 : k >> shift;
             take = h > prefix || (h == prefix && tie++ < need);
         }
-        if (take) out[place++] = id(p);
-    }
+        if (take) out[place++] = K > 0 ? ids[j] : id(p);
+    });
     if (tid == 0) s.picked_lens[at] = static_cast<int64_t>(s.n_sel - 1) * a.kv.ps + (pos - (P - 1) * a.kv.ps) + 1;
 }
 
@@ -448,21 +554,25 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
     if (B > 0 && x.n_pages > n_sel) {
         int tokens = 32;
         while (tokens > 1 && (tokens * x.a.G > kRows || tokens / 2 >= std::min(max_q, T))) tokens /= 2;
-        const int64_t tiles = (T + tokens - 1) / tokens + std::min(B, T), runs = (x.n_pages + kRun - 1) / kRun;
+        const int64_t tiles = tokens == 1 ? T : (T + tokens - 1) / tokens + std::min(B, T), runs = (x.n_pages + kRun - 1) / kRun;
         AIC_CHECK(tiles * c.kv_heads <= INT32_MAX, OutOfRange, "kv_select: too many rows in one call");
         const dim3 grid(static_cast<unsigned>(tiles * c.kv_heads), static_cast<unsigned>(std::min<int64_t>(runs, 65535)));
         auto run = [&](auto hd) {
             constexpr int D = decltype(hd)::value;
-            if (c.type == DType::Float32) kv_score_k<float, float, D><<<grid, kBlock, 0, s>>>(x, tokens);
-            else if (dt == DType::Float32) kv_score_k<float, bf16, D><<<grid, kBlock, 0, s>>>(x, tokens);
-            else kv_score_k<bf16, bf16, D><<<grid, kBlock, 0, s>>>(x, tokens);
+            const size_t lds = static_cast<size_t>(tokens * std::min(x.a.G, kRows / tokens)) * D * sizeof(double);  // at most 32 KB
+            if (c.type == DType::Float32) kv_score_k<float, float, D><<<grid, kBlock, lds, s>>>(x, tokens);
+            else if (dt == DType::Float32) kv_score_k<float, bf16, D><<<grid, kBlock, lds, s>>>(x, tokens);
+            else kv_score_k<bf16, bf16, D><<<grid, kBlock, lds, s>>>(x, tokens);
         };
         if (c.head_dim == 32) run(std::integral_constant<int, 32>{});
         else if (c.head_dim == 64) run(std::integral_constant<int, 64>{});
         else run(std::integral_constant<int, 128>{});
         AIC_LAUNCH_CHECK("kv_select scores");
     }
-    kv_pick_k<<<static_cast<unsigned>(picks), kBlock, 0, s>>>(x);
+    const auto grid = static_cast<unsigned>(picks);
+    if (x.n_pages <= 2 * kBlock) kv_pick_k<2><<<grid, kBlock, 0, s>>>(x);
+    else if (x.n_pages <= 8 * kBlock) kv_pick_k<8><<<grid, kBlock, 0, s>>>(x);
+    else kv_pick_k<0><<<grid, kBlock, 0, s>>>(x);
     AIC_LAUNCH_CHECK("kv_select");
 }
 
