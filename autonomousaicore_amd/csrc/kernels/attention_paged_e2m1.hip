@@ -391,14 +391,18 @@ __device__ __forceinline__ bool few4_part(const FewArgs<A>& f, const Part& pt, f
                     }
                 }
                 const char* none = reinterpret_cast<const char*>(&kNoPage);
-                constexpr int CH = L::CODES / 16;  // chunks of a tile; K's and then V's, 64 to a copy
-#pragma unroll 1
-                for (int i = 0; i < 2 * CH / 64; ++i) {
-                    const int u = i * 64 + fl, uk = u % CH, rr = uk / NC;
-                    const int64_t row = row_at(k0 + rr);
-                    dma16(row >= 0 ? (u < CH ? a.kv.kp : a.kv.vp) + row * RB + ((uk % NC ^ P::swz4(rr)) << 4) : none, dst + i * 1024);
-                }
                 const int64_t row = row_at(k0 + (fl & 31));
+                if constexpr (NC == 1) {  // one copy, K's by half of the lanes
+                    dma16(row >= 0 ? (fl < 32 ? a.kv.kp : a.kv.vp) + row * RB : none, dst);
+                } else {
+#pragma unroll(R == 16 ? 2 : 1)
+                    for (int i = 0; i < L::CODES / 1024; ++i) {
+                        const int rr = (i * 64 + fl) / NC;
+                        const int64_t at_row = row_at(k0 + rr), off = at_row * RB + ((fl % NC ^ P::swz4(rr)) << 4);
+                        dma16(at_row >= 0 ? a.kv.kp + off : none, dst + i * 1024);
+                        dma16(at_row >= 0 ? a.kv.vp + off : none, dst + L::CODES + i * 1024);
+                    }
+                }
                 dma_exps<HD>(row >= 0 ? reinterpret_cast<const char*>(fl >> 5 ? a.kv.ve : a.kv.ke) + row * NC : none, dst + 2 * L::CODES);
             };
             wait_vmcnt<0>();  // Q is there: left to the compiler, which does not count the copies, it would be waited for with all of them, at every tile
