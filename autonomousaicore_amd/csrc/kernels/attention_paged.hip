@@ -439,9 +439,9 @@ int64_t parts_bytes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64
     // the cache's type does not tell the queries' (codes serve both): room for either
     int64_t n = 0;
     const int64_t G = H / c.kv_heads;
-    const bool few = picked || few_rows(max_q, G, c.head_dim, c.type);
+    const bool few = picked || few_rows(B * c.kv_heads, max_q, max_len, G, c.head_dim, c.type);
     if (c.type != DType::Float32 && few)
-        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, c.type);
+        n = few_workspace(B, c.kv_heads, max_q, max_len, G, c.head_dim, c.type, picked);
     if (c.type != DType::Float32 && !few)
         n = plan_bytes(plan(B, T, max_len, H, c, 128), T, H, c.head_dim);
     if (c.type != DType::BFloat16)
@@ -465,7 +465,7 @@ void attend(A& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t
     a.vec_q = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq * size % 16 == 0;
     a.vec_o = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.ldo * size % 16 == 0;
 
-    const bool few = dt == DType::BFloat16 && (picked || few_rows(max_q, a.G, c.head_dim, c.type));
+    const bool few = dt == DType::BFloat16 && (picked || few_rows(B * c.kv_heads, max_q, max_len, a.G, c.head_dim, c.type));
     const int64_t R = dt == DType::BFloat16 ? 128 : f32_rows(B, T, max_q, max_len, H, c.kv_heads, c.head_dim, picked);
     Plan p = plan(B, T, max_len, H, c, R);
     const int64_t need = parts_bytes(c, B, T, max_q, max_len, H, picked);
@@ -480,7 +480,7 @@ void attend(A& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t
     if (need == 0) workspace = nullptr;
     if (few) {
         // need may be the other kernel's alone
-        const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, c.type) > 0;
+        const bool shares = few_workspace(B, c.kv_heads, max_q, max_len, a.G, c.head_dim, c.type, picked) > 0;
         attn_paged_few(a, max_q, c.type, static_cast<int>(c.head_dim), shares ? workspace : nullptr, s);
         return;
     }

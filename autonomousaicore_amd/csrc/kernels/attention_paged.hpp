@@ -350,8 +350,8 @@ void by_cache_type(DType type, F&& f) {
 
 // Few query rows per key/value head, bf16 queries (attention_paged_few.hip): row groups of `group` rows; with a
 // workspace the batch's keys are cut into equal shares, one per resident block.
-bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, DType type);
-int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type);
+bool few_rows(int64_t pairs, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type);
+int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type, bool picked);
 template <typename A>
 void attn_paged_few(const A& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s);
 

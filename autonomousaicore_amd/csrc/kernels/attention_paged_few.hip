@@ -426,17 +426,33 @@ int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * 
 // undivided group 0.3 us (head_dim 64) to 0.7 us (128).  One sequence of 1600 tokens, shares and whole: 13.3 and
 // 11.9 us with 12 heads of 64, 15.9 and 20.8 us with 8 of 128; of 2048: 13.3 and 13.9, 16.1 and 23.9 us.  With a group
 // for most CUs nothing is won by dividing up to 2048: 32 sequences with 8 heads of 128, 47.6 and 42.8 us.
-int64_t whole_len(int64_t pairs, int64_t head_dim) { return pairs >= 192 ? 2048 : head_dim < 128 ? 1536 : 1024; }
+// e2m1, whose tiles take less time to come: 32 sequences of 4096, 36.0 in shares and 32.5 us whole; 64 of them 54.3 and 55.7.
+// Rows with pages of their own are all of the same length, so that blocks that fill a round of the card end together:
+// 256 of 8192 tokens of 128, bf16 188.2 and 184.5 us, e2m1 64.2 and 60.3; 2600 of 4096, 946 and 525 us (shares take neighbouring
+// rows' pages from each other's cache); 128 of 4096, bf16 50.3 and 46.9, e2m1 30.1 and 31.7; of 8192, 102.1 and
+// 102.3, 46.1 and 55.0; but 288 of 4096, a round and a little, 113.4 and 135.9, 45.8 and 55.4; 384 of 8192 278 and 279, 99.5 and 108.
+int64_t whole_len(int64_t pairs, int64_t head_dim, DType type, bool picked) {
+    const bool one_round = pairs <= 256;
+    if (picked && (pairs >= 512 || (pairs >= 224 && one_round))) return kMaxLen;
+    if (picked ? pairs >= 128 && one_round : type == DType::UInt4 && head_dim == 128 && pairs >= 192 && one_round) return 4096;
+    return pairs >= 192 && !picked ? 2048 : head_dim < 128 ? 1536 : 1024;
+}
 
 }  // namespace
 
 // One group; or two where the cache is e4m3 and head_dim 128, whose tiles of 128 rows go through registers: 30 sequences of
 // up to 8000 tokens, 16 heads over 2, 64 rows: 41.6 us so, 66.6 us there; one sequence: 22.5 and 26.7 us; 96 rows on
 // up to 4000: 41.1 and 39.1 us.  bf16, 64 rows: 61.6 and 55.5 us; head_dim 64 25.0 and 22.7 us in e4m3.
-bool few_rows(int64_t max_q, int64_t G, int64_t head_dim, DType type) { return max_q * G <= (holds_codes(type) && head_dim == 128 ? 64 : 32); }
+// e2m1: two where there are 200000 keys to read.  64 rows over 8 heads of 128 of 8 sequences of 3000 tokens: 29.2 us so and 28.9 there; of 8000,
+// 41.1 and 48.3; 30 of 1000, 31.2 and 38.0; 16 of 1000, 30.7 and 24.0.  64 rows, 12 heads of 64: 4 of 8000, 27.7 and 33.0;
+// 16 of 1000, 20.3 and 24.3; 8 of 1000, 20.3 and 18.1.
+bool few_rows(int64_t pairs, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type) {
+    const bool two = type == DType::UInt4 ? pairs > 200000 / std::max<int64_t>(max_len, 1) : type == DType::UInt8 && head_dim == 128;
+    return max_q * G <= (two ? 64 : 32);
+}
 
-int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type) {
-    if (max_len <= whole_len(B * Hkv, head_dim)) return 0;
+int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, int64_t G, int64_t head_dim, DType type, bool picked) {
+    if (max_len <= whole_len(B * Hkv, head_dim, type, picked)) return 0;
     return (2 * resident(head_dim, type) * group_of(max_q, G) * (head_dim + 2) * 4 + (B + 1) * 8 + 15) / 16 * 16;
 }
 

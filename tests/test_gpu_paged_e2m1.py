@@ -145,6 +145,14 @@ def test_keys_split_among_blocks(dt, ns, lens, H, Hkv, hd):
         Call(p, H, dt).run(ws[:a.bytes() - 16])
 
 
+@pytest.mark.parametrize("ns,lens,H,Hkv,hd,ps,window", [
+    ([10] * 27, [3900] * 14 + [2700] * 13, 8, 2, 64, 24, 0), ([33, 0] + [40] * 18, [11200] + [9] + [4000] * 18, 1, 1, 128, 16, 700),
+    ([5] * 100, [2003] * 100, 16, 2, 32, 16, 0), ([1] * 200, [4090, 1] * 100, 2, 1, 128, 32, 0)])
+def test_batches_with_many_keys(ns, lens, H, Hkv, hd, ps, window):
+    """Two groups of rows over one cache, divided and whole."""
+    Call(Cache(ns, lens, Hkv, hd, ps, "e2m1", seed=hd), H, "bf16", window).run().check()
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("n,L,H,Hkv,hd,ps", [(1, 300, 8, 1, 128, 16), (1, 2000, 1, 1, 64, 24), (40, 100, 2, 1, 64, 16), (150, 400, 2, 1, 128, 64),
                                              (3, 700, 2, 1, 32, 8)])

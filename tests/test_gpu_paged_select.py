@@ -321,6 +321,14 @@ def test_chosen_pages_split_among_blocks(dt, cache, T, H, Hkv, hd, n_sel):
 
 
 @pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("T,H,Hkv,hd", [(17, 8, 8, 64), (30, 16, 8, 32), (38, 8, 8, 64), (75, 16, 8, 32)])
+def test_chosen_pages_of_many_rows(dt, cache, T, H, Hkv, hd):
+    """A block for each row and head, and blocks that share more rows than they have threads."""
+    p = Cache([1], [16 * 110], Hkv, hd, 16, cache, seed=T)
+    Picked(p, H, dt, *_random_pages(p, T, 105, T)).run().check()
+
+
+@pytest.mark.parametrize("dt,cache", TYPES)
 def test_chosen_pages_that_are_none(dt, cache):
     p = Cache([1], [400], 2, 64, 16, cache, seed=3)
     picked, lens = _random_pages(p, 6, 10, 1)
