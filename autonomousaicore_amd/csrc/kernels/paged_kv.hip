@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kBlock) void kv_write_k(PageView pv, Cut c, const T
 }
 
 // Elements of a unit of kv_read: 16 bytes of the cache, of e2m1 half as many (32 elements, four stores 64 bytes apart, would
-// leave a store's lanes 16 bytes of every 64: 8 x 2048 rows of 8 heads of 128 21.0 us for 14.5, 5.9 TB/s).
+// leave a store's lanes 16 bytes of every 64: prompts of 8 x 2048 rows of 8 heads of 128 21.0 us for 14.5, 3.8 TB/s).
 template <typename CT> constexpr int kRead = kE2<CT> ? 16 : kPer16<CT>;
 
 // Appending with the rotation on the way: a unit is 16 elements of a head, i .. i + 7 of its first half and the same of its second,

@@ -1,19 +1,19 @@
 // Choosing pages of a long cache for each query: bounds of the pages' keys, and the pages whose bounds promise most.
 //
 // bounds[page][kvh] holds, for each element, the least and the greatest value of the page's keys.  For a query q no key
-// of the page has more than sum_d max(q_d lo_d, q_d hi_d); a row's score of a page is the largest of
+// of the page has more than sum_d q_d (hi_d where q_d >= 0, else lo_d); a row's score of a page is the largest of
 // its group's heads' sums.  Scores are compared with one another, so they are added in 64 bits, where a bf16
 // product is exact and equal sums come out equal in any order that their digits allow: the choice does not
 // depend on how the sum is cut.
 //
 // kv_bounds_k: a wave per page and key/value head that the batch's rows touch; lanes hold 16 bytes of a key (8 of codes), the
-// wave's groups of lanes go over the keys in turn, with several loads in flight, and are joined at the end.  8 x 2048 e2m1 rows
-// of 8 heads of 128: 6.4 us, 2.0 TB/s; 32 rows: 6.5 us with the call, a launch's latency.
+// wave's groups of lanes go over the keys in turn, with several loads in flight, and are joined at the end.  Prompts of 8 x 4096
+// e2m1 rows of 8 heads of 128: 6.4 us, 2.0 TB/s; 32 rows: 6.5 us with the call, a launch's latency.
 // kv_score_k: tiles of up to 32 (token, head) pairs of one sequence and key/value head, their q in LDS as doubles, over a run of
 // pages; hd / 8 lanes hold a page's bounds in registers, all pages of a wave loaded at once, and go over the tile's rows.
 // Where a query's element is negative it meets the page's least, else the greatest: a choice of bits, one product of
-// 64 bits in place of two.  32 x 512 pages of 8 heads of 128: 16.2 us, 2.6 TB/s (a table entry and a page's bounds read for one
-// step at a time: 24.8); bound by the 64-bit sums' chains and the pages' latency.
+// 64 bits in place of two.  Sequences of 32 x 512 pages, 8 heads of 128: 13.9 us, 3.1 TB/s (a table entry and a page's bounds read for
+// one step at a time: 24.8); bound by the chain of loads from the batch's offsets to the pages.
 // kv_pick_k: a block per row and key/value head finds the score that separates the chosen pages (10 bits of
 // their order at a time, from the first bit in which they differ) and writes the pages in order of position.  The scores stay
 // in registers, a thread has neighbouring pages: 64 of 2048 pages 7.5 us (read from memory at each step: 14.6), 32 x 8 rows' 32 of
@@ -167,8 +167,6 @@ struct SelectArgs {
     int64_t* picked_lens;
 };
 constexpr int kRows = 32;       // (token, head) pairs of a tile
-constexpr int kWavePages = 16;  // pages of a wave
-constexpr int kRun = 4 * kWavePages;
 
 __device__ __forceinline__ int pages_of(const PageView& kv, int pos) { return pos < 0 ? 0 : kv.page_index(pos) + 1; }
 
@@ -219,9 +217,11 @@ template <> struct Bounds8<float> {
     }
 };
 
-template <typename T, typename BT, int HD>
+// NS: steps of a wave over its pages, all loaded at once.
+template <typename T, typename BT, int HD, int NS>
 __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
-    constexpr int L = HD / 8, PPS = 64 / L, NS = kWavePages / PPS;  // lanes of a page, pages of a step, steps of a wave
+    constexpr int L = HD / 8, PPS = 64 / L;                 // lanes of a page, pages of a step
+    constexpr int kWavePages = NS * PPS, kRun = 4 * kWavePages;
     // [pair][4][L] of two doubles: a lane's eight elements lie L doubles apart, so that its neighbours read other banks
     extern __shared__ __attribute__((aligned(16))) double2 qs[];
     const PagedArgs& a = s.a;
@@ -251,10 +251,11 @@ __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
 
     // heads of the group, kRows / tokens at a time (one chunk unless the group is larger than kRows)
     const int per = min(a.G, kRows / tokens);
-    for (int64_t run = first_run; run < most_pages; run += static_cast<int64_t>(gridDim.y) * kRun) {
+    auto page_id = [&](int64_t p) { return lane < kWavePages && p + lane < most_pages && p + lane < a.kv.ld_table ? tr[p + lane] : -1; };
+    const int64_t stride = static_cast<int64_t>(gridDim.y) * kRun;
+    int id = page_id(first_run + wave * kWavePages);
+    for (int64_t run = first_run; run < most_pages; run += stride) {
         const int p0 = static_cast<int>(run) + wave * kWavePages;
-        const int own = p0 + lane;
-        const int id = lane < kWavePages && own < most_pages && own < a.kv.ld_table ? tr[own] : -1;
         Bounds8<BT> bd[NS];
         bool valid[NS];
 #pragma unroll
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
             valid[k] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages);
             bd[k].load(static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid[k] ? page : 0) * Hkv + kvh) * 2 * HD + l * 8, HD);
         }
+        id = page_id(run + stride + wave * kWavePages);
         for (int g0 = 0; g0 < a.G; g0 += per) {
             const int ng = min(per, a.G - g0), rows = nt * ng;
             if (run != first_run || g0 > 0) __syncthreads();
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
                 for (int i = threadIdx.x; i < rows * HD; i += kBlock) {
                     const int r = i / HD, d = i % HD;
                     const float x = ld(static_cast<const T*>(a.q) + (sq.row0 + t0 + r / ng) * a.ldq + static_cast<int64_t>(kvh * a.G + g0 + r % ng) * HD, d);
-                    reinterpret_cast<double*>(qs)[r * HD + ((d & 7) >> 1) * (2 * L) + (d >> 3) * 2 + (d & 1)] = x;
+                    reinterpret_cast<double*>(qs)[r * HD + ((d & 7) >> 1) * (2 * L) + (d >> 3) * 2 + (d & 1)] = static_cast<double>(x) + 0.0;  // -0 as 0
                 }
                 __syncthreads();
             }
@@ -469,6 +471,9 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
     if (tid == 0) s.picked_lens[at] = static_cast<int64_t>(s.n_sel - 1) * a.kv.ps + (pos - (P - 1) * a.kv.ps) + 1;
 }
 
+// Blocks of kv_score_k: what the card holds at once, four to a CU, which go on to further runs of pages, their ids ahead (a block for every run,
+// two rounds of them: 16.2 us for 13.9).
+constexpr int64_t kScoreBlocks = 1024;
 int64_t longest_pages(const KVPages& c, int64_t max_len) { return (max_len + c.page_size - 1) / c.page_size; }
 
 void check_select(const KVPages& c, int64_t T, int64_t max_len) {
@@ -554,15 +559,23 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
     if (B > 0 && x.n_pages > n_sel) {
         int tokens = 32;
         while (tokens > 1 && (tokens * x.a.G > kRows || tokens / 2 >= std::min(max_q, T))) tokens /= 2;
-        const int64_t tiles = tokens == 1 ? T : (T + tokens - 1) / tokens + std::min(B, T), runs = (x.n_pages + kRun - 1) / kRun;
-        AIC_CHECK(tiles * c.kv_heads <= INT32_MAX, OutOfRange, "kv_select: too many rows in one call");
-        const dim3 grid(static_cast<unsigned>(tiles * c.kv_heads), static_cast<unsigned>(std::min<int64_t>(runs, 65535)));
-        auto run = [&](auto hd) {
-            constexpr int D = decltype(hd)::value;
+        const int64_t tiles = (tokens == 1 ? T : (T + tokens - 1) / tokens + std::min(B, T)) * c.kv_heads;
+        AIC_CHECK(tiles <= INT32_MAX, OutOfRange, "kv_select: too many rows in one call");
+        auto launch = [&](auto hd, auto steps) {
+            constexpr int D = decltype(hd)::value, NS = decltype(steps)::value, per = 4 * NS * (512 / D);
             const size_t lds = static_cast<size_t>(tokens * std::min(x.a.G, kRows / tokens)) * D * sizeof(double);  // at most 32 KB
-            if (c.type == DType::Float32) kv_score_k<float, float, D><<<grid, kBlock, lds, s>>>(x, tokens);
-            else if (dt == DType::Float32) kv_score_k<float, bf16, D><<<grid, kBlock, lds, s>>>(x, tokens);
-            else kv_score_k<bf16, bf16, D><<<grid, kBlock, lds, s>>>(x, tokens);
+            const int64_t runs = (x.n_pages + per - 1) / per, most = std::max<int64_t>(kScoreBlocks / tiles, 1);
+            const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>({runs, most, 65535})));
+            if (c.type == DType::Float32) kv_score_k<float, float, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
+            else if (dt == DType::Float32) kv_score_k<float, bf16, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
+            else kv_score_k<bf16, bf16, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
+        };
+        auto run = [&](auto hd) {
+            // 16 pages of a wave; one step's where that would leave CUs without a block: 2048 pages of 2 heads, 64 blocks 8.9, 256 7.1 us;
+            // of 256 sequences and heads, one step's 24.8
+            constexpr int NS = decltype(hd)::value / 32;
+            if (NS > 1 && tiles * ((x.n_pages + 63) / 64) < 256) launch(hd, std::integral_constant<int, 1>{});
+            else launch(hd, std::integral_constant<int, NS>{});
         };
         if (c.head_dim == 32) run(std::integral_constant<int, 32>{});
         else if (c.head_dim == 64) run(std::integral_constant<int, 64>{});

@@ -341,7 +341,7 @@ int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* of
 /* The choice: a row at position pos has P = pos / page_size + 1 pages and takes, for each key/value head, all of them if they are at
  * most n_sel, and otherwise the first `first` and the last `last` (at least 1: its own) ones and the n_sel - first - last others of the
  * greatest
- *   score = max over the head's query heads of sum_d max(q_d lo_d, q_d hi_d)
+ *   score = max over the head's query heads of sum_d q_d (hi_d where q_d >= 0, else lo_d)
  * which no q . k of the page's keys exceeds; sums in 64 bits, a NaN counts as infinity, ties go to the lower position.
  * q as in aic_hip_attn_paged.  picked [T][kv_heads][n_sel]: the pages' ids in order of position, then -1;
  * picked_lens [T][kv_heads]: the positions in them that the row sees, all but the last page whole.  A row of no sequence:

@@ -162,6 +162,16 @@ def test_what_is_no_number():
     a.run().check()
 
 
+def test_zeros_of_either_sign_beside_infinities():
+    """An element of q that is 0 or -0 meets the page's greatest."""
+    p = Cache([3], [900], 1, 32, 8, "bf16", seed=1)
+    a = Choice(p, 2, "bf16", 1, 2, 9)
+    a.q[0, 3], a.q[1, 3], a.q[1, 35], a.q[2, 35] = 0.0, -0.0, -0.0, 0.0
+    a.bounds[p.table[0, 30], 0, 0, 3] = float("-inf")
+    a.bounds[p.table[0, 60], 0, 1, 3] = float("inf")
+    a.run().check()
+
+
 @pytest.mark.parametrize("max_len", [1, 100, 333])
 def test_longer_than_promised(max_len):
     """Rows past max_len get a page that is none; the others are right, and nothing is written past the workspace."""
