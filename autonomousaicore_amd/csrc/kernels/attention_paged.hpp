@@ -165,6 +165,9 @@ __device__ __forceinline__ void part_of_keys(int& k_lo, int& k_hi, int split, in
     if (split + 1 < nsplit) k_hi = lo + 64 * static_cast<int>(n * static_cast<uint32_t>(split + 1) / static_cast<uint32_t>(nsplit));
 }
 
+// What lanes have stored to LDS, for other lanes of the wave: LDS works in order, so this is for the compiler alone.
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // ------------------------------------------------------------------------------- tiles
 // [KT][HD] tiles of T in LDS, 16-byte chunks swizzled per row.
 template <typename T, int HD>

@@ -34,8 +34,6 @@ __device__ __forceinline__ void dma_exps(const void* g, const void* lds) {
                      : "s"(__builtin_amdgcn_readfirstlane(l)), "v"(g)
                      : "memory", "m0");
 }
-// What lanes have stored to LDS, for other lanes of the wave: LDS works in order, so this is for the compiler alone.
-__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
 // Whether one of four bytes is 255.
 __device__ __forceinline__ bool any_nan_group(uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; }
 

@@ -14,6 +14,7 @@
 // Where a query's element is negative it meets the page's least, else the greatest: a choice of bits, one product of
 // 64 bits in place of two.  Sequences of 32 x 512 pages, 8 heads of 128: 13.9 us, 3.1 TB/s (a table entry and a page's bounds read for
 // one step at a time: 24.8); bound by the chain of loads from the batch's offsets to the pages.
+// kv_score_many_k: the same for chunks and large groups on the matrix units, also in 64 bits.
 // kv_pick_k: a block per row and key/value head finds the score that separates the chosen pages (10 bits of
 // their order at a time, from the first bit in which they differ) and writes the pages in order of position.  The scores stay
 // in registers, a thread has neighbouring pages: 64 of 2048 pages 7.5 us (read from memory at each step: 14.6), 32 x 8 rows' 32 of
@@ -217,104 +218,220 @@ template <> struct Bounds8<float> {
     }
 };
 
-// NS: steps of a wave over its pages, all loaded at once.
-template <typename T, typename BT, int HD, int NS>
-__global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
-    constexpr int L = HD / 8, PPS = 64 / L;                 // lanes of a page, pages of a step
-    constexpr int kWavePages = NS * PPS, kRun = 4 * kWavePages;
-    // [pair][4][L] of two doubles: a lane's eight elements lie L doubles apart, so that its neighbours read other banks
-    extern __shared__ __attribute__((aligned(16))) double2 qs[];
+// Tiles of up to kRows (token, head) pairs of a sequence and key/value head.
+struct ScoreTile {
+    Seq sq;
+    int b, kvh, t0, nt;  // first token and their number
+    int pages;           // that the last of them has, in the workspace's scores
+    int per;             // heads of the group at a time: all of them, unless they are more than kRows
+};
+// Tiles of `tokens` tokens; false: none, or nothing to choose from page `first` on.
+__device__ __forceinline__ bool score_tile(const SelectArgs& s, int tokens, int first, ScoreTile& x) {
     const PagedArgs& a = s.a;
-    const int Hkv = a.kv.Hkv, kvh = static_cast<int>(blockIdx.x) % Hkv, tile = static_cast<int>(blockIdx.x) / Hkv;
-    int b, local;
-    {
-        // tiles of `tokens` tokens: find_tile counts rows of one head
-        PagedArgs one = a;
-        one.G = 1;
-        bool found;
-        if (tokens == 32) found = find_tile<32>(one, tile, b, local);
-        else if (tokens == 16) found = find_tile<16>(one, tile, b, local);
-        else if (tokens == 8) found = find_tile<8>(one, tile, b, local);
-        else if (tokens == 4) found = find_tile<4>(one, tile, b, local);
-        else if (tokens == 2) found = find_tile<2>(one, tile, b, local);
-        else found = find_tile<1>(one, tile, b, local);
-        if (!found) return;
+    const int Hkv = a.kv.Hkv, tile = static_cast<int>(blockIdx.x) / Hkv;
+    x.kvh = static_cast<int>(blockIdx.x) % Hkv;
+    PagedArgs one = a;  // find_tile counts rows of one head
+    one.G = 1;
+    int local;
+    bool found;
+    if (tokens == 32) found = find_tile<32>(one, tile, x.b, local);
+    else if (tokens == 16) found = find_tile<16>(one, tile, x.b, local);
+    else if (tokens == 8) found = find_tile<8>(one, tile, x.b, local);
+    else if (tokens == 4) found = find_tile<4>(one, tile, x.b, local);
+    else if (tokens == 2) found = find_tile<2>(one, tile, x.b, local);
+    else found = find_tile<1>(one, tile, x.b, local);
+    if (!found) return false;
+    x.sq = wave_sequence(a, x.b);
+    x.t0 = local * tokens, x.nt = min(tokens, x.sq.n - x.t0);
+    x.per = min(a.G, kRows / tokens);
+    // rows past the workspace's pages have no scores (kv_pick_k)
+    x.pages = static_cast<int>(min(static_cast<int64_t>(pages_of(a.kv, x.sq.len - x.sq.n + x.t0 + x.nt - 1)), s.n_pages));
+    return x.pages > s.n_sel && first < x.pages - s.last;
+}
+// The tile's queries of heads g0 .. g0 + ng of the group, row (token, head): [row][4][L] of two doubles, the rows' starts
+// 16 bytes apart in the banks: a lane's eight neighbouring elements lie L doubles apart, and the same element of other rows in others.
+template <int HD> constexpr int kQueryRow = HD / 2 + 1;
+template <int HD> __device__ __forceinline__ int query_at(int d) { return ((d & 7) >> 1) * (HD / 8) + (d >> 3); }
+template <typename T, int HD>
+__device__ __forceinline__ void stage_queries(const SelectArgs& s, const ScoreTile& x, int g0, int ng, double2* qs) {
+    const PagedArgs& a = s.a;
+    for (int i = threadIdx.x; i < x.nt * ng * HD; i += kBlock) {
+        const int r = i / HD, d = i % HD, t = r / ng;
+        const float y = ld(static_cast<const T*>(a.q) + (x.sq.row0 + x.t0 + t) * a.ldq + static_cast<int64_t>(x.kvh * a.G + g0 + r - t * ng) * HD, d);
+        reinterpret_cast<double*>(qs + r * kQueryRow<HD> + query_at<HD>(d))[d & 1] = static_cast<double>(y) + 0.0;  // -0 as 0
     }
-    const Seq sq = wave_sequence(a, b);
-    const int t0 = local * tokens, nt = min(tokens, sq.n - t0);
-    // the last row's pages; rows past the workspace's have no scores (kv_pick_k)
-    const int most_pages = static_cast<int>(min(static_cast<int64_t>(pages_of(a.kv, sq.len - sq.n + t0 + nt - 1)), s.n_pages));
-    const int first_run = static_cast<int>(blockIdx.y) * kRun;
-    if (most_pages <= s.n_sel || first_run >= most_pages - s.last) return;  // nothing to choose here
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / L, l = lane % L;
-    const int32_t* tr = a.kv.table + b * a.kv.ld_table;
+}
+// A page's score over the group's heads; best: over those of this chunk of them.
+__device__ __forceinline__ void put_score(const SelectArgs& s, const ScoreTile& x, int t, int p, double best, bool valid, bool first_chunk) {
+    // a NaN; a page that is none: chosen, and the row's attention is NaN
+    if (best != best || !valid) best = INFINITY;
+    double* out = s.scores + ((x.sq.row0 + x.t0 + t) * s.a.kv.Hkv + x.kvh) * s.n_pages + p;
+    *out = first_chunk ? best : fmax(*out, best);
+}
 
-    // heads of the group, kRows / tokens at a time (one chunk unless the group is larger than kRows)
-    const int per = min(a.G, kRows / tokens);
-    auto page_id = [&](int64_t p) { return lane < kWavePages && p + lane < most_pages && p + lane < a.kv.ld_table ? tr[p + lane] : -1; };
-    const int64_t stride = static_cast<int64_t>(gridDim.y) * kRun;
-    int id = page_id(first_run + wave * kWavePages);
-    for (int64_t run = first_run; run < most_pages; run += stride) {
-        const int p0 = static_cast<int>(run) + wave * kWavePages;
-        Bounds8<BT> bd[NS];
-        bool valid[NS];
+// A wave's NS steps of pages, all loaded at once.
+template <typename BT, int HD, int NS>
+struct ScorePages {
+    static constexpr int L = HD / 8, PPS = 64 / L, PAGES = NS * PPS;  // lanes of a page, pages of a step and in all
+    Bounds8<BT> bd[NS];
+    bool valid[NS];
+    __device__ __forceinline__ void load(const SelectArgs& s, const ScoreTile& x, int id) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
-            const int page = __shfl(id, k * PPS + grp, 64);
-            valid[k] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.kv.n_pages);
-            bd[k].load(static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid[k] ? page : 0) * Hkv + kvh) * 2 * HD + l * 8, HD);
+            const int page = __shfl(id, k * PPS + lane / L, 64);
+            valid[k] = static_cast<uint32_t>(page) < static_cast<uint32_t>(s.a.kv.n_pages);
+            bd[k].load(static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid[k] ? page : 0) * s.a.kv.Hkv + x.kvh) * 2 * HD + lane % L * 8, HD);
         }
-        id = page_id(run + stride + wave * kWavePages);
-        for (int g0 = 0; g0 < a.G; g0 += per) {
-            const int ng = min(per, a.G - g0), rows = nt * ng;
-            if (run != first_run || g0 > 0) __syncthreads();
-            if (run == first_run || a.G > per) {  // else it is there
-                for (int i = threadIdx.x; i < rows * HD; i += kBlock) {
-                    const int r = i / HD, d = i % HD;
-                    const float x = ld(static_cast<const T*>(a.q) + (sq.row0 + t0 + r / ng) * a.ldq + static_cast<int64_t>(kvh * a.G + g0 + r % ng) * HD, d);
-                    reinterpret_cast<double*>(qs)[r * HD + ((d & 7) >> 1) * (2 * L) + (d >> 3) * 2 + (d & 1)] = static_cast<double>(x) + 0.0;  // -0 as 0
+    }
+    __device__ __forceinline__ void score(const SelectArgs& s, const ScoreTile& x, const double2* qs, int p0, int g0, int ng) const {
+        const int lane = threadIdx.x & 63, l = lane % L;
+        for (int t = 0; t < x.nt; ++t) {
+            double best[NS];
+#pragma unroll
+            for (int k = 0; k < NS; ++k) best[k] = -INFINITY;
+            for (int g = 0; g < ng; ++g) {
+                double q[8];
+                uint32_t neg[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double2 y = qs[(t * ng + g) * kQueryRow<HD> + j * L + l];
+                    q[2 * j] = y.x, q[2 * j + 1] = y.y;
                 }
-                __syncthreads();
-            }
-            if (p0 >= most_pages) continue;
-            for (int t = 0; t < nt; ++t) {
-                double best[NS];
 #pragma unroll
-                for (int k = 0; k < NS; ++k) best[k] = -INFINITY;
-                for (int g = 0; g < ng; ++g) {
-                    double q[8];
-                    uint32_t neg[8];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const double2 x = qs[(t * ng + g) * (HD / 2) + j * L + l];
-                        q[2 * j] = x.x, q[2 * j + 1] = x.y;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) neg[j] = static_cast<uint32_t>(static_cast<int64_t>(__double_as_longlong(q[j])) >> 63);
-#pragma unroll
-                    for (int k = 0; k < NS; ++k) {
-                        float x[8];
-                        bd[k].meet(neg, x);
-                        double sum = 0.0;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) sum = fma(q[j], static_cast<double>(x[j]), sum);
-                        sum = group_sum<L>(sum);
-                        best[k] = sum > best[k] || sum != sum ? sum : best[k];
-                    }
-                }
+                for (int j = 0; j < 8; ++j) neg[j] = static_cast<uint32_t>(__double_as_longlong(q[j]) >> 63);
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
-                    // a NaN; a page that is none: chosen, and the row's attention is NaN
-                    if (best[k] != best[k] || !valid[k]) best[k] = INFINITY;
-                    const int p = p0 + k * PPS + grp;
-                    if (l == 0 && p < most_pages) {
-                        double* out = s.scores + ((sq.row0 + t0 + t) * Hkv + kvh) * s.n_pages + p;
-                        *out = g0 > 0 ? fmax(*out, best[k]) : best[k];
-                    }
+                    float y[8];
+                    bd[k].meet(neg, y);
+                    double sum = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum = fma(q[j], static_cast<double>(y[j]), sum);
+                    sum = group_sum<L>(sum);
+                    best[k] = sum > best[k] || sum != sum ? sum : best[k];
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const int p = p0 + k * PPS + lane / L;
+                if (l == 0 && p < x.pages) put_score(s, x, t, p, best[k], valid[k], g0 == 0);
             }
         }
     }
+};
+
+// f(p0, id, g0, ng): the block's runs of 4 * PAGES pages, a wave's first page and its lanes' page ids, for each chunk of heads with its
+// queries staged; load(id) before the queries are.
+template <typename T, int HD, int PAGES, typename Load, typename F>
+__device__ __forceinline__ void over_runs(const SelectArgs& s, const ScoreTile& x, double2* qs, Load load, F f) {
+    const PagedArgs& a = s.a;
+    const int lane = threadIdx.x & 63, mine = static_cast<int>(threadIdx.x >> 6) * PAGES;
+    const int32_t* tr = a.kv.table + x.b * a.kv.ld_table;
+    const int64_t first = static_cast<int64_t>(blockIdx.y) * (4 * PAGES), stride = static_cast<int64_t>(gridDim.y) * (4 * PAGES);
+    auto page_id = [&](int64_t p) { return lane < PAGES && p + lane < x.pages && p + lane < a.kv.ld_table ? tr[p + lane] : -1; };
+    int id = page_id(first + mine);
+    for (int64_t run = first; run < x.pages; run += stride) {
+        const int p0 = static_cast<int>(run) + mine, now = id;
+        load(now);
+        id = page_id(run + stride + mine);
+        for (int g0 = 0; g0 < a.G; g0 += x.per) {
+            const int ng = min(x.per, a.G - g0);
+            if (run == first || a.G > x.per) {  // else they are there
+                if (run != first || g0 > 0) __syncthreads();
+                stage_queries<T, HD>(s, x, g0, ng, qs);
+                __syncthreads();
+            }
+            if (p0 < x.pages) f(p0, now, g0, ng);
+        }
+    }
+}
+
+template <typename T, typename BT, int HD, int NS>
+__global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
+    using P = ScorePages<BT, HD, NS>;
+    extern __shared__ __attribute__((aligned(16))) double2 qs[];
+    ScoreTile x;
+    if (!score_tile(s, tokens, static_cast<int>(blockIdx.y) * (4 * P::PAGES), x)) return;
+    P pages;
+    over_runs<T, HD, P::PAGES>(
+        s, x, qs, [&](int id) { pages.load(s, x, id); }, [&](int p0, int, int g0, int ng) { pages.score(s, x, qs, p0, g0, ng); });
+}
+
+// The same for many pairs, on the matrix units: sum_d of q+ hi and of q- lo, K = 2 HD in 64 bits; 16 pages of a wave, lane
+// (page, quarter of the columns).  An infinite bound would meet the zeros of the other sign: then as above.  512 rows of 32 heads over 8 on
+// 512 pages: 103 us, the matrix units busy 53% of it with two waves to a SIMD (both 16-row tiles of 32 pairs at once, the bounds
+// made 64 bits as they are used: the call 142 us for 114).
+template <typename T, typename BT, int HD>
+__global__ __launch_bounds__(kBlock) void kv_score_many_k(SelectArgs s, int tokens) {
+    using Plain = ScorePages<BT, HD, HD / 32>;
+    static_assert(Plain::PAGES == 16);
+    typedef double f64x4 __attribute__((ext_vector_type(4)));
+    constexpr int C = HD / 4, EV = 16 / sizeof(BT), NV = C / EV;  // columns of a lane, elements of a load, loads
+    extern __shared__ __attribute__((aligned(16))) double2 qs[];
+    ScoreTile x;
+    if (!score_tile(s, tokens, static_cast<int>(blockIdx.y) * 64, x)) return;
+    const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+    double* out = reinterpret_cast<double*>(qs + min(tokens * x.per, kRows) * kQueryRow<HD>) + static_cast<int>(threadIdx.x >> 6) * (kRows * 16);  // [row][16]
+    uint4 lo[NV], hi[NV];
+    bool valid = false;
+    auto load = [&](int id) {
+        const int page = __shfl(id, col, 64);
+        valid = static_cast<uint32_t>(page) < static_cast<uint32_t>(s.a.kv.n_pages);
+        const BT* p = static_cast<const BT*>(s.bounds) + (static_cast<int64_t>(valid ? page : 0) * s.a.kv.Hkv + x.kvh) * 2 * HD + quarter * C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            lo[i] = reinterpret_cast<const uint4*>(p)[i];
+            hi[i] = reinterpret_cast<const uint4*>(p + HD)[i];
+        }
+    };
+    auto value = [](const uint4& w, int j) {  // element j of 16 bytes
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        if constexpr (sizeof(BT) == 4) return static_cast<double>(__uint_as_float(v[j]));
+        else return static_cast<double>(__uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16));
+    };
+    over_runs<T, HD, 16>(s, x, qs, load, [&](int p0, int id, int g0, int ng) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) bad |= non_finite_bits<BT>(lo[i]) | non_finite_bits<BT>(hi[i]);
+        if (__builtin_expect(__ballot(bad != 0) != 0, 0)) {
+            Plain pages;
+            pages.load(s, x, id);
+            pages.score(s, x, qs, p0, g0, ng);
+            return;
+        }
+        // one 16-row tile after the other: the bounds stay in registers in 64 bits
+        const int rows = x.nt * ng;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+            f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+            const double2* q = qs + min(r0 + col, rows - 1) * kQueryRow<HD> + (quarter * C >> 3);
+#pragma unroll
+            for (int d = 0; d < C; d += 2) {
+                const double2 y = q[((d & 7) >> 1) * (HD / 8) + (d >> 3)];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(u ? y.y : y.x));
+                    const uint64_t neg = static_cast<uint64_t>(static_cast<int64_t>(bits) >> 63);
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(__longlong_as_double(static_cast<long long>(bits & neg)), value(lo[(d + u) / EV], (d + u) % EV), acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(__longlong_as_double(static_cast<long long>(bits & ~neg)), value(hi[(d + u) / EV], (d + u) % EV), acc, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[(r0 + 4 * e + quarter) * 16 + col] = acc[e];  // row 4 e + quarter
+        }
+        // lane: page col of every fourth token
+        wave_lds_fence();
+        const int p = p0 + col;
+        for (int t = quarter; t < x.nt; t += 4) {
+            double best = -INFINITY;
+            for (int g = 0; g < ng; ++g) {
+                const double sum = out[(t * ng + g) * 16 + col];
+                best = sum > best || sum != sum ? sum : best;
+            }
+            if (p < x.pages) put_score(s, x, t, p, best, valid, g0 == 0);
+        }
+        wave_lds_fence();
+    });
 }
 
 // -------------------------------------------------------------------------------- pick
@@ -474,6 +591,10 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
 // Blocks of kv_score_k: what the card holds at once, four to a CU, which go on to further runs of pages, their ids ahead (a block for every run,
 // two rounds of them: 16.2 us for 13.9).
 constexpr int64_t kScoreBlocks = 1024;
+// Pairs of a tile from which on the matrix units score them, 16 rows of a product being there in any case.  The call: 512 tokens of 32 heads over 8
+// on 512 pages, 113.7 us and 246.9 with kv_score_k; 2 x 8 tokens, 18.9 and 29.8; a token's 16 heads of a group, 32 sequences, 29.2 and 36.7; its 8, 40.8 and
+// 38.7.
+constexpr int64_t kManyPairs = 9;
 int64_t longest_pages(const KVPages& c, int64_t max_len) { return (max_len + c.page_size - 1) / c.page_size; }
 
 void check_select(const KVPages& c, int64_t T, int64_t max_len) {
@@ -561,18 +682,24 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
         while (tokens > 1 && (tokens * x.a.G > kRows || tokens / 2 >= std::min(max_q, T))) tokens /= 2;
         const int64_t tiles = (tokens == 1 ? T : (T + tokens - 1) / tokens + std::min(B, T)) * c.kv_heads;
         AIC_CHECK(tiles <= INT32_MAX, OutOfRange, "kv_select: too many rows in one call");
+        const int64_t pairs = tokens * std::min(x.a.G, kRows / tokens);
         auto launch = [&](auto hd, auto steps) {
             constexpr int D = decltype(hd)::value, NS = decltype(steps)::value, per = 4 * NS * (512 / D);
-            const size_t lds = static_cast<size_t>(tokens * std::min(x.a.G, kRows / tokens)) * D * sizeof(double);  // at most 32 KB
+            const size_t lds = static_cast<size_t>(pairs) * kQueryRow<D> * sizeof(double2);  // at most 33 KB
             const int64_t runs = (x.n_pages + per - 1) / per, most = std::max<int64_t>(kScoreBlocks / tiles, 1);
             const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(std::min<int64_t>({runs, most, 65535})));
-            if (c.type == DType::Float32) kv_score_k<float, float, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
+            if (NS == D / 32 && pairs >= kManyPairs) {
+                const size_t both = lds + 4 * kRows * 16 * sizeof(double);
+                if (c.type == DType::Float32) kv_score_many_k<float, float, D><<<grid, kBlock, both, s>>>(x, tokens);
+                else if (dt == DType::Float32) kv_score_many_k<float, bf16, D><<<grid, kBlock, both, s>>>(x, tokens);
+                else kv_score_many_k<bf16, bf16, D><<<grid, kBlock, both, s>>>(x, tokens);
+            } else if (c.type == DType::Float32) kv_score_k<float, float, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
             else if (dt == DType::Float32) kv_score_k<float, bf16, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
             else kv_score_k<bf16, bf16, D, NS><<<grid, kBlock, lds, s>>>(x, tokens);
         };
         auto run = [&](auto hd) {
-            // 16 pages of a wave; one step's where that would leave CUs without a block: 2048 pages of 2 heads, 64 blocks 8.9, 256 7.1 us;
-            // of 256 sequences and heads, one step's 24.8
+            // 16 pages of a wave; one step's where that would leave CUs without a block: the call on 2048 pages of 2 heads, 64 blocks
+            // 16.5, 256 13.9 us; 2 x 512 of 8 heads, 128 and 512 blocks, 10.9 and 10.7; 32 of them, 18.9 and 21.2
             constexpr int NS = decltype(hd)::value / 32;
             if (NS > 1 && tiles * ((x.n_pages + 63) / 64) < 256) launch(hd, std::integral_constant<int, 1>{});
             else launch(hd, std::integral_constant<int, NS>{});
@@ -583,6 +710,8 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
         AIC_LAUNCH_CHECK("kv_select scores");
     }
     const auto grid = static_cast<unsigned>(picks);
+    // the call, 2 kept, 8 kept and none: 512 pages, 32 x 8 rows, 19.4, 21.1 and 20.3 us; 2048 pages, 2 rows, 13.9 with 8 and 17.4 without,
+    // 32 x 8 rows 48.0 and 52.0
     if (x.n_pages <= 2 * kBlock) kv_pick_k<2><<<grid, kBlock, 0, s>>>(x);
     else if (x.n_pages <= 8 * kBlock) kv_pick_k<8><<<grid, kBlock, 0, s>>>(x);
     else kv_pick_k<0><<<grid, kBlock, 0, s>>>(x);

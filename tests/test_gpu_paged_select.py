@@ -162,10 +162,26 @@ def test_what_is_no_number():
     a.run().check()
 
 
-def test_zeros_of_either_sign_beside_infinities():
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("ns,lens,H,Hkv,hd,n_sel", [([37, 0, 1, 64], [900, 5, 300, 700], 8, 2, 128, 9), ([100], [800], 20, 1, 64, 12),
+                                                    ([2] * 9, [1100] * 9, 24, 2, 32, 5), ([5, 3], [3000, 2000], 40, 1, 128, 20)])
+def test_choice_of_many_rows(dt, ns, lens, H, Hkv, hd, n_sel):
+    """Chunks, large groups and groups of more than 32 heads; a page with infinities among the others."""
+    p = Cache(ns, lens, Hkv, hd, 16, dt, seed=hd)
+    a = Choice(p, H, dt, 1, 2, n_sel, pad=8, tied=hd == 32)
+    a.run().check()
+    a.bounds[p.table[0, 10], :, 1, 5] = float("inf")
+    a.bounds[p.table[0, 20], 0, 0, 7] = float("-inf")
+    a.bounds[p.table[0, 21], 0, :, 8] = float("nan")
+    a.q[0, 7], a.q[1, 5] = 0.0, -0.0
+    a.run().check()
+
+
+@pytest.mark.parametrize("H", [2, 16])
+def test_zeros_of_either_sign_beside_infinities(H):
     """An element of q that is 0 or -0 meets the page's greatest."""
     p = Cache([3], [900], 1, 32, 8, "bf16", seed=1)
-    a = Choice(p, 2, "bf16", 1, 2, 9)
+    a = Choice(p, H, "bf16", 1, 2, 9)
     a.q[0, 3], a.q[1, 3], a.q[1, 35], a.q[2, 35] = 0.0, -0.0, -0.0, 0.0
     a.bounds[p.table[0, 30], 0, 0, 3] = float("-inf")
     a.bounds[p.table[0, 60], 0, 1, 3] = float("inf")
