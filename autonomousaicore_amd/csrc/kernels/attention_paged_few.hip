@@ -458,7 +458,11 @@ int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, in
 
 template <typename A>
 void attn_paged_few(const A& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s) {
-    FewArgs<A> f{a, static_cast<int>(group_of(max_q, a.G)), 0, nullptr, nullptr, nullptr};
+    // e2m1 and picked pages: shares of two steps where there are few.  One token, 2 heads of 128, 64 pages of 64: 14.0 us so and 15.0 in fours (bf16 14.4 and
+    // 17.0); of 2000 tokens, 13.6 and 15.7; 8 heads, 64 pages, 14.1 and 15.3; but of 32000 tokens, 500 steps, 25.1 and 20.8.  (Other calls keep
+    // their parts, and so their sums' last bits.)
+    const int least = std::is_same_v<A, PickedArgs> || type == DType::UInt4 ? 2 : kLeast;
+    FewArgs<A> f{a, static_cast<int>(group_of(max_q, a.G)), 0, least, nullptr, nullptr, nullptr};
     if (workspace) {
         f.shares = static_cast<int>(resident(head_dim, type));
         f.part_o = static_cast<float*>(workspace);

@@ -11,6 +11,7 @@ struct FewArgs {
     A a;
     int group;         // query rows of a group, at most 32
     int shares;        // 0: a block per sequence and key/value head, nothing divided
+    int least;         // steps of a share at least, of a batch of up to kFewSteps
     int64_t* plan;     // [B + 1], as find_share leaves it
     float2* part_ml;   // [2 shares][group]: a share's first group's, then its last one's
     float* part_o;     // [2 shares][group][hd]
@@ -21,6 +22,7 @@ namespace {
 constexpr int kIds = 512;    // page ids in LDS at a time
 constexpr int kStep = 128;   // keys: a tile for each wave
 constexpr int kLeast = 4;    // steps of a share at least: a part costs a block about as much as three steps
+constexpr int kFewSteps = 256;  // a batch that leaves most CUs without a block even so
 // A sequence's place in the list of steps.
 struct Steps {
     Seq sq;
@@ -35,6 +37,11 @@ __device__ __forceinline__ Steps steps_of(const FewArgs<A>& f, const Seq& sq) {
     x.steps = max(1, (x.sq.len - x.lo + kStep - 1) / kStep);  // also of a sequence without keys: its rows are zeros
     x.groups = (x.sq.n * f.a.G + f.group - 1) / f.group;
     return x;
+}
+// Steps of a share, of `total` in at most `cuts`.
+template <typename A>
+__device__ __forceinline__ int64_t share_of(const FewArgs<A>& f, double total, int cuts) {
+    return max(static_cast<int64_t>(total <= kFewSteps ? f.least : kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
 }
 // Parts of a group of `steps` steps that is cut by itself.
 __device__ __forceinline__ int parts_of(int steps, int64_t share) {
@@ -91,7 +98,7 @@ __device__ __forceinline__ bool find_share(const FewArgs<A>& f, int g, int& b, S
         const double pairs = wave_all(groups, sum);
         const bool by_group = pairs * 4 <= f.shares;
         const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
-        const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
+        const int64_t share = share_of(f, total, cuts);
         if (by_group) {
             size = lane < f.a.B ? parts_of(own.steps, share) * groups : 0.0;
             total = wave_all(size, sum);
@@ -131,7 +138,7 @@ __device__ __forceinline__ bool find_share(const FewArgs<A>& f, int g, int& b, S
     block_scan(mine, sums[0], start, total);
     const bool by_group = pairs * 4 <= f.shares;
     const int cuts = f.shares - (by_group ? static_cast<int>(pairs) : 0);  // every group ends one part early
-    const int64_t share = max(static_cast<int64_t>(kLeast), static_cast<int64_t>((total + cuts - 1) / cuts));
+    const int64_t share = share_of(f, total, cuts);
     auto size = [&] { return (by_group ? parts_of(own.steps, share) : own.steps) * groups(); };
     if (by_group) {
         mine = 0.0;
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs<A> f) {
         any = __any(any);
         M = wave_all(M, [](float p, float q) { return fmaxf(p, q); });
         const float base = M == -INFINITY ? 0.0f : M;
-        constexpr int PL = HD >= 64 ? HD / 64 : 1;
+        constexpr int PL = HD >= 64 ? HD / 64 : 1, kAhead = 8;
         // a part's weight, of its row divided by its own sum
         auto weigh = [&](float2 ml) { return ml.y != 0.0f && ml.y != -1.0f ? __builtin_amdgcn_exp2f((ml.x - base) * a.c) * ml.y : 0.0f; };
         float own = weigh(first), o[PL] = {}, l = own;
@@ -281,24 +288,24 @@ __global__ __launch_bounds__(256) void attn_paged_few_join_k(FewArgs<A> f) {
             if (i0 > 0) own = weigh(state(i0 + lane));
             const float w = own * inv;
             uint64_t left = __ballot(own != 0.0f);
-            while (left) {  // four parts' rows at a time
-                int j[4];
-                float v[4][PL], ws[4];
-                bool live[4];
+            while (left) {  // eight parts' rows at a time
+                int j[kAhead];
+                float v[kAhead][PL], ws[kAhead];
+                bool live[kAhead];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < kAhead; ++k) {
                     live[k] = left != 0;
                     j[k] = live[k] ? __builtin_ctzll(left) : j[k > 0 ? k - 1 : 0];
                     ws[k] = __shfl(w, j[k], 64);
                     left &= left - 1;
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < kAhead; ++k)
 #pragma unroll
                     for (int u = 0; u < PL; ++u)
                         if (lane * PL < HD) v[k][u] = f.part_o[at(i0 + j[k]) * HD + lane * PL + u];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < kAhead; ++k)
 #pragma unroll
                     for (int u = 0; u < PL; ++u) o[u] = live[k] ? fmaf(ws[k], v[k][u], o[u]) : o[u];
             }
