@@ -359,7 +359,7 @@ __global__ __launch_bounds__(kBlock) void kv_score_k(SelectArgs s, int tokens) {
 
 // The same for many pairs, on the matrix units: sum_d of q+ hi and of q- lo, K = 2 HD in 64 bits; 16 pages of a wave, lane
 // (page, quarter of the columns).  An infinite bound would meet the zeros of the other sign: then as above.  512 rows of 32 heads over 8 on
-// 512 pages: 103 us, the matrix units busy 53% of it with two waves to a SIMD (both 16-row tiles of 32 pairs at once, the bounds
+// 512 pages: 103 us, the matrix units busy 58% of it with two waves to a SIMD (both 16-row tiles of 32 pairs at once, the bounds
 // made 64 bits as they are used: the call 142 us for 114).
 template <typename T, typename BT, int HD>
 __global__ __launch_bounds__(kBlock) void kv_score_many_k(SelectArgs s, int tokens) {
