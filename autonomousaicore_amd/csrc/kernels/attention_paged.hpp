@@ -92,10 +92,11 @@ struct Seq {
     int64_t row0;  // first packed row
     int n, len;    // queries, cached keys
 };
-// A picked row stands behind its pages' positions; length -1: nobody's row, left as it is.
+// A picked row stands behind its pages' positions; length -1: nobody's row, left as it is.  Past the pages: one position
+// without a place tells as much as all of them.
 __device__ __forceinline__ Seq sequence(const PickedArgs& a, int b) {
     const int64_t len = a.lens[b];
-    return {static_cast<uint32_t>(b) / static_cast<uint32_t>(a.kv.Hkv), len >= 0, static_cast<int>(min(max(len, int64_t{0}), kMaxLen))};
+    return {static_cast<uint32_t>(b) / static_cast<uint32_t>(a.kv.Hkv), len >= 0, static_cast<int>(min(max(len, int64_t{0}), a.kv.ld_table * a.kv.ps + 1))};
 }
 __device__ __forceinline__ Seq sequence(const PagedArgs& a, int b) {
     const int64_t lo = min(max(a.offsets[b], int64_t{0}), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);

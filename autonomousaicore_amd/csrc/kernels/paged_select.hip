@@ -489,7 +489,8 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
 
     // a thread's pages [q0, q1), of which those in [c0, c1) are free to choose
     const int run = K > 0 ? K : (P + kBlock - 1) / kBlock;
-    const int q0 = static_cast<int>(min(static_cast<int64_t>(tid) * run, static_cast<int64_t>(P))), q1 = min(q0 + run, P), c0 = s.first, c1 = P - s.last;
+    auto at_most = [&](int64_t p) { return static_cast<int>(min(p, static_cast<int64_t>(P))); };
+    const int q0 = at_most(static_cast<int64_t>(tid) * run), q1 = at_most(static_cast<int64_t>(tid + 1) * run), c0 = s.first, c1 = P - s.last;
     [[maybe_unused]] int32_t ids[K > 0 ? K : 1];
     uint64_t keys[K > 0 ? K : 1];
     if constexpr (K > 0) {

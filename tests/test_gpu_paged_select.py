@@ -366,6 +366,44 @@ def test_chosen_pages_that_are_none(dt, cache):
     Picked(p, 4, dt, picked, lens).run().check()
 
 
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("T,n_sel", [(4, 10), (3, 90), (130, 80)])
+def test_lengths_past_the_pages(dt, cache, T, n_sel):
+    """However large: NaN, as one position past them; the other rows as they are."""
+    p = Cache([1], [16 * (n_sel + 2)], 2, 32, 16, cache, seed=3)
+    picked, lens = _random_pages(p, T, n_sel, 1)
+    want = Picked(p, 4, dt, picked, lens).run().o.clone().view(T, 2, 64)
+    lens[1, 0], lens[2, 1] = 2 ** 31, 2 ** 62
+    got = Picked(p, 4, dt, picked, lens).run().o.view(T, 2, 64)
+    past = torch.zeros(T, 2, dtype=torch.bool, device="cuda")
+    past[1, 0] = past[2, 1] = True
+    assert torch.isnan(got[past]).all() and torch.equal(got[~past], want[~past])
+
+
+def test_two_streams_at_once():
+    """Choices and attention on two streams, with the streams' own scratch memory, as one after the other."""
+    calls, want = [], []
+    for seed in range(2):
+        p = Cache([3, 1], [5000, 3000], 2, 64, 16, "bf16", seed=seed)
+        a = Choice(p, 8, "bf16", 1, 2, 100, seed=seed)
+        a.run()
+        b = Picked(p, 8, "bf16", host(a.picked), host(a.lens), seed=seed).run()
+        want.append((a.picked.clone(), b.o.clone()))
+        calls.append((a, b, a.args(), (p.dev_table, p.dev_offs, p.dev_lens), b.args(), (p.dev_table, p.dev_offs, p.dev_lens)))
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(20):
+        for a, b, *_rest in calls:
+            a.picked.zero_(), b.o.fill_(7.0)  # rows of nobody stay
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, (a, b, c, _c, d, _d) in zip(streams, calls):
+                call("aic_hip_kv_select", *c, s.cuda_stream)
+                call("aic_hip_attn_paged_selected", *d, s.cuda_stream)
+        torch.cuda.synchronize()
+        for (a, b, *_rest), (picked, o) in zip(calls, want):
+            assert torch.equal(a.picked, picked) and torch.equal(b.o, o)
+
+
 @pytest.mark.parametrize("dt,cache", [("bf16", "e2m1"), ("bf16", "bf16"), ("f32", "f32")])
 def test_chosen_pages_captured(dt, cache):
     p = Cache([1], [4000], 2, 64, 16, cache, seed=5)
