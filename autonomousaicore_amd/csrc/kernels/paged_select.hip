@@ -230,19 +230,30 @@ __device__ __forceinline__ bool score_tile(const SelectArgs& s, int tokens, int 
     const PagedArgs& a = s.a;
     const int Hkv = a.kv.Hkv, tile = static_cast<int>(blockIdx.x) / Hkv;
     x.kvh = static_cast<int>(blockIdx.x) % Hkv;
-    PagedArgs one = a;  // find_tile counts rows of one head
-    one.G = 1;
-    int local;
-    bool found;
-    if (tokens == 32) found = find_tile<32>(one, tile, x.b, local);
-    else if (tokens == 16) found = find_tile<16>(one, tile, x.b, local);
-    else if (tokens == 8) found = find_tile<8>(one, tile, x.b, local);
-    else if (tokens == 4) found = find_tile<4>(one, tile, x.b, local);
-    else if (tokens == 2) found = find_tile<2>(one, tile, x.b, local);
-    else found = find_tile<1>(one, tile, x.b, local);
-    if (!found) return false;
-    x.sq = wave_sequence(a, x.b);
-    x.t0 = local * tokens, x.nt = min(tokens, x.sq.n - x.t0);
+    // 64 sequences per step, the found one's description from its lane
+    const int lane = threadIdx.x & 63, shift = __builtin_ctz(tokens);
+    x.b = -1;
+    int left = tile;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        Seq own{};
+        if (b0 + lane < a.B) own = sequence(a, b0 + lane);
+        const int tiles = (own.n >> shift) + ((own.n & (tokens - 1)) != 0), upto = wave_running_sum(tiles);
+        const uint64_t past = __ballot(left < upto);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            const auto row0 = static_cast<uint64_t>(own.row0);
+            x.b = b0 + l;
+            x.sq = {static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(at(static_cast<int>(row0 >> 32)))) << 32 |
+                                         static_cast<uint32_t>(at(static_cast<int>(row0)))),
+                    at(own.n), at(own.len)};
+            x.t0 = (left - at(upto - tiles)) << shift;
+            break;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (x.b < 0) return false;
+    x.nt = min(tokens, x.sq.n - x.t0);
     x.per = min(a.G, kRows / tokens);
     // rows past the workspace's pages have no scores (kv_pick_k)
     x.pages = static_cast<int>(min(static_cast<int64_t>(pages_of(a.kv, x.sq.len - x.sq.n + x.t0 + x.nt - 1)), s.n_pages));
