@@ -463,7 +463,7 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
     __shared__ uint4 bins[kBins / 4];
     __shared__ double ends[2][4];
     __shared__ int sums[3][4];
-    __shared__ int own_b, own_pos, cut_bin, cut_need, cut_count;
+    __shared__ int cut_bin, cut_need, cut_count;
 
     const double* scores = s.scores + at * s.n_pages;
     double kept[K > 0 ? K : 1];
@@ -471,19 +471,28 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
 #pragma unroll
         for (int j = 0; j < K; ++j) kept[j] = tid * K + j < s.n_pages ? scores[tid * K + j] : 0.0;
     }
-    if (tid == 0) own_b = -1, own_pos = -1;
-    __syncthreads();
-    for (int i = tid; i < a.B; i += kBlock) {
-        const int64_t from = a.offsets[i], to = a.offsets[i + 1], len = a.lens[i];
-        if (from <= t && t < to) {
-            const int64_t pos = len - (to - t);
-            own_b = i;
-            own_pos = pos < 0 || pos > kMaxLen ? -1 : static_cast<int>(pos);
+    // the row's sequence, by every wave for itself
+    int own_b = -1, pos = -1;
+    for (int b0 = 0; b0 < a.B && own_b < 0; b0 += 256) {
+        int64_t from[4], to[4], len[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = min(b0 + 64 * j + lane, a.B - 1);
+            from[j] = a.offsets[i], to[j] = a.offsets[i + 1], len[j] = a.lens[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint64_t here = __ballot(b0 + 64 * j + lane < a.B && from[j] <= t && t < to[j]);
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                const int64_t at_pos = len[j] - (to[j] - t);
+                own_b = b0 + 64 * j + l;
+                pos = __builtin_amdgcn_readlane(at_pos < 0 || at_pos > kMaxLen ? -1 : static_cast<int>(at_pos), l);
+            }
         }
     }
-    __syncthreads();
     const bool nobody = own_b < 0;
-    const int pos = own_pos, P = pages_of(a.kv, pos);
+    const int P = pages_of(a.kv, pos);
     int32_t* out = s.picked + at * s.n_sel;
     const int32_t* tr = a.kv.table + static_cast<int64_t>(nobody ? 0 : own_b) * a.kv.ld_table;
     auto id = [&](int p) { return p < a.kv.ld_table ? tr[p] : -1; };
