@@ -473,6 +473,7 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
     }
     // the row's sequence, by every wave for itself
     int own_b = -1, pos = -1;
+    bool past = false;  // of a sequence longer than lengths reach, whose tiles have scored other positions
     for (int b0 = 0; b0 < a.B && own_b < 0; b0 += 256) {
         int64_t from[4], to[4], len[4];
 #pragma unroll
@@ -487,7 +488,9 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
                 const int l = __builtin_ctzll(here);
                 const int64_t at_pos = len[j] - (to[j] - t);
                 own_b = b0 + 64 * j + l;
-                pos = __builtin_amdgcn_readlane(at_pos < 0 || at_pos > kMaxLen ? -1 : static_cast<int>(at_pos), l);
+                const int own_pos = at_pos < 0 ? -1 : len[j] > kMaxLen ? INT32_MAX : static_cast<int>(at_pos);
+                pos = __builtin_amdgcn_readlane(own_pos, l);
+                past = pos == INT32_MAX;
             }
         }
     }
@@ -496,7 +499,7 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
     int32_t* out = s.picked + at * s.n_sel;
     const int32_t* tr = a.kv.table + static_cast<int64_t>(nobody ? 0 : own_b) * a.kv.ld_table;
     auto id = [&](int p) { return p < a.kv.ld_table ? tr[p] : -1; };
-    if (P > s.n_pages) {  // past max_len: a position without a place, so that the row's attention is NaN
+    if (past || P > s.n_pages) {  // past max_len: a position without a place, so that the row's attention is NaN
         for (int i = tid; i < s.n_sel; i += kBlock) out[i] = -1;
         if (tid == 0) s.picked_lens[at] = 1;
         return;

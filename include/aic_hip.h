@@ -345,7 +345,8 @@ int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* of
  * which no q . k of the page's keys exceeds; sums in 64 bits, a NaN counts as infinity, ties go to the lower position.
  * q as in aic_hip_attn_paged.  picked [T][kv_heads][n_sel]: the pages' ids in order of position, then -1;
  * picked_lens [T][kv_heads]: the positions in them that the row sees, all but the last page whole.  A row of no sequence:
- * ids -1, length -1; at a position before 0: length 0; past max_len: id -1, length 1.  A page id outside [0, n_pages) is chosen as it is.
+ * ids -1, length -1; at a position before 0: ids -1, length 0; in a page behind that of position max_len - 1, or of a sequence longer than
+ * 2^31 - 4096: ids -1, length 1, so that its attention is NaN.  A page id outside [0, n_pages) is chosen as it is.
  * max_q: for the choice of forms.  max_len: the longest lens[b].  workspace: as aic_hip_attn_paged,
  * aic_hip_kv_select_workspace(cache, T, max_len) bytes; a captured call must bring one (InvalidState). */
 int64_t aic_hip_kv_select_workspace(const aic_kv_pages* cache, int64_t T, int64_t max_len); /* negative: -(error code) */
