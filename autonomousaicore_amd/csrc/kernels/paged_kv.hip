@@ -104,8 +104,10 @@ struct Cut {
     uint32_t mul;  // unit / ncol = unit * mul >> 32, exact for several rows' 1024 units; 0: one row
 };
 
+constexpr int kPastAll = -2;    // a position past 2^31 - 1
+
 // The places of the block's rows: page * Hkv * ps + slot, -1: none, -2: a row of no sequence.  where: their positions, -1
-// before 0 and for rows of no sequence.
+// before 0 and for rows of no sequence, or kPastAll.
 __device__ __forceinline__ void block_places(const PageView& pv, const Cut& c, int64_t t0, int64_t (&at)[kMaxRows], int* where = nullptr) {
     const int b0 = block_sequence(c.offsets, c.B, t0);
     const int r = static_cast<int>(threadIdx.x);
@@ -121,7 +123,8 @@ __device__ __forceinline__ void block_places(const PageView& pv, const Cut& c, i
         if (t < c.T && b >= 0 && b < c.B) {
             const int64_t pos = c.lens[b] - (end - t);
             place = -1;
-            if (pos >= 0 && pos <= INT32_MAX) {
+            if (pos > INT32_MAX) p = kPastAll;
+            else if (pos >= 0) {
                 const int64_t row = pv.row(pv.table + b * pv.ld_table, static_cast<int>(pos), 0);
                 if (row >= 0) place = row;
                 p = static_cast<int>(pos);
@@ -287,9 +290,9 @@ __global__ __launch_bounds__(kBlock) void kv_append_k(PageView pv, Cut c, Turn a
         const int u = u0 + i * kBlock, uu = min(u, last), r = row_of_unit(c, uu), col = uu - r * c.ncol, hh = col / LPH, d = col % LPH * 8;
         const bool q = hh < a.H, mine = u <= last;
         const int h = q ? hh : hh < heads ? hh - a.H : hh - heads;
-        const int p = pos[r];  // -1: of no sequence, or before 0
-        const bool past = p >= a.n_pos;
-        if (hh < heads && p >= 0) {
+        const int p = pos[r];
+        const bool turned = p != -1, past = p == kPastAll || p >= a.n_pos;
+        if (hh < heads && turned) {
             float cs[8], sn[8];
             const int64_t row = static_cast<int64_t>(past ? 0 : p) * (HD / 2) + d;
             load_row<float, 8>(a.cos_t + row, a.vec_t, cs);
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(kBlock) void kv_append_k(PageView pv, Cut c, Turn a
             }
         }
         if (q) {
-            if (mine && p >= 0) {
+            if (mine && turned) {
                 T* o = static_cast<T*>(a.q_out) + (t0 + r) * a.ld_qo + static_cast<int64_t>(h) * HD + d;
                 store_row<T, 8>(o, a.vec_qo, x1[i]);
                 store_row<T, 8>(o + HD / 2, a.vec_qo, x2[i]);

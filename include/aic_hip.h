@@ -300,7 +300,7 @@ int aic_hip_kv_read(const aic_kv_pages* cache, void* k, void* v, int64_t ld, con
  * positions, v as it is.  cos_t, sin_t: fp32 [n_pos, head_dim / 2] as aic_hip_rope_tables builds them; with x1, x2 the elements i and
  * i + head_dim / 2 of a head, y1 = x1 c - x2 s, y2 = x1 s + x2 c in fp32, each product and sum rounded, then one rounding to the
  * type, or the cache's codes.  Rows without a place in the cache: q is turned, k and v are not written.  Rows at a position before 0
- * are left as they are; at positions from n_pos on q_out is NaN, and k and v are not written.
+ * are left as they are; at positions from n_pos on, and past 2^31 - 1, q_out is NaN, and k and v are not written.
  * Replaces: RotaryPositionEmbedding::forward with its start position (include/nn/rope.hpp:23-112) and the cache's append
  * (include/nn/attention.hpp:49-120), which know one position for all sequences. */
 int aic_hip_kv_append(const aic_kv_pages* cache, const void* q, int64_t ld_q, void* q_out, int64_t ld_qo, int64_t H, const void* k,

@@ -8,6 +8,7 @@ pytestmark = pytest.mark.gpu
 
 from tests.gpu_util import host  # noqa: E402
 from tests.paged_codes_ref import Cache  # noqa: E402
+from tests.test_gpu_paged_append import TYPES, Append  # noqa: E402
 from tests.test_gpu_paged_select import Choice, Picked  # noqa: E402
 
 REACH = 2 ** 31 - 4096
@@ -52,3 +53,13 @@ def test_choice_of_many_rows_past_the_range():
     want[0][:40], want[1][:40] = -1, 1
     a.run()
     assert np.array_equal(host(a.lens), want[1]) and np.array_equal(host(a.picked), want[0])
+
+
+# ------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dt,cache", TYPES)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_past_the_range(dt, cache, in_place):
+    """q is NaN and nothing is written where positions are past 2^31 - 1, as from n_pos on; a chunk that reaches over it; the others as ever."""
+    p = Cache([2, 1, 3, 4], [300, 290, 300, 40], 2, 64, 16, cache, seed=3)
+    p.lens[1], p.lens[2] = 2 ** 40, 2 ** 31 + 1
+    Append(p, 4, dt, n_pos=300, in_place=in_place).check()
