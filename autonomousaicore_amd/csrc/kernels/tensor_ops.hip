@@ -350,9 +350,9 @@ void strided_copy(const void* src, int64_t offset, int ndim, const int64_t* shap
 void cast(const void* src, DType from, void* dst, DType to, int64_t n, hipStream_t s) {
     AIC_CHECK(n >= 0, InvalidArgument, "cast: negative count");
     const int f = static_cast<int>(from), t = static_cast<int>(to);
-    // the reference's table (src/tensor/tensor.cpp:392-407)
-    const bool known = f == t || (f == 0 && t >= 1 && t <= 4) || (t == 0 && f >= 1 && f <= 4) || (f == 4 && t == 3) ||
-                       (f == 3 && t == 4);
+    // the reference's table (src/tensor/tensor.cpp:392-407); of a type without a whole number of bytes, or none, not even to itself
+    const bool known = (f == t && dtype_size(from) > 0) || (f == 0 && t >= 1 && t <= 4) || (t == 0 && f >= 1 && f <= 4) ||
+                       (f == 4 && t == 3) || (f == 3 && t == 4);
     AIC_CHECK(known, NotImplemented, "Type cast from ", dtype_name(from), " to ", dtype_name(to), " not implemented");
     if (n == 0) return;
     AIC_CHECK(src && dst, InvalidArgument, "cast: null pointer");

@@ -692,7 +692,7 @@ int aic_qlora_linear_backward(aic_qlora_linear* m, const void* dy, void* dx, flo
 int aic_hip_strided_copy(const void* src, int64_t offset, int ndim, const int64_t* shape, const int64_t* strides,
                          int64_t elem_size, void* dst, aic_stream stream);
 /* n elements from -> to for the reference's cast table (f32<->f16, f32<->bf16, f32<->i64,
- * f32<->i32, i64<->i32), with its rounding and NaN encodings (include/core/dtype.hpp:65-133);
+ * f32<->i32, i64<->i32, and each of its types to itself), with its rounding and NaN encodings (include/core/dtype.hpp:65-133);
  * any other pair fails with NotImplemented (8).
  * Replaces: Tensor::to(DType) (src/tensor/tensor.cpp:359-410), a host round trip on the GPU. */
 int aic_hip_cast(const void* src, aic_dtype from, void* dst, aic_dtype to, int64_t n, aic_stream stream);
