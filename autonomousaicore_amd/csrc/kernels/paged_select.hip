@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kBlock) void kv_bounds_k(BoundArgs a) {
 struct SelectArgs {
     PagedArgs a;        // kv, q, ldq, T, offsets, lens, B, H, G, vec_q
     const void* bounds;
-    double* scores;     // [T][Hkv][n_pages]
+    double* scores;     // [T][Hkv][n_pages]; null: every row takes all its pages
     int64_t n_pages;    // of the longest cache
     int first, last, n_sel;
     int32_t* picked;
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
 
     const double* scores = s.scores + at * s.n_pages;
     double kept[K > 0 ? K : 1];
-    if constexpr (K > 0) {  // on their way before the row is known; what lies behind its pages is not used
+    if (K > 0 && s.scores) {  // on their way before the row is known; what lies behind its pages is not used
 #pragma unroll
         for (int j = 0; j < K; ++j) kept[j] = tid * K + j < s.n_pages ? scores[tid * K + j] : 0.0;
     }
@@ -665,7 +665,7 @@ int64_t kv_select_workspace(const KVPages& c, int64_t T, int64_t max_len) {
 void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q, const int64_t* offsets, const int64_t* lens, int64_t B,
                int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t first, int64_t last, int64_t n_sel, int32_t* picked,
                int64_t* picked_lens, void* workspace, int64_t workspace_bytes, DType dt, hipStream_t s) {
-    const int64_t need = kv_select_workspace(c, T, max_len);
+    const int64_t most = kv_select_workspace(c, T, max_len);
     AIC_CHECK(B >= 0 && B <= INT32_MAX, InvalidArgument, "kv_select: B must be 0 .. 2^31 - 1");
     AIC_CHECK(max_q >= 0, InvalidArgument, "kv_select: max_q must not be negative");
     AIC_CHECK(dt == DType::Float32 || dt == DType::BFloat16, DTypeMismatch, "kv_select: queries are float32 or bfloat16");
@@ -681,6 +681,8 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
     if (T == 0) return;
     AIC_CHECK(bounds && q && picked && picked_lens && (B == 0 || (offsets && lens)), InvalidArgument, "kv_select: null pointer");
     AIC_CHECK(reinterpret_cast<uintptr_t>(bounds) % 16 == 0, InvalidArgument, "kv_select: the bounds must be 16-byte aligned");
+    const bool scored = B > 0 && longest_pages(c, max_len) > n_sel;
+    const int64_t need = scored ? most : 0;
     const StreamScratchUse use(s);
     if (workspace) {
         AIC_CHECK(workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, InvalidArgument,
@@ -695,13 +697,13 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
     x.a.offsets = offsets, x.a.lens = lens;
     x.a.B = static_cast<int>(B), x.a.H = static_cast<int>(H), x.a.G = static_cast<int>(H / c.kv_heads);
     x.bounds = bounds;
-    x.scores = static_cast<double*>(workspace);
+    x.scores = scored ? static_cast<double*>(workspace) : nullptr;
     x.n_pages = longest_pages(c, max_len);
     x.first = static_cast<int>(first), x.last = static_cast<int>(last), x.n_sel = static_cast<int>(n_sel);
     x.picked = picked, x.picked_lens = picked_lens;
     const int64_t picks = T * c.kv_heads;
     AIC_CHECK(picks <= INT32_MAX, OutOfRange, "kv_select: too many rows in one call");
-    if (B > 0 && x.n_pages > n_sel) {
+    if (scored) {
         int tokens = 32;
         while (tokens > 1 && (tokens * x.a.G > kRows || tokens / 2 >= std::min(max_q, T))) tokens /= 2;
         const int64_t tiles = (tokens == 1 ? T : (T + tokens - 1) / tokens + std::min(B, T)) * c.kv_heads;

@@ -348,7 +348,8 @@ int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* of
  * ids -1, length -1; at a position before 0: ids -1, length 0; in a page behind that of position max_len - 1, or of a sequence longer than
  * 2^31 - 4096: ids -1, length 1, so that its attention is NaN.  A page id outside [0, n_pages) is chosen as it is.
  * max_q: for the choice of forms.  max_len: the longest lens[b].  workspace: as aic_hip_attn_paged,
- * aic_hip_kv_select_workspace(cache, T, max_len) bytes; a captured call must bring one (InvalidState). */
+ * aic_hip_kv_select_workspace(cache, T, max_len) bytes, none where max_len is at most n_sel pages; a captured call must bring one
+ * (InvalidState). */
 int64_t aic_hip_kv_select_workspace(const aic_kv_pages* cache, int64_t T, int64_t max_len); /* negative: -(error code) */
 int aic_hip_kv_select(const aic_kv_pages* cache, const void* bounds, const void* q, int64_t ld_q, const int64_t* offsets,
                       const int64_t* lens, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, int64_t first, int64_t last,
