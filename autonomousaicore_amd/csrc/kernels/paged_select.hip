@@ -3,8 +3,8 @@
 // bounds[page][kvh] holds, for each element, the least and the greatest value of the page's keys.  For a query q no key
 // of the page has more than sum_d q_d (hi_d where q_d >= 0, else lo_d); a row's score of a page is the largest of
 // its group's heads' sums.  Scores are compared with one another, so they are added in 64 bits, where a bf16
-// product is exact and equal sums come out equal in any order that their digits allow: the choice does not
-// depend on how the sum is cut.
+// product is exact and equal sums that 53 bits hold come out equal in any order: the choice does not depend on how such a sum is
+// cut.  Longer ones are rounded, so that pages whose scores agree in nearly all of 53 bits may change places between the forms below.
 //
 // kv_bounds_k: a wave per page and key/value head that the batch's rows touch; lanes hold 16 bytes of a key (8 of codes), the
 // wave's groups of lanes go over the keys in turn, with several loads in flight, and are joined at the end.  Prompts of 8 x 4096
@@ -67,6 +67,14 @@ __device__ __forceinline__ void load_key(const char* p, uint32_t byte, float (&x
 #pragma unroll
         for (int j = 0; j < EPL; ++j) x[j] = static_cast<float>(y[j]);
     }
+}
+
+// A bound as bf16: the least values towards -infinity, the greatest ones towards infinity.  Only of an e4m3 cache are there any between
+// the type's numbers, below its least one, 2^-133: to the nearest, a bound could leave a key out.
+template <bool UP>
+__device__ __forceinline__ bf16 bound_bf16(float x) {
+    const uint32_t u = __float_as_uint(x), away = UP ? x > 0.0f : x < 0.0f;
+    return __builtin_bit_cast(bf16, static_cast<uint16_t>((u + (away ? 0xffffu : 0u)) >> 16));
 }
 
 // f, idempotent, over the lanes that stand at the same place of their groups of L.
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(kBlock) void kv_bounds_k(BoundArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) lo[j] = across_groups<L>(lo[j], least), hi[j] = across_groups<L>(hi[j], most);
-    if (grp < 2) {  // one group writes the least, the next one the greatest values; exact: each is a cached value
+    if (grp < 2) {  // one group writes the least, the next one the greatest values
         using BT = std::conditional_t<std::is_same_v<CT, float>, float, bf16>;
         BT* out = static_cast<BT*>(a.bounds) + ((static_cast<int64_t>(page) * a.kv.Hkv + kvh) * 2 + grp) * HD + d0;
         constexpr int W = 16 / sizeof(BT);
@@ -151,7 +159,10 @@ __global__ __launch_bounds__(kBlock) void kv_bounds_k(BoundArgs a) {
         for (int j = 0; j < EPL; j += W) {
             vec_t y;
 #pragma unroll
-            for (int u = 0; u < W; ++u) y[u] = static_cast<BT>(grp == 0 ? lo[j + u] : hi[j + u]);
+            for (int u = 0; u < W; ++u) {
+                if constexpr (kE4<CT>) y[u] = grp == 0 ? bound_bf16<false>(lo[j + u]) : bound_bf16<true>(hi[j + u]);
+                else y[u] = static_cast<BT>(grp == 0 ? lo[j + u] : hi[j + u]);  // exact: each is a cached value
+            }
             *reinterpret_cast<vec_t*>(out + j) = y;
         }
     }

@@ -331,9 +331,10 @@ int aic_hip_attn_paged(const aic_kv_pages* cache, const void* q, int64_t ld_q, v
                        int64_t workspace_bytes, aic_dtype dt, aic_stream stream);
 /* Attention over chosen pages of long caches, in three calls.
  *
- * Bounds: bounds [n_pages][kv_heads][2][head_dim] (16-byte aligned; fp32 for an fp32 cache, otherwise bf16, which holds every cached value) gets,
+ * Bounds: bounds [n_pages][kv_heads][2][head_dim] (16-byte aligned; fp32 for an fp32 cache, otherwise bf16) gets,
  * for every page that the batch's rows stand in, the least and the greatest of each element over the page's keys
- * at positions below lens[b]; NaN where one of them is.  Other pages' bounds stay as they are: call it after each
+ * at positions below lens[b]; NaN where one of them is.  bf16 holds every cached value but for e4m3's bits below 2^-133: there the least
+ * is bf16's next number below, the greatest the next above.  Other pages' bounds stay as they are: call it after each
  * aic_hip_kv_write or aic_hip_kv_append of a batch, with the same offsets and lens.  Rows of two sequences must not stand in
  * one page (full pages may be shared).  Pages without a place are left out. */
 int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* offsets, const int64_t* lens, int64_t B, int64_t T,
@@ -342,7 +343,8 @@ int aic_hip_kv_bounds(const aic_kv_pages* cache, void* bounds, const int64_t* of
  * most n_sel, and otherwise the first `first` and the last `last` (at least 1: its own) ones and the n_sel - first - last others of the
  * greatest
  *   score = max over the head's query heads of sum_d q_d (hi_d where q_d >= 0, else lo_d)
- * which no q . k of the page's keys exceeds; sums in 64 bits, a NaN counts as infinity, ties go to the lower position.
+ * which no q . k of the page's keys exceeds; sums in 64 bits (of products beyond 53 bits rounded, in an order that may differ between sizes),
+ * a NaN counts as infinity, ties go to the lower position.
  * q as in aic_hip_attn_paged.  picked [T][kv_heads][n_sel]: the pages' ids in order of position, then -1;
  * picked_lens [T][kv_heads]: the positions in them that the row sees, all but the last page whole.  A row of no sequence:
  * ids -1, length -1; at a position before 0: ids -1, length 0; in a page behind that of position max_len - 1, or of a sequence longer than
