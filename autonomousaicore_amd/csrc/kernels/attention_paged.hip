@@ -427,10 +427,10 @@ void check_sizes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t 
 
 }  // namespace
 
-// Bytes of the parts of a call's sizes; picked: of rows with pages of their own, a sequence each (bf16 queries then always go to the
-// few rows' kernel).
 namespace {
 
+// Bytes of the parts of a call's sizes; picked: of rows with pages of their own, a sequence each (bf16 queries then always go to the
+// few rows' kernel).
 int64_t parts_bytes(const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t max_len, int64_t H, bool picked) {
     check_sizes(c, B, T, max_q, max_len, H);
     check_cache_shape(c, "attn_paged");
@@ -497,7 +497,7 @@ void attend(A& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t
         constexpr int D = decltype(hd)::value;
         const auto grid = static_cast<unsigned>(blocks);
         if constexpr (sizeof(X) == 2) {
-            if constexpr (!picked) attn_paged_tiles(a, c.type, D, grid, s);
+            attn_paged_tiles(a, c.type, D, grid, s);
         } else if (R <= 4) {
             attn_paged_f32_few(a, static_cast<int>(R), c.type, D, grid, s);
         } else {
@@ -520,7 +520,7 @@ void attend(A& a, const KVPages& c, int64_t B, int64_t T, int64_t max_q, int64_t
     };
     auto types = [&](auto hd) {
         if (dt == DType::Float32) run(float{}, hd);
-        else run(bf16{}, hd);
+        else if constexpr (!picked) run(bf16{}, hd);  // picked: the few rows' kernel, always
     };
     if (c.head_dim == 32) types(std::integral_constant<int, 32>{});
     else if (c.head_dim == 64) types(std::integral_constant<int, 64>{});

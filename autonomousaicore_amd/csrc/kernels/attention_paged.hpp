@@ -249,11 +249,6 @@ struct Rows {
             m = m_new;
         }
     }
-    // Whether a tile's row maxima would move the reference maximum, of any row.
-    __device__ __forceinline__ bool moves(float mx, float c) const {
-        mx = facing_op<32>(mx, [](float x, float y) { return fmaxf(x, y); });
-        return __ballot((mx - m) * c > kLazyRescale) != 0;
-    }
     // A tile's weights of this half of the wave join the sum.
     __device__ __forceinline__ void add(float sum) { l += facing_op<32>(sum, [](float x, float y) { return x + y; }); }
     // -m in log2 units, less down; a row that has seen only scores of -infinity counts from zero
