@@ -427,13 +427,18 @@ int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * 
 // 11.9 us with 12 heads of 64, 15.9 and 20.8 us with 8 of 128; of 2048: 13.3 and 13.9, 16.1 and 23.9 us.  With a group
 // for most CUs nothing is won by dividing up to 2048: 32 sequences with 8 heads of 128, 47.6 and 42.8 us.
 // e2m1, whose tiles take less time to come: 32 sequences of 4096, 36.0 in shares and 32.5 us whole; 64 of them 54.3 and 55.7.
-// Rows with pages of their own are all of the same length, so that blocks that fill a round of the card end together:
-// 256 of 8192 tokens of 128, bf16 188.2 and 184.5 us, e2m1 64.2 and 60.3; 2600 of 4096, 946 and 525 us (shares take neighbouring
-// rows' pages from each other's cache); 128 of 4096, bf16 50.3 and 46.9, e2m1 30.1 and 31.7; of 8192, 102.1 and
-// 102.3, 46.1 and 55.0; but 288 of 4096, a round and a little, 113.4 and 135.9, 45.8 and 55.4; 384 of 8192 278 and 279, 99.5 and 108.
+// Rows with pages of their own, heads of 128, shares and whole.  Rows of one length, as those of long caches mostly are, end together where
+// their blocks fill a round of the card: 256 of 8192 tokens, bf16 191 and 188 us, e2m1 69 and 62; 128 of 4096, bf16 50.3 and 46.9, e2m1
+// 30.1 and 31.7; of 8192, 102.1 and 102.3, 46.1 and 55.0; but 288 of 4096, a round and a little, 118 and 140, 48 and 57; 384 of
+// 8192 280 and 283; 512, 364 and 361, e2m1 124 and 114.  A caller's lengths may differ: 8 long rows among 216 of 1024 tokens are left alone at
+// the end, of 4096 30 and 48 us, of 8192 35 and 83, of 32768 54 and 296; with 504, 59 and 60, 58 and 94, 76 and 307.  So whole up to 8192.
+// From 2048 on at any length: these are a chunk's rows, which choose the same pages and take them from each other's cache while their blocks
+// run in step: 2600 of 4096, 808 and 486 us, of 16384, 3242 and 1653, of a quarter of that and more, 1886 and 1134 (pages chosen at random:
+// 3316 and 3388, 2029 and 2075); 8 of 32768 among 2592 of 1024, 267 and 380.
 int64_t whole_len(int64_t pairs, int64_t head_dim, DType type, bool picked) {
     const bool one_round = pairs <= 256;
-    if (picked && (pairs >= 512 || (pairs >= 224 && one_round))) return kMaxLen;
+    if (picked && pairs >= 2048) return kMaxLen;
+    if (picked && (pairs >= 512 || (pairs >= 224 && one_round))) return 8192;
     if (picked ? pairs >= 128 && one_round : type == DType::UInt4 && head_dim == 128 && pairs >= 192 && one_round) return 4096;
     return pairs >= 192 && !picked ? 2048 : head_dim < 128 ? 1536 : 1024;
 }
