@@ -426,7 +426,8 @@ int64_t group_of(int64_t max_q, int64_t G) { return std::clamp<int64_t>(max_q * 
 // undivided group 0.3 us (head_dim 64) to 0.7 us (128).  One sequence of 1600 tokens, shares and whole: 13.3 and
 // 11.9 us with 12 heads of 64, 15.9 and 20.8 us with 8 of 128; of 2048: 13.3 and 13.9, 16.1 and 23.9 us.  With a group
 // for most CUs nothing is won by dividing up to 2048: 32 sequences with 8 heads of 128, 47.6 and 42.8 us.
-// e2m1, whose tiles take less time to come: 32 sequences of 4096, 36.0 in shares and 32.5 us whole; 64 of them 54.3 and 55.7.
+// e2m1, whose tiles take less time to come: 32 sequences of 4096, 37.1 in shares and 32.8 us whole, of a quarter of that and more 31.2 and
+// 31.8, 24 sequences 34.4 and 32.0, 29.8 and 31.8 (one of 4096 among others of 512, 20 and 31); 64 of them 54.3 and 55.7.
 // Rows with pages of their own, heads of 128, shares and whole.  Rows of one length, as those of long caches mostly are, end together where
 // their blocks fill a round of the card: 256 of 8192 tokens, bf16 191 and 188 us, e2m1 69 and 62; 128 of 4096, bf16 50.3 and 46.9, e2m1
 // 30.1 and 31.7; of 8192, 102.1 and 102.3, 46.1 and 55.0; but 288 of 4096, a round and a little, 118 and 140, 48 and 57; 384 of
@@ -463,9 +464,9 @@ int64_t few_workspace(int64_t B, int64_t Hkv, int64_t max_q, int64_t max_len, in
 
 template <typename A>
 void attn_paged_few(const A& a, int64_t max_q, DType type, int head_dim, void* workspace, hipStream_t s) {
-    // e2m1 and picked pages: shares of two steps where there are few.  One token, 2 heads of 128, 64 pages of 64: 14.0 us so and 15.0 in fours (bf16 14.4 and
-    // 17.0); of 2000 tokens, 13.6 and 15.7; 8 heads, 64 pages, 14.1 and 15.3; but of 32000 tokens, 500 steps, 25.1 and 20.8.  (Other calls keep
-    // their parts, and so their sums' last bits.)
+    // e2m1 and picked pages: shares of two steps where there are few.  One token, 2 heads of 128, 64 pages of 64: 13.6 us so and 15.1 in fours (bf16 14.4 and
+    // 16.2), 256 pages, 18.0 and 17.5; of 2000 tokens, 13.4 and 15.5; of 16000, 250 steps, 18.3 and 17.6; of 32000, 24.9 and 20.7; 8 heads, 64
+    // pages, 14.0 and 15.7.  (Other calls keep their parts, and so their sums' last bits.)
     const int least = std::is_same_v<A, PickedArgs> || type == DType::UInt4 ? 2 : kLeast;
     FewArgs<A> f{a, static_cast<int>(group_of(max_q, a.G)), 0, least, nullptr, nullptr, nullptr};
     if (workspace) {

@@ -17,8 +17,8 @@
 // kv_score_many_k: the same for chunks and large groups on the matrix units, also in 64 bits.
 // kv_pick_k: a block per row and key/value head finds the score that separates the chosen pages (10 bits of
 // their order at a time, from the first bit in which they differ) and writes the pages in order of position.  The scores stay
-// in registers, a thread has neighbouring pages: 64 of 2048 pages 7.5 us (read from memory at each step: 14.6), 32 x 8 rows' 32 of
-// 512 4.8 (9.6): steps of a block that wait for one another.
+// in registers, a thread has neighbouring pages: 64 of 2048 pages 7.7 us, 32 x 8 rows' 64 of 512 5.2, steps of a block that wait for one
+// another (read from memory at each step, the calls take 17.3 for 13.8 and 19.9 for 19.0).
 #include <algorithm>
 
 #include "../runtime/memory_pool.hpp"
@@ -627,8 +627,9 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
 // two rounds of them: 16.2 us for 13.9).
 constexpr int64_t kScoreBlocks = 1024;
 // Pairs of a tile from which on the matrix units score them, 16 rows of a product being there in any case.  The call: 512 tokens of 32 heads over 8
-// on 512 pages, 113.7 us and 246.9 with kv_score_k; 2 x 8 tokens, 18.9 and 29.8; a token's 16 heads of a group, 32 sequences, 29.2 and 36.7; its 8, 40.8 and
-// 38.7.
+// on 512 pages, 113.9 us and 244 with kv_score_k; 2 x 8 tokens, 18.5 and 29.4; 16 x 5 tokens of 2 heads, 24.4 and 28.2; a token's 16 heads of a group,
+// 32 sequences, 27.8 and 35.2; its 8, 40.3 and 38.4.  Tiles so few that a wave takes one step's pages (below) do not come here: one sequence of 512 pages,
+// 32 heads over 8, 8 tokens, 20.4 so and 18.2 here, 4 tokens, 14.9 and 14.3, 2 tokens, 12.1 and 13.8.
 constexpr int64_t kManyPairs = 9;
 int64_t longest_pages(const KVPages& c, int64_t max_len) { return (max_len + c.page_size - 1) / c.page_size; }
 
@@ -736,7 +737,7 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
         };
         auto run = [&](auto hd) {
             // 16 pages of a wave; one step's where that would leave CUs without a block: the call on 2048 pages of 2 heads, 64 blocks
-            // 16.5, 256 13.9 us; 2 x 512 of 8 heads, 128 and 512 blocks, 10.9 and 10.7; 32 of them, 18.9 and 21.2
+            // 16.5, 256 13.8 us; 2 x 512 of 8 heads, 128 and 512 blocks, 11.5 and 11.5; 8 of them, 12.0 and 12.4; 32, 19.0 and 20.4
             constexpr int NS = decltype(hd)::value / 32;
             if (NS > 1 && tiles * ((x.n_pages + 63) / 64) < 256) launch(hd, std::integral_constant<int, 1>{});
             else launch(hd, std::integral_constant<int, NS>{});
@@ -747,8 +748,8 @@ void kv_select(const KVPages& c, const void* bounds, const void* q, int64_t ld_q
         AIC_LAUNCH_CHECK("kv_select scores");
     }
     const auto grid = static_cast<unsigned>(picks);
-    // the call, 2 kept, 8 kept and none: 512 pages, 32 x 8 rows, 19.4, 21.1 and 20.3 us; 2048 pages, 2 rows, 13.9 with 8 and 17.4 without,
-    // 32 x 8 rows 48.0 and 52.0
+    // the call, 2 kept, 8 kept and none: 512 pages, 32 x 8 rows, 19.0, 20.9 and 19.9 us; 2048 pages, 2 rows, 13.8 with 8 and 17.3 without,
+    // 32 x 8 rows 46.3 and 50.6
     if (x.n_pages <= 2 * kBlock) kv_pick_k<2><<<grid, kBlock, 0, s>>>(x);
     else if (x.n_pages <= 8 * kBlock) kv_pick_k<8><<<grid, kBlock, 0, s>>>(x);
     else kv_pick_k<0><<<grid, kBlock, 0, s>>>(x);

@@ -315,8 +315,9 @@ int aic_hip_kv_append(const aic_kv_pages* cache, const void* q, int64_t ld_q, vo
  * row that sees a position without a place in the cache is NaN.  What a row does not see does not
  * reach it, infinities and NaN included.  Values of all sizes from 2^-117 to the largest keep their digits, next to one another
  * too: rows whose sums over finite v would leave fp32's range (and rows that see an infinity or NaN in a v)
- * take twice the time, in chunks on e4m3 caches with the largest powers up to three times.  q . k is held in fp32 before the
- * scale.  scale > 0.
+ * take twice the time, in chunks on e4m3 caches with the largest powers, or on e2m1 caches with a NaN group, up to three times.
+ * q . k is held in fp32 before the scale, and so are the weights' sums; bf16 queries' weights are rounded to bf16 for the product with v.
+ * scale > 0.
  * max_q and max_len: the most rows of a sequence and the longest lens[b], for the choice of
  * kernels; larger values in offsets and lens give right results, slower.
  * workspace: device memory of at least aic_hip_attn_paged_workspace(...) bytes for the same sizes,
