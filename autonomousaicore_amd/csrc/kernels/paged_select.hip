@@ -499,9 +499,8 @@ __global__ __launch_bounds__(kBlock) void kv_pick_k(SelectArgs s) {
                 const int l = __builtin_ctzll(here);
                 const int64_t at_pos = len[j] - (to[j] - t);
                 own_b = b0 + 64 * j + l;
-                const int own_pos = at_pos < 0 ? -1 : len[j] > kMaxLen ? INT32_MAX : static_cast<int>(at_pos);
-                pos = __builtin_amdgcn_readlane(own_pos, l);
-                past = pos == INT32_MAX;
+                pos = __builtin_amdgcn_readlane(at_pos < 0 ? -1 : static_cast<int>(min(at_pos, kMaxLen)), l);
+                past = pos >= 0 && __ballot(len[j] > kMaxLen) >> l & 1;
             }
         }
     }
